@@ -52,7 +52,10 @@ def _build(force: bool, verbose: bool, defines, tag: str) -> str:
     os.makedirs(LIB_DIR, exist_ok=True)
     obj_dir = os.path.join(HERE, "build" + ("_" + tag if tag else ""))
     os.makedirs(obj_dir, exist_ok=True)
-    flags = ["-O3", "-std=c++17", "--offload-arch=" + ARCH, "-fPIC", "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function"]
+    flags = ["-O3", "-std=c++17", "--offload-arch=" + ARCH, "-fPIC", "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function",
+             # no packed fp32 arithmetic: the compiler forms it from ordinary float code, and some of its forms have given
+             # wrong results on the target now and then (the host pass does not know the feature and says so)
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     flags += ["-D" + d for d in defines]
     procs, objs = [], []
     for src in sources():
