@@ -11,7 +11,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libhhrl_hip.so")
 
-ACT_NONE, ACT_RELU, ACT_TANH, ACT_SIGMOID = 0, 1, 2, 3
+ACT_NONE, ACT_RELU, ACT_TANH, ACT_SIGMOID, ACT_SILU = 0, 1, 2, 3, 4
 
 _P = C.c_void_p
 _I = C.c_int
@@ -19,7 +19,7 @@ _L = C.c_long
 _F = C.c_float
 _D = C.c_double
 
-ABI_VERSION = 104            # HHRL_ABI_VERSION of include/hhrl_hip.h
+ABI_VERSION = 105            # HHRL_ABI_VERSION of include/hhrl_hip.h
 
 
 class LstmDesc(C.Structure):
@@ -80,6 +80,31 @@ class LinearBwdDesc(C.Structure):
                 ("dx", _P), ("lddx", _I), ("dx_accumulate", _I), ("dw", _P), ("db", _P),
                 ("K", _I), ("N", _I), ("act", _I)]
 
+
+GDR_MAX_K, GDR_MAX_V = 128, 512
+
+
+class GdrDesc(C.Structure):
+    """hhrl_gdr_desc of include/hhrl_hip.h."""
+    _fields_ = [("dtype", _I), ("n_seq", _I), ("rows", _L), ("Hk", _I), ("Hv", _I), ("K", _I), ("V", _I), ("scale", _F),
+                ("starts", _P), ("lens", _P), ("q", _P), ("k", _P), ("v", _P), ("ldq", _L), ("ldk", _L), ("ldv", _L),
+                ("g", _P), ("beta", _P), ("ldg", _L), ("ldbeta", _L), ("o", _P), ("ldo", _L), ("s0", _P), ("s1", _P),
+                ("no_backward", _I), ("d_o", _P), ("lddo", _L), ("d_s1", _P), ("d_s0", _P),
+                ("dq", _P), ("dk", _P), ("dv", _P), ("lddq", _L), ("lddk", _L), ("lddv", _L),
+                ("dg", _P), ("dbeta", _P), ("lddg", _L), ("lddbeta", _L), ("ws", _P), ("ws_floats", _L)]
+
+
+class BlockNormDesc(C.Structure):
+    """hhrl_block_norm_desc of include/hhrl_hip.h."""
+    _fields_ = [("dtype", _I), ("M", _L), ("H", _I), ("D", _I), ("post", _I), ("pre", _I), ("gate_act", _I), ("gate_rows", _L),
+                ("alpha", _F), ("scale", _F), ("eps", _F),
+                ("x", _P), ("y", _P), ("gate", _P), ("ldx", _L), ("ldy", _L), ("ldgate", _L),
+                ("w_post", _P), ("b_post", _P), ("w_pre", _P), ("b_pre", _P), ("out", _P), ("h", _P), ("ldo", _L), ("ldh", _L),
+                ("d_out", _P), ("d_h", _P), ("lddo", _L), ("lddh", _L),
+                ("dx", _P), ("dy", _P), ("dgate", _P), ("lddx", _L), ("lddy", _L), ("lddgate", _L),
+                ("dw_post", _P), ("db_post", _P), ("dw_pre", _P), ("db_pre", _P), ("ws", _P), ("ws_floats", _L)]
+
+
 # name -> (restype, argtypes); mirrors include/hhrl_hip.h one to one
 SIGNATURES = {
     "hhrl_version": (_I, []),
@@ -123,6 +148,13 @@ SIGNATURES = {
     "hhrl_lstm_backward": (_I, [_P, _P, _I, _P, _P, _I, _I, _I, _I, _P]),
     "hhrl_lstm_forward_group": (_I, [_P, _I, _I, _I, _I, _P]),
     "hhrl_lstm_backward_group": (_I, [_P, _I, _I, _I, _I, _P]),
+    "hhrl_gdr_workspace_floats": (_L, [_I, _I, _L, _I, _I, _I, _I, _I, _I]),
+    "hhrl_gdr_forward": (_I, [_P, _P]),
+    "hhrl_gdr_backward": (_I, [_P, _P]),
+    "hhrl_gdr_step": (_I, [_I, _I, _I, _I, _I, _I, _F, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _I, _P, _P]),
+    "hhrl_block_norm_workspace_floats": (_L, [_L, _I, _I, _L]),
+    "hhrl_block_norm_forward": (_I, [_P, _P]),
+    "hhrl_block_norm_backward": (_I, [_P, _P]),
     "hhrl_adam_step": (_I, [_P, _P, _P, _P, _L, _D, _D, _D, _D, _I, _D, _P]),
     "hhrl_adam_step_copy": (_I, [_P, _P, _P, _P, _L, _D, _D, _D, _D, _I, _D, _P, _P, _P]),
     "hhrl_adam_stage": (_I, [_P, _D, _D, _D, _D, _I, _D, _P]),

@@ -1,0 +1,280 @@
+"""Sequence layers beside the BiLSTM of `ops`: the gated delta rule (`GatedDelta`: a matrix state per head, whole
+sequences forward and backward, one token per agent against a pool of states) and the norms before and after a block with
+its gate and residual scale (`BlockNorm`).
+
+Operands are torch tensors on the current device; every call enqueues on torch's current stream and returns at once.
+Outputs, gradients and workspaces are the caller's: a call allocates nothing, so it can be recorded into a HIP graph.
+What a call cannot take (type, shape, strides, device) raises ValueError before anything is launched; errors of the
+library raise `_lib.HipError`.  A workspace belongs to one forward and its backward at a time: calls that may run at once
+(two streams, two graphs) need one each.  Tensors that another stream writes or frees are ordered by the caller, as for
+any torch operation."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import ACT_NONE, ACT_SIGMOID, ACT_SILU, check
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}            # HHRL_F32, HHRL_BF16
+_NORMS = {"none": 0, "rms": 1, "layer": 2}                 # HHRL_NORM_*
+_GATES = {"none": ACT_NONE, "sigmoid": ACT_SIGMOID, "silu": ACT_SILU}
+
+
+def _need(ok: bool, msg: str) -> None:
+    if not ok:
+        raise ValueError(msg)
+
+
+def _dtype_code(dtype) -> int:
+    _need(dtype in _DTYPES, "dtype %s: float32 and bfloat16 are supported" % (dtype,))
+    return _DTYPES[dtype]
+
+
+def _on_device(name: str, t: torch.Tensor) -> None:
+    _need(t.is_cuda, "%s is on %s, not on a GPU" % (name, t.device))
+    _need(t.device.index == torch.cuda.current_device(),
+          "%s is on %s, the current device is cuda:%d" % (name, t.device, torch.cuda.current_device()))
+
+
+def _tensor(name: str, t, shape, dtype) -> int:
+    """Checks a contiguous tensor of a given shape; its address."""
+    _need(isinstance(t, torch.Tensor), "%s is not a tensor" % name)
+    _need(tuple(t.shape) == tuple(shape), "%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
+    _need(t.dtype == dtype, "%s is %s, not %s" % (name, t.dtype, dtype))
+    _need(t.is_contiguous(), "%s is not contiguous" % name)
+    _on_device(name, t)
+    return t.data_ptr()
+
+
+def _rows(name: str, t, lead, tail, dtype):
+    """Checks a tensor [*lead, *tail] whose tail is contiguous and whose leading dimensions are rows at one distance
+    (a column range of a wider buffer qualifies): its address and that distance in elements."""
+    _need(isinstance(t, torch.Tensor), "%s is not a tensor" % name)
+    _need(tuple(t.shape) == tuple(lead) + tuple(tail), "%s has shape %s, not %s" % (name, tuple(t.shape), tuple(lead) + tuple(tail)))
+    _need(t.dtype == dtype, "%s is %s, not %s" % (name, t.dtype, dtype))
+    _on_device(name, t)
+    n, width = len(lead), 1
+    for size, stride in zip(reversed(t.shape[n:]), reversed(t.stride()[n:])):
+        _need(size == 1 or stride == width, "%s: the elements of a row are not contiguous (strides %s)" % (name, t.stride()))
+        width *= size
+    ld = None
+    inner = 1                                     # rows below the dimension at hand
+    for size, stride in zip(reversed(t.shape[:n]), reversed(t.stride()[:n])):
+        if size > 1:
+            if ld is None and stride % inner == 0:
+                ld = stride // inner
+            _need(ld is not None and stride == ld * inner, "%s: its rows are not at one distance (strides %s)" % (name, t.stride()))
+        inner *= size
+    ld = width if ld is None else ld
+    _need(ld >= width, "%s: rows overlap (strides %s)" % (name, t.stride()))
+    return t.data_ptr(), ld
+
+
+class GatedDelta:
+    """Shapes and scale of a gated delta rule layer: Hk key heads of K elements, Hv value heads of V elements (value head
+    h reads key head h // (Hv // Hk)).  Per value head, with the log decay g_t <= 0 and the step size beta_t:
+
+        S <- exp(g_t) S;   S <- S + beta_t k_t (v_t - S^T k_t)^T;   o_t = scale * S^T q_t       (scale: K ** -0.5)
+
+    q, k, v, o and their gradients are `dtype`; g, beta, states and their gradients float32.  Sequences come as
+    [B, T, heads, width] (`lens`: B int32 numbers of valid tokens, the rest of a row is padding) or packed as
+    [rows, heads, width] with `starts` (n + 1 ascending int32 numbers; rows behind starts[n] belong to nobody).  Padding is
+    neither read nor written."""
+
+    def __init__(self, Hk: int, Hv: int, K: int, V: int, dtype=torch.float32, scale: Optional[float] = None):
+        self.code = _dtype_code(dtype)
+        _need(Hk > 0 and Hv > 0 and Hv % Hk == 0, "Hv=%d is not a multiple of Hk=%d" % (Hv, Hk))
+        _need(0 < K <= _lib.GDR_MAX_K and 0 < V <= _lib.GDR_MAX_V, "K=%d V=%d: up to %d, %d supported" % (K, V, _lib.GDR_MAX_K, _lib.GDR_MAX_V))
+        self.Hk, self.Hv, self.K, self.V, self.dtype = Hk, Hv, K, V, dtype
+        self.scale = float(K) ** -0.5 if scale is None else float(scale)
+        self._lib = _lib.load()
+
+    def workspace(self, n_seq: int, rows: int, device, packed: bool = True, no_backward: bool = False) -> torch.Tensor:
+        """Workspace for n_seq sequences of `rows` tokens in all (of one padded length if not packed); what serves packed
+        sequences serves as many padded ones too."""
+        n = self._lib.hhrl_gdr_workspace_floats(self.code, n_seq, rows, int(packed), self.Hk, self.Hv, self.K, self.V, int(no_backward))
+        _need(n > 0, "no workspace for n_seq=%d rows=%d" % (n_seq, rows))
+        return torch.empty(n, dtype=torch.float32, device=device)
+
+    def _desc(self, q, k, v, g, beta, ws, starts, lens):
+        d = _lib.GdrDesc()
+        _need(isinstance(q, torch.Tensor), "q is not a tensor")
+        if starts is not None:
+            _need(lens is None, "starts and lens")
+            _need(q.dim() == 3, "packed q has shape %s, not [rows, Hk, K]" % (tuple(q.shape),))
+            lead = (q.shape[0],)
+            _need(isinstance(starts, torch.Tensor) and starts.dim() == 1 and starts.numel() >= 2, "starts: n_seq + 1 numbers")
+            n_seq = starts.numel() - 1
+            d.starts = _tensor("starts", starts, (n_seq + 1,), torch.int32)
+        else:
+            _need(q.dim() == 4, "q has shape %s, not [B, T, Hk, K]" % (tuple(q.shape),))
+            lead = tuple(q.shape[:2])
+            n_seq = lead[0]
+            if lens is not None:
+                d.lens = _tensor("lens", lens, (n_seq,), torch.int32)
+        rows = 1
+        for s in lead:
+            rows *= s
+        _need(rows > 0, "no tokens")
+        d.dtype, d.n_seq, d.rows = self.code, n_seq, rows
+        d.Hk, d.Hv, d.K, d.V, d.scale = self.Hk, self.Hv, self.K, self.V, self.scale
+        d.q, d.ldq = _rows("q", q, lead, (self.Hk, self.K), self.dtype)
+        d.k, d.ldk = _rows("k", k, lead, (self.Hk, self.K), self.dtype)
+        d.v, d.ldv = _rows("v", v, lead, (self.Hv, self.V), self.dtype)
+        d.g, d.ldg = _rows("g", g, lead, (self.Hv,), torch.float32)
+        d.beta, d.ldbeta = _rows("beta", beta, lead, (self.Hv,), torch.float32)
+        _need(isinstance(ws, torch.Tensor), "ws is not a tensor")
+        d.ws, d.ws_floats = _tensor("ws", ws, (ws.numel(),), torch.float32), ws.numel()
+        return d, lead, n_seq
+
+    def _state(self, name, t, n_seq):
+        return _tensor(name, t, (n_seq, self.Hv, self.K, self.V), torch.float32) if t is not None else None
+
+    def fwd(self, q, k, v, g, beta, o, ws, s0=None, s1=None, starts=None, lens=None, no_backward: bool = False) -> None:
+        """Writes o and, where given, s1 (states behind the sequences, from s0 or zero).  Leaves in ws what `bwd` of the
+        same inputs reads, unless no_backward."""
+        d, lead, n = self._desc(q, k, v, g, beta, ws, starts, lens)
+        d.o, d.ldo = _rows("o", o, lead, (self.Hv, self.V), self.dtype)
+        d.s0, d.s1 = self._state("s0", s0, n), self._state("s1", s1, n)
+        d.no_backward = int(no_backward)
+        check(self._lib.hhrl_gdr_forward(C.byref(d), _lib.stream_ptr()))
+
+    def bwd(self, q, k, v, g, beta, d_o, dq, dk, dv, dg, dbeta, ws, d_s1=None, d_s0=None, starts=None, lens=None) -> None:
+        """Gradients of <d_o, o> + <d_s1, s1> (either None: absent), written to dq, dk, dv, dg, dbeta and d_s0; ws as the
+        forward call of the same inputs left it."""
+        d, lead, n = self._desc(q, k, v, g, beta, ws, starts, lens)
+        if d_o is not None:
+            d.d_o, d.lddo = _rows("d_o", d_o, lead, (self.Hv, self.V), self.dtype)
+        d.d_s1, d.d_s0 = self._state("d_s1", d_s1, n), self._state("d_s0", d_s0, n)
+        d.dq, d.lddq = _rows("dq", dq, lead, (self.Hk, self.K), self.dtype)
+        d.dk, d.lddk = _rows("dk", dk, lead, (self.Hk, self.K), self.dtype)
+        d.dv, d.lddv = _rows("dv", dv, lead, (self.Hv, self.V), self.dtype)
+        d.dg, d.lddg = _rows("dg", dg, lead, (self.Hv,), torch.float32)
+        d.dbeta, d.lddbeta = _rows("dbeta", dbeta, lead, (self.Hv,), torch.float32)
+        check(self._lib.hhrl_gdr_backward(C.byref(d), _lib.stream_ptr()))
+
+    def step(self, q, k, v, g, beta, o, state, state_out=None, slots=None) -> None:
+        """One token for each of B rows (q, k [B, Hk, K], v, o [B, Hv, V], g, beta [B, Hv]) against a pool of states
+        [n, Hv, K, V]: row b moves state slots[b] (None: state b) into state_out (None: in place).  A negative slot: the
+        row is idle, its output 0.  A slot past the pool, or one that an earlier row names: output NaN, no state moves."""
+        _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q is not [B, Hk, K]")
+        B = q.shape[0]
+        _need(B > 0, "no rows")
+        _need(isinstance(state, torch.Tensor) and state.dim() == 4 and state.shape[0] > 0, "state is not [n, Hv, K, V]")
+        n = state.shape[0]
+        sp = self._state("state", state, n)
+        so = sp if state_out is None else self._state("state_out", state_out, n)
+        ptrs = []
+        for name, t, tail, dt in (("q", q, (self.Hk, self.K), self.dtype), ("k", k, (self.Hk, self.K), self.dtype),
+                                  ("v", v, (self.Hv, self.V), self.dtype), ("g", g, (self.Hv,), torch.float32),
+                                  ("beta", beta, (self.Hv,), torch.float32), ("o", o, (self.Hv, self.V), self.dtype)):
+            ptrs += _rows(name, t, (B,), tail, dt)
+        sl = _tensor("slots", slots, (B,), torch.int32) if slots is not None else None
+        _need(slots is not None or B <= n, "%d rows for %d states" % (B, n))
+        check(self._lib.hhrl_gdr_step(self.code, B, self.Hk, self.Hv, self.K, self.V, self.scale, *ptrs, sp, so, n, sl, _lib.stream_ptr()))
+
+
+class BlockNorm:
+    """Norms after a block (`post`) and before the next (`pre`) with the block's gate and residual scale:
+
+        r = alpha * x + scale * a(gate) * post(y);    h = pre(r)
+
+    per group of D elements (H groups per row), in one pass over the rows.  post, pre: "none", "rms", "layer", each with
+    optional float32 weight and bias [D]; gate_act a: "none", "sigmoid", "silu".  x, y, gate, out (r), h and their gradients
+    are `dtype`, [M, H, D], or [M, D] if H is 1; with gate_rows > 1 (H 1) the gate is float32 [ceil(M / gate_rows), D], a row
+    for every gate_rows rows of x.  Without x there is no residual stream, without y only the norm in front of a block."""
+
+    PARAMS = ("w_post", "b_post", "w_pre", "b_pre")
+
+    def __init__(self, D: int, H: int = 1, post: str = "none", pre: str = "none", gate_act: str = "none", gate_rows: int = 1,
+                 alpha: float = 1.0, scale: float = 1.0, eps: float = 1e-6, dtype=torch.float32):
+        self.code = _dtype_code(dtype)
+        _need(post in _NORMS and pre in _NORMS, "norms %r, %r: none, rms or layer" % (post, pre))
+        _need(gate_act in _GATES, "gate_act %r: none, sigmoid or silu" % (gate_act,))
+        _need(0 < D <= 8192 and H > 0, "H=%d D=%d: D up to 8192" % (H, D))
+        _need(gate_rows >= 1 and (gate_rows == 1 or H == 1), "gate_rows=%d with H=%d" % (gate_rows, H))
+        _need(eps >= 0, "eps=%g" % eps)
+        self.D, self.H, self.post, self.pre, self.gate_act, self.gate_rows = D, H, post, pre, gate_act, gate_rows
+        self.alpha, self.scale, self.eps, self.dtype = float(alpha), float(scale), float(eps), dtype
+        self._lib = _lib.load()
+
+    def workspace(self, M: int, device) -> torch.Tensor:
+        """Workspace of `bwd` for M rows."""
+        n = self._lib.hhrl_block_norm_workspace_floats(M, self.H, self.D, self.gate_rows)
+        _need(n > 0, "no workspace for M=%d" % M)
+        return torch.empty(n, dtype=torch.float32, device=device)
+
+    def _act(self, name, t, M):
+        tail = (self.H, self.D) if t.dim() == 3 or self.H > 1 else (self.D,)
+        return _rows(name, t, (M,), tail, self.dtype)
+
+    def _gate(self, name, t, M):
+        if self.gate_rows == 1:
+            return self._act(name, t, M)
+        return _rows(name, t, (-(-M // self.gate_rows),), (1, self.D) if t.dim() == 3 else (self.D,), torch.float32)
+
+    def _desc(self, x, y, gate, params):
+        d = _lib.BlockNormDesc()
+        first = x if x is not None else y
+        _need(isinstance(first, torch.Tensor), "neither x nor y")
+        M = first.shape[0] if first.dim() else 0
+        _need(M > 0, "no rows")
+        _need(y is not None or (gate is None and self.post == "none"), "a gate or a post norm without y")
+        d.dtype, d.M, d.H, d.D = self.code, M, self.H, self.D
+        d.post, d.pre, d.gate_act, d.gate_rows = _NORMS[self.post], _NORMS[self.pre], _GATES[self.gate_act], self.gate_rows
+        d.alpha, d.scale, d.eps = self.alpha, self.scale, self.eps
+        for name, t in (("x", x), ("y", y)):
+            if t is not None:
+                _need(isinstance(t, torch.Tensor), "%s is not a tensor" % name)
+                p, ld = self._act(name, t, M)
+                setattr(d, name, p)
+                setattr(d, "ld" + name, ld)
+        if gate is not None:
+            _need(isinstance(gate, torch.Tensor), "gate is not a tensor")
+            d.gate, d.ldgate = self._gate("gate", gate, M)
+        for name, t in zip(self.PARAMS, params):
+            if t is not None:
+                _need(getattr(self, name[2:]) != "none", "%s without a %s norm" % (name, name[2:]))
+                setattr(d, name, _tensor(name, t, (self.D,), torch.float32))
+        return d, M
+
+    def fwd(self, x=None, y=None, gate=None, w_post=None, b_post=None, w_pre=None, b_pre=None, out=None, h=None) -> None:
+        """Writes r to out and pre(r) to h (either may be None; both may be x or y)."""
+        d, M = self._desc(x, y, gate, (w_post, b_post, w_pre, b_pre))
+        _need(out is not None or h is not None, "neither out nor h")
+        _need(self.pre == "none" or h is not None, "a pre norm without h")
+        if out is not None:
+            d.out, d.ldo = self._act("out", out, M)
+        if h is not None:
+            d.h, d.ldh = self._act("h", h, M)
+        check(self._lib.hhrl_block_norm_forward(C.byref(d), _lib.stream_ptr()))
+
+    def bwd(self, x=None, y=None, gate=None, w_post=None, b_post=None, w_pre=None, b_pre=None, d_out=None, d_h=None,
+            dx=None, dy=None, dgate=None, dw_post=None, db_post=None, dw_pre=None, db_pre=None, ws=None) -> None:
+        """Gradients of <d_out, r> + <d_h, h> (either None: absent) from the forward call's inputs: dx, dy, dgate are
+        written, parameter gradients added to; those that are None are skipped.  ws: needed for parameter gradients and for
+        the gradient of a gate with gate_rows > 1."""
+        d, M = self._desc(x, y, gate, (w_post, b_post, w_pre, b_pre))
+        _need(d_out is not None or d_h is not None, "neither d_out nor d_h")
+        for name, t, of in (("dx", dx, x), ("dy", dy, y), ("dgate", dgate, gate)):
+            _need(t is None or of is not None, "%s without %s" % (name, name[1:]))
+        if d_out is not None:
+            d.d_out, d.lddo = self._act("d_out", d_out, M)
+        if d_h is not None:
+            d.d_h, d.lddh = self._act("d_h", d_h, M)
+        if dx is not None:
+            d.dx, d.lddx = self._act("dx", dx, M)
+        if dy is not None:
+            d.dy, d.lddy = self._act("dy", dy, M)
+        if dgate is not None:
+            d.dgate, d.lddgate = self._gate("dgate", dgate, M)
+        for name, t in zip(self.PARAMS, (dw_post, db_post, dw_pre, db_pre)):
+            if t is not None:
+                _need(getattr(self, name[2:]) != "none" and (name[2:] == "post" or d_h is not None), "d%s without its norm" % name)
+                setattr(d, "d" + name, _tensor("d" + name, t, (self.D,), torch.float32))
+        if ws is not None:
+            d.ws, d.ws_floats = _tensor("ws", ws, (ws.numel(),), torch.float32), ws.numel()
+        check(self._lib.hhrl_block_norm_backward(C.byref(d), _lib.stream_ptr()))

@@ -32,6 +32,15 @@ extern "C" {
 #define HHRL_ACT_RELU 1
 #define HHRL_ACT_TANH 2
 #define HHRL_ACT_SIGMOID 3
+#define HHRL_ACT_SILU 4 /* gates of hhrl_block_norm_* only */
+
+/* Element types of the sequence layers' activations (hhrl_gdr_*, hhrl_block_norm_*). */
+#define HHRL_F32 0
+#define HHRL_BF16 1
+
+#define HHRL_NORM_NONE 0
+#define HHRL_NORM_RMS 1   /* v / sqrt(mean(v^2) + eps) */
+#define HHRL_NORM_LAYER 2 /* (v - mean) / sqrt(var + eps), var the mean squared deviation */
 
 /* Library identification / diagnostics. */
 /* The ABI version this header describes; hhrl_version() returns the one the library was built with.  A binding checks
@@ -40,8 +49,9 @@ extern "C" {
  * 102: hhrl_mlp3_backward_group_adam (hhrl_adam_ride), hhrl_td3_target_mse_zeroed added.
  * 103: hhrl_mlp3_desc gained the mse_* fields; hhrl_mlp3_slab_floats is positive for every M (one more entry per row).
  * 104: hhrl_gcopy_desc.gather gained 2 (flat copy), 3 (standard normals) and 4 (scattered rows); row numbers may lie in
- *      pinned memory. */
-#define HHRL_ABI_VERSION 104
+ *      pinned memory.
+ * 105: hhrl_gdr_*, hhrl_block_norm_* added. */
+#define HHRL_ABI_VERSION 105
 int hhrl_version(void);
 const char* hhrl_last_error(void);
 
@@ -388,6 +398,89 @@ typedef struct {
 } hhrl_lstm_desc;
 int hhrl_lstm_forward_group(const hhrl_lstm_desc* descs, int n, int B, int T, int H, void* stream);
 int hhrl_lstm_backward_group(const hhrl_lstm_desc* descs, int n, int B, int T, int H, void* stream);
+
+/* --------------------------------------------------------- sequence layers
+ * No counterpart in the reference: recurrent layers whose training is parallel over the sequence, beside its BiLSTM
+ * (algorithm.py:141-156).  Activations are HHRL_F32 or HHRL_BF16 (`dtype`); decays, step sizes, states, parameters
+ * and parameter gradients are fp32.  Leading dimensions are longs, in elements.
+ *
+ * Gated delta rule: one matrix state S [K, V] per value head, moved by every token t:
+ *   S <- exp(g_t) S;   S <- S + beta_t k_t (v_t - S^T k_t)^T;   o_t = scale * S^T q_t.
+ * q, k: Hk heads of K elements per token, v, o: Hv heads of V elements (Hv a multiple of Hk; value head h reads key
+ * head h / (Hv/Hk)), heads contiguous, ld* from token to token; g (log decay, <= 0; -infinity forgets the state) and
+ * beta: Hv per token.  1 <= K <= HHRL_GDR_MAX_K, 1 <= V <= HHRL_GDR_MAX_V.
+ * Sequences: `starts` null: n_seq sequences of T = rows / n_seq tokens behind each other, of which the first lens[n]
+ * hold data (lens null: all).  `starts` (n_seq + 1 device ints): sequence n is rows starts[n] .. starts[n+1] - 1 of
+ * `rows` packed rows; it may be empty.  Numbers outside 0 .. rows (or 0 .. T) are clamped; starts has to ascend.
+ * Rows of no sequence are neither read nor written, in any operand; what they hold does not matter.
+ * s0 [n_seq, Hv, K, V]: states before the first token (null: zero); s1: receives the states behind the last (null: not
+ * wanted; may be s0).  A sequence without tokens hands its state on.
+ * Forward writes o.  Unless no_backward is set it leaves in ws what the backward call reads; ws
+ * (hhrl_gdr_workspace_floats, 16-byte aligned) must then stay untouched until that call, which takes the same inputs
+ * and writes dq, dk, dv (dtype), dg, dbeta and, where given, d_s0 (gradients with respect to q .. s0 of
+ * <d_o, o> + <d_s1, s1>; d_o and d_s1 may not both be null).
+ * The products run on bf16 matrix instructions with every fp32 operand as three bf16 terms: results carry fp32
+ * accuracy for either dtype, o and the input gradients are rounded once.  No atomics: the same bits on every run.
+ * A non-finite number in a token may spread to the 63 tokens before it (they share a chunk) and to all behind it. */
+#define HHRL_GDR_MAX_K 128
+#define HHRL_GDR_MAX_V 512
+typedef struct {
+  int dtype;
+  int n_seq; long rows;
+  int Hk, Hv, K, V;
+  float scale;
+  const int* starts; const int* lens;
+  const void *q, *k, *v; long ldq, ldk, ldv;
+  const float *g, *beta; long ldg, ldbeta;
+  void* o; long ldo;
+  const float* s0; float* s1;
+  int no_backward;
+  const void* d_o; long lddo;
+  const float* d_s1; float* d_s0;
+  void *dq, *dk, *dv; long lddq, lddk, lddv;
+  float *dg, *dbeta; long lddg, lddbeta;
+  float* ws; long ws_floats;
+} hhrl_gdr_desc;
+long hhrl_gdr_workspace_floats(int dtype, int n_seq, long rows, int packed, int Hk, int Hv, int K, int V, int no_backward);
+int hhrl_gdr_forward(const hhrl_gdr_desc* d, void* stream);
+int hhrl_gdr_backward(const hhrl_gdr_desc* d, void* stream);
+/* One token for each of B rows against a pool of states [n_slots, Hv, K, V] (an agent acting, a decoding step): row b
+ * moves state slots[b] (null: state b) and reads its output from it.  state_out: the pool that receives the moved
+ * states (may be state_in; slots that no row names are left alone).  A row whose slot is negative is idle: its output
+ * is zero and no state moves.  A slot >= n_slots, or one that an earlier row of the call names already, is an error
+ * that only the device sees: that row's output is NaN and no state moves for it.  No workspace. */
+int hhrl_gdr_step(int dtype, int B, int Hk, int Hv, int K, int V, float scale, const void* q, long ldq, const void* k, long ldk,
+                  const void* v, long ldv, const float* g, long ldg, const float* beta, long ldbeta, void* o, long ldo,
+                  const float* state_in, float* state_out, int n_slots, const int* slots, void* stream);
+
+/* Norms before and after a block with its gate and residual scale, one pass over the rows:
+ *   r = alpha*x + scale * a(gate) * post(y);    h = pre(r)
+ * M tokens of H groups of D elements (ld* from token to token, groups contiguous), each group normalised by itself:
+ * H = 1 between two blocks, H = heads behind the gated delta rule.  x null: no residual stream (0); y null: only the
+ * norm in front of a block; pre = HHRL_NORM_NONE: h, if wanted, is r.  post(y) = norm(y) * w_post + b_post, pre alike;
+ * w null: 1, b null: 0 (D floats each, shared by the groups).  a: HHRL_ACT_NONE, _SIGMOID, _SILU; gate null: 1.
+ * gate_rows = 1: one gate element per element (dtype).  gate_rows > 1 (H = 1): tokens m of one m / gate_rows share an
+ * fp32 gate row (modulation of a sequence; gate_rows >= M: one learned gate per channel).
+ * out (r) and h are rounded from the same fp32 row; either may be null; both may be x or y.
+ * Backward forms everything again from the inputs (no saved statistics).  d_out, d_h: gradients of r and h, either may
+ * be null.  dx, dy, dgate are written, dw_*, db_* ADDED to; any may be null.  Parameter gradients and a shared gate's
+ * need ws (hhrl_block_norm_workspace_floats, 16-byte aligned); sums are made in a fixed order.  D <= 8192. */
+typedef struct {
+  int dtype;
+  long M; int H, D;
+  int post, pre, gate_act; long gate_rows;
+  float alpha, scale, eps;
+  const void *x, *y, *gate; long ldx, ldy, ldgate;
+  const float *w_post, *b_post, *w_pre, *b_pre;
+  void *out, *h; long ldo, ldh;
+  const void *d_out, *d_h; long lddo, lddh;
+  void *dx, *dy, *dgate; long lddx, lddy, lddgate;
+  float *dw_post, *db_post, *dw_pre, *db_pre;
+  float* ws; long ws_floats;
+} hhrl_block_norm_desc;
+long hhrl_block_norm_workspace_floats(long M, int H, int D, long gate_rows);
+int hhrl_block_norm_forward(const hhrl_block_norm_desc* d, void* stream);
+int hhrl_block_norm_backward(const hhrl_block_norm_desc* d, void* stream);
 
 /* --------------------------------------------------------------- optimiser
  * torch.optim.Adam.step with default betas/eps on one flat buffer
