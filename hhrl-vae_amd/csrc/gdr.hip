@@ -37,9 +37,8 @@ using sb::bf16x8;
 using sb::f32x4;
 
 constexpr int kC = 64;             // tokens per chunk
-constexpr int kVt = 32;            // state columns per workgroup of a scan
 constexpr int kLdT = kC + 8;       // row stride of an LDS image that runs along the tokens (16 rows: 16 distinct bank groups)
-constexpr int kLdM = kC + 4;       // row stride of the fp32 images of the triangular solve
+constexpr int kLdM = kC + 4;       // row stride of an fp32 image
 constexpr float kGMin = -1e4f;     // log decays are clamped here: exp() of it is 0, and infinities would leave NaN differences
 
 struct GdrArgs {
@@ -64,9 +63,10 @@ struct GdrArgs {
   float *dg, *dbeta;
   long lddg, lddbeta;
   int pack, train, vp, nvt;
-  // ws, per chunk and key head: k, q [terms][64][Kp] (pack), their transposes [terms][Kp][64];
-  //     per chunk and value head: M, P and their transposes [terms][64][64], five rows of 64 floats, and for the
-  //     backward pass W, Y [64][vp] and S, dS [Kp][vp], fp32
+  // ws, per chunk and key head: k, q [64][terms][Kp] (pack), their transposes [Kp][terms][64];
+  //     per chunk and value head: M, P and their transposes [64][terms][64], five rows of 64 floats, and for the
+  //     backward pass W, Y [64][vp] and S, dS [Kp][vp], fp32.  The terms of a row lie side by side, so that a lane's
+  //     fragments are at constant offsets from one address.
   __bf16 *kpk, *qpk, *kt, *qt, *m, *p, *mt, *pt;
   float *vec, *w, *y, *s, *ds;
 };
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         *reinterpret_cast<bf16x8*>(dst + (p * kC + i) * LDK + c) = t[p];
-        if (a.pack) *reinterpret_cast<bf16x8*>(pk + ((long)p * kC + i) * Kp + c) = t[p];
+        if (a.pack) *reinterpret_cast<bf16x8*>(pk + ((long)i * NP + p) * Kp + c) = t[p];
       }
     }
   }
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
       bf16x8 t;
 #pragma unroll
       for (int e = 0; e < 8; ++e) t[e] = src[(p * kC + i0 + e) * LDK + k];
-      *reinterpret_cast<bf16x8*>(dst + ((long)p * Kp + k) * kC + i0) = t;
+      *reinterpret_cast<bf16x8*>(dst + ((long)k * NP + p) * kC + i0) = t;
     }
   }
   f32x4 kk[4], qk[4];
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
     const int row = tid >> 2, c0 = (tid & 3) * 16;
     for (int what = 0; what < (a.train ? 4 : 2); ++what) {
       const float* const src = what & 1 ? pm : mm;
-      __bf16* const dst = (what == 0 ? a.m : what == 1 ? a.p : what == 2 ? a.mt : a.pt) + vs * 3 * kC * kC + row * kC + c0;
+      __bf16* const dst = (what == 0 ? a.m : what == 1 ? a.p : what == 2 ? a.mt : a.pt) + (vs * kC + row) * 3 * kC + c0;
       const int si = what < 2 ? kLdM : 1, sj = what < 2 ? 1 : kLdM;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
         bf16x8 t[3];
         sb::split8<3>(x, t);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dst + p * kC * kC + 8 * h) = t[p];
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dst + p * kC + 8 * h) = t[p];
       }
     }
   }
@@ -302,9 +302,9 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
 // --------------------------------------------------------------------------------------------------------- scans
 // Workgroup -> (sequence, value head, column tile).  Workgroups go to the eight XCDs in turn: the column tiles of one
 // head read the same k, q, M and P, so they are dealt to one XCD (one L2), eight workgroups apart.
-__device__ __forceinline__ bool scan_tile(const GdrArgs& a, int& n, int& hv, int& v0) {
+__device__ __forceinline__ bool scan_tile(const GdrArgs& a, int vt, int& n, int& hv, int& v0) {
   const int xcd = blockIdx.x & 7, u = blockIdx.x >> 3;
-  v0 = (u % a.nvt) * kVt;
+  v0 = (u % a.nvt) * vt;
   const long pair = (long)(u / a.nvt) * 8 + xcd;
   if (pair >= (long)a.n_seq * a.Hv) return false;
   n = (int)(pair / a.Hv);
@@ -312,351 +312,566 @@ __device__ __forceinline__ bool scan_tile(const GdrArgs& a, int& n, int& hv, int
   return true;
 }
 
-template <int NP, int KB2>
+// LDS of a scan, in bytes: images of bf16 terms run along K (S) or along the tokens (X), fp32 images along the tokens (F);
+// a row per state column
+template <int NP, int KB2, int NT>
 struct ScanLds {
-  static constexpr int Kp = 64 * KB2, LDS_S = Kp + 8;
-  static constexpr int S = 3 * kVt * LDS_S, X = 3 * kVt * kLdT;
-  static constexpr int bytes = 2 * (S + 3 * X + (NP == 3 ? X : kVt * kLdT));      // the last: dO as it is (backward)
+  static constexpr int Kp = 64 * KB2, VT = 16 * NT, LDS_S = Kp + 8;
+  static constexpr int S = 3 * VT * LDS_S, X = 3 * VT * kLdT, F = VT * kLdM;     // elements
+  static constexpr int fwd_bytes = 2 * (S + 2 * X) + 4 * F;
+  static constexpr int bwd_bytes = 2 * (S + 3 * X + NP * VT * kLdT) + 8 * F;
 };
 
-// A-operand rows of k or q: token 16*wave + lr of a chunk, from the packed terms or from the caller's rows
+// Operand rows of k or q, token 16*w + lr of a chunk, from the packed terms or from the caller's rows.  Requests have
+// no conditions (a conditional one is waited for where its branch joins): a row behind the sequence reads the last one
+// instead, and the results it reaches are masked.
 template <int NP, int KB>
-__device__ __forceinline__ void load_rows(bf16x8 (&f)[KB][NP], const GdrArgs& a, const void* raw, long ld, const __bf16* packed,
-                                          long hs, int hk, long row, bool in, int i, int lg) {
-  constexpr int Kp = 32 * KB;
-  if (NP == 1 && !a.pack) {
-    const __bf16* const p = static_cast<const __bf16*>(raw) + row * ld + (long)hk * Kp + 8 * lg;
+struct RowPtr {
+  static constexpr int Kp = 32 * KB;
+  const __bf16* p;
+  long step, back;
+  int over;                                    // this row of the first chunk less the sequence's last row
+  __device__ __forceinline__ RowPtr(const GdrArgs& a, const void* raw, long ld, const __bf16* packed, long slot0, int hk, long start, int len,
+                                    int i, int lg) {
+    if (NP == 1 && !a.pack) {
+      p = static_cast<const __bf16*>(raw) + (start + i) * ld + (long)hk * Kp + 8 * lg;
+      step = kC * ld;
+      back = ld;
+    } else {
+      p = packed + ((slot0 * a.Hk + hk) * kC + i) * NP * Kp + 8 * lg;
+      step = (long)a.Hk * NP * kC * Kp;
+      back = 0;
+    }
+    over = i - (len - 1);
+  }
+  __device__ __forceinline__ void load(bf16x8 (&f)[KB][NP], int c) const {
+    const __bf16* const r = p + c * step - max(0, c * kC + over) * back;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      if (in) {
-        f[kb][0] = *reinterpret_cast<const bf16x8*>(p + 32 * kb);
-      } else {
+    for (int kb = 0; kb < KB; ++kb) sb::load_frag<NP>(f[kb], r + 32 * kb, Kp);
+  }
+};
+// Elements of v or dO in the layout of a result (rows ib + e, columns v0 + 16*t + lr), requested the same way and kept
+// as they come; get() is 0 outside the sequence and the head
+template <typename T, int NT>
+struct ColPtr {
+  const T* p[NT];
+  long ld;
+  int ib, len;
+  bool in[NT];
+  unsigned x[NT][4];
+  __device__ __forceinline__ ColPtr(const void* src, long ld_, long start, int len_, int hv, int V, int v0, int lr, int ib_) : ld(ld_), ib(ib_), len(len_) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[kb][0][e] = (__bf16)0.f;
+    for (int t = 0; t < NT; ++t) {
+      const int v = v0 + 16 * t + lr;
+      in[t] = v < V;
+      p[t] = static_cast<const T*>(src) + start * ld + (long)hv * V + (in[t] ? v : V - 1);
+    }
+  }
+  __device__ __forceinline__ void load(int c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const long off = (long)min(c * kC + ib + e, len - 1) * ld;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (sizeof(T) == 2) x[t][e] = *reinterpret_cast<const unsigned short*>(p[t] + off);
+        else x[t][e] = *reinterpret_cast<const unsigned*>(p[t] + off);
       }
     }
-  } else {
-    const __bf16* const p = packed + (hs * NP * kC + i) * Kp + 8 * lg;
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) sb::load_frag<NP>(f[kb], p + 32 * kb, (long)kC * Kp);
   }
+  __device__ __forceinline__ f32x4 get(int t, int valid) const {
+    f32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = in[t] && ib + e < valid ? __uint_as_float(sizeof(T) == 2 ? x[t][e] << 16 : x[t][e]) : 0.f;
+    return r;
+  }
+};
+__device__ __forceinline__ f32x4 rows_below(const f32x4& x, int ib, int valid) {
+  f32x4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = ib + e < valid ? x[e] : 0.f;
+  return r;
+}
+// a result tile of o or dv into the caller's rows
+template <typename T, int NT>
+__device__ __forceinline__ void store_cols(void* dst, long ld, long row0, int valid, int hv, int V, int v0, int ib, int lr, const f32x4 (&x)[NT]) {
+  T* const p = static_cast<T*>(dst) + (row0 + ib) * ld + (long)hv * V + v0 + lr;
+  if (valid == kC && v0 + 16 * NT <= V) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) p[e * ld + 16 * t] = (T)x[t][e];
+    return;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (ib + e < valid && v0 + 16 * t + lr < V) p[e * ld + 16 * t] = (T)x[t][e];
+}
+// the state tile of a scan's chain wave w: rows 16*(KB2*w + t) + 4*lg + e, columns v0 + 16*u + lr
+template <int KB2, int NT>
+__device__ __forceinline__ void load_state(f32x4 (&S)[KB2][NT], const float* s, const GdrArgs& a, long nh, int w, int v0, int lr, int lg) {
+#pragma unroll
+  for (int t = 0; t < KB2; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = 16 * (KB2 * w + t) + 4 * lg + e, v = v0 + 16 * u + lr;
+        S[t][u][e] = s && k < a.K && v < a.V ? s[(nh * a.K + k) * a.V + v] : 0.f;
+      }
+}
+template <int KB2, int NT>
+__device__ __forceinline__ void store_state(const f32x4 (&S)[KB2][NT], float* s, const GdrArgs& a, long nh, int w, int v0, int lr, int lg) {
+#pragma unroll
+  for (int t = 0; t < KB2; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = 16 * (KB2 * w + t) + 4 * lg + e, v = v0 + 16 * u + lr;
+        if (k < a.K && v < a.V) s[(nh * a.K + k) * a.V + v] = S[t][u][e];
+      }
 }
 
-template <typename T, int NP, int KB2>
-__global__ __launch_bounds__(256, 2) void gdr_scan_fwd_kernel(GdrArgs a) {
-  using L = ScanLds<NP, KB2>;
-  constexpr int Kp = L::Kp, KB = Kp / 32, LDS_S = L::LDS_S;
+// Per-token factors of a chunk, rows ib .. ib + 3
+struct ScanVec {
+  f32x4 gam, tail, beta;
+  float last;
+  __device__ __forceinline__ void load(const float* vec, int ib) {
+    gam = *reinterpret_cast<const f32x4*>(vec + kGam * kC + ib);
+    tail = *reinterpret_cast<const f32x4*>(vec + kTail * kC + ib);
+    beta = *reinterpret_cast<const f32x4*>(vec + kBeta * kC + ib);
+    last = vec[kGam * kC + kC - 1];
+  }
+};
+// the two 32-wide halves of a row of M, P or a transpose; `low` / `high`: whether this wave's rows reach them
+template <int N>
+__device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* row, bool low, bool high) {
+  if (low) sb::load_frag<N>(f[0], row, kC);
+  if (high) sb::load_frag<N>(f[1], row + 32, kC);
+}
+
+// A scan is bound by its chain: state -> K S -> W -> state, chunk after chunk, and inside it by the instructions its waves
+// issue (splitting results into terms, addressing; the matrix products are a third).  So four waves of the workgroup do
+// nothing but the chain, and four others what hangs on it: the output o, one chunk behind (forward), or what only depends
+// on dO, one chunk ahead, and the stores of Y and dV (backward).  Everything a chunk needs from memory is requested while
+// the chunk in front of it is worked on, behind the last use of its registers.
+template <typename T, int NP, int KB2, int NT>
+__global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
+  using L = ScanLds<NP, KB2, NT>;
+  constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT, LDS_S = L::LDS_S;
+  constexpr int NO = NP == 1 ? 2 : 3;                      // terms behind o: a bf16 o takes 2^-17, an fp32 one all three
   extern __shared__ __align__(16) char smem[];
-  __bf16* const sl = reinterpret_cast<__bf16*>(smem);      // [3][32][LDS_S] S, a row per column
-  __bf16* const xl = sl + L::S;                            // [3][32][kLdT]  beta (V - gam K S)
-  __bf16* const wl = xl + L::X;                            // W
-  __bf16* const ul = wl + L::X;                            // exp(G_C - G) W
+  __bf16* const sl = reinterpret_cast<__bf16*>(smem);      // [3][VT][LDS_S] S
+  __bf16* const xl = sl + L::S;                            // [3][VT][kLdT]  beta (V - gam K S)
+  __bf16* const ul = xl + L::X;                            // [3][VT][kLdT]  exp(G_C - G) W
+  float* const wl = reinterpret_cast<float*>(ul + L::X);   // [VT][kLdM]     W
   int n, hv, v0;
-  if (!scan_tile(a, n, hv, v0)) return;
+  if (!scan_tile(a, VT, n, hv, v0)) return;
   const int hk = hv / a.rep;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, w = (tid >> 6) & 3, lr = lane & 15, lg = lane >> 4;
   long start, slot0;
   int len;
   seq_range(a, n, start, len, slot0);
   const int nc = (len + kC - 1) / kC;
-  const int ib = 16 * wave + 4 * lg;                       // first of the four tokens of a result register group
-  const int nkb = wave < 2 ? 1 : 2;                        // M and P are lower triangular: rows < 32 read 32 columns
+  const int ib = 16 * w + 4 * lg, ia = 16 * w + lr;        // first of four result rows; operand row
+  const bool high = w >= 2;                                // M and P are lower triangular: rows < 32 read 32 columns
+  const long nh = (long)n * a.Hv + hv;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
-  f32x4 S[KB2][2];                                         // rows 16*(KB2*wave + t) + 4*lg + e, columns v0 + 16*c + lr
+  if (tid < 256) {                                         // ---- the chain
+    f32x4 S[KB2][NT];
+    load_state<KB2, NT>(S, a.s0, a, nh, w, v0, lr, lg);
+    if (nc > 0) {
+      bf16x8 kf[KB][NP], mf[2][3], ktf[KB2][2][NP];
+      const RowPtr<NP, KB> kp(a, a.k, a.ldk, a.kpk, slot0, hk, start, len, ia, lg);
+      ColPtr<T, NT> vp(a.v, a.ldv, start, len, hv, a.V, v0, lr, ib);
+      ScanVec vn;
+      const float* vecp = a.vec + (slot0 * a.Hv + hv) * kVecs * kC;
+      const __bf16* mp = a.m + ((slot0 * a.Hv + hv) * kC + ia) * 3 * kC + 8 * lg;
+      const __bf16* ktp = a.kt + ((slot0 * a.Hk + hk) * Kp + 16 * KB2 * w + lr) * NP * kC + 8 * lg;
+      auto load_kt = [&]() {
 #pragma unroll
-  for (int t = 0; t < KB2; ++t)
+        for (int t = 0; t < KB2; ++t)
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+          for (int kb = 0; kb < 2; ++kb) sb::load_frag<NP>(ktf[t][kb], ktp + 16 * t * NP * kC + 32 * kb, kC);
+      };
+      kp.load(kf, 0);
+      vp.load(0);
+      vn.load(vecp, ib);
+      load_tri<3>(mf, mp, true, high);
+      load_kt();
+      for (int c = 0; c < nc; ++c) {
+        const int valid = min(kC, len - c * kC), next = min(c + 1, nc - 1);
+        const long adv = next - c;                         // 0 behind the last chunk: its operands are read again, to no use
+        vecp += adv * a.Hv * kVecs * kC;
+        mp += adv * a.Hv * 3 * kC * kC;
+        ktp += adv * a.Hk * NP * Kp * kC;
+        const long vs = (slot0 + c) * a.Hv + hv;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = 16 * (KB2 * wave + t) + 4 * lg + e, v = v0 + 16 * c + lr;
-        S[t][c][e] = a.s0 && k < a.K && v < a.V ? a.s0[(((long)n * a.Hv + hv) * a.K + k) * a.V + v] : 0.f;
-      }
-  for (int c = 0; c < nc; ++c) {
-    const long slot = slot0 + c, hs = slot * a.Hk + hk, vs = slot * a.Hv + hv;
-    const long row0 = start + (long)c * kC;
-    const int valid = min(kC, len - c * kC);
-    const float* const vec = a.vec + vs * kVecs * kC;
-    const f32x4 gam = *reinterpret_cast<const f32x4*>(vec + kGam * kC + ib);
-    const f32x4 tail = *reinterpret_cast<const f32x4*>(vec + kTail * kC + ib);
-    const f32x4 beta = *reinterpret_cast<const f32x4*>(vec + kBeta * kC + ib);
-    const float last = vec[kGam * kC + kC - 1];
-    bf16x8 kf[KB][NP], qf[KB][NP];
-    const int ia = 16 * wave + lr;
-    load_rows<NP, KB>(kf, a, a.k, a.ldk, a.kpk, hs, hk, row0 + ia, ia < valid, ia, lg);
-    load_rows<NP, KB>(qf, a, a.q, a.ldq, a.qpk, hs, hk, row0 + ia, ia < valid, ia, lg);
-    f32x4 vv[2];
+        for (int t = 0; t < KB2; ++t)
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+          for (int u = 0; u < NT; ++u)
+            sb::split_store4<3>(sl + (16 * u + lr) * LDS_S + 16 * (KB2 * w + t) + 4 * lg, VT * LDS_S, S[t][u]);
+        lds_barrier();
+        f32x4 ks[NT];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int v = v0 + 16 * t + lr;
-        vv[t][e] = ib + e < valid && v < a.V ? (float)static_cast<const T*>(a.v)[(row0 + ib + e) * a.ldv + (long)hv * a.V + v] : 0.f;
-      }
+        for (int t = 0; t < NT; ++t) ks[t] = zero;
 #pragma unroll
-    for (int t = 0; t < KB2; ++t)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int k = 16 * (KB2 * wave + t) + 4 * lg;
-        sb::split_store4<3>(sl + (16 * u + lr) * LDS_S + k, kVt * LDS_S, S[t][u]);
+          for (int t = 0; t < NT; ++t) {
+            bf16x8 b[3];
+            sb::load_frag<3>(b, sl + (16 * t + lr) * LDS_S + 32 * kb + 8 * lg, VT * LDS_S);
+            sb::mma<NP, 3>(ks[t], kf[kb], b);
+          }
+        kp.load(kf, next);
+        const ScanVec vc = vn;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          sb::split_store4<3>(xl + (16 * t + lr) * kLdT + ib, VT * kLdT, rows_below(vc.beta * (vp.get(t, valid) - vc.gam * ks[t]), ib, valid));
+        vp.load(next);
+        vn.load(vecp, ib);
         if (a.train) {
+          float* const sp = a.s + (vs * Kp + 16 * KB2 * w + 4 * lg) * a.vp + v0 + lr;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) a.s[(vs * Kp + k + e) * a.vp + v0 + 16 * u + lr] = S[t][u][e];
+          for (int t = 0; t < KB2; ++t)
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sp[(16 * t + e) * a.vp + 16 * u] = S[t][u][e];
         }
-      }
-    lds_barrier();
-    f32x4 ks[2], qs[2];
-    ks[0] = ks[1] = qs[0] = qs[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        lds_barrier();
+        f32x4 wt[NT];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+        for (int t = 0; t < NT; ++t) wt[t] = zero;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        bf16x8 b[3];
-        sb::load_frag<3>(b, sl + (16 * t + lr) * LDS_S + 32 * kb + 8 * lg, kVt * LDS_S);
-        sb::mma<NP, 3>(ks[t], kf[kb], b);
-        sb::mma<NP, 3>(qs[t], qf[kb], b);
-      }
+        for (int kb = 0; kb < 2; ++kb)
+          if (kb == 0 || high)
 #pragma unroll
-    for (int t = 0; t < 2; ++t) sb::split_store4<3>(xl + (16 * t + lr) * kLdT + ib, kVt * kLdT, beta * (vv[t] - gam * ks[t]));
-    lds_barrier();
-    f32x4 w[2];
-    w[0] = w[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const __bf16* const mrow = a.m + vs * 3 * kC * kC + ia * kC + 8 * lg;
-    for (int kb = 0; kb < nkb; ++kb) {
-      bf16x8 mf[3];
-      sb::load_frag<3>(mf, mrow + 32 * kb, kC * kC);
+            for (int t = 0; t < NT; ++t) {
+              bf16x8 b[3];
+              sb::load_frag<3>(b, xl + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+              sb::mma<3, 3>(wt[t], mf[kb], b);
+            }
+        load_tri<3>(mf, mp, true, high);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        bf16x8 b[3];
-        sb::load_frag<3>(b, xl + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, kVt * kLdT);
-        sb::mma<3, 3>(w[t], mf, b);
+        for (int t = 0; t < NT; ++t) {
+          sb::split_store4<3>(ul + (16 * t + lr) * kLdT + ib, VT * kLdT, vc.tail * wt[t]);
+          *reinterpret_cast<f32x4*>(wl + (16 * t + lr) * kLdM + ib) = wt[t];
+        }
+        lds_barrier();
+#pragma unroll
+        for (int t = 0; t < KB2; ++t)
+#pragma unroll
+          for (int u = 0; u < NT; ++u) S[t][u] *= vc.last;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int u = 0; u < NT; ++u) {
+            bf16x8 b[3];
+            sb::load_frag<3>(b, ul + (16 * u + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+#pragma unroll
+            for (int t = 0; t < KB2; ++t) sb::mma<NP, 3>(S[t][u], ktf[t][kb], b);
+          }
+        load_kt();
       }
     }
+    if (a.s1) store_state<KB2, NT>(S, a.s1, a, nh, w, v0, lr, lg);
+  } else if (nc > 0) {                                     // ---- the output, between the chain's barriers
+    bf16x8 qf[KB][NP], pf[2][NO];
+    f32x4 qs[NT], gam;
+    const RowPtr<NP, KB> qp(a, a.q, a.ldq, a.qpk, slot0, hk, start, len, ia, lg);
+    const __bf16* pp = a.p + ((slot0 * a.Hv + hv) * kC + ia) * 3 * kC + 8 * lg;
+    const float* gp = a.vec + (slot0 * a.Hv + hv) * kVecs * kC + kGam * kC + ib;
+    // o of chunk c from qs = gam (Q S) and W, which the chain has left in wl
+    auto finish = [&](int c) {
+      const long vs = (slot0 + c) * a.Hv + hv;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      sb::split_store4<3>(wl + (16 * t + lr) * kLdT + ib, kVt * kLdT, w[t]);
-      sb::split_store4<3>(ul + (16 * t + lr) * kLdT + ib, kVt * kLdT, tail * w[t]);
+      for (int kb = 0; kb < 2; ++kb)
+        if (kb == 0 || high)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            float x[8];
+            const float* const src = wl + (16 * t + lr) * kLdM + 32 * kb + 8 * lg;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const f32x4 y = *reinterpret_cast<const f32x4*>(src + 4 * h);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[4 * h + e] = y[e];
+            }
+            bf16x8 b[NO];
+            sb::split8<NO>(x, b);
+            sb::mma<NO, NO>(qs[t], pf[kb], b);
+          }
       if (a.train) {
+        float* const wp = a.w + (vs * kC + ib) * a.vp + v0 + lr;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a.w[(vs * kC + ib + e) * a.vp + v0 + 16 * t + lr] = w[t][e];
-      }
-    }
-    lds_barrier();
-    const __bf16* const ktr = a.kt + hs * NP * Kp * kC + 8 * lg;
+        for (int t = 0; t < NT; ++t) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(wl + (16 * t + lr) * kLdM + ib);
 #pragma unroll
-    for (int t = 0; t < KB2; ++t) {
-      S[t][0] *= last;
-      S[t][1] *= last;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        bf16x8 f[NP];
-        sb::load_frag<NP>(f, ktr + (16 * (KB2 * wave + t) + lr) * kC + 32 * kb, Kp * kC);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          bf16x8 b[3];
-          sb::load_frag<3>(b, ul + (16 * u + lr) * kLdT + 32 * kb + 8 * lg, kVt * kLdT);
-          sb::mma<NP, 3>(S[t][u], f, b);
+          for (int e = 0; e < 4; ++e) wp[e * a.vp + 16 * t] = y[e];
         }
       }
-    }
-    const __bf16* const prow = a.p + vs * 3 * kC * kC + ia * kC + 8 * lg;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) qs[t] *= gam;
-    for (int kb = 0; kb < nkb; ++kb) {
-      bf16x8 pf[3];
-      sb::load_frag<3>(pf, prow + 32 * kb, kC * kC);
+      for (int t = 0; t < NT; ++t) qs[t] *= a.scale;
+      store_cols<T, NT>(a.o, a.ldo, start + (long)c * kC, min(kC, len - c * kC), hv, a.V, v0, ib, lr, qs);
+    };
+    qp.load(qf, 0);
+    for (int c = 0; c < nc; ++c) {
+      if (c > 0) finish(c - 1);
+      load_tri<NO>(pf, pp, true, high);
+      gam = *reinterpret_cast<const f32x4*>(gp);
+      pp += (long)a.Hv * 3 * kC * kC;
+      gp += (long)a.Hv * kVecs * kC;
+      lds_barrier();
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        bf16x8 b[3];
-        sb::load_frag<3>(b, wl + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, kVt * kLdT);
-        sb::mma<3, 3>(qs[t], pf, b);
-      }
-    }
+      for (int t = 0; t < NT; ++t) qs[t] = zero;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int v = v0 + 16 * t + lr;
-        if (ib + e < valid && v < a.V) static_cast<T*>(a.o)[(row0 + ib + e) * a.ldo + (long)hv * a.V + v] = (T)(a.scale * qs[t][e]);
-      }
-  }
-  if (a.s1) {
-#pragma unroll
-    for (int t = 0; t < KB2; ++t)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = 16 * (KB2 * wave + t) + 4 * lg + e, v = v0 + 16 * u + lr;
-          if (k < a.K && v < a.V) a.s1[(((long)n * a.Hv + hv) * a.K + k) * a.V + v] = S[t][u][e];
+        for (int t = 0; t < NT; ++t) {
+          bf16x8 b[NO];
+          sb::load_frag<NO>(b, sl + (16 * t + lr) * LDS_S + 32 * kb + 8 * lg, VT * LDS_S);
+          sb::mma<NP, NO>(qs[t], qf[kb], b);
         }
+      qp.load(qf, min(c + 1, nc - 1));
+#pragma unroll
+      for (int t = 0; t < NT; ++t) qs[t] *= gam;
+      lds_barrier();
+      lds_barrier();
+    }
+    finish(nc - 1);
   }
 }
 
-template <typename T, int NP, int KB2>
-__global__ __launch_bounds__(256, 2) void gdr_scan_bwd_kernel(GdrArgs a) {
-  using L = ScanLds<NP, KB2>;
-  constexpr int Kp = L::Kp, KB = Kp / 32, LDS_S = L::LDS_S;
+template <typename T, int NP, int KB2, int NT>
+__global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
+  using L = ScanLds<NP, KB2, NT>;
+  constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT, LDS_S = L::LDS_S;
   extern __shared__ __align__(16) char smem[];
-  __bf16* const dl = reinterpret_cast<__bf16*>(smem);      // [3][32][LDS_S] dS'
-  __bf16* const gl = dl + L::S;                            // [3][32][kLdT]  scale gam dO
-  __bf16* const zl = gl + L::X;                            // Z
-  __bf16* const yl = zl + L::X;                            // -gam beta Y
-  __bf16* const ol = yl + L::X;                            // [NP][32][kLdT] dO
+  __bf16* const dl = reinterpret_cast<__bf16*>(smem);      // [3][VT][LDS_S] dS'
+  __bf16* const gl = dl + L::S;                            // [3][VT][kLdT]  scale gam dO
+  __bf16* const zl = gl + L::X;                            // [3][VT][kLdT]  Z
+  __bf16* const yl = zl + L::X;                            // [3][VT][kLdT]  -gam beta Y
+  __bf16* const ol = yl + L::X;                            // [NP][VT][kLdT] dO
+  float* const zp = reinterpret_cast<float*>(ol + NP * VT * kLdT);   // [VT][kLdM] scale P^T dO
+  float* const yf = zp + L::F;                             // [VT][kLdM] Y
   int n, hv, v0;
-  if (!scan_tile(a, n, hv, v0)) return;
+  if (!scan_tile(a, VT, n, hv, v0)) return;
   const int hk = hv / a.rep;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, w = (tid >> 6) & 3, lr = lane & 15, lg = lane >> 4;
   long start, slot0;
   int len;
   seq_range(a, n, start, len, slot0);
   const int nc = (len + kC - 1) / kC;
-  const int ib = 16 * wave + 4 * lg, ia = 16 * wave + lr;
-  const int kb0 = wave < 2 ? 0 : 1;                        // P^T and M^T are upper triangular
+  const int ib = 16 * w + 4 * lg, ia = 16 * w + lr;
+  const bool low = w < 2;                                  // P^T and M^T are upper triangular: rows >= 32 read the last 32 columns
+  const long nh = (long)n * a.Hv + hv;
+  const long slot1 = slot0 + nc - 1;                       // the last chunk, where the walk begins
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
-  f32x4 dS[KB2][2];
+  // Barriers of a chunk: 1 (dl), 2 (zl), 3 (yl, yf; gl, zp by the others).  Two more in front of the walk.
+  if (tid < 256) {                                         // ---- the chain
+    f32x4 dS[KB2][NT];
+    load_state<KB2, NT>(dS, a.d_s1, a, nh, w, v0, lr, lg);
+    if (nc > 0) {
+      bf16x8 kf[KB][NP], mf[2][3], ktf[KB2][2][NP], qtf[KB2][2][NP];
+      const RowPtr<NP, KB> kp(a, a.k, a.ldk, a.kpk, slot0, hk, start, len, ia, lg);
+      ScanVec vn;
+      const float* vecp = a.vec + (slot1 * a.Hv + hv) * kVecs * kC;
+      const __bf16* mp = a.mt + ((slot1 * a.Hv + hv) * kC + ia) * 3 * kC + 8 * lg;
+      long tp = ((slot1 * a.Hk + hk) * Kp + 16 * KB2 * w + lr) * NP * kC + 8 * lg;
+      auto load_t = [&]() {
 #pragma unroll
-  for (int t = 0; t < KB2; ++t)
+        for (int t = 0; t < KB2; ++t)
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+          for (int kb = 0; kb < 2; ++kb) {
+            sb::load_frag<NP>(qtf[t][kb], a.qt + tp + 16 * t * NP * kC + 32 * kb, kC);
+            sb::load_frag<NP>(ktf[t][kb], a.kt + tp + 16 * t * NP * kC + 32 * kb, kC);
+          }
+      };
+      kp.load(kf, nc - 1);
+      vn.load(vecp, ib);
+      load_tri<3>(mf, mp, low, true);
+      load_t();
+      lds_barrier();
+      lds_barrier();
+      for (int c = nc - 1; c >= 0; --c) {
+        const int valid = min(kC, len - c * kC), next = max(c - 1, 0);
+        const long adv = c - next;
+        vecp -= adv * a.Hv * kVecs * kC;
+        mp -= adv * a.Hv * 3 * kC * kC;
+        tp -= adv * a.Hk * NP * Kp * kC;
+        const ScanVec vc = vn;
+        const long vs = (slot0 + c) * a.Hv + hv;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = 16 * (KB2 * wave + t) + 4 * lg + e, v = v0 + 16 * c + lr;
-        dS[t][c][e] = a.d_s1 && k < a.K && v < a.V ? a.d_s1[(((long)n * a.Hv + hv) * a.K + k) * a.V + v] : 0.f;
-      }
-  for (int c = nc - 1; c >= 0; --c) {
-    const long slot = slot0 + c, hs = slot * a.Hk + hk, vs = slot * a.Hv + hv;
-    const long row0 = start + (long)c * kC;
-    const int valid = min(kC, len - c * kC);
-    const float* const vec = a.vec + vs * kVecs * kC;
-    const f32x4 gam = *reinterpret_cast<const f32x4*>(vec + kGam * kC + ib);
-    const f32x4 tail = *reinterpret_cast<const f32x4*>(vec + kTail * kC + ib);
-    const f32x4 beta = *reinterpret_cast<const f32x4*>(vec + kBeta * kC + ib);
-    const float last = vec[kGam * kC + kC - 1];
-    bf16x8 kf[KB][NP];
-    load_rows<NP, KB>(kf, a, a.k, a.ldk, a.kpk, hs, hk, row0 + ia, ia < valid, ia, lg);
+        for (int t = 0; t < KB2; ++t)
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      f32x4 d;
+          for (int u = 0; u < NT; ++u)
+            sb::split_store4<3>(dl + (16 * u + lr) * LDS_S + 16 * (KB2 * w + t) + 4 * lg, VT * LDS_S, dS[t][u]);
+        lds_barrier();
+        f32x4 z[NT], y[NT];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int v = v0 + 16 * t + lr;
-        d[e] = a.d_o && ib + e < valid && v < a.V ? (float)static_cast<const T*>(a.d_o)[(row0 + ib + e) * a.lddo + (long)hv * a.V + v] : 0.f;
-      }
-      sb::split_store4<NP>(ol + (16 * t + lr) * kLdT + ib, kVt * kLdT, d);
-      sb::split_store4<3>(gl + (16 * t + lr) * kLdT + ib, kVt * kLdT, a.scale * gam * d);
-    }
+        for (int t = 0; t < NT; ++t) z[t] = y[t] = zero;
 #pragma unroll
-    for (int t = 0; t < KB2; ++t)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int k = 16 * (KB2 * wave + t) + 4 * lg;
-        sb::split_store4<3>(dl + (16 * u + lr) * LDS_S + k, kVt * LDS_S, dS[t][u]);
+          for (int t = 0; t < NT; ++t) {
+            bf16x8 b[3];
+            sb::load_frag<3>(b, dl + (16 * t + lr) * LDS_S + 32 * kb + 8 * lg, VT * LDS_S);
+            sb::mma<NP, 3>(z[t], kf[kb], b);
+          }
+        kp.load(kf, next);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a.ds[(vs * Kp + k + e) * a.vp + v0 + 16 * u + lr] = dS[t][u][e];
-      }
-    lds_barrier();
-    f32x4 z[2], y[2];
-    z[0] = z[1] = y[0] = y[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        bf16x8 b[3];
-        sb::load_frag<3>(b, dl + (16 * t + lr) * LDS_S + 32 * kb + 8 * lg, kVt * LDS_S);
-        sb::mma<NP, 3>(z[t], kf[kb], b);
-      }
-    const __bf16* const prow = a.pt + vs * 3 * kC * kC + ia * kC + 8 * lg;
-    for (int kb = kb0; kb < 2; ++kb) {
-      bf16x8 f[3];
-      sb::load_frag<3>(f, prow + 32 * kb, kC * kC);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        bf16x8 b[NP];
-        sb::load_frag<NP>(b, ol + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, kVt * kLdT);
-        sb::mma<3, NP>(y[t], f, b);
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) sb::split_store4<3>(zl + (16 * t + lr) * kLdT + ib, kVt * kLdT, a.scale * y[t] + tail * z[t]);
-    lds_barrier();
-    y[0] = y[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const __bf16* const mrow = a.mt + vs * 3 * kC * kC + ia * kC + 8 * lg;
-    for (int kb = kb0; kb < 2; ++kb) {
-      bf16x8 f[3];
-      sb::load_frag<3>(f, mrow + 32 * kb, kC * kC);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        bf16x8 b[3];
-        sb::load_frag<3>(b, zl + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, kVt * kLdT);
-        sb::mma<3, 3>(y[t], f, b);
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      sb::split_store4<3>(yl + (16 * t + lr) * kLdT + ib, kVt * kLdT, -gam * beta * y[t]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int v = v0 + 16 * t + lr;
-        a.y[(vs * kC + ib + e) * a.vp + v] = y[t][e];
-        if (ib + e < valid && v < a.V) static_cast<T*>(a.dv)[(row0 + ib + e) * a.lddv + (long)hv * a.V + v] = (T)(beta[e] * y[t][e]);
-      }
-    }
-    lds_barrier();
-    const __bf16* const ktr = a.kt + hs * NP * Kp * kC + 8 * lg;
-    const __bf16* const qtr = a.qt + hs * NP * Kp * kC + 8 * lg;
-#pragma unroll
-    for (int t = 0; t < KB2; ++t) {
-      dS[t][0] *= last;
-      dS[t][1] *= last;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        bf16x8 f[NP], h[NP];
-        const int off = (16 * (KB2 * wave + t) + lr) * kC + 32 * kb;
-        sb::load_frag<NP>(f, ktr + off, Kp * kC);
-        sb::load_frag<NP>(h, qtr + off, Kp * kC);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          bf16x8 b[3];
-          sb::load_frag<3>(b, gl + (16 * u + lr) * kLdT + 32 * kb + 8 * lg, kVt * kLdT);
-          sb::mma<NP, 3>(dS[t][u], h, b);
-          sb::load_frag<3>(b, yl + (16 * u + lr) * kLdT + 32 * kb + 8 * lg, kVt * kLdT);
-          sb::mma<NP, 3>(dS[t][u], f, b);
+        for (int t = 0; t < NT; ++t) {
+          const f32x4 p = *reinterpret_cast<const f32x4*>(zp + (16 * t + lr) * kLdM + ib);
+          sb::split_store4<3>(zl + (16 * t + lr) * kLdT + ib, VT * kLdT, rows_below(p + vc.tail * z[t], ib, valid));
         }
+        vn.load(vecp, ib);
+        float* const sp = a.ds + (vs * Kp + 16 * KB2 * w + 4 * lg) * a.vp + v0 + lr;
+#pragma unroll
+        for (int t = 0; t < KB2; ++t)
+#pragma unroll
+          for (int u = 0; u < NT; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sp[(16 * t + e) * a.vp + 16 * u] = dS[t][u][e];
+        lds_barrier();
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          if (kb == 1 || low)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              bf16x8 b[3];
+              sb::load_frag<3>(b, zl + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+              sb::mma<3, 3>(y[t], mf[kb], b);
+            }
+        load_tri<3>(mf, mp, low, true);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          sb::split_store4<3>(yl + (16 * t + lr) * kLdT + ib, VT * kLdT, -vc.gam * vc.beta * y[t]);
+          *reinterpret_cast<f32x4*>(yf + (16 * t + lr) * kLdM + ib) = y[t];
+        }
+        lds_barrier();
+#pragma unroll
+        for (int t = 0; t < KB2; ++t)
+#pragma unroll
+          for (int u = 0; u < NT; ++u) dS[t][u] *= vc.last;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int u = 0; u < NT; ++u) {
+            bf16x8 b[3], g[3];
+            sb::load_frag<3>(g, gl + (16 * u + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+            sb::load_frag<3>(b, yl + (16 * u + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+#pragma unroll
+            for (int t = 0; t < KB2; ++t) {
+              sb::mma<NP, 3>(dS[t][u], qtf[t][kb], g);
+              sb::mma<NP, 3>(dS[t][u], ktf[t][kb], b);
+            }
+          }
+        load_t();
       }
     }
-    lds_barrier();                                 // gl and yl have been read: the next chunk writes gl before its first barrier
-  }
-  if (a.d_s0) {
+    if (a.d_s0) store_state<KB2, NT>(dS, a.d_s0, a, nh, w, v0, lr, lg);
+  } else if (nc > 0) {                                     // ---- dO's share, ahead of the chain; Y and dV, behind it
+    bf16x8 pf[2][3];
+    const bool has_do = a.d_o != nullptr;
+    ColPtr<T, NT> dp(has_do ? a.d_o : a.v, has_do ? a.lddo : a.ldv, start, len, hv, a.V, v0, lr, ib);
+    const __bf16* const pt = a.pt + ((slot0 * a.Hv + hv) * kC + ia) * 3 * kC + 8 * lg;
+    const float* const vec = a.vec + (slot0 * a.Hv + hv) * kVecs * kC + ib;
+    const long pstep = (long)a.Hv * 3 * kC * kC, vstep = (long)a.Hv * kVecs * kC;
+    f32x4 d[NT], dn[NT];                                   // dO of the chunk at hand and of the next one
+    auto share = [&]() {                                   // zp of the chunk whose dO is in ol and whose P^T is in pf
+      f32x4 z[NT];
 #pragma unroll
-    for (int t = 0; t < KB2; ++t)
+      for (int t = 0; t < NT; ++t) z[t] = zero;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int kb = 0; kb < 2; ++kb)
+        if (kb == 1 || low)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = 16 * (KB2 * wave + t) + 4 * lg + e, v = v0 + 16 * u + lr;
-          if (k < a.K && v < a.V) a.d_s0[(((long)n * a.Hv + hv) * a.K + k) * a.V + v] = dS[t][u][e];
-        }
+          for (int t = 0; t < NT; ++t) {
+            bf16x8 b[NP];
+            sb::load_frag<NP>(b, ol + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+            sb::mma<3, NP>(z[t], pf[kb], b);
+          }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(zp + (16 * t + lr) * kLdM + ib) = a.scale * z[t];
+    };
+    dp.load(nc - 1);
+    load_tri<3>(pf, pt + (nc - 1) * pstep, low, true);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      dn[t] = dp.get(t, has_do ? len - (nc - 1) * kC : 0);
+      sb::split_store4<NP>(ol + (16 * t + lr) * kLdT + ib, VT * kLdT, dn[t]);
+    }
+    dp.load(max(nc - 2, 0));
+    lds_barrier();
+    share();
+    load_tri<3>(pf, pt + max(nc - 2, 0) * pstep, low, true);
+    lds_barrier();
+    for (int c = nc - 1; c >= 0; --c) {
+      const int next = max(c - 1, 0), next2 = max(c - 2, 0);
+      const f32x4 gam = *reinterpret_cast<const f32x4*>(vec + c * vstep + kGam * kC);
+      const f32x4 beta = *reinterpret_cast<const f32x4*>(vec + c * vstep + kBeta * kC);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) { d[t] = dn[t]; dn[t] = dp.get(t, has_do ? min(kC, len - next * kC) : 0); }
+      dp.load(next2);
+      lds_barrier();                                       // 1: the chain has read the previous chunk's gl
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        sb::split_store4<3>(gl + (16 * t + lr) * kLdT + ib, VT * kLdT, a.scale * gam * d[t]);
+        sb::split_store4<NP>(ol + (16 * t + lr) * kLdT + ib, VT * kLdT, dn[t]);
+      }
+      lds_barrier();                                       // 2: the chain has read zp
+      share();
+      load_tri<3>(pf, pt + next2 * pstep, low, true);
+      lds_barrier();                                       // 3
+      float* const yp = a.y + (((slot0 + c) * a.Hv + hv) * kC + ib) * a.vp + v0 + lr;
+      f32x4 y[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        y[t] = *reinterpret_cast<const f32x4*>(yf + (16 * t + lr) * kLdM + ib);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) yp[e * a.vp + 16 * t] = y[t][e];
+        y[t] *= beta;
+      }
+      store_cols<T, NT>(a.dv, a.lddv, start + (long)c * kC, min(kC, len - c * kC), hv, a.V, v0, ib, lr, y);
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------------------------ gradients
 // One workgroup per chunk and key head; the value heads of the key head one after the other, so that dq and dk are summed
-// in registers in a fixed order.  A wave holds 16 tokens against all of K; S, dS' and W pass through LDS 32 columns at a
-// time as bf16 terms.
+// in registers in a fixed order.  Eight waves: 16 tokens against half of K each.  S, dS', W, Y and dO pass through LDS 32
+// columns at a time as bf16 terms; the next 32 columns are on their way from memory meanwhile.
+template <int NP, int KB2>
+struct GradsLds {
+  static constexpr int Kp = 64 * KB2, LDV = 40;              // 32 columns + 8: 16 rows in 16 distinct bank groups
+  static constexpr int cols = 3 * LDV * (2 * Kp + 2 * kC) + NP * LDV * kC;       // elements: S, dS', W, Y, dO
+  static constexpr int tri = 4 * 3 * kC * kLdT;              // R, B and their transposes, over them afterwards
+  static constexpr int over = 2 * (cols > tri ? cols : tri);
+  static constexpr int bytes = over + (8 * kC + 8) * 4;
+};
 template <typename T, int NP, int KB2, bool GROUP>
-__global__ __launch_bounds__(256, 1) void gdr_grads_kernel(GdrArgs a) {
-  constexpr int Kp = 64 * KB2, KT = Kp / 16, LDV = 40;       // 32 columns + 8: 16 rows in 16 distinct bank groups
+__global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
+  using L = GradsLds<NP, KB2>;
+  constexpr int Kp = L::Kp, LDV = L::LDV, KT = Kp / 32;      // k tiles of a wave
   extern __shared__ __align__(16) char smem[];
   __bf16* const sl = reinterpret_cast<__bf16*>(smem);        // [3][Kp][LDV]
   __bf16* const dl = sl + 3 * Kp * LDV;                      // [3][Kp][LDV]
   __bf16* const wl = dl + 3 * Kp * LDV;                      // [3][64][LDV]
-  __bf16* const rl = reinterpret_cast<__bf16*>(smem);        // over them afterwards: R and B, then their transposes
-  __bf16* const bl = rl + 3 * kC * kLdT;                     // [3][64][kLdT]
-  constexpr int kOver = 2 * 3 * LDV * (2 * Kp + kC) > 2 * 2 * 3 * kC * kLdT ? 2 * 3 * LDV * (2 * Kp + kC) : 2 * 2 * 3 * kC * kLdT;
-  float* const rows = reinterpret_cast<float*>(smem + kOver);      // [4][64]: Y.v, dG without the state's share, dbeta's rest, k.(tail E3)
-  float* const red = rows + 4 * kC;                                // [4]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
+  __bf16* const yl = wl + 3 * kC * LDV;                      // [3][64][LDV]
+  __bf16* const ol = yl + 3 * kC * LDV;                      // [NP][64][LDV]
+  __bf16* const rl = reinterpret_cast<__bf16*>(smem);        // [3][64][kLdT] each
+  __bf16* const bl = rl + 3 * kC * kLdT;
+  __bf16* const rt = bl + 3 * kC * kLdT;
+  __bf16* const bt = rt + 3 * kC * kLdT;
+  float* const rows = reinterpret_cast<float*>(smem + L::over);    // [2 halves][3][64]: shares of dG, of dbeta, k.(tail E3)
+  float* const yv = rows + 6 * kC;                                 // [64] Y.v
+  float* const red = yv + kC;                                      // [8]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, w = wave >> 1, half = wave & 1, lr = lane & 15, lg = lane >> 4;
   const long slot = blockIdx.x;
   const int hk = blockIdx.y;
   long row0;
@@ -664,8 +879,12 @@ __global__ __launch_bounds__(256, 1) void gdr_grads_kernel(GdrArgs a) {
   slot_chunk(a, slot, row0, valid);
   if (valid == 0) return;
   const long hs = slot * a.Hk + hk;
-  const int ib = 16 * wave + 4 * lg, ia = 16 * wave + lr;
+  const int ib = 16 * w + 4 * lg, ia = 16 * w + lr, kt0 = 16 * KT * half;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  const bool has_do = a.d_o != nullptr;
+  // cooperative loads: 8 columns of a row per thread
+  const int gi = (tid & 255) >> 2, gc = (tid & 3) * 8;       // token and columns of W, dO (threads 0..255), Y, v (the others)
+  const long rowc = row0 + min(gi, valid - 1);
 
   f32x4 dqs[GROUP ? KT : 1], dks[GROUP ? KT : 1];
   if (GROUP) {
@@ -675,94 +894,102 @@ __global__ __launch_bounds__(256, 1) void gdr_grads_kernel(GdrArgs a) {
   for (int r = 0; r < a.rep; ++r) {
     const int hv = hk * a.rep + r;
     const long vs = slot * a.Hv + hv;
-    f32x4 e1[KT], e2[KT], e3[KT], dp[4], da[4];
+    f32x4 e1[KT], e2[KT], e3[KT], dp[2], da[2];
 #pragma unroll
     for (int t = 0; t < KT; ++t) e1[t] = e2[t] = e3[t] = zero;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) dp[t] = da[t] = zero;
-    float sdot = 0.f, yv = 0.f;
+    for (int t = 0; t < 2; ++t) dp[t] = da[t] = zero;
+    float sdot = 0.f, ydot = 0.f;
+    const bool has_s = KB2 == 2 || tid < 256;
+    const float* const ps = a.s + (vs * Kp + (tid >> 2) % Kp) * a.vp + gc;
+    const float* const pd = a.ds + (vs * Kp + (tid >> 2) % Kp) * a.vp + gc;
+    const float* const pw = (tid < 256 ? a.w : a.y) + (vs * kC + gi) * a.vp + gc;
+    const T* const px = tid < 256 ? (has_do ? static_cast<const T*>(a.d_o) + rowc * a.lddo + (long)hv * a.V : static_cast<const T*>(a.v))
+                                  : static_cast<const T*>(a.v) + rowc * a.ldv + (long)hv * a.V;
+    f32x4 xs[2], xd[2], xw[2];
+    unsigned xo[8];
+    auto request = [&](int vb) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        xs[h] = *reinterpret_cast<const f32x4*>(ps + vb + 4 * h);
+        xd[h] = *reinterpret_cast<const f32x4*>(pd + vb + 4 * h);
+        xw[h] = *reinterpret_cast<const f32x4*>(pw + vb + 4 * h);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int v = min(vb + gc + e, a.V - 1);
+        if constexpr (sizeof(T) == 2) xo[e] = *reinterpret_cast<const unsigned short*>(px + v);
+        else xo[e] = *reinterpret_cast<const unsigned*>(px + v);
+      }
+    };
+    request(0);
     for (int vb = 0; vb < a.vp; vb += 32) {
       __syncthreads();
-#pragma unroll
-      for (int u0 = 0; u0 < Kp * 4; u0 += 256) {
-        const int u = u0 + tid, k = u >> 2, c = (u & 3) * 8;
-        const float* const ps = a.s + (vs * Kp + k) * a.vp + vb + c;
-        const float* const pd = a.ds + (vs * Kp + k) * a.vp + vb + c;
-        float x[8], d[8];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const f32x4 t = *reinterpret_cast<const f32x4*>(ps + 4 * h), w = *reinterpret_cast<const f32x4*>(pd + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { x[4 * h + e] = t[e]; d[4 * h + e] = w[e]; sdot = fmaf(t[e], w[e], sdot); }
-        }
-        bf16x8 t[3];
-        sb::split8<3>(x, t);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(sl + (p * Kp + k) * LDV + c) = t[p];
-        sb::split8<3>(d, t);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dl + (p * Kp + k) * LDV + c) = t[p];
-      }
       {
-        const int i = tid >> 2, c = (tid & 3) * 8;
-        const float* const pw = a.w + (vs * kC + i) * a.vp + vb + c;
         float x[8];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const f32x4 t = *reinterpret_cast<const f32x4*>(pw + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[4 * h + e] = t[e];
-        }
         bf16x8 t[3];
+        if (has_s) {
+          const int k = tid >> 2;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) { x[e] = xs[e >> 2][e & 3]; sdot = fmaf(x[e], xd[e >> 2][e & 3], sdot); }
+          sb::split8<3>(x, t);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(sl + (p * Kp + k) * LDV + gc) = t[p];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = xd[e >> 2][e & 3];
+          sb::split8<3>(x, t);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dl + (p * Kp + k) * LDV + gc) = t[p];
+        }
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          o[e] = gi < valid && vb + gc + e < a.V ? __uint_as_float(sizeof(T) == 2 ? xo[e] << 16 : xo[e]) : 0.f;
+        __bf16* const dst = (tid < 256 ? wl : yl) + gi * LDV + gc;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = xw[e >> 2][e & 3];
         sb::split8<3>(x, t);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(wl + (p * kC + i) * LDV + c) = t[p];
-      }
-      // this wave's rows of dO, Y and W
-      bf16x8 of[NP], yf[3], wf[3];
-      {
-        float x[8], y[8];
-        const float* const py = a.y + (vs * kC + ia) * a.vp + vb + 8 * lg;
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dst + p * kC * LDV) = t[p];
+        if (tid < 256) {
+          bf16x8 u[NP];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const f32x4 t = *reinterpret_cast<const f32x4*>(py + 4 * h);
+          for (int e = 0; e < 8; ++e) o[e] = has_do ? o[e] : 0.f;
+          sb::split8<NP>(o, u);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[4 * h + e] = t[e];
+          for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(ol + (p * kC + gi) * LDV + gc) = u[p];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ydot = fmaf(x[e], o[e], ydot);
         }
-        sb::split8<3>(y, yf);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int v = vb + 8 * lg + e;
-          const bool in = ia < valid && v < a.V;
-          x[e] = a.d_o && in ? (float)static_cast<const T*>(a.d_o)[(row0 + ia) * a.lddo + (long)hv * a.V + v] : 0.f;
-          if (in) yv = fmaf(y[e], (float)static_cast<const T*>(a.v)[(row0 + ia) * a.ldv + (long)hv * a.V + v], yv);
-        }
-        sb::split8<NP>(x, of);
       }
       __syncthreads();
+      request(min(vb + 32, a.vp - 32));
+      bf16x8 of[NP], yf[3], wf[3];
+      sb::load_frag<NP>(of, ol + ia * LDV + 8 * lg, kC * LDV);
+      sb::load_frag<3>(yf, yl + ia * LDV + 8 * lg, kC * LDV);
       sb::load_frag<3>(wf, wl + ia * LDV + 8 * lg, kC * LDV);
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
-        bf16x8 b[3];
-        sb::load_frag<3>(b, sl + (16 * t + lr) * LDV + 8 * lg, Kp * LDV);
+        bf16x8 b[3], d[3];
+        sb::load_frag<3>(b, sl + (kt0 + 16 * t + lr) * LDV + 8 * lg, Kp * LDV);
+        sb::load_frag<3>(d, dl + (kt0 + 16 * t + lr) * LDV + 8 * lg, Kp * LDV);
         sb::mma<NP, 3>(e1[t], of, b);
         sb::mma<3, 3>(e2[t], yf, b);
-        sb::load_frag<3>(b, dl + (16 * t + lr) * LDV + 8 * lg, Kp * LDV);
-        sb::mma<3, 3>(e3[t], wf, b);
+        sb::mma<3, 3>(e3[t], wf, d);
       }
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        if (t <= wave) {
+      for (int t = 0; t < 2; ++t) {
+        const int jt = 2 * t + half;
+        if (jt <= w) {
           bf16x8 b[3];
-          sb::load_frag<3>(b, wl + (16 * t + lr) * LDV + 8 * lg, kC * LDV);
+          sb::load_frag<3>(b, wl + (16 * jt + lr) * LDV + 8 * lg, kC * LDV);
           sb::mma<NP, 3>(dp[t], of, b);
           sb::mma<3, 3>(da[t], yf, b);
         }
       }
     }
-    yv += __shfl_xor(yv, 16, 64);
-    yv += __shfl_xor(yv, 32, 64);
-    sdot = wave_sum(sdot);
+    // ---- the chunk's own part
     const float* const vec = a.vec + vs * kVecs * kC;
     const f32x4 gam = *reinterpret_cast<const f32x4*>(vec + kGam * kC + ib);
     const f32x4 tail = *reinterpret_cast<const f32x4*>(vec + kTail * kC + ib);
@@ -770,12 +997,17 @@ __global__ __launch_bounds__(256, 1) void gdr_grads_kernel(GdrArgs a) {
     const f32x4 ghi = *reinterpret_cast<const f32x4*>(vec + kGHi * kC + ib);
     const f32x4 glo = *reinterpret_cast<const f32x4*>(vec + kGLo * kC + ib);
     const float last = vec[kGam * kC + kC - 1];
+    const __bf16* const ktr = a.kt + (hs * Kp + kt0 + lr) * NP * kC;
+    const __bf16* const qtr = a.qt + (hs * Kp + kt0 + lr) * NP * kC;
+    ydot += __shfl_xor(ydot, 1, 64);
+    ydot += __shfl_xor(ydot, 2, 64);
+    sdot = wave_sum(sdot);
     __syncthreads();
-    if (lg == 0) rows[ia] = yv;
+    if (tid >= 256 && (tid & 3) == 0) yv[gi] = ydot;
     if (lane == 0) red[wave] = sdot;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int j = 16 * t + lr;
+    for (int t = 0; t < 2; ++t) {
+      const int jt = 2 * t + half, j = 16 * jt + lr;
       const float hj = vec[kGHi * kC + j], lj = vec[kGLo * kC + j];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -791,6 +1023,8 @@ __global__ __launch_bounds__(256, 1) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
         for (int p = 0; p < 3; ++p) bl[(p * kC + i) * kLdT + j] = x[p];
       }
+      sb::split_store4<3>(rt + j * kLdT + ib, kC * kLdT, dp[t]);
+      sb::split_store4<3>(bt + j * kLdT + ib, kC * kLdT, beta * da[t]);
     }
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
@@ -798,65 +1032,56 @@ __global__ __launch_bounds__(256, 1) void gdr_grads_kernel(GdrArgs a) {
       e2[t] *= -gam;
       e3[t] *= tail;
     }
-    __syncthreads();
-    const __bf16* const ktr = a.kt + hs * NP * Kp * kC + lr * kC + 8 * lg;
-    const __bf16* const qtr = a.qt + hs * NP * Kp * kC + lr * kC + 8 * lg;
-    for (int kb = 0; kb < (wave < 2 ? 1 : 2); ++kb) {
-      bf16x8 rf[3], bf[3];
-      sb::load_frag<3>(rf, rl + ia * kLdT + 32 * kb + 8 * lg, kC * kLdT);
-      sb::load_frag<3>(bf, bl + ia * kLdT + 32 * kb + 8 * lg, kC * kLdT);
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        bf16x8 b[NP];
-        sb::load_frag<NP>(b, ktr + 16 * t * kC + 32 * kb, Kp * kC);
-        sb::mma<3, NP>(e1[t], rf, b);
-        sb::mma<3, NP>(e2[t], bf, b);
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      sb::split_store4<3>(rl + (16 * t + lr) * kLdT + ib, kC * kLdT, dp[t]);
-      sb::split_store4<3>(bl + (16 * t + lr) * kLdT + ib, kC * kLdT, beta * da[t]);
-    }
-    // row sums that need k and q as fp32, and k.(tail E3) before the other terms join
-    f32x4 dg = zero, db = zero, st = zero;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = 16 * t + lr;
-        const bool in = ib + e < valid && k < a.K;
-        const float kv = in ? (float)static_cast<const T*>(a.k)[(row0 + ib + e) * a.ldk + (long)hk * a.K + k] : 0.f;
-        const float qv = in ? (float)static_cast<const T*>(a.q)[(row0 + ib + e) * a.ldq + (long)hk * a.K + k] : 0.f;
-        dg[e] = fmaf(qv, e1[t][e], dg[e]);
-        db[e] = fmaf(kv, e2[t][e], db[e]);
-        st[e] = fmaf(kv, e3[t][e], st[e]);
-      }
-    __syncthreads();
-    for (int kb = wave < 2 ? 0 : 1; kb < 2; ++kb) {
-      bf16x8 rf[3], bf[3];
-      sb::load_frag<3>(rf, rl + ia * kLdT + 32 * kb + 8 * lg, kC * kLdT);
-      sb::load_frag<3>(bf, bl + ia * kLdT + 32 * kb + 8 * lg, kC * kLdT);
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        bf16x8 b[NP];
-        sb::load_frag<NP>(b, qtr + 16 * t * kC + 32 * kb, Kp * kC);
-        sb::mma<3, NP>(e3[t], rf, b);
-        sb::load_frag<NP>(b, ktr + 16 * t * kC + 32 * kb, Kp * kC);
-        sb::mma<3, NP>(e3[t], bf, b);
-      }
-    }
-    f32x4 kc = zero;
+    // k and q in the layout of a result: four tokens of one column, from the transposes
+    f32x4 kv[KT], qv[KT];
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
+      kv[t] = qv[t] = zero;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int k = 16 * t + lr;
-        const bool in = ib + e < valid && k < a.K;
-        const float kv = in ? (float)static_cast<const T*>(a.k)[(row0 + ib + e) * a.ldk + (long)hk * a.K + k] : 0.f;
-        kc[e] = fmaf(kv, e3[t][e], kc[e]);
+      for (int p = NP - 1; p >= 0; --p) {
+        const bf16x4 x = *reinterpret_cast<const bf16x4*>(ktr + (16 * t * NP + p) * kC + ib);
+        const bf16x4 y = *reinterpret_cast<const bf16x4*>(qtr + (16 * t * NP + p) * kC + ib);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { kv[t][e] += (float)x[e]; qv[t][e] += (float)y[e]; }
       }
+    }
+    f32x4 dg = zero, db = zero, st = zero, kc = zero;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) st += kv[t] * e3[t];
+    __syncthreads();
+#pragma unroll 1
+    for (int kb = 0; kb < 2; ++kb) {                         // not unrolled: fragments of both halves at once would not fit the registers
+      if (kb == 0 || w >= 2) {
+        bf16x8 rf[3], bf[3];
+        sb::load_frag<3>(rf, rl + ia * kLdT + 32 * kb + 8 * lg, kC * kLdT);
+        sb::load_frag<3>(bf, bl + ia * kLdT + 32 * kb + 8 * lg, kC * kLdT);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          bf16x8 b[NP];
+          sb::load_frag<NP>(b, ktr + 16 * t * NP * kC + 32 * kb + 8 * lg, kC);
+          sb::mma<3, NP>(e1[t], rf, b);
+          sb::mma<3, NP>(e2[t], bf, b);
+        }
+      }
+      if (kb == 1 || w < 2) {
+        bf16x8 rf[3], bf[3];
+        sb::load_frag<3>(rf, rt + ia * kLdT + 32 * kb + 8 * lg, kC * kLdT);
+        sb::load_frag<3>(bf, bt + ia * kLdT + 32 * kb + 8 * lg, kC * kLdT);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          bf16x8 b[NP];
+          sb::load_frag<NP>(b, qtr + 16 * t * NP * kC + 32 * kb + 8 * lg, kC);
+          sb::mma<3, NP>(e3[t], rf, b);
+          sb::load_frag<NP>(b, ktr + 16 * t * NP * kC + 32 * kb + 8 * lg, kC);
+          sb::mma<3, NP>(e3[t], bf, b);
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      dg += qv[t] * e1[t];
+      db += kv[t] * e2[t];
+      kc += kv[t] * e3[t];
       e2[t] = e2[t] * beta + e3[t];                          // dk of this value head
       if (GROUP) { dqs[t] += e1[t]; dks[t] += e2[t]; }
     }
@@ -869,16 +1094,22 @@ __global__ __launch_bounds__(256, 1) void gdr_grads_kernel(GdrArgs a) {
         y += __shfl_xor(y, off, 64);
         z += __shfl_xor(z, off, 64);
       }
-      if (lr == 0) { rows[kC + ib + e] = x; rows[2 * kC + ib + e] = y; rows[3 * kC + ib + e] = z; }
+      if (lr == 0) {
+        float* const p = rows + half * 3 * kC + ib + e;
+        p[0] = x; p[kC] = y; p[2 * kC] = z;
+      }
     }
     __syncthreads();
     if (wave == 0) {
       // <dS', S'> = gam_C <dS', S> + sum_i k_i.(tail E3)_i reaches every token of the chunk, dG_i those up to i
-      double share = rows[3 * kC + lane];
+      double share = (double)rows[2 * kC + lane] + rows[5 * kC + lane];
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1) share += __shfl_xor(share, off, 64);
-      share += (double)last * ((double)red[0] + red[1] + red[2] + red[3]);
-      double s = rows[kC + lane];
+      double sd = 0.0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sd += red[i];
+      share += (double)last * sd;
+      double s = (double)rows[lane] + rows[3 * kC + lane];
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
         const double down = __shfl_down(s, off, 64);
@@ -886,21 +1117,21 @@ __global__ __launch_bounds__(256, 1) void gdr_grads_kernel(GdrArgs a) {
       }
       if (lane < valid) {
         a.dg[(row0 + lane) * a.lddg + hv] = (float)(s + share);
-        a.dbeta[(row0 + lane) * a.lddbeta + hv] = rows[lane] + rows[2 * kC + lane];
+        a.dbeta[(row0 + lane) * a.lddbeta + hv] = yv[lane] + (rows[kC + lane] + rows[4 * kC + lane]);
       }
     }
     if (r == a.rep - 1) {
+      T* const pq = static_cast<T*>(a.dq) + (row0 + ib) * a.lddq + (long)hk * a.K + kt0 + lr;
+      T* const pk = static_cast<T*>(a.dk) + (row0 + ib) * a.lddk + (long)hk * a.K + kt0 + lr;
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
         const f32x4 dq = GROUP ? dqs[t] : e1[t], dk = GROUP ? dks[t] : e2[t];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = 16 * t + lr;
-          if (ib + e < valid && k < a.K) {
-            static_cast<T*>(a.dq)[(row0 + ib + e) * a.lddq + (long)hk * a.K + k] = (T)dq[e];
-            static_cast<T*>(a.dk)[(row0 + ib + e) * a.lddk + (long)hk * a.K + k] = (T)dk[e];
+        for (int e = 0; e < 4; ++e)
+          if (ib + e < valid && kt0 + 16 * t + lr < a.K) {
+            pq[e * a.lddq + 16 * t] = (T)dq[e];
+            pk[e * a.lddk + 16 * t] = (T)dk[e];
           }
-        }
       }
     }
   }
@@ -1033,7 +1264,7 @@ long slots_of(int n_seq, long rows, bool packed) {
 // ws: offsets in floats (every array a multiple of 64 floats); returns the total.  Rows that the scans read in place
 // (bf16, K = 64 or 128, 16-byte aligned) are not packed; the size leaves room for them where alignment may forbid it.
 long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, int Hk, int Hv, int K, int V, bool train) {
-  const long ns = slots_of(n_seq, rows, packed), kp = padded_k(K), np = dtype == HHRL_BF16 ? 1 : 3, vp = (V + kVt - 1) / kVt * kVt;
+  const long ns = slots_of(n_seq, rows, packed), kp = padded_k(K), np = dtype == HHRL_BF16 ? 1 : 3, vp = (V + 31) / 32 * 32;
   long off = 0;
   auto take = [&](long floats) { float* p = ws ? ws + off : nullptr; off += (floats + 63) & ~63L; return p; };
   auto take16 = [&](long n) { return reinterpret_cast<__bf16*>(take((n + 1) / 2)); };
@@ -1056,7 +1287,7 @@ long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, 
   if (a) {
     a->kpk = t.kpk; a->qpk = t.qpk; a->kt = t.kt; a->qt = t.qt; a->m = t.m; a->p = t.p; a->mt = t.mt; a->pt = t.pt;
     a->vec = t.vec; a->w = t.w; a->y = t.y; a->s = t.s; a->ds = t.ds;
-    a->n_slots = ns; a->vp = (int)vp; a->nvt = (int)(vp / kVt);
+    a->n_slots = ns; a->vp = (int)vp;
   }
   return off;
 }
@@ -1076,7 +1307,7 @@ int gdr_check(const hhrl_gdr_desc* d, const char* who) {
                "%s: leading dimension of an input too small", who);
   const long ns = slots_of(d->n_seq, d->rows, d->starts != nullptr);
   HHRL_REQUIRE(ns < (1L << 31), "%s: %ld chunks", who, ns);
-  const long blocks = ((long)d->n_seq * d->Hv + 7) / 8 * 8 * ((d->V + kVt - 1) / kVt);
+  const long blocks = ((long)d->n_seq * d->Hv + 7) / 8 * 8 * ((d->V + 31) / 32 * 2);
   HHRL_REQUIRE(blocks < (1L << 31), "%s: n_seq*Hv too large", who);
   return HHRL_OK;
 }
@@ -1098,48 +1329,61 @@ int gdr_fill(const hhrl_gdr_desc* d, GdrArgs& a, bool train, const char* who) {
   return HHRL_OK;
 }
 
+// Columns per workgroup of a scan: 32 (two result tiles per wave) where that fills the chip's 256 CUs, else 16: twice the
+// workgroups, and a shorter chain from chunk to chunk.
+#ifndef SCAN_NT
+#define SCAN_NT(wgs32) ((wgs32) >= 256 ? 2 : 1)
+#endif
+int scan_tiles(const GdrArgs& a) { return SCAN_NT((long)a.n_seq * a.Hv * (a.vp / 32)); }
+
+template <typename T, int NP, int KB2, int NT>
+int run_scan(GdrArgs a, bool bwd, hipStream_t st, double flops) {
+  a.nvt = a.vp / (16 * NT);
+  const unsigned grid = (unsigned)(((long)a.n_seq * a.Hv + 7) / 8 * 8 * a.nvt);
+  if (bwd) {
+    constexpr int lds = ScanLds<NP, KB2, NT>::bwd_bytes;
+    HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(&gdr_scan_bwd_kernel<T, NP, KB2, NT>), lds, "gdr_backward"));
+    ProfScope ps("gdr_scan_bwd_kernel", st, flops, 0.0);
+    hipLaunchKernelGGL((gdr_scan_bwd_kernel<T, NP, KB2, NT>), dim3(grid), dim3(512), lds, st, a);
+  } else {
+    constexpr int lds = ScanLds<NP, KB2, NT>::fwd_bytes;
+    HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(&gdr_scan_fwd_kernel<T, NP, KB2, NT>), lds, "gdr_forward"));
+    ProfScope ps("gdr_scan_fwd_kernel", st, flops, 0.0);
+    hipLaunchKernelGGL((gdr_scan_fwd_kernel<T, NP, KB2, NT>), dim3(grid), dim3(512), lds, st, a);
+  }
+  return launch_status(bwd ? "gdr_scan_bwd_kernel" : "gdr_scan_fwd_kernel");
+}
+template <typename T, int NP, int KB2>
+int run_scan(const GdrArgs& a, bool bwd, hipStream_t st, double flops) {
+  return scan_tiles(a) == 2 ? run_scan<T, NP, KB2, 2>(a, bwd, st, flops) : run_scan<T, NP, KB2, 1>(a, bwd, st, flops);
+}
+
 template <typename T, int NP, int KB2>
 int run_fwd(const GdrArgs& a, hipStream_t st, double flops) {
   constexpr int Kp = 64 * KB2;
   constexpr int over = 2 * NP * kC * (Kp + 8) * 2 > 2 * kC * kLdM * 4 ? 2 * NP * kC * (Kp + 8) * 2 : 2 * kC * kLdM * 4;
   constexpr int lds_prep = over + 2 * kC * kLdM * 4 + 3 * kC * 4;
-  constexpr int lds_scan = ScanLds<NP, KB2>::bytes;
-  const void* prep = reinterpret_cast<const void*>(&gdr_prep_kernel<T, NP, KB2>);
-  const void* scan = reinterpret_cast<const void*>(&gdr_scan_fwd_kernel<T, NP, KB2>);
-  HHRL_TRY(ensure_dyn_lds(prep, lds_prep, "gdr_forward"));
-  HHRL_TRY(ensure_dyn_lds(scan, lds_scan, "gdr_forward"));
+  HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(&gdr_prep_kernel<T, NP, KB2>), lds_prep, "gdr_forward"));
   {
     ProfScope ps("gdr_prep_kernel", st, 0.0, 0.0);
     hipLaunchKernelGGL((gdr_prep_kernel<T, NP, KB2>), dim3((unsigned)a.n_slots, a.Hk), dim3(256), lds_prep, st, a);
   }
   HHRL_TRY(launch_status("gdr_prep_kernel"));
-  const unsigned grid = (unsigned)(((long)a.n_seq * a.Hv + 7) / 8 * 8 * a.nvt);
-  ProfScope ps("gdr_scan_fwd_kernel", st, flops, 0.0);
-  hipLaunchKernelGGL((gdr_scan_fwd_kernel<T, NP, KB2>), dim3(grid), dim3(256), lds_scan, st, a);
-  return launch_status("gdr_scan_fwd_kernel");
+  return run_scan<T, NP, KB2>(a, false, st, flops);
 }
 
 template <typename T, int NP, int KB2, bool GROUP>
 int run_grads(const GdrArgs& a, hipStream_t st, double flops) {
-  constexpr int Kp = 64 * KB2, LDV = 40;
-  constexpr int over = 2 * 3 * LDV * (2 * Kp + kC) > 2 * 2 * 3 * kC * kLdT ? 2 * 3 * LDV * (2 * Kp + kC) : 2 * 2 * 3 * kC * kLdT;
-  constexpr int lds = over + (4 * kC + 4) * 4;
+  constexpr int lds = GradsLds<NP, KB2>::bytes;
   HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(&gdr_grads_kernel<T, NP, KB2, GROUP>), lds, "gdr_backward"));
   ProfScope ps("gdr_grads_kernel", st, flops, 0.0);
-  hipLaunchKernelGGL((gdr_grads_kernel<T, NP, KB2, GROUP>), dim3((unsigned)a.n_slots, a.Hk), dim3(256), lds, st, a);
+  hipLaunchKernelGGL((gdr_grads_kernel<T, NP, KB2, GROUP>), dim3((unsigned)a.n_slots, a.Hk), dim3(512), lds, st, a);
   return launch_status("gdr_grads_kernel");
 }
 
 template <typename T, int NP, int KB2>
 int run_bwd(const GdrArgs& a, hipStream_t st, double flops) {
-  constexpr int lds = ScanLds<NP, KB2>::bytes;
-  HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(&gdr_scan_bwd_kernel<T, NP, KB2>), lds, "gdr_backward"));
-  const unsigned grid = (unsigned)(((long)a.n_seq * a.Hv + 7) / 8 * 8 * a.nvt);
-  {
-    ProfScope ps("gdr_scan_bwd_kernel", st, flops, 0.0);
-    hipLaunchKernelGGL((gdr_scan_bwd_kernel<T, NP, KB2>), dim3(grid), dim3(256), lds, st, a);
-  }
-  HHRL_TRY(launch_status("gdr_scan_bwd_kernel"));
+  HHRL_TRY((run_scan<T, NP, KB2>(a, true, st, flops)));
   return a.rep > 1 ? run_grads<T, NP, KB2, true>(a, st, flops) : run_grads<T, NP, KB2, false>(a, st, flops);
 }
 

@@ -33,44 +33,50 @@ def _dtype_code(dtype) -> int:
     return _DTYPES[dtype]
 
 
-def _on_device(name: str, t: torch.Tensor) -> None:
-    _need(t.is_cuda, "%s is on %s, not on a GPU" % (name, t.device))
-    _need(t.device.index == torch.cuda.current_device(),
-          "%s is on %s, the current device is cuda:%d" % (name, t.device, torch.cuda.current_device()))
-
-
-def _tensor(name: str, t, shape, dtype) -> int:
-    """Checks a contiguous tensor of a given shape; its address."""
+def _fail(name: str, t, shape, dtype, dev: int) -> None:
+    """Says what is wrong with an operand that failed a check."""
     _need(isinstance(t, torch.Tensor), "%s is not a tensor" % name)
     _need(tuple(t.shape) == tuple(shape), "%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
     _need(t.dtype == dtype, "%s is %s, not %s" % (name, t.dtype, dtype))
+    _need(t.is_cuda, "%s is on %s, not on a GPU" % (name, t.device))
+    _need(t.get_device() == dev, "%s is on %s, the current device is cuda:%d" % (name, t.device, dev))
+
+
+def _tensor(name: str, t, shape, dtype, dev: int) -> int:
+    """Checks a contiguous tensor of a given shape; its address."""
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype or t.get_device() != dev:
+        _fail(name, t, shape, dtype, dev)
     _need(t.is_contiguous(), "%s is not contiguous" % name)
-    _on_device(name, t)
     return t.data_ptr()
 
 
-def _rows(name: str, t, lead, tail, dtype):
-    """Checks a tensor [*lead, *tail] whose tail is contiguous and whose leading dimensions are rows at one distance
+def _rows(name: str, t, shape, n: int, width: int, dtype, dev: int):
+    """Checks a tensor whose first n dimensions are rows of `width` contiguous elements, at one distance from each other
     (a column range of a wider buffer qualifies): its address and that distance in elements."""
-    _need(isinstance(t, torch.Tensor), "%s is not a tensor" % name)
-    _need(tuple(t.shape) == tuple(lead) + tuple(tail), "%s has shape %s, not %s" % (name, tuple(t.shape), tuple(lead) + tuple(tail)))
-    _need(t.dtype == dtype, "%s is %s, not %s" % (name, t.dtype, dtype))
-    _on_device(name, t)
-    n, width = len(lead), 1
-    for size, stride in zip(reversed(t.shape[n:]), reversed(t.stride()[n:])):
-        _need(size == 1 or stride == width, "%s: the elements of a row are not contiguous (strides %s)" % (name, t.stride()))
-        width *= size
-    ld = None
-    inner = 1                                     # rows below the dimension at hand
-    for size, stride in zip(reversed(t.shape[:n]), reversed(t.stride()[:n])):
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype or t.get_device() != dev:
+        _fail(name, t, shape, dtype, dev)
+    if t.is_contiguous():
+        return t.data_ptr(), width
+    strides, inner = t.stride(), 1
+    for size, stride in zip(reversed(shape[n:]), reversed(strides[n:])):
+        _need(size == 1 or stride == inner, "%s: the elements of a row are not contiguous (strides %s)" % (name, strides))
+        inner *= size
+    ld, inner = None, 1                           # inner: rows below the dimension at hand
+    for size, stride in zip(reversed(shape[:n]), reversed(strides[:n])):
         if size > 1:
             if ld is None and stride % inner == 0:
                 ld = stride // inner
-            _need(ld is not None and stride == ld * inner, "%s: its rows are not at one distance (strides %s)" % (name, t.stride()))
+            _need(ld is not None and stride == ld * inner, "%s: its rows are not at one distance (strides %s)" % (name, strides))
         inner *= size
     ld = width if ld is None else ld
-    _need(ld >= width, "%s: rows overlap (strides %s)" % (name, t.stride()))
+    _need(ld >= width, "%s: rows overlap (strides %s)" % (name, strides))
     return t.data_ptr(), ld
+
+
+def _device() -> int:
+    if not torch.cuda.is_initialized():
+        _need(torch.cuda.is_available(), "no GPU")
+    return torch.cuda.current_device()
 
 
 class GatedDelta:
@@ -99,82 +105,88 @@ class GatedDelta:
         _need(n > 0, "no workspace for n_seq=%d rows=%d" % (n_seq, rows))
         return torch.empty(n, dtype=torch.float32, device=device)
 
-    def _desc(self, q, k, v, g, beta, ws, starts, lens):
+    def _desc(self, q, k, v, g, beta, ws, starts, lens, dev):
         d = _lib.GdrDesc()
         _need(isinstance(q, torch.Tensor), "q is not a tensor")
         if starts is not None:
             _need(lens is None, "starts and lens")
             _need(q.dim() == 3, "packed q has shape %s, not [rows, Hk, K]" % (tuple(q.shape),))
             lead = (q.shape[0],)
+            rows = lead[0]
             _need(isinstance(starts, torch.Tensor) and starts.dim() == 1 and starts.numel() >= 2, "starts: n_seq + 1 numbers")
             n_seq = starts.numel() - 1
-            d.starts = _tensor("starts", starts, (n_seq + 1,), torch.int32)
+            d.starts = _tensor("starts", starts, (n_seq + 1,), torch.int32, dev)
         else:
             _need(q.dim() == 4, "q has shape %s, not [B, T, Hk, K]" % (tuple(q.shape),))
             lead = tuple(q.shape[:2])
-            n_seq = lead[0]
+            n_seq, rows = lead[0], lead[0] * lead[1]
             if lens is not None:
-                d.lens = _tensor("lens", lens, (n_seq,), torch.int32)
-        rows = 1
-        for s in lead:
-            rows *= s
+                d.lens = _tensor("lens", lens, (n_seq,), torch.int32, dev)
         _need(rows > 0, "no tokens")
+        n = len(lead)
+        key, val, head = (lead + (self.Hk, self.K), n, self.Hk * self.K, self.dtype, dev), \
+            (lead + (self.Hv, self.V), n, self.Hv * self.V, self.dtype, dev), (lead + (self.Hv,), n, self.Hv, torch.float32, dev)
         d.dtype, d.n_seq, d.rows = self.code, n_seq, rows
         d.Hk, d.Hv, d.K, d.V, d.scale = self.Hk, self.Hv, self.K, self.V, self.scale
-        d.q, d.ldq = _rows("q", q, lead, (self.Hk, self.K), self.dtype)
-        d.k, d.ldk = _rows("k", k, lead, (self.Hk, self.K), self.dtype)
-        d.v, d.ldv = _rows("v", v, lead, (self.Hv, self.V), self.dtype)
-        d.g, d.ldg = _rows("g", g, lead, (self.Hv,), torch.float32)
-        d.beta, d.ldbeta = _rows("beta", beta, lead, (self.Hv,), torch.float32)
+        d.q, d.ldq = _rows("q", q, *key)
+        d.k, d.ldk = _rows("k", k, *key)
+        d.v, d.ldv = _rows("v", v, *val)
+        d.g, d.ldg = _rows("g", g, *head)
+        d.beta, d.ldbeta = _rows("beta", beta, *head)
         _need(isinstance(ws, torch.Tensor), "ws is not a tensor")
-        d.ws, d.ws_floats = _tensor("ws", ws, (ws.numel(),), torch.float32), ws.numel()
-        return d, lead, n_seq
+        d.ws_floats = ws.numel()
+        d.ws = _tensor("ws", ws, (d.ws_floats,), torch.float32, dev)
+        return d, n_seq, key, val, head
 
-    def _state(self, name, t, n_seq):
-        return _tensor(name, t, (n_seq, self.Hv, self.K, self.V), torch.float32) if t is not None else None
+    def _state(self, name, t, n_seq, dev):
+        return _tensor(name, t, (n_seq, self.Hv, self.K, self.V), torch.float32, dev) if t is not None else None
 
     def fwd(self, q, k, v, g, beta, o, ws, s0=None, s1=None, starts=None, lens=None, no_backward: bool = False) -> None:
-        """Writes o and, where given, s1 (states behind the sequences, from s0 or zero).  Leaves in ws what `bwd` of the
-        same inputs reads, unless no_backward."""
-        d, lead, n = self._desc(q, k, v, g, beta, ws, starts, lens)
-        d.o, d.ldo = _rows("o", o, lead, (self.Hv, self.V), self.dtype)
-        d.s0, d.s1 = self._state("s0", s0, n), self._state("s1", s1, n)
+        """Writes o and, where given, s1 (states behind the sequences, from s0 or zero; may be s0).  Leaves in ws what `bwd`
+        of the same inputs reads, unless no_backward."""
+        dev = _device()
+        d, n, _, val, _ = self._desc(q, k, v, g, beta, ws, starts, lens, dev)
+        d.o, d.ldo = _rows("o", o, *val)
+        d.s0, d.s1 = self._state("s0", s0, n, dev), self._state("s1", s1, n, dev)
         d.no_backward = int(no_backward)
         check(self._lib.hhrl_gdr_forward(C.byref(d), _lib.stream_ptr()))
 
     def bwd(self, q, k, v, g, beta, d_o, dq, dk, dv, dg, dbeta, ws, d_s1=None, d_s0=None, starts=None, lens=None) -> None:
         """Gradients of <d_o, o> + <d_s1, s1> (either None: absent), written to dq, dk, dv, dg, dbeta and d_s0; ws as the
         forward call of the same inputs left it."""
-        d, lead, n = self._desc(q, k, v, g, beta, ws, starts, lens)
+        dev = _device()
+        d, n, key, val, head = self._desc(q, k, v, g, beta, ws, starts, lens, dev)
         if d_o is not None:
-            d.d_o, d.lddo = _rows("d_o", d_o, lead, (self.Hv, self.V), self.dtype)
-        d.d_s1, d.d_s0 = self._state("d_s1", d_s1, n), self._state("d_s0", d_s0, n)
-        d.dq, d.lddq = _rows("dq", dq, lead, (self.Hk, self.K), self.dtype)
-        d.dk, d.lddk = _rows("dk", dk, lead, (self.Hk, self.K), self.dtype)
-        d.dv, d.lddv = _rows("dv", dv, lead, (self.Hv, self.V), self.dtype)
-        d.dg, d.lddg = _rows("dg", dg, lead, (self.Hv,), torch.float32)
-        d.dbeta, d.lddbeta = _rows("dbeta", dbeta, lead, (self.Hv,), torch.float32)
+            d.d_o, d.lddo = _rows("d_o", d_o, *val)
+        d.d_s1, d.d_s0 = self._state("d_s1", d_s1, n, dev), self._state("d_s0", d_s0, n, dev)
+        d.dq, d.lddq = _rows("dq", dq, *key)
+        d.dk, d.lddk = _rows("dk", dk, *key)
+        d.dv, d.lddv = _rows("dv", dv, *val)
+        d.dg, d.lddg = _rows("dg", dg, *head)
+        d.dbeta, d.lddbeta = _rows("dbeta", dbeta, *head)
         check(self._lib.hhrl_gdr_backward(C.byref(d), _lib.stream_ptr()))
 
     def step(self, q, k, v, g, beta, o, state, state_out=None, slots=None) -> None:
         """One token for each of B rows (q, k [B, Hk, K], v, o [B, Hv, V], g, beta [B, Hv]) against a pool of states
         [n, Hv, K, V]: row b moves state slots[b] (None: state b) into state_out (None: in place).  A negative slot: the
         row is idle, its output 0.  A slot past the pool, or one that an earlier row names: output NaN, no state moves."""
+        dev = _device()
         _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q is not [B, Hk, K]")
-        B = q.shape[0]
-        _need(B > 0, "no rows")
-        _need(isinstance(state, torch.Tensor) and state.dim() == 4 and state.shape[0] > 0, "state is not [n, Hv, K, V]")
-        n = state.shape[0]
-        sp = self._state("state", state, n)
-        so = sp if state_out is None else self._state("state_out", state_out, n)
-        ptrs = []
-        for name, t, tail, dt in (("q", q, (self.Hk, self.K), self.dtype), ("k", k, (self.Hk, self.K), self.dtype),
-                                  ("v", v, (self.Hv, self.V), self.dtype), ("g", g, (self.Hv,), torch.float32),
-                                  ("beta", beta, (self.Hv,), torch.float32), ("o", o, (self.Hv, self.V), self.dtype)):
-            ptrs += _rows(name, t, (B,), tail, dt)
-        sl = _tensor("slots", slots, (B,), torch.int32) if slots is not None else None
-        _need(slots is not None or B <= n, "%d rows for %d states" % (B, n))
-        check(self._lib.hhrl_gdr_step(self.code, B, self.Hk, self.Hv, self.K, self.V, self.scale, *ptrs, sp, so, n, sl, _lib.stream_ptr()))
+        _need(isinstance(state, torch.Tensor) and state.dim() == 4, "state is not [n, Hv, K, V]")
+        B, n = q.shape[0], state.shape[0]
+        _need(B > 0 and n > 0, "%d rows for %d states" % (B, n))
+        Hk, Hv, K, V, dt = self.Hk, self.Hv, self.K, self.V, self.dtype
+        key, val, head = ((B, Hk, K), 1, Hk * K, dt, dev), ((B, Hv, V), 1, Hv * V, dt, dev), ((B, Hv), 1, Hv, torch.float32, dev)
+        sp = self._state("state", state, n, dev)
+        so = sp if state_out is None else self._state("state_out", state_out, n, dev)
+        sl = None
+        if slots is not None:
+            sl = _tensor("slots", slots, (B,), torch.int32, dev)
+        else:
+            _need(B <= n, "%d rows for %d states" % (B, n))
+        check(self._lib.hhrl_gdr_step(self.code, B, Hk, Hv, K, V, self.scale, *_rows("q", q, *key), *_rows("k", k, *key),
+                                      *_rows("v", v, *val), *_rows("g", g, *head), *_rows("beta", beta, *head), *_rows("o", o, *val),
+                                      sp, so, n, sl, _lib.stream_ptr()))
 
 
 class BlockNorm:
@@ -199,6 +211,7 @@ class BlockNorm:
         _need(eps >= 0, "eps=%g" % eps)
         self.D, self.H, self.post, self.pre, self.gate_act, self.gate_rows = D, H, post, pre, gate_act, gate_rows
         self.alpha, self.scale, self.eps, self.dtype = float(alpha), float(scale), float(eps), dtype
+        self._kinds = _NORMS[post], _NORMS[pre], _GATES[gate_act], gate_rows
         self._lib = _lib.load()
 
     def workspace(self, M: int, device) -> torch.Tensor:
@@ -207,49 +220,49 @@ class BlockNorm:
         _need(n > 0, "no workspace for M=%d" % M)
         return torch.empty(n, dtype=torch.float32, device=device)
 
-    def _act(self, name, t, M):
-        tail = (self.H, self.D) if t.dim() == 3 or self.H > 1 else (self.D,)
-        return _rows(name, t, (M,), tail, self.dtype)
+    def _shape(self, first, M, dev):
+        """What an activation of M rows has to look like: as [M, H, D], or [M, D] if that is how the first one comes."""
+        flat = self.H == 1 and isinstance(first, torch.Tensor) and first.dim() == 2
+        return ((M, self.D) if flat else (M, self.H, self.D), 1, self.H * self.D, self.dtype, dev)
 
-    def _gate(self, name, t, M):
+    def _gate_shape(self, t, M, act, dev):
         if self.gate_rows == 1:
-            return self._act(name, t, M)
-        return _rows(name, t, (-(-M // self.gate_rows),), (1, self.D) if t.dim() == 3 else (self.D,), torch.float32)
+            return act
+        n = -(-M // self.gate_rows)
+        return ((n, self.D) if isinstance(t, torch.Tensor) and t.dim() == 2 else (n, 1, self.D), 1, self.D, torch.float32, dev)
 
-    def _desc(self, x, y, gate, params):
+    def _desc(self, x, y, gate, params, dev):
         d = _lib.BlockNormDesc()
         first = x if x is not None else y
-        _need(isinstance(first, torch.Tensor), "neither x nor y")
-        M = first.shape[0] if first.dim() else 0
+        _need(isinstance(first, torch.Tensor) and first.dim() > 0, "neither x nor y")
+        M = first.shape[0]
         _need(M > 0, "no rows")
         _need(y is not None or (gate is None and self.post == "none"), "a gate or a post norm without y")
+        act = self._shape(first, M, dev)
         d.dtype, d.M, d.H, d.D = self.code, M, self.H, self.D
-        d.post, d.pre, d.gate_act, d.gate_rows = _NORMS[self.post], _NORMS[self.pre], _GATES[self.gate_act], self.gate_rows
+        d.post, d.pre, d.gate_act, d.gate_rows = self._kinds
         d.alpha, d.scale, d.eps = self.alpha, self.scale, self.eps
-        for name, t in (("x", x), ("y", y)):
-            if t is not None:
-                _need(isinstance(t, torch.Tensor), "%s is not a tensor" % name)
-                p, ld = self._act(name, t, M)
-                setattr(d, name, p)
-                setattr(d, "ld" + name, ld)
+        if x is not None:
+            d.x, d.ldx = _rows("x", x, *act)
+        if y is not None:
+            d.y, d.ldy = _rows("y", y, *act)
         if gate is not None:
-            _need(isinstance(gate, torch.Tensor), "gate is not a tensor")
-            d.gate, d.ldgate = self._gate("gate", gate, M)
+            d.gate, d.ldgate = _rows("gate", gate, *self._gate_shape(gate, M, act, dev))
         for name, t in zip(self.PARAMS, params):
             if t is not None:
                 _need(getattr(self, name[2:]) != "none", "%s without a %s norm" % (name, name[2:]))
-                setattr(d, name, _tensor(name, t, (self.D,), torch.float32))
-        return d, M
+                setattr(d, name, _tensor(name, t, (self.D,), torch.float32, dev))
+        return d, M, act
 
     def fwd(self, x=None, y=None, gate=None, w_post=None, b_post=None, w_pre=None, b_pre=None, out=None, h=None) -> None:
         """Writes r to out and pre(r) to h (either may be None; both may be x or y)."""
-        d, M = self._desc(x, y, gate, (w_post, b_post, w_pre, b_pre))
+        d, M, act = self._desc(x, y, gate, (w_post, b_post, w_pre, b_pre), _device())
         _need(out is not None or h is not None, "neither out nor h")
         _need(self.pre == "none" or h is not None, "a pre norm without h")
         if out is not None:
-            d.out, d.ldo = self._act("out", out, M)
+            d.out, d.ldo = _rows("out", out, *act)
         if h is not None:
-            d.h, d.ldh = self._act("h", h, M)
+            d.h, d.ldh = _rows("h", h, *act)
         check(self._lib.hhrl_block_norm_forward(C.byref(d), _lib.stream_ptr()))
 
     def bwd(self, x=None, y=None, gate=None, w_post=None, b_post=None, w_pre=None, b_pre=None, d_out=None, d_h=None,
@@ -257,24 +270,27 @@ class BlockNorm:
         """Gradients of <d_out, r> + <d_h, h> (either None: absent) from the forward call's inputs: dx, dy, dgate are
         written, parameter gradients added to; those that are None are skipped.  ws: needed for parameter gradients and for
         the gradient of a gate with gate_rows > 1."""
-        d, M = self._desc(x, y, gate, (w_post, b_post, w_pre, b_pre))
+        dev = _device()
+        d, M, act = self._desc(x, y, gate, (w_post, b_post, w_pre, b_pre), dev)
         _need(d_out is not None or d_h is not None, "neither d_out nor d_h")
         for name, t, of in (("dx", dx, x), ("dy", dy, y), ("dgate", dgate, gate)):
             _need(t is None or of is not None, "%s without %s" % (name, name[1:]))
         if d_out is not None:
-            d.d_out, d.lddo = self._act("d_out", d_out, M)
+            d.d_out, d.lddo = _rows("d_out", d_out, *act)
         if d_h is not None:
-            d.d_h, d.lddh = self._act("d_h", d_h, M)
+            d.d_h, d.lddh = _rows("d_h", d_h, *act)
         if dx is not None:
-            d.dx, d.lddx = self._act("dx", dx, M)
+            d.dx, d.lddx = _rows("dx", dx, *act)
         if dy is not None:
-            d.dy, d.lddy = self._act("dy", dy, M)
+            d.dy, d.lddy = _rows("dy", dy, *act)
         if dgate is not None:
-            d.dgate, d.lddgate = self._gate("dgate", dgate, M)
+            d.dgate, d.lddgate = _rows("dgate", dgate, *self._gate_shape(dgate, M, act, dev))
         for name, t in zip(self.PARAMS, (dw_post, db_post, dw_pre, db_pre)):
             if t is not None:
                 _need(getattr(self, name[2:]) != "none" and (name[2:] == "post" or d_h is not None), "d%s without its norm" % name)
-                setattr(d, "d" + name, _tensor("d" + name, t, (self.D,), torch.float32))
+                setattr(d, "d" + name, _tensor("d" + name, t, (self.D,), torch.float32, dev))
         if ws is not None:
-            d.ws, d.ws_floats = _tensor("ws", ws, (ws.numel(),), torch.float32), ws.numel()
+            _need(isinstance(ws, torch.Tensor), "ws is not a tensor")
+            d.ws_floats = ws.numel()
+            d.ws = _tensor("ws", ws, (d.ws_floats,), torch.float32, dev)
         check(self._lib.hhrl_block_norm_backward(C.byref(d), _lib.stream_ptr()))
