@@ -852,7 +852,8 @@ struct GradsLds {
   static constexpr int cols = 3 * LDV * (2 * Kp + 2 * kC) + NP * LDV * kC;       // elements: S, dS', W, Y, dO
   static constexpr int tri = 4 * 3 * kC * kLdT;              // R, B and their transposes, over them afterwards
   static constexpr int over = 2 * (cols > tri ? cols : tri);
-  static constexpr int bytes = over + (8 * kC + 8) * 4;
+  static constexpr int kq = NP == 1 ? 2 * 2 * Kp * kLdT : 0;                     // bytes: k and q of the chunk, transposed (three terms do not fit)
+  static constexpr int bytes = over + kq + (8 * kC + 8) * 4;
 };
 template <typename T, int NP, int KB2, bool GROUP>
 __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
@@ -868,7 +869,9 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
   __bf16* const bl = rl + 3 * kC * kLdT;
   __bf16* const rt = bl + 3 * kC * kLdT;
   __bf16* const bt = rt + 3 * kC * kLdT;
-  float* const rows = reinterpret_cast<float*>(smem + L::over);    // [2 halves][3][64]: shares of dG, of dbeta, k.(tail E3)
+  __bf16* const kl = reinterpret_cast<__bf16*>(smem + L::over);    // NP == 1: [Kp][kLdT] each
+  __bf16* const ql = kl + Kp * kLdT;
+  float* const rows = reinterpret_cast<float*>(smem + L::over + L::kq);    // [2 halves][3][64]: shares of dG, of dbeta, k.(tail E3)
   float* const yv = rows + 6 * kC;                                 // [64] Y.v
   float* const red = yv + kC;                                      // [8]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, w = wave >> 1, half = wave & 1, lr = lane & 15, lg = lane >> 4;
@@ -886,6 +889,27 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
   const int gi = (tid & 255) >> 2, gc = (tid & 3) * 8;       // token and columns of W, dO (threads 0..255), Y, v (the others)
   const long rowc = row0 + min(gi, valid - 1);
 
+  // the chunk's k and q, transposed: fragments along the tokens, and single columns in the layout of a result
+  constexpr int TS = NP == 1 ? kLdT : NP * kC;               // from column to column
+  const __bf16 *ktr, *qtr;
+  if constexpr (NP == 1) {
+    const bf16x8* const gk = reinterpret_cast<const bf16x8*>(a.kt + hs * Kp * kC);
+    const bf16x8* const gq = reinterpret_cast<const bf16x8*>(a.qt + hs * Kp * kC);
+    bf16x8 x[Kp / 64], y[Kp / 64];
+#pragma unroll
+    for (int u = 0; u < Kp / 64; ++u) { x[u] = gk[u * 512 + tid]; y[u] = gq[u * 512 + tid]; }
+#pragma unroll
+    for (int u = 0; u < Kp / 64; ++u) {
+      const int at = (u * 64 + (tid >> 3)) * kLdT + (tid & 7) * 8;
+      *reinterpret_cast<bf16x8*>(kl + at) = x[u];
+      *reinterpret_cast<bf16x8*>(ql + at) = y[u];
+    }
+    ktr = kl + (kt0 + lr) * TS;
+    qtr = ql + (kt0 + lr) * TS;
+  } else {
+    ktr = a.kt + (hs * Kp + kt0 + lr) * TS;
+    qtr = a.qt + (hs * Kp + kt0 + lr) * TS;
+  }
   f32x4 dqs[GROUP ? KT : 1], dks[GROUP ? KT : 1];
   if (GROUP) {
 #pragma unroll
@@ -997,8 +1021,21 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
     const f32x4 ghi = *reinterpret_cast<const f32x4*>(vec + kGHi * kC + ib);
     const f32x4 glo = *reinterpret_cast<const f32x4*>(vec + kGLo * kC + ib);
     const float last = vec[kGam * kC + kC - 1];
-    const __bf16* const ktr = a.kt + (hs * Kp + kt0 + lr) * NP * kC;
-    const __bf16* const qtr = a.qt + (hs * Kp + kt0 + lr) * NP * kC;
+    float hj[2], lj[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      hj[t] = vec[kGHi * kC + 16 * (2 * t + half) + lr];
+      lj[t] = vec[kGLo * kC + 16 * (2 * t + half) + lr];
+    }
+    bf16x4 kr[KT][NP], qr[KT][NP];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        kr[t][p] = *reinterpret_cast<const bf16x4*>(ktr + 16 * t * TS + p * kC + ib);
+        qr[t][p] = *reinterpret_cast<const bf16x4*>(qtr + 16 * t * TS + p * kC + ib);
+      }
+    __builtin_amdgcn_sched_barrier(0);                       // all of these requests together, in front of what waits for them
     ydot += __shfl_xor(ydot, 1, 64);
     ydot += __shfl_xor(ydot, 2, 64);
     sdot = wave_sum(sdot);
@@ -1008,11 +1045,10 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int jt = 2 * t + half, j = 16 * jt + lr;
-      const float hj = vec[kGHi * kC + j], lj = vec[kGLo * kC + j];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = ib + e;
-        const float d = i >= j ? expf((ghi[e] - hj) + (glo[e] - lj)) : 0.f;
+        const float d = i >= j ? expf((ghi[e] - hj[t]) + (glo[e] - lj[t])) : 0.f;
         dp[t][e] = i >= j ? a.scale * dp[t][e] * d : 0.f;
         da[t][e] = i > j ? -da[t][e] * d : 0.f;
         __bf16 x[3];
@@ -1038,12 +1074,9 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
     for (int t = 0; t < KT; ++t) {
       kv[t] = qv[t] = zero;
 #pragma unroll
-      for (int p = NP - 1; p >= 0; --p) {
-        const bf16x4 x = *reinterpret_cast<const bf16x4*>(ktr + (16 * t * NP + p) * kC + ib);
-        const bf16x4 y = *reinterpret_cast<const bf16x4*>(qtr + (16 * t * NP + p) * kC + ib);
+      for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { kv[t][e] += (float)x[e]; qv[t][e] += (float)y[e]; }
-      }
+        for (int e = 0; e < 4; ++e) { kv[t][e] += (float)kr[t][p][e]; qv[t][e] += (float)qr[t][p][e]; }
     }
     f32x4 dg = zero, db = zero, st = zero, kc = zero;
 #pragma unroll
@@ -1058,7 +1091,7 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
           bf16x8 b[NP];
-          sb::load_frag<NP>(b, ktr + 16 * t * NP * kC + 32 * kb + 8 * lg, kC);
+          sb::load_frag<NP>(b, ktr + 16 * t * TS + 32 * kb + 8 * lg, kC);
           sb::mma<3, NP>(e1[t], rf, b);
           sb::mma<3, NP>(e2[t], bf, b);
         }
@@ -1070,9 +1103,9 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
           bf16x8 b[NP];
-          sb::load_frag<NP>(b, qtr + 16 * t * NP * kC + 32 * kb + 8 * lg, kC);
+          sb::load_frag<NP>(b, qtr + 16 * t * TS + 32 * kb + 8 * lg, kC);
           sb::mma<3, NP>(e3[t], rf, b);
-          sb::load_frag<NP>(b, ktr + 16 * t * NP * kC + 32 * kb + 8 * lg, kC);
+          sb::load_frag<NP>(b, ktr + 16 * t * TS + 32 * kb + 8 * lg, kC);
           sb::mma<3, NP>(e3[t], bf, b);
         }
       }
