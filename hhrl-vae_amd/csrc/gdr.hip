@@ -69,6 +69,7 @@ struct GdrArgs {
   //     fragments are at constant offsets from one address.
   __bf16 *kpk, *qpk, *kt, *qt, *m, *p, *mt, *pt;
   float *vec, *w, *y, *s, *ds;
+  float* nobody;                   // 64 floats that stores of nobody's elements go to
 };
 enum { kGam = 0, kTail = 1, kBeta = 2, kGHi = 3, kGLo = 4, kVecs = 5 };
 
@@ -318,8 +319,8 @@ template <int NP, int KB2, int NT>
 struct ScanLds {
   static constexpr int Kp = 64 * KB2, VT = 16 * NT, LDS_S = Kp + 8;
   static constexpr int S = 3 * VT * LDS_S, X = 3 * VT * kLdT, F = VT * kLdM;     // elements
-  static constexpr int fwd_bytes = 2 * (S + 2 * X) + 4 * F;
-  static constexpr int bwd_bytes = 2 * (S + 3 * X + NP * VT * kLdT) + 8 * F;
+  static constexpr int fwd_bytes = 2 * (S + 2 * X) + 8 * F;
+  static constexpr int bwd_bytes = 2 * (S + 3 * X + NP * VT * kLdT) + 12 * F;
 };
 
 // Operand rows of k or q, token 16*w + lr of a chunk, from the packed terms or from the caller's rows.  Requests have
@@ -391,22 +392,19 @@ __device__ __forceinline__ f32x4 rows_below(const f32x4& x, int ib, int valid) {
   for (int e = 0; e < 4; ++e) r[e] = ib + e < valid ? x[e] : 0.f;
   return r;
 }
-// a result tile of o or dv into the caller's rows
+// a result tile of o or dv into the caller's rows.  Without conditions too: what is waited for later (loads and stores come
+// back in order) is counted from the instructions on every path.  Elements that are nobody's go to a corner of ws.
 template <typename T, int NT>
-__device__ __forceinline__ void store_cols(void* dst, long ld, long row0, int valid, int hv, int V, int v0, int ib, int lr, const f32x4 (&x)[NT]) {
+__device__ __forceinline__ void store_cols(void* dst, long ld, long row0, int valid, int hv, int V, int v0, int ib, int lr, const f32x4 (&x)[NT], float* nobody) {
   T* const p = static_cast<T*>(dst) + (row0 + ib) * ld + (long)hv * V + v0 + lr;
-  if (valid == kC && v0 + 16 * NT <= V) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) p[e * ld + 16 * t] = (T)x[t][e];
-    return;
-  }
+  T* const trash = reinterpret_cast<T*>(nobody) + lr;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (ib + e < valid && v0 + 16 * t + lr < V) p[e * ld + 16 * t] = (T)x[t][e];
+    for (int e = 0; e < 4; ++e) {
+      T* const q = ib + e < valid && v0 + 16 * t + lr < V ? p + e * ld + 16 * t : trash;
+      *q = (T)x[t][e];
+    }
 }
 // the state tile of a scan's chain wave w: rows 16*(KB2*w + t) + 4*lg + e, columns v0 + 16*u + lr
 template <int KB2, int NT>
@@ -445,11 +443,12 @@ struct ScanVec {
     last = vec[kGam * kC + kC - 1];
   }
 };
-// the two 32-wide halves of a row of M, P or a transpose; `low` / `high`: whether this wave's rows reach them
+// the two 32-wide halves of a row of M, P or a transpose.  Half `f` of a wave whose rows do not reach it reads the other
+// one again (from the first-level cache): a request under a condition would be waited for at once.
 template <int N>
 __device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* row, bool low, bool high) {
-  if (low) sb::load_frag<N>(f[0], row, kC);
-  if (high) sb::load_frag<N>(f[1], row + 32, kC);
+  sb::load_frag<N>(f[0], row + (low ? 0 : 32), kC);
+  sb::load_frag<N>(f[1], row + (high ? 32 : 0), kC);
 }
 
 // A scan is bound by its chain: state -> K S -> W -> state, chunk after chunk, and inside it by the instructions its waves
@@ -457,7 +456,7 @@ __device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* row, b
 // nothing but the chain, and four others what hangs on it: the output o, one chunk behind (forward), or what only depends
 // on dO, one chunk ahead, and the stores of Y and dV (backward).  Everything a chunk needs from memory is requested while
 // the chunk in front of it is worked on, behind the last use of its registers.
-template <typename T, int NP, int KB2, int NT>
+template <typename T, int NP, int KB2, int NT, bool TRAIN>
 __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
   using L = ScanLds<NP, KB2, NT>;
   constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT, LDS_S = L::LDS_S;
@@ -466,7 +465,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
   __bf16* const sl = reinterpret_cast<__bf16*>(smem);      // [3][VT][LDS_S] S
   __bf16* const xl = sl + L::S;                            // [3][VT][kLdT]  beta (V - gam K S)
   __bf16* const ul = xl + L::X;                            // [3][VT][kLdT]  exp(G_C - G) W
-  float* const wl = reinterpret_cast<float*>(ul + L::X);   // [VT][kLdM]     W
+  float* const wl = reinterpret_cast<float*>(ul + L::X);   // [2][VT][kLdM]  W, of the chunk at hand and the one in front of it
   int n, hv, v0;
   if (!scan_tile(a, VT, n, hv, v0)) return;
   const int hk = hv / a.rep;
@@ -533,7 +532,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
           sb::split_store4<3>(xl + (16 * t + lr) * kLdT + ib, VT * kLdT, rows_below(vc.beta * (vp.get(t, valid) - vc.gam * ks[t]), ib, valid));
         vp.load(next);
         vn.load(vecp, ib);
-        if (a.train) {
+        if constexpr (TRAIN) {
           float* const sp = a.s + (vs * Kp + 16 * KB2 * w + 4 * lg) * a.vp + v0 + lr;
 #pragma unroll
           for (int t = 0; t < KB2; ++t)
@@ -559,7 +558,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           sb::split_store4<3>(ul + (16 * t + lr) * kLdT + ib, VT * kLdT, vc.tail * wt[t]);
-          *reinterpret_cast<f32x4*>(wl + (16 * t + lr) * kLdM + ib) = wt[t];
+          *reinterpret_cast<f32x4*>(wl + (c & 1) * L::F + (16 * t + lr) * kLdM + ib) = wt[t];
         }
         lds_barrier();
 #pragma unroll
@@ -581,20 +580,21 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
     if (a.s1) store_state<KB2, NT>(S, a.s1, a, nh, w, v0, lr, lg);
   } else if (nc > 0) {                                     // ---- the output, between the chain's barriers
     bf16x8 qf[KB][NP], pf[2][NO];
-    f32x4 qs[NT], gam;
+    f32x4 qs[NT], qn[NT];
     const RowPtr<NP, KB> qp(a, a.q, a.ldq, a.qpk, slot0, hk, start, len, ia, lg);
     const __bf16* pp = a.p + ((slot0 * a.Hv + hv) * kC + ia) * 3 * kC + 8 * lg;
     const float* gp = a.vec + (slot0 * a.Hv + hv) * kVecs * kC + kGam * kC + ib;
     // o of chunk c from qs = gam (Q S) and W, which the chain has left in wl
     auto finish = [&](int c) {
       const long vs = (slot0 + c) * a.Hv + hv;
+      const float* const wc = wl + (c & 1) * L::F;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
         if (kb == 0 || high)
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             float x[8];
-            const float* const src = wl + (16 * t + lr) * kLdM + 32 * kb + 8 * lg;
+            const float* const src = wc + (16 * t + lr) * kLdM + 32 * kb + 8 * lg;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const f32x4 y = *reinterpret_cast<const f32x4*>(src + 4 * h);
@@ -605,41 +605,41 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
             sb::split8<NO>(x, b);
             sb::mma<NO, NO>(qs[t], pf[kb], b);
           }
-      if (a.train) {
+      if constexpr (TRAIN) {
         float* const wp = a.w + (vs * kC + ib) * a.vp + v0 + lr;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(wl + (16 * t + lr) * kLdM + ib);
+          const f32x4 y = *reinterpret_cast<const f32x4*>(wc + (16 * t + lr) * kLdM + ib);
 #pragma unroll
           for (int e = 0; e < 4; ++e) wp[e * a.vp + 16 * t] = y[e];
         }
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) qs[t] *= a.scale;
-      store_cols<T, NT>(a.o, a.ldo, start + (long)c * kC, min(kC, len - c * kC), hv, a.V, v0, ib, lr, qs);
+      store_cols<T, NT>(a.o, a.ldo, start + (long)c * kC, min(kC, len - c * kC), hv, a.V, v0, ib, lr, qs, a.nobody);
     };
     qp.load(qf, 0);
     for (int c = 0; c < nc; ++c) {
-      if (c > 0) finish(c - 1);
-      load_tri<NO>(pf, pp, true, high);
-      gam = *reinterpret_cast<const f32x4*>(gp);
-      pp += (long)a.Hv * 3 * kC * kC;
+      const f32x4 gam = *reinterpret_cast<const f32x4*>(gp);
       gp += (long)a.Hv * kVecs * kC;
       lds_barrier();
 #pragma unroll
-      for (int t = 0; t < NT; ++t) qs[t] = zero;
+      for (int t = 0; t < NT; ++t) qn[t] = zero;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           bf16x8 b[NO];
           sb::load_frag<NO>(b, sl + (16 * t + lr) * LDS_S + 32 * kb + 8 * lg, VT * LDS_S);
-          sb::mma<NP, NO>(qs[t], qf[kb], b);
+          sb::mma<NP, NO>(qn[t], qf[kb], b);
         }
       qp.load(qf, min(c + 1, nc - 1));
-#pragma unroll
-      for (int t = 0; t < NT; ++t) qs[t] *= gam;
       lds_barrier();
+      if (c > 0) finish(c - 1);
+      load_tri<NO>(pf, pp, true, high);
+      pp += (long)a.Hv * 3 * kC * kC;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) qs[t] = qn[t] * gam;
       lds_barrier();
     }
     finish(nc - 1);
@@ -657,7 +657,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
   __bf16* const yl = zl + L::X;                            // [3][VT][kLdT]  -gam beta Y
   __bf16* const ol = yl + L::X;                            // [NP][VT][kLdT] dO
   float* const zp = reinterpret_cast<float*>(ol + NP * VT * kLdT);   // [VT][kLdM] scale P^T dO
-  float* const yf = zp + L::F;                             // [VT][kLdM] Y
+  float* const yf = zp + L::F;                             // [2][VT][kLdM] Y, of the chunk at hand and the one behind it
   int n, hv, v0;
   if (!scan_tile(a, VT, n, hv, v0)) return;
   const int hk = hv / a.rep;
@@ -751,7 +751,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           sb::split_store4<3>(yl + (16 * t + lr) * kLdT + ib, VT * kLdT, -vc.gam * vc.beta * y[t]);
-          *reinterpret_cast<f32x4*>(yf + (16 * t + lr) * kLdM + ib) = y[t];
+          *reinterpret_cast<f32x4*>(yf + (c & 1) * L::F + (16 * t + lr) * kLdM + ib) = y[t];
         }
         lds_barrier();
 #pragma unroll
@@ -811,10 +811,23 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
     share();
     load_tri<3>(pf, pt + max(nc - 2, 0) * pstep, low, true);
     lds_barrier();
+    // Y and dV of chunk c, which the chain has left in yf
+    auto finish = [&](int c, const f32x4& beta) {
+      float* const yp = a.y + (((slot0 + c) * a.Hv + hv) * kC + ib) * a.vp + v0 + lr;
+      f32x4 y[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        y[t] = *reinterpret_cast<const f32x4*>(yf + (c & 1) * L::F + (16 * t + lr) * kLdM + ib);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) yp[e * a.vp + 16 * t] = y[t][e];
+        y[t] *= beta;
+      }
+      store_cols<T, NT>(a.dv, a.lddv, start + (long)c * kC, min(kC, len - c * kC), hv, a.V, v0, ib, lr, y, a.nobody);
+    };
+    f32x4 gam = *reinterpret_cast<const f32x4*>(vec + (nc - 1) * vstep + kGam * kC), beta = *reinterpret_cast<const f32x4*>(vec + (nc - 1) * vstep + kBeta * kC);
+    f32x4 before = zero;                                   // beta of the chunk behind
     for (int c = nc - 1; c >= 0; --c) {
       const int next = max(c - 1, 0), next2 = max(c - 2, 0);
-      const f32x4 gam = *reinterpret_cast<const f32x4*>(vec + c * vstep + kGam * kC);
-      const f32x4 beta = *reinterpret_cast<const f32x4*>(vec + c * vstep + kBeta * kC);
 #pragma unroll
       for (int t = 0; t < NT; ++t) { d[t] = dn[t]; dn[t] = dp.get(t, has_do ? min(kC, len - next * kC) : 0); }
       dp.load(next2);
@@ -824,21 +837,16 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
         sb::split_store4<3>(gl + (16 * t + lr) * kLdT + ib, VT * kLdT, a.scale * gam * d[t]);
         sb::split_store4<NP>(ol + (16 * t + lr) * kLdT + ib, VT * kLdT, dn[t]);
       }
+      gam = *reinterpret_cast<const f32x4*>(vec + next * vstep + kGam * kC);
       lds_barrier();                                       // 2: the chain has read zp
       share();
       load_tri<3>(pf, pt + next2 * pstep, low, true);
+      if (c < nc - 1) finish(c + 1, before);
+      before = beta;
+      beta = *reinterpret_cast<const f32x4*>(vec + next * vstep + kBeta * kC);
       lds_barrier();                                       // 3
-      float* const yp = a.y + (((slot0 + c) * a.Hv + hv) * kC + ib) * a.vp + v0 + lr;
-      f32x4 y[NT];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        y[t] = *reinterpret_cast<const f32x4*>(yf + (16 * t + lr) * kLdM + ib);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) yp[e * a.vp + 16 * t] = y[t][e];
-        y[t] *= beta;
-      }
-      store_cols<T, NT>(a.dv, a.lddv, start + (long)c * kC, min(kC, len - c * kC), hv, a.V, v0, ib, lr, y);
     }
+    finish(0, before);
   }
 }
 
@@ -1308,6 +1316,7 @@ long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, 
   t.m = take16(ns * Hv * 3 * kC * kC);
   t.p = take16(ns * Hv * 3 * kC * kC);
   t.vec = take(ns * Hv * kVecs * kC);
+  t.nobody = take(64);
   if (train) {
     t.qt = take16(ns * Hk * np * kC * kp);
     t.mt = take16(ns * Hv * 3 * kC * kC);
@@ -1319,7 +1328,7 @@ long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, 
   }
   if (a) {
     a->kpk = t.kpk; a->qpk = t.qpk; a->kt = t.kt; a->qt = t.qt; a->m = t.m; a->p = t.p; a->mt = t.mt; a->pt = t.pt;
-    a->vec = t.vec; a->w = t.w; a->y = t.y; a->s = t.s; a->ds = t.ds;
+    a->vec = t.vec; a->w = t.w; a->y = t.y; a->s = t.s; a->ds = t.ds; a->nobody = t.nobody;
     a->n_slots = ns; a->vp = (int)vp;
   }
   return off;
@@ -1380,9 +1389,10 @@ int run_scan(GdrArgs a, bool bwd, hipStream_t st, double flops) {
     hipLaunchKernelGGL((gdr_scan_bwd_kernel<T, NP, KB2, NT>), dim3(grid), dim3(512), lds, st, a);
   } else {
     constexpr int lds = ScanLds<NP, KB2, NT>::fwd_bytes;
-    HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(&gdr_scan_fwd_kernel<T, NP, KB2, NT>), lds, "gdr_forward"));
+    void (*const fn)(GdrArgs) = a.train ? gdr_scan_fwd_kernel<T, NP, KB2, NT, true> : gdr_scan_fwd_kernel<T, NP, KB2, NT, false>;
+    HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(fn), lds, "gdr_forward"));
     ProfScope ps("gdr_scan_fwd_kernel", st, flops, 0.0);
-    hipLaunchKernelGGL((gdr_scan_fwd_kernel<T, NP, KB2, NT>), dim3(grid), dim3(512), lds, st, a);
+    hipLaunchKernelGGL(fn, dim3(grid), dim3(512), lds, st, a);
   }
   return launch_status(bwd ? "gdr_scan_bwd_kernel" : "gdr_scan_fwd_kernel");
 }
