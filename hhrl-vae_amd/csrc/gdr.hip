@@ -65,26 +65,25 @@ struct GdrArgs {
   int pack, train, vp, nvt;
   // ws, per chunk and key head: k, q [64][terms][Kp] (pack), their transposes [Kp][terms][64];
   //     per chunk and value head: M, P and their transposes [64][terms][64], five rows of 64 floats, and for the
-  //     backward pass W, Y [64][vp] and S, dS [Kp][vp], fp32.  The terms of a row lie side by side, so that a lane's
+  //     backward pass W, Y [vp/32][64][32] and S, dS [vp/32][Kp][32], fp32 (tiles of 32 columns).  The terms of a row lie side by side, so that a lane's
   //     fragments are at constant offsets from one address.
   __bf16 *kpk, *qpk, *kt, *qt, *m, *p, *mt, *pt;
   float *vec, *w, *y, *s, *ds;
-  float* nobody;                   // 64 floats that stores of nobody's elements go to
 };
 enum { kGam = 0, kTail = 1, kBeta = 2, kGHi = 3, kGLo = 4, kVecs = 5 };
 
 __device__ __forceinline__ long clampl(long v, long lo, long hi) { return v < lo ? lo : v > hi ? hi : v; }
 
-// rows [start, start + len) of sequence n and the place of its first chunk.  Packed sequences of any lengths:
+// rows [start, start + len) of sequence n (the same n in the whole wave) and the place of its first chunk.  Packed sequences of any lengths:
 // floor(start/64) + n leaves every sequence at least ceil(len/64) places.
 __device__ __forceinline__ void seq_range(const GdrArgs& a, int n, long& start, int& len, long& slot0) {
   if (a.starts) {
-    start = clampl(a.starts[n], 0, a.rows);
-    len = (int)(clampl(a.starts[n + 1], start, a.rows) - start);
+    start = clampl(__builtin_amdgcn_readfirstlane(a.starts[n]), 0, a.rows);
+    len = (int)(clampl(__builtin_amdgcn_readfirstlane(a.starts[n + 1]), start, a.rows) - start);
     slot0 = start / kC + n;
   } else {
     start = (long)n * a.T;
-    len = a.lens ? (int)clampl(a.lens[n], 0, a.T) : a.T;
+    len = a.lens ? (int)clampl(__builtin_amdgcn_readfirstlane(a.lens[n]), 0, a.T) : a.T;
     slot0 = (long)n * a.cpt;
   }
 }
@@ -308,8 +307,8 @@ __device__ __forceinline__ bool scan_tile(const GdrArgs& a, int vt, int& n, int&
   v0 = (u % a.nvt) * vt;
   const long pair = (long)(u / a.nvt) * 8 + xcd;
   if (pair >= (long)a.n_seq * a.Hv) return false;
-  n = (int)(pair / a.Hv);
-  hv = (int)(pair - (long)n * a.Hv);
+  n = __builtin_amdgcn_readfirstlane((int)(pair / a.Hv));
+  hv = __builtin_amdgcn_readfirstlane((int)(pair - (long)n * a.Hv));
   return true;
 }
 
@@ -323,88 +322,111 @@ struct ScanLds {
   static constexpr int bwd_bytes = 2 * (S + 3 * X + NP * VT * kLdT) + 12 * F;
 };
 
-// Operand rows of k or q, token 16*w + lr of a chunk, from the packed terms or from the caller's rows.  Requests have
-// no conditions (a conditional one is waited for where its branch joins): a row behind the sequence reads the last one
-// instead, and the results it reaches are masked.
+// Rows of the caller's tensors go through buffer descriptors: a base that moves from chunk to chunk in scalar registers, a
+// lane's offset that never changes, and the size of what the sequence has left, behind which a load gives 0 and a store is
+// dropped.  So rows behind the sequence need no test, no request has a condition (a conditional one would be waited for
+// where its branch joins), and a chunk costs no address arithmetic on the vector unit.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+constexpr unsigned kNoColumn = 0x80000000u;      // an offset behind every size
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, long offset, long bytes) {
+  // (descriptor word 3: 32-bit data, no swizzle)
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base)) + offset, 0, (int)bytes, 0x00027000);
+}
+// Operand rows of k or q, token 16*w + lr of a chunk, from the packed terms (whose rows behind the sequence are 0) or from
+// the caller's rows
 template <int NP, int KB>
 struct RowPtr {
   static constexpr int Kp = 32 * KB;
-  const __bf16* p;
-  long step, back;
-  int over;                                    // this row of the first chunk less the sequence's last row
-  __device__ __forceinline__ RowPtr(const GdrArgs& a, const void* raw, long ld, const __bf16* packed, long slot0, int hk, long start, int len,
-                                    int i, int lg) {
+  const char* base;
+  long step, row;                              // bytes from chunk to chunk and from row to row
+  unsigned at;
+  int len;
+  __device__ __forceinline__ RowPtr(const GdrArgs& a, const void* raw, long ld, const __bf16* packed, long slot0, int hk, long start, int len_,
+                                    int i, int lg) : len(len_) {
     if (NP == 1 && !a.pack) {
-      p = static_cast<const __bf16*>(raw) + (start + i) * ld + (long)hk * Kp + 8 * lg;
-      step = kC * ld;
-      back = ld;
+      base = static_cast<const char*>(raw) + (start * ld + (long)hk * Kp) * 2;
+      row = ld * 2;
+      step = kC * row;
     } else {
-      p = packed + ((slot0 * a.Hk + hk) * kC + i) * NP * Kp + 8 * lg;
-      step = (long)a.Hk * NP * kC * Kp;
-      back = 0;
+      base = reinterpret_cast<const char*>(packed + (slot0 * a.Hk + hk) * kC * NP * Kp);
+      row = NP * Kp * 2;
+      step = (long)a.Hk * kC * row;
+      len = 0x7fffffff;                        // all rows of a packed chunk are there
     }
-    over = i - (len - 1);
+    at = i * (unsigned)row + 16 * lg;
   }
   __device__ __forceinline__ void load(bf16x8 (&f)[KB][NP], int c) const {
-    const __bf16* const r = p + c * step - max(0, c * kC + over) * back;
+    const int have = min(kC, len - c * kC);
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(base, c * step, (have - 1) * row + NP * Kp * 2);
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) sb::load_frag<NP>(f[kb], r + 32 * kb, Kp);
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+        f[kb][p] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(r, at + (p * Kp + 32 * kb) * 2, 0, 0));
   }
 };
-// Elements of v or dO in the layout of a result (rows ib + e, columns v0 + 16*t + lr), requested the same way and kept
-// as they come; get() is 0 outside the sequence and the head
+// Elements of v or dO in the layout of a result (rows ib + e, columns v0 + 16*t + lr), kept as they come
 template <typename T, int NT>
 struct ColPtr {
-  const T* p[NT];
-  long ld;
-  int ib, len;
-  bool in[NT];
-  unsigned x[NT][4];
-  __device__ __forceinline__ ColPtr(const void* src, long ld_, long start, int len_, int hv, int V, int v0, int lr, int ib_) : ld(ld_), ib(ib_), len(len_) {
+  const char* base;
+  long row, width;
+  int len;
+  unsigned at[NT][4], x[NT][4];
+  __device__ __forceinline__ ColPtr(const void* src, long ld, long start, int len_, int hv, int V, int v0, int lr, int ib) : len(len_) {
+    base = static_cast<const char*>(src) + (start * ld + (long)hv * V) * sizeof(T);
+    row = ld * sizeof(T);
+    width = (long)V * sizeof(T);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int v = v0 + 16 * t + lr;
-      in[t] = v < V;
-      p[t] = static_cast<const T*>(src) + start * ld + (long)hv * V + (in[t] ? v : V - 1);
-    }
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int v = v0 + 16 * t + lr;
+        at[t][e] = v < V ? (ib + e) * (unsigned)row + v * (unsigned)sizeof(T) : kNoColumn;
+      }
+  }
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk(int c) const {
+    return rows_rsrc(base, (long)c * kC * row, (min(kC, len - c * kC) - 1) * row + width);
   }
   __device__ __forceinline__ void load(int c) {
+    const __amdgpu_buffer_rsrc_t r = chunk(c);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const long off = (long)min(c * kC + ib + e, len - 1) * ld;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if constexpr (sizeof(T) == 2) x[t][e] = *reinterpret_cast<const unsigned short*>(p[t] + off);
-        else x[t][e] = *reinterpret_cast<const unsigned*>(p[t] + off);
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 2) x[t][e] = __builtin_amdgcn_raw_buffer_load_b16(r, at[t][e], 0, 0);
+        else x[t][e] = __builtin_amdgcn_raw_buffer_load_b32(r, at[t][e], 0, 0);
       }
-    }
   }
-  __device__ __forceinline__ f32x4 get(int t, int valid) const {
+  __device__ __forceinline__ f32x4 get(int t) const {
     f32x4 r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = in[t] && ib + e < valid ? __uint_as_float(sizeof(T) == 2 ? x[t][e] << 16 : x[t][e]) : 0.f;
+    for (int e = 0; e < 4; ++e) r[e] = __uint_as_float(sizeof(T) == 2 ? x[t][e] << 16 : x[t][e]);
     return r;
   }
 };
-__device__ __forceinline__ f32x4 rows_below(const f32x4& x, int ib, int valid) {
-  f32x4 r;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) r[e] = ib + e < valid ? x[e] : 0.f;
-  return r;
-}
-// a result tile of o or dv into the caller's rows.  Without conditions too: what is waited for later (loads and stores come
-// back in order) is counted from the instructions on every path.  Elements that are nobody's go to a corner of ws.
+// a result tile of o or dv into the caller's rows
 template <typename T, int NT>
-__device__ __forceinline__ void store_cols(void* dst, long ld, long row0, int valid, int hv, int V, int v0, int ib, int lr, const f32x4 (&x)[NT], float* nobody) {
-  T* const p = static_cast<T*>(dst) + (row0 + ib) * ld + (long)hv * V + v0 + lr;
-  T* const trash = reinterpret_cast<T*>(nobody) + lr;
+struct ColOut : ColPtr<T, NT> {
+  using ColPtr<T, NT>::ColPtr;
+  __device__ __forceinline__ void store(int c, const f32x4 (&y)[NT]) const {
+    const __amdgpu_buffer_rsrc_t r = this->chunk(c);
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      T* const q = ib + e < valid && v0 + 16 * t + lr < V ? p + e * ld + 16 * t : trash;
-      *q = (T)x[t][e];
-    }
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)y[t][e]), r, this->at[t][e], 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y[t][e]), r, this->at[t][e], 0, 0);
+      }
+  }
+};
+template <int NP, int KB2>
+__device__ __forceinline__ void load_kt(bf16x8 (&f)[KB2][2][NP], const __bf16* base, unsigned at) {
+#pragma unroll
+  for (int t = 0; t < KB2; ++t)
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int p = 0; p < NP; ++p) f[t][kb][p] = *reinterpret_cast<const bf16x8*>(base + (at + (16 * t * NP + p) * kC + 32 * kb));
 }
 // the state tile of a scan's chain wave w: rows 16*(KB2*w + t) + 4*lg + e, columns v0 + 16*u + lr
 template <int KB2, int NT>
@@ -446,9 +468,13 @@ struct ScanVec {
 // the two 32-wide halves of a row of M, P or a transpose.  Half `f` of a wave whose rows do not reach it reads the other
 // one again (from the first-level cache): a request under a condition would be waited for at once.
 template <int N>
-__device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* row, bool low, bool high) {
-  sb::load_frag<N>(f[0], row + (low ? 0 : 32), kC);
-  sb::load_frag<N>(f[1], row + (high ? 32 : 0), kC);
+__device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* base, unsigned lane_at, bool low, bool high) {
+  const unsigned at0 = lane_at + (low ? 0 : 32), at1 = lane_at + (high ? 32 : 0);
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    f[0][q] = *reinterpret_cast<const bf16x8*>(base + (at0 + q * kC));
+    f[1][q] = *reinterpret_cast<const bf16x8*>(base + (at1 + q * kC));
+  }
 }
 
 // A scan is bound by its chain: state -> K S -> W -> state, chunk after chunk, and inside it by the instructions its waves
@@ -488,21 +514,16 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
       ColPtr<T, NT> vp(a.v, a.ldv, start, len, hv, a.V, v0, lr, ib);
       ScanVec vn;
       const float* vecp = a.vec + (slot0 * a.Hv + hv) * kVecs * kC;
-      const __bf16* mp = a.m + ((slot0 * a.Hv + hv) * kC + ia) * 3 * kC + 8 * lg;
-      const __bf16* ktp = a.kt + ((slot0 * a.Hk + hk) * Kp + 16 * KB2 * w + lr) * NP * kC + 8 * lg;
-      auto load_kt = [&]() {
-#pragma unroll
-        for (int t = 0; t < KB2; ++t)
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb) sb::load_frag<NP>(ktf[t][kb], ktp + 16 * t * NP * kC + 32 * kb, kC);
-      };
+      const __bf16* mp = a.m + (slot0 * a.Hv + hv) * 3 * kC * kC;
+      const __bf16* ktp = a.kt + (slot0 * a.Hk + hk) * Kp * NP * kC;
+      const unsigned mat = ia * 3 * kC + 8 * lg, ktat = (16 * KB2 * w + lr) * NP * kC + 8 * lg;
       kp.load(kf, 0);
       vp.load(0);
       vn.load(vecp, ib);
-      load_tri<3>(mf, mp, true, high);
-      load_kt();
+      load_tri<3>(mf, mp, mat, true, high);
+      load_kt<NP, KB2>(ktf, ktp, ktat);
       for (int c = 0; c < nc; ++c) {
-        const int valid = min(kC, len - c * kC), next = min(c + 1, nc - 1);
+        const int next = min(c + 1, nc - 1);
         const long adv = next - c;                         // 0 behind the last chunk: its operands are read again, to no use
         vecp += adv * a.Hv * kVecs * kC;
         mp += adv * a.Hv * 3 * kC * kC;
@@ -529,17 +550,18 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
         const ScanVec vc = vn;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-          sb::split_store4<3>(xl + (16 * t + lr) * kLdT + ib, VT * kLdT, rows_below(vc.beta * (vp.get(t, valid) - vc.gam * ks[t]), ib, valid));
+          sb::split_store4<3>(xl + (16 * t + lr) * kLdT + ib, VT * kLdT, vc.beta * (vp.get(t) - vc.gam * ks[t]));
         vp.load(next);
         vn.load(vecp, ib);
         if constexpr (TRAIN) {
-          float* const sp = a.s + (vs * Kp + 16 * KB2 * w + 4 * lg) * a.vp + v0 + lr;
+          float* const sp = a.s + ((vs * (a.vp / 32) + v0 / 32) * Kp) * 32 + (v0 & 16);
+          const unsigned at = (16 * KB2 * w + 4 * lg) * 32 + lr;
 #pragma unroll
           for (int t = 0; t < KB2; ++t)
 #pragma unroll
             for (int u = 0; u < NT; ++u)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) sp[(16 * t + e) * a.vp + 16 * u] = S[t][u][e];
+              for (int e = 0; e < 4; ++e) sp[at + (16 * t + e) * 32 + 16 * u] = S[t][u][e];
         }
         lds_barrier();
         f32x4 wt[NT];
@@ -554,7 +576,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
               sb::load_frag<3>(b, xl + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
               sb::mma<3, 3>(wt[t], mf[kb], b);
             }
-        load_tri<3>(mf, mp, true, high);
+        load_tri<3>(mf, mp, mat, true, high);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           sb::split_store4<3>(ul + (16 * t + lr) * kLdT + ib, VT * kLdT, vc.tail * wt[t]);
@@ -574,54 +596,59 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
 #pragma unroll
             for (int t = 0; t < KB2; ++t) sb::mma<NP, 3>(S[t][u], ktf[t][kb], b);
           }
-        load_kt();
+        load_kt<NP, KB2>(ktf, ktp, ktat);
       }
     }
     if (a.s1) store_state<KB2, NT>(S, a.s1, a, nh, w, v0, lr, lg);
   } else if (nc > 0) {                                     // ---- the output, between the chain's barriers
+    // Chunk c: Q S behind barrier 1, the first half of P W behind barrier 3, the second behind the next chunk's barrier 2,
+    // the store behind its barrier 1 after that: no stretch between two barriers is longer than the chain's.
     bf16x8 qf[KB][NP], pf[2][NO];
-    f32x4 qs[NT], qn[NT];
+    f32x4 qn[NT], qs[NT], qo[NT];
     const RowPtr<NP, KB> qp(a, a.q, a.ldq, a.qpk, slot0, hk, start, len, ia, lg);
-    const __bf16* pp = a.p + ((slot0 * a.Hv + hv) * kC + ia) * 3 * kC + 8 * lg;
-    const float* gp = a.vec + (slot0 * a.Hv + hv) * kVecs * kC + kGam * kC + ib;
-    // o of chunk c from qs = gam (Q S) and W, which the chain has left in wl
-    auto finish = [&](int c) {
-      const long vs = (slot0 + c) * a.Hv + hv;
+    const __bf16* pp = a.p + (slot0 * a.Hv + hv) * 3 * kC * kC;
+    const unsigned pat = ia * 3 * kC + 8 * lg;
+    ColOut<T, NT> op(a.o, a.ldo, start, len, hv, a.V, v0, lr, ib);
+    const float* gp = a.vec + (slot0 * a.Hv + hv) * kVecs * kC + kGam * kC;
+    auto pw = [&](int c, int kb) {                         // qs += P W, columns 32*kb of P; W as the chain left it in wl
       const float* const wc = wl + (c & 1) * L::F;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        if (kb == 0 || high)
+      for (int t = 0; t < NT; ++t) {
+        float x[8];
+        const float* const src = wc + (16 * t + lr) * kLdM + 32 * kb + 8 * lg;
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            float x[8];
-            const float* const src = wc + (16 * t + lr) * kLdM + 32 * kb + 8 * lg;
+        for (int h = 0; h < 2; ++h) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(src + 4 * h);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const f32x4 y = *reinterpret_cast<const f32x4*>(src + 4 * h);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[4 * h + e] = y[e];
-            }
-            bf16x8 b[NO];
-            sb::split8<NO>(x, b);
-            sb::mma<NO, NO>(qs[t], pf[kb], b);
-          }
+          for (int e = 0; e < 4; ++e) x[4 * h + e] = y[e];
+        }
+        bf16x8 b[NO];
+        sb::split8<NO>(x, b);
+        sb::mma<NO, NO>(qs[t], pf[kb], b);
+      }
+    };
+    auto second = [&](int c) {                             // the second half, and W for the backward pass
+      if (high) pw(c, 1);
+      load_tri<NO>(pf, pp, pat, true, high);
+      pp += c + 2 < nc ? (long)a.Hv * 3 * kC * kC : 0;
       if constexpr (TRAIN) {
-        float* const wp = a.w + (vs * kC + ib) * a.vp + v0 + lr;
+        float* const wp = a.w + ((((slot0 + c) * a.Hv + hv) * (a.vp / 32) + v0 / 32) * kC) * 32 + (v0 & 16);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(wc + (16 * t + lr) * kLdM + ib);
+          const f32x4 y = *reinterpret_cast<const f32x4*>(wl + (c & 1) * L::F + (16 * t + lr) * kLdM + ib);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) wp[e * a.vp + 16 * t] = y[e];
+          for (int e = 0; e < 4; ++e) wp[(unsigned)(ib * 32 + lr) + e * 32 + 16 * t] = y[e];
         }
       }
 #pragma unroll
-      for (int t = 0; t < NT; ++t) qs[t] *= a.scale;
-      store_cols<T, NT>(a.o, a.ldo, start + (long)c * kC, min(kC, len - c * kC), hv, a.V, v0, ib, lr, qs, a.nobody);
+      for (int t = 0; t < NT; ++t) qo[t] = qs[t] * a.scale;
     };
+    auto store = [&](int c) { op.store(c, qo); };
     qp.load(qf, 0);
+    load_tri<NO>(pf, pp, pat, true, high);
+    pp += nc > 1 ? (long)a.Hv * 3 * kC * kC : 0;
+    f32x4 gam = *reinterpret_cast<const f32x4*>(gp + (unsigned)ib);
     for (int c = 0; c < nc; ++c) {
-      const f32x4 gam = *reinterpret_cast<const f32x4*>(gp);
-      gp += (long)a.Hv * kVecs * kC;
       lds_barrier();
 #pragma unroll
       for (int t = 0; t < NT; ++t) qn[t] = zero;
@@ -634,15 +661,19 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
           sb::mma<NP, NO>(qn[t], qf[kb], b);
         }
       qp.load(qf, min(c + 1, nc - 1));
+      if (c > 1) store(c - 2);
       lds_barrier();
-      if (c > 0) finish(c - 1);
-      load_tri<NO>(pf, pp, true, high);
-      pp += (long)a.Hv * 3 * kC * kC;
+      if (c > 0) second(c - 1);
 #pragma unroll
       for (int t = 0; t < NT; ++t) qs[t] = qn[t] * gam;
+      gp += c + 1 < nc ? (long)a.Hv * kVecs * kC : 0;
+      gam = *reinterpret_cast<const f32x4*>(gp + (unsigned)ib);
       lds_barrier();
+      pw(c, 0);
     }
-    finish(nc - 1);
+    if (nc > 1) store(nc - 2);
+    second(nc - 1);
+    store(nc - 1);
   }
 }
 
@@ -681,29 +712,26 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
       const RowPtr<NP, KB> kp(a, a.k, a.ldk, a.kpk, slot0, hk, start, len, ia, lg);
       ScanVec vn;
       const float* vecp = a.vec + (slot1 * a.Hv + hv) * kVecs * kC;
-      const __bf16* mp = a.mt + ((slot1 * a.Hv + hv) * kC + ia) * 3 * kC + 8 * lg;
-      long tp = ((slot1 * a.Hk + hk) * Kp + 16 * KB2 * w + lr) * NP * kC + 8 * lg;
+      const __bf16* mp = a.mt + (slot1 * a.Hv + hv) * 3 * kC * kC;
+      const __bf16 *ktp = a.kt + (slot1 * a.Hk + hk) * Kp * NP * kC, *qtp = a.qt + (slot1 * a.Hk + hk) * Kp * NP * kC;
+      const unsigned mat = ia * 3 * kC + 8 * lg, ktat = (16 * KB2 * w + lr) * NP * kC + 8 * lg;
       auto load_t = [&]() {
-#pragma unroll
-        for (int t = 0; t < KB2; ++t)
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            sb::load_frag<NP>(qtf[t][kb], a.qt + tp + 16 * t * NP * kC + 32 * kb, kC);
-            sb::load_frag<NP>(ktf[t][kb], a.kt + tp + 16 * t * NP * kC + 32 * kb, kC);
-          }
+        load_kt<NP, KB2>(qtf, qtp, ktat);
+        load_kt<NP, KB2>(ktf, ktp, ktat);
       };
       kp.load(kf, nc - 1);
       vn.load(vecp, ib);
-      load_tri<3>(mf, mp, low, true);
+      load_tri<3>(mf, mp, mat, low, true);
       load_t();
       lds_barrier();
       lds_barrier();
       for (int c = nc - 1; c >= 0; --c) {
-        const int valid = min(kC, len - c * kC), next = max(c - 1, 0);
+        const int next = max(c - 1, 0);
         const long adv = c - next;
         vecp -= adv * a.Hv * kVecs * kC;
         mp -= adv * a.Hv * 3 * kC * kC;
-        tp -= adv * a.Hk * NP * Kp * kC;
+        ktp -= adv * a.Hk * NP * Kp * kC;
+        qtp -= adv * a.Hk * NP * Kp * kC;
         const ScanVec vc = vn;
         const long vs = (slot0 + c) * a.Hv + hv;
 #pragma unroll
@@ -727,16 +755,17 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const f32x4 p = *reinterpret_cast<const f32x4*>(zp + (16 * t + lr) * kLdM + ib);
-          sb::split_store4<3>(zl + (16 * t + lr) * kLdT + ib, VT * kLdT, rows_below(p + vc.tail * z[t], ib, valid));
+          sb::split_store4<3>(zl + (16 * t + lr) * kLdT + ib, VT * kLdT, p + vc.tail * z[t]);
         }
         vn.load(vecp, ib);
-        float* const sp = a.ds + (vs * Kp + 16 * KB2 * w + 4 * lg) * a.vp + v0 + lr;
+        float* const sp = a.ds + ((vs * (a.vp / 32) + v0 / 32) * Kp) * 32 + (v0 & 16);
+        const unsigned at = (16 * KB2 * w + 4 * lg) * 32 + lr;
 #pragma unroll
         for (int t = 0; t < KB2; ++t)
 #pragma unroll
           for (int u = 0; u < NT; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sp[(16 * t + e) * a.vp + 16 * u] = dS[t][u][e];
+            for (int e = 0; e < 4; ++e) sp[at + (16 * t + e) * 32 + 16 * u] = dS[t][u][e];
         lds_barrier();
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -747,7 +776,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
               sb::load_frag<3>(b, zl + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
               sb::mma<3, 3>(y[t], mf[kb], b);
             }
-        load_tri<3>(mf, mp, low, true);
+        load_tri<3>(mf, mp, mat, low, true);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           sb::split_store4<3>(yl + (16 * t + lr) * kLdT + ib, VT * kLdT, -vc.gam * vc.beta * y[t]);
@@ -778,9 +807,11 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
   } else if (nc > 0) {                                     // ---- dO's share, ahead of the chain; Y and dV, behind it
     bf16x8 pf[2][3];
     const bool has_do = a.d_o != nullptr;
-    ColPtr<T, NT> dp(has_do ? a.d_o : a.v, has_do ? a.lddo : a.ldv, start, len, hv, a.V, v0, lr, ib);
-    const __bf16* const pt = a.pt + ((slot0 * a.Hv + hv) * kC + ia) * 3 * kC + 8 * lg;
-    const float* const vec = a.vec + (slot0 * a.Hv + hv) * kVecs * kC + ib;
+    ColPtr<T, NT> dp(has_do ? a.d_o : a.v, has_do ? a.lddo : a.ldv, start, len, hv, has_do ? a.V : 0, v0, lr, ib);
+    const __bf16* const pt = a.pt + (slot0 * a.Hv + hv) * 3 * kC * kC;
+    const unsigned pat = ia * 3 * kC + 8 * lg;
+    ColOut<T, NT> vo(a.dv, a.lddv, start, len, hv, a.V, v0, lr, ib);
+    const float* const vec = a.vec + (slot0 * a.Hv + hv) * kVecs * kC;
     const long pstep = (long)a.Hv * 3 * kC * kC, vstep = (long)a.Hv * kVecs * kC;
     f32x4 d[NT], dn[NT];                                   // dO of the chunk at hand and of the next one
     auto share = [&]() {                                   // zp of the chunk whose dO is in ol and whose P^T is in pf
@@ -800,36 +831,36 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
       for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(zp + (16 * t + lr) * kLdM + ib) = a.scale * z[t];
     };
     dp.load(nc - 1);
-    load_tri<3>(pf, pt + (nc - 1) * pstep, low, true);
+    load_tri<3>(pf, pt + (nc - 1) * pstep, pat, low, true);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      dn[t] = dp.get(t, has_do ? len - (nc - 1) * kC : 0);
+      dn[t] = dp.get(t);
       sb::split_store4<NP>(ol + (16 * t + lr) * kLdT + ib, VT * kLdT, dn[t]);
     }
     dp.load(max(nc - 2, 0));
     lds_barrier();
     share();
-    load_tri<3>(pf, pt + max(nc - 2, 0) * pstep, low, true);
+    load_tri<3>(pf, pt + max(nc - 2, 0) * pstep, pat, low, true);
     lds_barrier();
     // Y and dV of chunk c, which the chain has left in yf
     auto finish = [&](int c, const f32x4& beta) {
-      float* const yp = a.y + (((slot0 + c) * a.Hv + hv) * kC + ib) * a.vp + v0 + lr;
+      float* const yp = a.y + ((((slot0 + c) * a.Hv + hv) * (a.vp / 32) + v0 / 32) * kC) * 32 + (v0 & 16);
       f32x4 y[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         y[t] = *reinterpret_cast<const f32x4*>(yf + (c & 1) * L::F + (16 * t + lr) * kLdM + ib);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) yp[e * a.vp + 16 * t] = y[t][e];
+        for (int e = 0; e < 4; ++e) yp[(unsigned)(ib * 32 + lr) + e * 32 + 16 * t] = y[t][e];
         y[t] *= beta;
       }
-      store_cols<T, NT>(a.dv, a.lddv, start + (long)c * kC, min(kC, len - c * kC), hv, a.V, v0, ib, lr, y, a.nobody);
+      vo.store(c, y);
     };
-    f32x4 gam = *reinterpret_cast<const f32x4*>(vec + (nc - 1) * vstep + kGam * kC), beta = *reinterpret_cast<const f32x4*>(vec + (nc - 1) * vstep + kBeta * kC);
+    f32x4 gam = *reinterpret_cast<const f32x4*>(vec + (nc - 1) * vstep + kGam * kC + (unsigned)ib), beta = *reinterpret_cast<const f32x4*>(vec + (nc - 1) * vstep + kBeta * kC + (unsigned)ib);
     f32x4 before = zero;                                   // beta of the chunk behind
     for (int c = nc - 1; c >= 0; --c) {
       const int next = max(c - 1, 0), next2 = max(c - 2, 0);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) { d[t] = dn[t]; dn[t] = dp.get(t, has_do ? min(kC, len - next * kC) : 0); }
+      for (int t = 0; t < NT; ++t) { d[t] = dn[t]; dn[t] = dp.get(t); }
       dp.load(next2);
       lds_barrier();                                       // 1: the chain has read the previous chunk's gl
 #pragma unroll
@@ -837,13 +868,13 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
         sb::split_store4<3>(gl + (16 * t + lr) * kLdT + ib, VT * kLdT, a.scale * gam * d[t]);
         sb::split_store4<NP>(ol + (16 * t + lr) * kLdT + ib, VT * kLdT, dn[t]);
       }
-      gam = *reinterpret_cast<const f32x4*>(vec + next * vstep + kGam * kC);
+      gam = *reinterpret_cast<const f32x4*>(vec + next * vstep + kGam * kC + (unsigned)ib);
       lds_barrier();                                       // 2: the chain has read zp
       share();
-      load_tri<3>(pf, pt + next2 * pstep, low, true);
+      load_tri<3>(pf, pt + next2 * pstep, pat, low, true);
       if (c < nc - 1) finish(c + 1, before);
       before = beta;
-      beta = *reinterpret_cast<const f32x4*>(vec + next * vstep + kBeta * kC);
+      beta = *reinterpret_cast<const f32x4*>(vec + next * vstep + kBeta * kC + (unsigned)ib);
       lds_barrier();                                       // 3
     }
     finish(0, before);
@@ -933,9 +964,9 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
     for (int t = 0; t < 2; ++t) dp[t] = da[t] = zero;
     float sdot = 0.f, ydot = 0.f;
     const bool has_s = KB2 == 2 || tid < 256;
-    const float* const ps = a.s + (vs * Kp + (tid >> 2) % Kp) * a.vp + gc;
-    const float* const pd = a.ds + (vs * Kp + (tid >> 2) % Kp) * a.vp + gc;
-    const float* const pw = (tid < 256 ? a.w : a.y) + (vs * kC + gi) * a.vp + gc;
+    const float* const ps = a.s + (vs * (a.vp / 32) * Kp + (tid >> 2) % Kp) * 32 + gc;
+    const float* const pd = a.ds + (vs * (a.vp / 32) * Kp + (tid >> 2) % Kp) * 32 + gc;
+    const float* const pw = (tid < 256 ? a.w : a.y) + (vs * (a.vp / 32) * kC + gi) * 32 + gc;
     const T* const px = tid < 256 ? (has_do ? static_cast<const T*>(a.d_o) + rowc * a.lddo + (long)hv * a.V : static_cast<const T*>(a.v))
                                   : static_cast<const T*>(a.v) + rowc * a.ldv + (long)hv * a.V;
     f32x4 xs[2], xd[2], xw[2];
@@ -943,9 +974,9 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
     auto request = [&](int vb) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        xs[h] = *reinterpret_cast<const f32x4*>(ps + vb + 4 * h);
-        xd[h] = *reinterpret_cast<const f32x4*>(pd + vb + 4 * h);
-        xw[h] = *reinterpret_cast<const f32x4*>(pw + vb + 4 * h);
+        xs[h] = *reinterpret_cast<const f32x4*>(ps + vb * Kp + 4 * h);
+        xd[h] = *reinterpret_cast<const f32x4*>(pd + vb * Kp + 4 * h);
+        xw[h] = *reinterpret_cast<const f32x4*>(pw + vb * kC + 4 * h);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -1316,7 +1347,6 @@ long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, 
   t.m = take16(ns * Hv * 3 * kC * kC);
   t.p = take16(ns * Hv * 3 * kC * kC);
   t.vec = take(ns * Hv * kVecs * kC);
-  t.nobody = take(64);
   if (train) {
     t.qt = take16(ns * Hk * np * kC * kp);
     t.mt = take16(ns * Hv * 3 * kC * kC);
@@ -1328,7 +1358,7 @@ long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, 
   }
   if (a) {
     a->kpk = t.kpk; a->qpk = t.qpk; a->kt = t.kt; a->qt = t.qt; a->m = t.m; a->p = t.p; a->mt = t.mt; a->pt = t.pt;
-    a->vec = t.vec; a->w = t.w; a->y = t.y; a->s = t.s; a->ds = t.ds; a->nobody = t.nobody;
+    a->vec = t.vec; a->w = t.w; a->y = t.y; a->s = t.s; a->ds = t.ds;
     a->n_slots = ns; a->vp = (int)vp;
   }
   return off;
@@ -1347,6 +1377,8 @@ int gdr_check(const hhrl_gdr_desc* d, const char* who) {
   HHRL_REQUIRE(d->q && d->k && d->v && d->g && d->beta, "%s: null input", who);
   HHRL_REQUIRE(d->ldq >= (long)d->Hk * d->K && d->ldk >= (long)d->Hk * d->K && d->ldv >= (long)d->Hv * d->V && d->ldg >= d->Hv && d->ldbeta >= d->Hv,
                "%s: leading dimension of an input too small", who);
+  const long most = 1L << 22;                    // offsets inside a chunk are 31-bit byte numbers
+  HHRL_REQUIRE(d->ldq < most && d->ldk < most && d->ldv < most, "%s: leading dimension of an input beyond %ld", who, most - 1);
   const long ns = slots_of(d->n_seq, d->rows, d->starts != nullptr);
   HHRL_REQUIRE(ns < (1L << 31), "%s: %ld chunks", who, ns);
   const long blocks = ((long)d->n_seq * d->Hv + 7) / 8 * 8 * ((d->V + 31) / 32 * 2);
@@ -1453,6 +1485,7 @@ long hhrl_gdr_workspace_floats(int dtype, int n_seq, long rows, int packed, int 
 int hhrl_gdr_forward(const hhrl_gdr_desc* d, void* stream) {
   HHRL_TRY(gdr_check(d, "gdr_forward"));
   HHRL_REQUIRE(d->o && d->ldo >= (long)d->Hv * d->V, "gdr_forward: o null or ldo=%ld too small", d->ldo);
+  HHRL_REQUIRE(d->ldo < (1L << 22), "gdr_forward: ldo=%ld too large", d->ldo);
   GdrArgs a = {};
   HHRL_TRY(gdr_fill(d, a, !d->no_backward, "gdr_forward"));
   a.o = d->o; a.ldo = d->ldo; a.s0 = d->s0; a.s1 = d->s1;
@@ -1468,6 +1501,7 @@ int hhrl_gdr_backward(const hhrl_gdr_desc* d, void* stream) {
   HHRL_REQUIRE(d->dq && d->dk && d->dv && d->dg && d->dbeta, "gdr_backward: null gradient");
   HHRL_REQUIRE((!d->d_o || d->lddo >= (long)d->Hv * d->V) && d->lddq >= (long)d->Hk * d->K && d->lddk >= (long)d->Hk * d->K && d->lddv >= (long)d->Hv * d->V &&
                d->lddg >= d->Hv && d->lddbeta >= d->Hv, "gdr_backward: leading dimension of a gradient too small");
+  HHRL_REQUIRE((!d->d_o || d->lddo < (1L << 22)) && d->lddv < (1L << 22), "gdr_backward: leading dimension of d_o or dv too large");
   GdrArgs a = {};
   HHRL_TRY(gdr_fill(d, a, true, "gdr_backward"));
   a.d_o = d->d_o; a.lddo = d->lddo; a.d_s1 = d->d_s1; a.d_s0 = d->d_s0;

@@ -19,7 +19,27 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// x = h + m + l up to 2^-27 |x|; each term rounded to nearest even, so the remainders are exact in fp32
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// two numbers rounded to bf16 (to nearest even), the first in the low half
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const f32x2 v = {a, b};
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+}
+// x = h + m + l up to 2^-27 |x|; each term rounded to nearest even, so the remainders are exact in fp32.  Two numbers at a
+// time (one conversion instruction packs a pair): 11 instructions, 15 one by one.
+template <int N>
+__device__ __forceinline__ void split2(float a, float b, unsigned (&t)[N]) {
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    t[q] = pack2(a, b);
+    if (q + 1 < N) {
+      a -= __uint_as_float(t[q] << 16);
+      b -= __uint_as_float(t[q] & 0xffff0000u);
+    }
+  }
+}
 __device__ __forceinline__ void split3(float x, __bf16& h, __bf16& m, __bf16& l) {
   h = (__bf16)x;
   const float r = x - (float)h;
@@ -30,26 +50,25 @@ __device__ __forceinline__ void split3(float x, __bf16& h, __bf16& m, __bf16& l)
 // N terms of x at p[0], p[stride], ...
 template <int N>
 __device__ __forceinline__ void split_store4(__bf16* p, int stride, const f32x4& x) {
-  bf16x4 t[3];
+  unsigned a[N], b[N];
+  split2<N>(x[0], x[1], a);
+  split2<N>(x[2], x[3], b);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    __bf16 h, m, l;
-    split3(x[e], h, m, l);
-    t[0][e] = h; t[1][e] = m; t[2][e] = l;
-  }
-#pragma unroll
-  for (int q = 0; q < N; ++q) *reinterpret_cast<bf16x4*>(p + q * stride) = t[q];
+  for (int q = 0; q < N; ++q) *reinterpret_cast<uint2*>(p + q * stride) = make_uint2(a[q], b[q]);
 }
 template <int N>
 __device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&t)[N]) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 r[N];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    __bf16 h, m, l;
-    split3(x[e], h, m, l);
-    t[0][e] = h;
-    if constexpr (N > 1) t[1][e] = m;
-    if constexpr (N > 2) t[2][e] = l;
+  for (int e = 0; e < 4; ++e) {
+    unsigned a[N];
+    split2<N>(x[2 * e], x[2 * e + 1], a);
+#pragma unroll
+    for (int q = 0; q < N; ++q) r[q][e] = a[q];
   }
+#pragma unroll
+  for (int q = 0; q < N; ++q) t[q] = __builtin_bit_cast(bf16x8, r[q]);
 }
 
 // acc += A B from NA and NB terms: the partial products whose weights add up to less than the longer operand's length
