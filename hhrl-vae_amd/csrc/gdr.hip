@@ -468,13 +468,14 @@ struct ScanVec {
 // the two 32-wide halves of a row of M, P or a transpose.  Half `f` of a wave whose rows do not reach it reads the other
 // one again (from the first-level cache): a request under a condition would be waited for at once.
 template <int N>
-__device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* base, unsigned lane_at, bool low, bool high) {
-  const unsigned at0 = lane_at + (low ? 0 : 32), at1 = lane_at + (high ? 32 : 0);
+__device__ __forceinline__ void load_half(bf16x8 (&f)[N], const __bf16* base, unsigned at) {
 #pragma unroll
-  for (int q = 0; q < N; ++q) {
-    f[0][q] = *reinterpret_cast<const bf16x8*>(base + (at0 + q * kC));
-    f[1][q] = *reinterpret_cast<const bf16x8*>(base + (at1 + q * kC));
-  }
+  for (int q = 0; q < N; ++q) f[q] = *reinterpret_cast<const bf16x8*>(base + (at + q * kC));
+}
+template <int N>
+__device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* base, unsigned at, bool low, bool high) {
+  load_half<N>(f[0], base, at + (low ? 0 : 32));
+  load_half<N>(f[1], base, at + (high ? 32 : 0));
 }
 
 // A scan is bound by its chain: state -> K S -> W -> state, chunk after chunk, and inside it by the instructions its waves
@@ -606,7 +607,8 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
     bf16x8 qf[KB][NP], pf[2][NO];
     f32x4 qn[NT], qs[NT], qo[NT];
     const RowPtr<NP, KB> qp(a, a.q, a.ldq, a.qpk, slot0, hk, start, len, ia, lg);
-    const __bf16* pp = a.p + (slot0 * a.Hv + hv) * 3 * kC * kC;
+    const __bf16* const pp = a.p + (slot0 * a.Hv + hv) * 3 * kC * kC;
+    const long pstep = (long)a.Hv * 3 * kC * kC;
     const unsigned pat = ia * 3 * kC + 8 * lg;
     ColOut<T, NT> op(a.o, a.ldo, start, len, hv, a.V, v0, lr, ib);
     const float* gp = a.vec + (slot0 * a.Hv + hv) * kVecs * kC + kGam * kC;
@@ -629,8 +631,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
     };
     auto second = [&](int c) {                             // the second half, and W for the backward pass
       if (high) pw(c, 1);
-      load_tri<NO>(pf, pp, pat, true, high);
-      pp += c + 2 < nc ? (long)a.Hv * 3 * kC * kC : 0;
+      load_half<NO>(pf[1], pp + min(c + 1, nc - 1) * pstep, pat + (high ? 32 : 0));
       if constexpr (TRAIN) {
         float* const wp = a.w + ((((slot0 + c) * a.Hv + hv) * (a.vp / 32) + v0 / 32) * kC) * 32 + (v0 & 16);
 #pragma unroll
@@ -646,7 +647,6 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
     auto store = [&](int c) { op.store(c, qo); };
     qp.load(qf, 0);
     load_tri<NO>(pf, pp, pat, true, high);
-    pp += nc > 1 ? (long)a.Hv * 3 * kC * kC : 0;
     f32x4 gam = *reinterpret_cast<const f32x4*>(gp + (unsigned)ib);
     for (int c = 0; c < nc; ++c) {
       lds_barrier();
@@ -670,6 +670,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
       gam = *reinterpret_cast<const f32x4*>(gp + (unsigned)ib);
       lds_barrier();
       pw(c, 0);
+      load_half<NO>(pf[0], pp + min(c + 1, nc - 1) * pstep, pat);
     }
     if (nc > 1) store(nc - 2);
     second(nc - 1);
