@@ -62,15 +62,18 @@ struct GdrArgs {
   long lddq, lddk, lddv;
   float *dg, *dbeta;
   long lddg, lddbeta;
-  int pack, train, vp, nvt;
+  int pack, wide, train, vp, nvt;
   // ws, per chunk and key head: k, q [64][terms][Kp] (pack), their transposes [Kp][terms][64];
-  //     per chunk and value head: M, P and their transposes [64][terms][64], five rows of 64 floats, and for the
+  //     per chunk and value head: M, P (two terms for bf16: what o takes) and their transposes [64][terms][64], five rows of 64 floats, and for the
   //     backward pass W, Y [vp/32][64][32] and S, dS [vp/32][Kp][32], fp32 (tiles of 32 columns).  The terms of a row lie side by side, so that a lane's
   //     fragments are at constant offsets from one address.
   __bf16 *kpk, *qpk, *kt, *qt, *m, *p, *mt, *pt;
   float *vec, *w, *y, *s, *ds;
 };
 enum { kGam = 0, kTail = 1, kBeta = 2, kGHi = 3, kGLo = 4, kVecs = 5 };
+
+// exp(x) for x <= 0, to 2^-24 |x| of itself, so to 2^-25 of the largest decay, 1 (the exponential instruction is base two)
+__device__ __forceinline__ float decay(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 
 __device__ __forceinline__ long clampl(long v, long lo, long hi) { return v < lo ? lo : v > hi ? hi : v; }
 
@@ -109,22 +112,41 @@ __device__ __forceinline__ void slot_chunk(const GdrArgs& a, long slot, long& ro
   valid = at < 0 || at >= len ? 0 : (int)min((long)kC, len - at);
 }
 
+// Rows of the caller's tensors go through buffer descriptors: a base that moves from chunk to chunk in scalar registers, a
+// lane's offset that never changes, and the size of what the sequence has left, behind which a load gives 0 and a store is
+// dropped.  So rows behind the sequence need no test, no request has a condition (a conditional one would be waited for
+// where its branch joins), and a chunk costs no address arithmetic on the vector unit.
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+constexpr unsigned kNoColumn = 0x80000000u;      // an offset behind every size
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, long offset, long bytes) {
+  // (descriptor word 3: 32-bit data, no swizzle)
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base)) + offset, 0, (int)bytes, 0x00027000);
+}
 // ------------------------------------------------------------------------------------------------------------ prep
 // One workgroup per chunk and key head: k k^T and q k^T once, then per value head of the key head the decays, the
 // triangular inverse and P.  The inverse goes by blocks: 16 x 16 on the diagonal by substitution (a lane per column), then
-// the blocks below them, 16 and 32 wide, as -M22 (L21 M11) on the fp32 matrix instruction.
+// the blocks below them, 16 and 32 wide, as -M22 (L21 M11) on the fp32 matrix instruction.  P is written straight from the
+// registers of a product: four elements of a row from k q^T, of a column (for the transpose) from q k^T.  The 32 x 32
+// blocks beyond the diagonal are neither written nor read.
+template <int NP, int KB2>
+struct PrepLds {
+  static constexpr int Kp = 64 * KB2, LDK = Kp + 8;
+  static constexpr int kq = 2 * NP * kC * LDK * 2;             // bytes: k and q as terms
+  static constexpr int img = (2 * kC + 32) * kLdM * 4;         // I + A, its inverse, a product of the solve: over them once they are used
+  static constexpr int over = kq > img ? kq : img;
+  static constexpr int bytes = over + 3 * kC * 4;
+};
 template <typename T, int NP, int KB2>
-__global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
-  constexpr int Kp = 64 * KB2, LDK = Kp + 8, KG = Kp / 8;
+__global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs a) {
+  using L = PrepLds<NP, KB2>;
+  constexpr int Kp = L::Kp, LDK = L::LDK, KG = Kp / 8, NO = NP == 1 ? 2 : 3;
   extern __shared__ __align__(16) char smem[];
   __bf16* const kl = reinterpret_cast<__bf16*>(smem);          // [NP][64][LDK]
   __bf16* const ql = kl + NP * kC * LDK;
-  float* const pm = reinterpret_cast<float*>(smem);            // over kl, once the products are done: P, products of the solve
-  float* const tm = pm + kC * kLdM;
-  constexpr int kOver = 2 * NP * kC * LDK * 2 > 2 * kC * kLdM * 4 ? 2 * NP * kC * LDK * 2 : 2 * kC * kLdM * 4;
-  float* const lm = reinterpret_cast<float*>(smem + kOver);    // [64][kLdM] I + A
+  float* const lm = reinterpret_cast<float*>(smem);            // [64][kLdM] I + A
   float* const mm = lm + kC * kLdM;                            // [64][kLdM] its inverse
-  float* const gh = mm + kC * kLdM;
+  float* const tm = mm + kC * kLdM;                            // [32][kLdM]
+  float* const gh = reinterpret_cast<float*>(smem + L::over);
   float* const gl = gh + kC;
   float* const be = gl + kC;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
@@ -137,50 +159,85 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
   const long hs = slot * a.Hk + hk;
 
   // k and q as bf16 terms; what lies beyond the sequence or the head's width becomes 0 and is not read
-  for (int side = 0; side < 2; ++side) {
-    const T* src = static_cast<const T*>(side ? a.q : a.k) + row0 * (side ? a.ldq : a.ldk) + (long)hk * a.K;
-    const long ld = side ? a.ldq : a.ldk;
-    __bf16* const dst = side ? ql : kl;
-    __bf16* const pk = (side ? a.qpk : a.kpk) + hs * NP * kC * Kp;
-    const bool whole = !a.pack;                     // rows of Kp elements, 16-byte aligned
-    for (int u = tid; u < kC * KG; u += 256) {
-      const int i = u / KG, c = (u - i * KG) * 8;
-      bf16x8 t[NP];
-      if constexpr (NP == 1) {
-        if (whole && i < valid) {
-          t[0] = *reinterpret_cast<const bf16x8*>(src + i * ld + c);
+  if (NP == 1 && !a.pack) {                                    // rows of Kp elements, 16-byte aligned
+    constexpr int U = kC * KG / 256;
+    bf16x8 x[2][U];
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      const long ld = side ? a.ldq : a.ldk;
+      const __amdgpu_buffer_rsrc_t r = rows_rsrc(side ? a.q : a.k, (row0 * ld + (long)hk * Kp) * 2, ((valid - 1) * ld + Kp) * 2);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int g = u * 256 + tid, i = g / KG, c = (g - i * KG) * 8;
+        x[side][u] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(r, (i * (unsigned)ld + c) * 2, 0, 0));
+      }
+    }
+#pragma unroll
+    for (int side = 0; side < 2; ++side)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int g = u * 256 + tid, i = g / KG, c = (g - i * KG) * 8;
+        *reinterpret_cast<bf16x8*>((side ? ql : kl) + i * LDK + c) = x[side][u];
+      }
+  } else {
+    for (int side = 0; side < 2; ++side) {
+      const long ld = side ? a.ldq : a.ldk;
+      const T* const src = static_cast<const T*>(side ? a.q : a.k) + row0 * ld + (long)hk * a.K;
+      __bf16* const dst = side ? ql : kl;
+      __bf16* const pk = (side ? a.qpk : a.kpk) + hs * kC * NP * Kp;
+      for (int u = tid; u < kC * KG; u += 256) {
+        const int i = u / KG, c = (u - i * KG) * 8;
+        // (unconditional requests of elements that are there, then a choice)
+        const T* const p = src + min(i, valid - 1) * ld;
+        T raw[8];
+        if (a.wide) {                                          // K % 8 == 0, 16-byte aligned rows
+          const u32x4* const q = reinterpret_cast<const u32x4*>(p + min(c, a.K - 8));
+          u32x4 y[sizeof(T) / 2];
+#pragma unroll
+          for (int h = 0; h < (int)sizeof(T) / 2; ++h) y[h] = q[h];
+          __builtin_memcpy(raw, y, sizeof(raw));
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) t[0][e] = i < valid && c + e < a.K ? (__bf16)src[i * ld + c + e] : (__bf16)0.f;
+          for (int e = 0; e < 8; ++e) raw[e] = p[min(c + e, a.K - 1)];
         }
-      } else {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = i < valid && c + e < a.K ? (float)src[i * ld + c + e] : 0.f;
+        for (int e = 0; e < 8; ++e) x[e] = i < valid && c + e < a.K ? (float)raw[e] : 0.f;
+        bf16x8 t[NP];
         sb::split8<NP>(x, t);
-      }
 #pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        *reinterpret_cast<bf16x8*>(dst + (p * kC + i) * LDK + c) = t[p];
-        if (a.pack) *reinterpret_cast<bf16x8*>(pk + ((long)i * NP + p) * Kp + c) = t[p];
+        for (int p = 0; p < NP; ++p) {
+          *reinterpret_cast<bf16x8*>(dst + (p * kC + i) * LDK + c) = t[p];
+          if (a.pack) *reinterpret_cast<bf16x8*>(pk + ((long)i * NP + p) * Kp + c) = t[p];
+        }
       }
     }
   }
   __syncthreads();
+  // the transposes: two columns of eight tokens per thread
   for (int side = 0; side < (a.train ? 2 : 1); ++side) {
     const __bf16* const src = side ? ql : kl;
     __bf16* const dst = (side ? a.qt : a.kt) + hs * NP * Kp * kC;
-    for (int u = tid; u < NP * Kp * 8; u += 256) {
-      const int k = u % Kp, r = u / Kp, i0 = (r & 7) * 8, p = r >> 3;
-      bf16x8 t;
+    for (int u = tid; u < NP * (Kp / 2) * 8; u += 256) {
+      const int k = u % (Kp / 2) * 2, r = u / (Kp / 2), i0 = (r & 7) * 8, p = r >> 3;
+      unsigned x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) t[e] = src[(p * kC + i0 + e) * LDK + k];
-      *reinterpret_cast<bf16x8*>(dst + ((long)k * NP + p) * kC + i0) = t;
+      for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const unsigned*>(src + (p * kC + i0 + e) * LDK + k);
+      u32x4 lo, hi;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        lo[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x05040100u);       // low halves of two tokens
+        hi[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x07060302u);       // high halves
+      }
+      *reinterpret_cast<u32x4*>(dst + ((long)k * NP + p) * kC + i0) = lo;
+      *reinterpret_cast<u32x4*>(dst + ((long)(k + 1) * NP + p) * kC + i0) = hi;
     }
   }
-  f32x4 kk[4], qk[4];
+  // rows 16*wave.. against the tiles of columns in front of them: k k^T, q k^T (its transpose's source), and k q^T with the
+  // roles changed: rows of the wave's tile are the columns j of P
+  f32x4 kk[4], qk[4], kq[4];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) kk[t] = qk[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < 4; ++t) kk[t] = qk[t] = kq[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int kb = 0; kb < Kp / 32; ++kb) {
     bf16x8 ka[NP], qa[NP];
@@ -193,7 +250,8 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
         bf16x8 b[NP];
         sb::load_frag<NP>(b, kl + (16 * t + lr) * LDK + 32 * kb + 8 * lg, kC * LDK);
         sb::mma<NP, NP>(kk[t], ka, b);
-        sb::mma<NP, NP>(qk[t], qa, b);
+        if (a.train) sb::mma<NP, NP>(qk[t], qa, b);
+        sb::mma<NP, NP>(kq[t], b, qa);                         // row 16*t + ..: k's token j, column 16*wave + lr: q's token i
       }
     }
   }
@@ -204,9 +262,10 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
     // every wave holds token `lane`: running sum of the log decays in fp64, kept as two floats
     {
       const bool in = lane < valid;
-      float gi = in ? a.g[(row0 + lane) * a.ldg + hv] : 0.f;
-      const float bi = in ? a.beta[(row0 + lane) * a.ldbeta + hv] : 0.f;
-      gi = gi < kGMin ? kGMin : gi;
+      const long row = row0 + min(lane, valid - 1);
+      float gi = a.g[row * a.ldg + hv], bi = a.beta[row * a.ldbeta + hv];
+      gi = in ? gi < kGMin ? kGMin : gi : 0.f;
+      bi = in ? bi : 0.f;
       double G = gi;
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
@@ -226,31 +285,48 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
       }
     }
     __syncthreads();
-    const int ib = 16 * wave + 4 * lg;
+    const int ib = 16 * wave + 4 * lg, iq = 16 * wave + lr;
+    __bf16* const pp = a.p + vs * kC * NO * kC;
+    __bf16* const pt = a.pt + vs * kC * 3 * kC;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int j = 16 * t + lr;
+      const int j = 16 * t + lr, jb = 16 * t + 4 * lg;
+      f32x4 x;
       const float hj = gh[j], lj = gl[j];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = ib + e;
-        const float d = i >= j ? expf((gh[i] - hj) + (gl[i] - lj)) : 0.f;
+        const float d = i >= j ? decay((gh[i] - hj) + (gl[i] - lj)) : 0.f;
         lm[i * kLdM + j] = i > j ? be[i] * kk[t][e] * d : i == j ? 1.f : 0.f;
-        pm[i * kLdM + j] = i >= j ? qk[t][e] * d : 0.f;
         mm[i * kLdM + j] = 0.f;
+        x[e] = i >= j ? qk[t][e] * d : 0.f;
       }
+      if (a.train && ((t < 2) || (wave >= 2))) sb::split_store4<3>(pt + j * 3 * kC + ib, kC, x);       // PT rows j >= 32 hold columns i >= 32
+      const float hi = gh[iq], lo = gl[iq];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = iq >= jb + e ? kq[t][e] * decay((hi - gh[jb + e]) + (lo - gl[jb + e])) : 0.f;
+      if (t < 2 || wave >= 2) sb::split_store4<NO>(pp + iq * NO * kC + jb, kC, x);
     }
     __syncthreads();
     {
       // diagonal block `wave`: column lr of the inverse by substitution
-      const float* const L = lm + 16 * wave * kLdM + 16 * wave;
+      const float* const D = lm + 16 * wave * kLdM + 16 * wave;
       float x[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float s = i == lr ? 1.f : 0.f;
+        // (rows of L requested one by one: all at once would not fit the registers)
+        if (i > 0) asm volatile("" : "+v"(x[i - 1])::"memory");
+        f32x4 row[4];
 #pragma unroll
-        for (int j = 0; j < i; ++j) s = fmaf(-L[i * kLdM + j], x[j], s);
-        x[i] = s;
+        for (int q = 0; q < 4; ++q)
+          if (4 * q < i) row[q] = *reinterpret_cast<const f32x4*>(D + i * kLdM + 4 * q);
+        float s0 = i == lr ? 1.f : 0.f, s1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < i; ++j) {
+          if (j & 1) s1 = fmaf(-row[j >> 2][j & 3], x[j], s1);
+          else s0 = fmaf(-row[j >> 2][j & 3], x[j], s0);
+        }
+        x[i] = s0 + s1;
       }
       if (lg == 0) {
 #pragma unroll
@@ -263,33 +339,32 @@ __global__ __launch_bounds__(256) void gdr_prep_kernel(GdrArgs a) {
       // 16 x 16 below the diagonal of the two 32 x 32 blocks
       const int o1 = 32 * wave, o2 = o1 + 16;
       mt::f32x4 c = mt::wave_mma16<16, kLdM, 1, kLdM, 1>(lm + o2 * kLdM + o1, mm + o1 * kLdM + o1, lane, zero);
-      mt::store_block16<kLdM>(tm, o2, 0, c, lane);
+      mt::store_block16<kLdM>(tm, 16 * wave, 0, c, lane);
       mt::wave_sync();
-      c = mt::wave_mma16<16, kLdM, 1, kLdM, 1>(mm + o2 * kLdM + o2, tm + o2 * kLdM, lane, zero);
+      c = mt::wave_mma16<16, kLdM, 1, kLdM, 1>(mm + o2 * kLdM + o2, tm + 16 * wave * kLdM, lane, zero);
       mt::store_block16<kLdM>(mm, o2, o1, -c, lane);
     }
     __syncthreads();
     {
       const int ti = 16 * (wave >> 1), tj = 16 * (wave & 1);
       mt::f32x4 c = mt::wave_mma16<32, kLdM, 1, kLdM, 1>(lm + (32 + ti) * kLdM, mm + tj, lane, zero);
-      __syncthreads();
       mt::store_block16<kLdM>(tm, ti, tj, c, lane);
       __syncthreads();
       c = mt::wave_mma16<32, kLdM, 1, kLdM, 1>(mm + (32 + ti) * kLdM + 32, tm + tj, lane, zero);
       mt::store_block16<kLdM>(mm, 32 + ti, tj, -c, lane);
     }
     __syncthreads();
-    // 16 elements of a row (or of a column, for the transposes the backward scan reads) per thread
+    // 16 elements of a row (or of a column, for the transpose the backward scan reads) per thread
     const int row = tid >> 2, c0 = (tid & 3) * 16;
-    for (int what = 0; what < (a.train ? 4 : 2); ++what) {
-      const float* const src = what & 1 ? pm : mm;
-      __bf16* const dst = (what == 0 ? a.m : what == 1 ? a.p : what == 2 ? a.mt : a.pt) + (vs * kC + row) * 3 * kC + c0;
-      const int si = what < 2 ? kLdM : 1, sj = what < 2 ? 1 : kLdM;
+    for (int what = 0; what < (a.train ? 2 : 1); ++what) {
+      if (what == 0 ? row < 32 && c0 >= 32 : row >= 32 && c0 < 32) continue;
+      __bf16* const dst = (what == 0 ? a.m : a.mt) + (vs * kC + row) * 3 * kC + c0;
+      const int si = what == 0 ? kLdM : 1, sj = what == 0 ? 1 : kLdM;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = src[row * si + (c0 + 8 * h + e) * sj];
+        for (int e = 0; e < 8; ++e) x[e] = mm[row * si + (c0 + 8 * h + e) * sj];
         bf16x8 t[3];
         sb::split8<3>(x, t);
 #pragma unroll
@@ -322,16 +397,6 @@ struct ScanLds {
   static constexpr int bwd_bytes = 2 * (S + 3 * X + NP * VT * kLdT) + 12 * F;
 };
 
-// Rows of the caller's tensors go through buffer descriptors: a base that moves from chunk to chunk in scalar registers, a
-// lane's offset that never changes, and the size of what the sequence has left, behind which a load gives 0 and a store is
-// dropped.  So rows behind the sequence need no test, no request has a condition (a conditional one would be waited for
-// where its branch joins), and a chunk costs no address arithmetic on the vector unit.
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-constexpr unsigned kNoColumn = 0x80000000u;      // an offset behind every size
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, long offset, long bytes) {
-  // (descriptor word 3: 32-bit data, no swizzle)
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base)) + offset, 0, (int)bytes, 0x00027000);
-}
 // Operand rows of k or q, token 16*w + lr of a chunk, from the packed terms (whose rows behind the sequence are 0) or from
 // the caller's rows
 template <int NP, int KB>
@@ -607,9 +672,9 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
     bf16x8 qf[KB][NP], pf[2][NO];
     f32x4 qn[NT], qs[NT], qo[NT];
     const RowPtr<NP, KB> qp(a, a.q, a.ldq, a.qpk, slot0, hk, start, len, ia, lg);
-    const __bf16* const pp = a.p + (slot0 * a.Hv + hv) * 3 * kC * kC;
-    const long pstep = (long)a.Hv * 3 * kC * kC;
-    const unsigned pat = ia * 3 * kC + 8 * lg;
+    const __bf16* const pp = a.p + (slot0 * a.Hv + hv) * NO * kC * kC;
+    const long pstep = (long)a.Hv * NO * kC * kC;
+    const unsigned pat = ia * NO * kC + 8 * lg;
     ColOut<T, NT> op(a.o, a.ldo, start, len, hv, a.V, v0, lr, ib);
     const float* gp = a.vec + (slot0 * a.Hv + hv) * kVecs * kC + kGam * kC;
     auto pw = [&](int c, int kb) {                         // qs += P W, columns 32*kb of P; W as the chain left it in wl
@@ -1088,7 +1153,7 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = ib + e;
-        const float d = i >= j ? expf((ghi[e] - hj[t]) + (glo[e] - lj[t])) : 0.f;
+        const float d = i >= j ? decay((ghi[e] - hj[t]) + (glo[e] - lj[t])) : 0.f;
         dp[t][e] = i >= j ? a.scale * dp[t][e] * d : 0.f;
         da[t][e] = i > j ? -da[t][e] * d : 0.f;
         __bf16 x[3];
@@ -1346,7 +1411,7 @@ long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, 
   t.qpk = take16(ns * Hk * np * kC * kp);
   t.kt = take16(ns * Hk * np * kC * kp);
   t.m = take16(ns * Hv * 3 * kC * kC);
-  t.p = take16(ns * Hv * 3 * kC * kC);
+  t.p = take16(ns * Hv * (np == 1 ? 2 : 3) * kC * kC);
   t.vec = take(ns * Hv * kVecs * kC);
   if (train) {
     t.qt = take16(ns * Hk * np * kC * kp);
@@ -1400,7 +1465,8 @@ int gdr_fill(const hhrl_gdr_desc* d, GdrArgs& a, bool train, const char* who) {
   a.q = d->q; a.k = d->k; a.v = d->v; a.ldq = d->ldq; a.ldk = d->ldk; a.ldv = d->ldv;
   a.g = d->g; a.beta = d->beta; a.ldg = d->ldg; a.ldbeta = d->ldbeta;
   a.train = train;
-  a.pack = !(d->dtype == HHRL_BF16 && d->K == padded_k(d->K) && a16(d->q) && a16(d->k) && d->ldq % 8 == 0 && d->ldk % 8 == 0);
+  a.wide = d->K % 8 == 0 && a16(d->q) && a16(d->k) && d->ldq % 8 == 0 && d->ldk % 8 == 0;
+  a.pack = !(d->dtype == HHRL_BF16 && d->K == padded_k(d->K) && a.wide);
   return HHRL_OK;
 }
 
@@ -1436,9 +1502,7 @@ int run_scan(const GdrArgs& a, bool bwd, hipStream_t st, double flops) {
 
 template <typename T, int NP, int KB2>
 int run_fwd(const GdrArgs& a, hipStream_t st, double flops) {
-  constexpr int Kp = 64 * KB2;
-  constexpr int over = 2 * NP * kC * (Kp + 8) * 2 > 2 * kC * kLdM * 4 ? 2 * NP * kC * (Kp + 8) * 2 : 2 * kC * kLdM * 4;
-  constexpr int lds_prep = over + 2 * kC * kLdM * 4 + 3 * kC * 4;
+  constexpr int lds_prep = PrepLds<NP, KB2>::bytes;
   HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(&gdr_prep_kernel<T, NP, KB2>), lds_prep, "gdr_forward"));
   {
     ProfScope ps("gdr_prep_kernel", st, 0.0, 0.0);
