@@ -955,7 +955,10 @@ template <int NP, int KB2>
 struct GradsLds {
   static constexpr int Kp = 64 * KB2, LDV = 40;              // 32 columns + 8: 16 rows in 16 distinct bank groups
   static constexpr int cols = 3 * LDV * (2 * Kp + 2 * kC) + NP * LDV * kC;       // elements: S, dS', W, Y, dO
-  static constexpr int tri = 4 * 3 * kC * kLdT;              // R, B and their transposes, over them afterwards
+  // afterwards, over them: R, B and their transposes; where k and q do not stay in LDS (three terms), 32 tokens of those and
+  // of k and q at a time
+  static constexpr int LDH = 32 + 8;
+  static constexpr int tri = NP == 1 ? 4 * 3 * kC * kLdT : 4 * 3 * kC * LDH + 2 * NP * Kp * LDH;
   static constexpr int over = 2 * (cols > tri ? cols : tri);
   static constexpr int kq = NP == 1 ? 2 * 2 * Kp * kLdT : 0;                     // bytes: k and q of the chunk, transposed (three terms do not fit)
   static constexpr int bytes = over + kq + (8 * kC + 8) * 4;
@@ -970,12 +973,14 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
   __bf16* const wl = dl + 3 * Kp * LDV;                      // [3][64][LDV]
   __bf16* const yl = wl + 3 * kC * LDV;                      // [3][64][LDV]
   __bf16* const ol = yl + 3 * kC * LDV;                      // [NP][64][LDV]
-  __bf16* const rl = reinterpret_cast<__bf16*>(smem);        // [3][64][kLdT] each
-  __bf16* const bl = rl + 3 * kC * kLdT;
-  __bf16* const rt = bl + 3 * kC * kLdT;
-  __bf16* const bt = rt + 3 * kC * kLdT;
-  __bf16* const kl = reinterpret_cast<__bf16*>(smem + L::over);    // NP == 1: [Kp][kLdT] each
-  __bf16* const ql = kl + Kp * kLdT;
+  constexpr int LDR = NP == 1 ? kLdT : L::LDH;
+  __bf16* const rl = reinterpret_cast<__bf16*>(smem);        // [3][64][LDR] each
+  __bf16* const bl = rl + 3 * kC * LDR;
+  __bf16* const rt = bl + 3 * kC * LDR;
+  __bf16* const bt = rt + 3 * kC * LDR;
+  // k and q, transposed: for the kernel's length (one term, [Kp][kLdT] each) or 32 tokens at a time ([NP][Kp][LDH] each)
+  __bf16* const kl = NP == 1 ? reinterpret_cast<__bf16*>(smem + L::over) : bt + 3 * kC * LDR;
+  __bf16* const ql = kl + (NP == 1 ? Kp * kLdT : NP * Kp * L::LDH);
   float* const rows = reinterpret_cast<float*>(smem + L::over + L::kq);    // [2 halves][3][64]: shares of dG, of dbeta, k.(tail E3)
   float* const yv = rows + 6 * kC;                                 // [64] Y.v
   float* const red = yv + kC;                                      // [8]
@@ -994,9 +999,6 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
   const int gi = (tid & 255) >> 2, gc = (tid & 3) * 8;       // token and columns of W, dO (threads 0..255), Y, v (the others)
   const long rowc = row0 + min(gi, valid - 1);
 
-  // the chunk's k and q, transposed: fragments along the tokens, and single columns in the layout of a result
-  constexpr int TS = NP == 1 ? kLdT : NP * kC;               // from column to column
-  const __bf16 *ktr, *qtr;
   if constexpr (NP == 1) {
     const bf16x8* const gk = reinterpret_cast<const bf16x8*>(a.kt + hs * Kp * kC);
     const bf16x8* const gq = reinterpret_cast<const bf16x8*>(a.qt + hs * Kp * kC);
@@ -1009,11 +1011,6 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
       *reinterpret_cast<bf16x8*>(kl + at) = x[u];
       *reinterpret_cast<bf16x8*>(ql + at) = y[u];
     }
-    ktr = kl + (kt0 + lr) * TS;
-    qtr = ql + (kt0 + lr) * TS;
-  } else {
-    ktr = a.kt + (hs * Kp + kt0 + lr) * TS;
-    qtr = a.qt + (hs * Kp + kt0 + lr) * TS;
   }
   f32x4 dqs[GROUP ? KT : 1], dks[GROUP ? KT : 1];
   if (GROUP) {
@@ -1132,87 +1129,146 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
       hj[t] = vec[kGHi * kC + 16 * (2 * t + half) + lr];
       lj[t] = vec[kGLo * kC + 16 * (2 * t + half) + lr];
     }
-    bf16x4 kr[KT][NP], qr[KT][NP];
+    // k and q in the layout of a result: four tokens of one column, from the transposes or from the caller's rows
+    bf16x4 kr[NP == 1 ? KT : 1], qr[NP == 1 ? KT : 1];
+    unsigned kx[NP == 1 ? 1 : KT][4], qx[NP == 1 ? 1 : KT][4];
+    if constexpr (NP == 1) {
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        kr[t][p] = *reinterpret_cast<const bf16x4*>(ktr + 16 * t * TS + p * kC + ib);
-        qr[t][p] = *reinterpret_cast<const bf16x4*>(qtr + 16 * t * TS + p * kC + ib);
+      for (int t = 0; t < KT; ++t) {
+        kr[t] = *reinterpret_cast<const bf16x4*>(kl + (kt0 + 16 * t + lr) * kLdT + ib);
+        qr[t] = *reinterpret_cast<const bf16x4*>(ql + (kt0 + 16 * t + lr) * kLdT + ib);
       }
+    } else {
+      const __amdgpu_buffer_rsrc_t rk = rows_rsrc(a.k, (row0 * a.ldk + (long)hk * a.K) * 4, ((valid - 1) * a.ldk + a.K) * 4);
+      const __amdgpu_buffer_rsrc_t rq = rows_rsrc(a.q, (row0 * a.ldq + (long)hk * a.K) * 4, ((valid - 1) * a.ldq + a.K) * 4);
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = kt0 + 16 * t + lr;
+          kx[t][e] = __builtin_amdgcn_raw_buffer_load_b32(rk, k < a.K ? ((ib + e) * (unsigned)a.ldk + k) * 4 : kNoColumn, 0, 0);
+          qx[t][e] = __builtin_amdgcn_raw_buffer_load_b32(rq, k < a.K ? ((ib + e) * (unsigned)a.ldq + k) * 4 : kNoColumn, 0, 0);
+        }
+    }
     __builtin_amdgcn_sched_barrier(0);                       // all of these requests together, in front of what waits for them
     ydot += __shfl_xor(ydot, 1, 64);
     ydot += __shfl_xor(ydot, 2, 64);
     sdot = wave_sum(sdot);
-    __syncthreads();
-    if (tid >= 256 && (tid & 3) == 0) yv[gi] = ydot;
-    if (lane == 0) red[wave] = sdot;
+    f32x4 kv[KT], qv[KT];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        kv[t][e] = NP == 1 ? (float)kr[NP == 1 ? t : 0][e] : __uint_as_float(kx[NP == 1 ? 0 : t][e]);
+        qv[t][e] = NP == 1 ? (float)qr[NP == 1 ? t : 0][e] : __uint_as_float(qx[NP == 1 ? 0 : t][e]);
+      }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int jt = 2 * t + half, j = 16 * jt + lr;
+      const int j = 16 * (2 * t + half) + lr;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = ib + e;
         const float d = i >= j ? decay((ghi[e] - hj[t]) + (glo[e] - lj[t])) : 0.f;
         dp[t][e] = i >= j ? a.scale * dp[t][e] * d : 0.f;
         da[t][e] = i > j ? -da[t][e] * d : 0.f;
-        __bf16 x[3];
-        sb::split3(dp[t][e], x[0], x[1], x[2]);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) rl[(p * kC + i) * kLdT + j] = x[p];
-        sb::split3(da[t][e], x[0], x[1], x[2]);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) bl[(p * kC + i) * kLdT + j] = x[p];
       }
-      sb::split_store4<3>(rt + j * kLdT + ib, kC * kLdT, dp[t]);
-      sb::split_store4<3>(bt + j * kLdT + ib, kC * kLdT, beta * da[t]);
     }
+    f32x4 dg = zero, db = zero, st = zero, kc = zero;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       e1[t] *= a.scale * gam;
       e2[t] *= -gam;
       e3[t] *= tail;
+      st += kv[t] * e3[t];
     }
-    // k and q in the layout of a result: four tokens of one column, from the transposes
-    f32x4 kv[KT], qv[KT];
+    // R and B (columns j0..) and their transposes (rows' tokens i0..) into LDS
+    auto put = [&](int t, int j0) {
+      const int j = 16 * (2 * t + half) + lr;
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      kv[t] = qv[t] = zero;
+      for (int e = 0; e < 4; ++e) {
+        __bf16 x[3];
+        sb::split3(dp[t][e], x[0], x[1], x[2]);
 #pragma unroll
-      for (int p = NP - 1; p >= 0; --p)
+        for (int p = 0; p < 3; ++p) rl[(p * kC + ib + e) * LDR + j - j0] = x[p];
+        sb::split3(da[t][e], x[0], x[1], x[2]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { kv[t][e] += (float)kr[t][p][e]; qv[t][e] += (float)qr[t][p][e]; }
-    }
-    f32x4 dg = zero, db = zero, st = zero, kc = zero;
-#pragma unroll
-    for (int t = 0; t < KT; ++t) st += kv[t] * e3[t];
-    __syncthreads();
-#pragma unroll 1
-    for (int kb = 0; kb < 2; ++kb) {                         // not unrolled: fragments of both halves at once would not fit the registers
+        for (int p = 0; p < 3; ++p) bl[(p * kC + ib + e) * LDR + j - j0] = x[p];
+      }
+    };
+    auto put_t = [&](int t, int i0) {
+      const int j = 16 * (2 * t + half) + lr;
+      sb::split_store4<3>(rt + j * LDR + ib - i0, kC * LDR, dp[t]);
+      sb::split_store4<3>(bt + j * LDR + ib - i0, kC * LDR, beta * da[t]);
+    };
+    // the products of 32 tokens: at = where they begin in the images
+    auto join = [&](int kb, int at) {
+      constexpr int KS = NP == 1 ? kLdT : L::LDH, KP = NP * Kp;  // from column to column, from term to term (in columns)
+      const __bf16* const kf = kl + (kt0 + lr) * KS + at + 8 * lg;
+      const __bf16* const qf = ql + (kt0 + lr) * KS + at + 8 * lg;
       if (kb == 0 || w >= 2) {
         bf16x8 rf[3], bf[3];
-        sb::load_frag<3>(rf, rl + ia * kLdT + 32 * kb + 8 * lg, kC * kLdT);
-        sb::load_frag<3>(bf, bl + ia * kLdT + 32 * kb + 8 * lg, kC * kLdT);
+        sb::load_frag<3>(rf, rl + ia * LDR + at + 8 * lg, kC * LDR);
+        sb::load_frag<3>(bf, bl + ia * LDR + at + 8 * lg, kC * LDR);
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
           bf16x8 b[NP];
-          sb::load_frag<NP>(b, ktr + 16 * t * TS + 32 * kb + 8 * lg, kC);
+          sb::load_frag<NP>(b, kf + 16 * t * KS, Kp * KS);
           sb::mma<3, NP>(e1[t], rf, b);
           sb::mma<3, NP>(e2[t], bf, b);
         }
       }
       if (kb == 1 || w < 2) {
         bf16x8 rf[3], bf[3];
-        sb::load_frag<3>(rf, rt + ia * kLdT + 32 * kb + 8 * lg, kC * kLdT);
-        sb::load_frag<3>(bf, bt + ia * kLdT + 32 * kb + 8 * lg, kC * kLdT);
+        sb::load_frag<3>(rf, rt + ia * LDR + at + 8 * lg, kC * LDR);
+        sb::load_frag<3>(bf, bt + ia * LDR + at + 8 * lg, kC * LDR);
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
           bf16x8 b[NP];
-          sb::load_frag<NP>(b, qtr + 16 * t * TS + 32 * kb + 8 * lg, kC);
+          sb::load_frag<NP>(b, qf + 16 * t * KS, Kp * KS);
           sb::mma<3, NP>(e3[t], rf, b);
-          sb::load_frag<NP>(b, ktr + 16 * t * TS + 32 * kb + 8 * lg, kC);
+          sb::load_frag<NP>(b, kf + 16 * t * KS, Kp * KS);
           sb::mma<3, NP>(e3[t], bf, b);
         }
+      }
+    };
+    __syncthreads();
+    if (tid >= 256 && (tid & 3) == 0) yv[gi] = ydot;
+    if (lane == 0) red[wave] = sdot;
+    if constexpr (NP == 1) {
+      put(0, 0);
+      put(1, 0);
+      put_t(0, 0);
+      put_t(1, 0);
+      __syncthreads();
+#pragma unroll 1
+      for (int kb = 0; kb < 2; ++kb) join(kb, 32 * kb);      // not unrolled: fragments of both halves at once would not fit the registers
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        // 16 bytes of a term's row (32 tokens are four) per thread: columns tid/4, tid/4 + 128, ..
+        constexpr int U = (NP * Kp + 127) / 128;
+        bf16x8 x[2][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int row = min(u * 128 + (tid >> 2), NP * Kp - 1), p = row / Kp, k = row - p * Kp;
+          const long at = ((hs * Kp + k) * NP + p) * kC + 32 * kb + 8 * (tid & 3);
+          x[0][u] = *reinterpret_cast<const bf16x8*>(a.kt + at);
+          x[1][u] = *reinterpret_cast<const bf16x8*>(a.qt + at);
+        }
+        if (kb) __syncthreads();                             // the first half's images have been read
+        put(kb, 32 * kb);
+        if ((w >> 1) == kb) {
+          put_t(0, 32 * kb);
+          put_t(1, 32 * kb);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int at = min(u * 128 + (tid >> 2), NP * Kp - 1) * L::LDH + 8 * (tid & 3);    // (the last row's copies are the same)
+          *reinterpret_cast<bf16x8*>(kl + at) = x[0][u];
+          *reinterpret_cast<bf16x8*>(ql + at) = x[1][u];
+        }
+        __syncthreads();
+        join(kb, 0);
       }
     }
 #pragma unroll
