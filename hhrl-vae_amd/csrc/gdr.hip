@@ -69,6 +69,10 @@ struct GdrArgs {
   //     fragments are at constant offsets from one address.
   __bf16 *kpk, *qpk, *kt, *qt, *m, *p, *mt, *pt;
   float *vec, *w, *y, *s, *ds;
+  // segments of long sequences: segs of seg_chunks chunks each (1: the whole sequence), grid_segs of them in a launch; per
+  // value head and segment M and its transpose [Kp][Kp], N [Kp][vp], and the state (gradient) it starts from [Kp][vp]
+  int segs, seg_chunks, grid_segs;
+  float *seg_m, *seg_mt, *seg_n, *seg_s;
 };
 enum { kGam = 0, kTail = 1, kBeta = 2, kGHi = 3, kGLo = 4, kVecs = 5 };
 
@@ -375,13 +379,15 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
 }
 
 // --------------------------------------------------------------------------------------------------------- scans
-// Workgroup -> (sequence, value head, column tile).  Workgroups go to the eight XCDs in turn: the column tiles of one
+// Workgroup -> (sequence, value head, segment, column tile).  Workgroups go to the eight XCDs in turn: the column tiles of one
 // head read the same k, q, M and P, so they are dealt to one XCD (one L2), eight workgroups apart.
-__device__ __forceinline__ bool scan_tile(const GdrArgs& a, int vt, int& n, int& hv, int& v0) {
+__device__ __forceinline__ bool scan_tile(const GdrArgs& a, int vt, int& n, int& hv, int& v0, int& seg) {
   const int xcd = blockIdx.x & 7, u = blockIdx.x >> 3;
   v0 = (u % a.nvt) * vt;
-  const long pair = (long)(u / a.nvt) * 8 + xcd;
-  if (pair >= (long)a.n_seq * a.Hv) return false;
+  const long unit = (long)(u / a.nvt) * 8 + xcd;
+  if (unit >= (long)a.n_seq * a.Hv * a.grid_segs) return false;
+  const long pair = unit / a.grid_segs;
+  seg = __builtin_amdgcn_readfirstlane((int)(unit - pair * a.grid_segs));
   n = __builtin_amdgcn_readfirstlane((int)(pair / a.Hv));
   hv = __builtin_amdgcn_readfirstlane((int)(pair - (long)n * a.Hv));
   return true;
@@ -519,6 +525,26 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[KB2][NT], float* s,
       }
 }
 
+// the same tile of a state of a segment, [Kp][ld] without bounds to keep
+template <int KB2, int NT>
+__device__ __forceinline__ void load_seg(f32x4 (&S)[KB2][NT], const float* s, int ld, int w, int v0, int lr, int lg) {
+#pragma unroll
+  for (int t = 0; t < KB2; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[t][u][e] = s[(16 * (KB2 * w + t) + 4 * lg + e) * ld + v0 + 16 * u + lr];
+}
+template <int KB2, int NT>
+__device__ __forceinline__ void store_seg(const f32x4 (&S)[KB2][NT], float* s, int ld, int w, int v0, int lr, int lg) {
+#pragma unroll
+  for (int t = 0; t < KB2; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[(16 * (KB2 * w + t) + 4 * lg + e) * ld + v0 + 16 * u + lr] = S[t][u][e];
+}
+
 // Per-token factors of a chunk, rows ib .. ib + 3
 struct ScanVec {
   f32x4 gam, tail, beta;
@@ -548,6 +574,108 @@ __device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* base, 
 // nothing but the chain, and four others what hangs on it: the output o, one chunk behind (forward), or what only depends
 // on dO, one chunk ahead, and the stores of Y and dV (backward).  Everything a chunk needs from memory is requested while
 // the chunk in front of it is worked on, behind the last use of its registers.
+// The chain: chunks c0 .. c1 - 1 of a sequence, four waves, S in their registers.  BARE: nobody hangs on it (no W is left in
+// wl).  vcols: V, or 0 for columns without a v (and v0 what it may).
+template <typename T, int NP, int KB2, int NT, bool TRAIN, bool BARE>
+__device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT], __bf16* sl, __bf16* xl, __bf16* ul, float* wl, int hv, int vcols,
+                                           int v0, long start, int len, long slot0, int c0, int c1) {
+  using L = ScanLds<NP, KB2, NT>;
+  constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT, LDS_S = L::LDS_S;
+  const int hk = hv / a.rep, lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
+  const int ib = 16 * w + 4 * lg, ia = 16 * w + lr;        // first of four result rows; operand row
+  const bool high = w >= 2;                                // M is lower triangular: rows < 32 read 32 columns
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  bf16x8 kf[KB][NP], mf[2][3], ktf[KB2][2][NP];
+  const RowPtr<NP, KB> kp(a, a.k, a.ldk, a.kpk, slot0, hk, start, len, ia, lg);
+  ColPtr<T, NT> vp(a.v, a.ldv, start, len, hv, vcols, v0, lr, ib);
+  ScanVec vn;
+  const float* vecp = a.vec + ((slot0 + c0) * a.Hv + hv) * kVecs * kC;
+  const __bf16* mp = a.m + ((slot0 + c0) * a.Hv + hv) * 3 * kC * kC;
+  const __bf16* ktp = a.kt + ((slot0 + c0) * a.Hk + hk) * Kp * NP * kC;
+  const unsigned mat = ia * 3 * kC + 8 * lg, ktat = (16 * KB2 * w + lr) * NP * kC + 8 * lg;
+  kp.load(kf, c0);
+  vp.load(c0);
+  vn.load(vecp, ib);
+  load_tri<3>(mf, mp, mat, true, high);
+  load_kt<NP, KB2>(ktf, ktp, ktat);
+  for (int c = c0; c < c1; ++c) {
+    const int next = min(c + 1, c1 - 1);
+    const long adv = next - c;                         // 0 behind the last chunk: its operands are read again, to no use
+    vecp += adv * a.Hv * kVecs * kC;
+    mp += adv * a.Hv * 3 * kC * kC;
+    ktp += adv * a.Hk * NP * Kp * kC;
+    const long vs = (slot0 + c) * a.Hv + hv;
+#pragma unroll
+    for (int t = 0; t < KB2; ++t)
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+        sb::split_store4<3>(sl + (16 * u + lr) * LDS_S + 16 * (KB2 * w + t) + 4 * lg, VT * LDS_S, S[t][u]);
+    lds_barrier();
+    f32x4 ks[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) ks[t] = zero;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        bf16x8 b[3];
+        sb::load_frag<3>(b, sl + (16 * t + lr) * LDS_S + 32 * kb + 8 * lg, VT * LDS_S);
+        sb::mma<NP, 3>(ks[t], kf[kb], b);
+      }
+    kp.load(kf, next);
+    const ScanVec vc = vn;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      sb::split_store4<3>(xl + (16 * t + lr) * kLdT + ib, VT * kLdT, vc.beta * (vp.get(t) - vc.gam * ks[t]));
+    vp.load(next);
+    vn.load(vecp, ib);
+    if constexpr (TRAIN) {
+      float* const sp = a.s + ((vs * (a.vp / 32) + v0 / 32) * Kp) * 32 + (v0 & 16);
+      const unsigned at = (16 * KB2 * w + 4 * lg) * 32 + lr;
+#pragma unroll
+      for (int t = 0; t < KB2; ++t)
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sp[at + (16 * t + e) * 32 + 16 * u] = S[t][u][e];
+    }
+    lds_barrier();
+    f32x4 wt[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) wt[t] = zero;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+      if (kb == 0 || high)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          bf16x8 b[3];
+          sb::load_frag<3>(b, xl + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+          sb::mma<3, 3>(wt[t], mf[kb], b);
+        }
+    load_tri<3>(mf, mp, mat, true, high);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      sb::split_store4<3>(ul + (16 * t + lr) * kLdT + ib, VT * kLdT, vc.tail * wt[t]);
+      if constexpr (!BARE) *reinterpret_cast<f32x4*>(wl + (c & 1) * L::F + (16 * t + lr) * kLdM + ib) = wt[t];
+    }
+    lds_barrier();
+#pragma unroll
+    for (int t = 0; t < KB2; ++t)
+#pragma unroll
+      for (int u = 0; u < NT; ++u) S[t][u] *= vc.last;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        bf16x8 b[3];
+        sb::load_frag<3>(b, ul + (16 * u + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+#pragma unroll
+        for (int t = 0; t < KB2; ++t) sb::mma<NP, 3>(S[t][u], ktf[t][kb], b);
+      }
+    load_kt<NP, KB2>(ktf, ktp, ktat);
+  }
+}
+
 template <typename T, int NP, int KB2, int NT, bool TRAIN>
 __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
   using L = ScanLds<NP, KB2, NT>;
@@ -558,14 +686,16 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
   __bf16* const xl = sl + L::S;                            // [3][VT][kLdT]  beta (V - gam K S)
   __bf16* const ul = xl + L::X;                            // [3][VT][kLdT]  exp(G_C - G) W
   float* const wl = reinterpret_cast<float*>(ul + L::X);   // [2][VT][kLdM]  W, of the chunk at hand and the one in front of it
-  int n, hv, v0;
-  if (!scan_tile(a, VT, n, hv, v0)) return;
+  int n, hv, v0, seg;
+  if (!scan_tile(a, VT, n, hv, v0, seg)) return;
   const int hk = hv / a.rep;
   const int tid = threadIdx.x, lane = tid & 63, w = (tid >> 6) & 3, lr = lane & 15, lg = lane >> 4;
   long start, slot0;
   int len;
   seq_range(a, n, start, len, slot0);
   const int nc = (len + kC - 1) / kC;
+  const int c0 = seg * a.seg_chunks, c1 = min(nc, c0 + a.seg_chunks);
+  if (seg > 0 && c0 >= nc) return;
   const int ib = 16 * w + 4 * lg, ia = 16 * w + lr;        // first of four result rows; operand row
   const bool high = w >= 2;                                // M and P are lower triangular: rows < 32 read 32 columns
   const long nh = (long)n * a.Hv + hv;
@@ -573,110 +703,21 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
 
   if (tid < 256) {                                         // ---- the chain
     f32x4 S[KB2][NT];
-    load_state<KB2, NT>(S, a.s0, a, nh, w, v0, lr, lg);
-    if (nc > 0) {
-      bf16x8 kf[KB][NP], mf[2][3], ktf[KB2][2][NP];
-      const RowPtr<NP, KB> kp(a, a.k, a.ldk, a.kpk, slot0, hk, start, len, ia, lg);
-      ColPtr<T, NT> vp(a.v, a.ldv, start, len, hv, a.V, v0, lr, ib);
-      ScanVec vn;
-      const float* vecp = a.vec + (slot0 * a.Hv + hv) * kVecs * kC;
-      const __bf16* mp = a.m + (slot0 * a.Hv + hv) * 3 * kC * kC;
-      const __bf16* ktp = a.kt + (slot0 * a.Hk + hk) * Kp * NP * kC;
-      const unsigned mat = ia * 3 * kC + 8 * lg, ktat = (16 * KB2 * w + lr) * NP * kC + 8 * lg;
-      kp.load(kf, 0);
-      vp.load(0);
-      vn.load(vecp, ib);
-      load_tri<3>(mf, mp, mat, true, high);
-      load_kt<NP, KB2>(ktf, ktp, ktat);
-      for (int c = 0; c < nc; ++c) {
-        const int next = min(c + 1, nc - 1);
-        const long adv = next - c;                         // 0 behind the last chunk: its operands are read again, to no use
-        vecp += adv * a.Hv * kVecs * kC;
-        mp += adv * a.Hv * 3 * kC * kC;
-        ktp += adv * a.Hk * NP * Kp * kC;
-        const long vs = (slot0 + c) * a.Hv + hv;
-#pragma unroll
-        for (int t = 0; t < KB2; ++t)
-#pragma unroll
-          for (int u = 0; u < NT; ++u)
-            sb::split_store4<3>(sl + (16 * u + lr) * LDS_S + 16 * (KB2 * w + t) + 4 * lg, VT * LDS_S, S[t][u]);
-        lds_barrier();
-        f32x4 ks[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) ks[t] = zero;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            bf16x8 b[3];
-            sb::load_frag<3>(b, sl + (16 * t + lr) * LDS_S + 32 * kb + 8 * lg, VT * LDS_S);
-            sb::mma<NP, 3>(ks[t], kf[kb], b);
-          }
-        kp.load(kf, next);
-        const ScanVec vc = vn;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-          sb::split_store4<3>(xl + (16 * t + lr) * kLdT + ib, VT * kLdT, vc.beta * (vp.get(t) - vc.gam * ks[t]));
-        vp.load(next);
-        vn.load(vecp, ib);
-        if constexpr (TRAIN) {
-          float* const sp = a.s + ((vs * (a.vp / 32) + v0 / 32) * Kp) * 32 + (v0 & 16);
-          const unsigned at = (16 * KB2 * w + 4 * lg) * 32 + lr;
-#pragma unroll
-          for (int t = 0; t < KB2; ++t)
-#pragma unroll
-            for (int u = 0; u < NT; ++u)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) sp[at + (16 * t + e) * 32 + 16 * u] = S[t][u][e];
-        }
-        lds_barrier();
-        f32x4 wt[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) wt[t] = zero;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-          if (kb == 0 || high)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              bf16x8 b[3];
-              sb::load_frag<3>(b, xl + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
-              sb::mma<3, 3>(wt[t], mf[kb], b);
-            }
-        load_tri<3>(mf, mp, mat, true, high);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          sb::split_store4<3>(ul + (16 * t + lr) * kLdT + ib, VT * kLdT, vc.tail * wt[t]);
-          *reinterpret_cast<f32x4*>(wl + (c & 1) * L::F + (16 * t + lr) * kLdM + ib) = wt[t];
-        }
-        lds_barrier();
-#pragma unroll
-        for (int t = 0; t < KB2; ++t)
-#pragma unroll
-          for (int u = 0; u < NT; ++u) S[t][u] *= vc.last;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int u = 0; u < NT; ++u) {
-            bf16x8 b[3];
-            sb::load_frag<3>(b, ul + (16 * u + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
-#pragma unroll
-            for (int t = 0; t < KB2; ++t) sb::mma<NP, 3>(S[t][u], ktf[t][kb], b);
-          }
-        load_kt<NP, KB2>(ktf, ktp, ktat);
-      }
-    }
-    if (a.s1) store_state<KB2, NT>(S, a.s1, a, nh, w, v0, lr, lg);
-  } else if (nc > 0) {                                     // ---- the output, between the chain's barriers
+    if (seg == 0) load_state<KB2, NT>(S, a.s0, a, nh, w, v0, lr, lg);
+    else load_seg<KB2, NT>(S, a.seg_s + (nh * a.segs + seg) * Kp * a.vp, a.vp, w, v0, lr, lg);
+    if (c0 < c1) scan_chain<T, NP, KB2, NT, TRAIN, false>(a, S, sl, xl, ul, wl, hv, a.V, v0, start, len, slot0, c0, c1);
+    if (a.s1 && c1 == nc) store_state<KB2, NT>(S, a.s1, a, nh, w, v0, lr, lg);
+  } else if (c0 < c1) {                                    // ---- the output, between the chain's barriers
     // Chunk c: Q S behind barrier 1, the first half of P W behind barrier 3, the second behind the next chunk's barrier 2,
     // the store behind its barrier 1 after that: no stretch between two barriers is longer than the chain's.
     bf16x8 qf[KB][NP], pf[2][NO];
     f32x4 qn[NT], qs[NT], qo[NT];
     const RowPtr<NP, KB> qp(a, a.q, a.ldq, a.qpk, slot0, hk, start, len, ia, lg);
-    const __bf16* const pp = a.p + (slot0 * a.Hv + hv) * NO * kC * kC;
+    const __bf16* const pp = a.p + ((slot0 + c0) * a.Hv + hv) * NO * kC * kC;
     const long pstep = (long)a.Hv * NO * kC * kC;
     const unsigned pat = ia * NO * kC + 8 * lg;
     ColOut<T, NT> op(a.o, a.ldo, start, len, hv, a.V, v0, lr, ib);
-    const float* gp = a.vec + (slot0 * a.Hv + hv) * kVecs * kC + kGam * kC;
+    const float* gp = a.vec + ((slot0 + c0) * a.Hv + hv) * kVecs * kC + kGam * kC;
     auto pw = [&](int c, int kb) {                         // qs += P W, columns 32*kb of P; W as the chain left it in wl
       const float* const wc = wl + (c & 1) * L::F;
 #pragma unroll
@@ -696,7 +737,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
     };
     auto second = [&](int c) {                             // the second half, and W for the backward pass
       if (high) pw(c, 1);
-      load_half<NO>(pf[1], pp + min(c + 1, nc - 1) * pstep, pat + (high ? 32 : 0));
+      load_half<NO>(pf[1], pp + (min(c + 1, c1 - 1) - c0) * pstep, pat + (high ? 32 : 0));
       if constexpr (TRAIN) {
         float* const wp = a.w + ((((slot0 + c) * a.Hv + hv) * (a.vp / 32) + v0 / 32) * kC) * 32 + (v0 & 16);
 #pragma unroll
@@ -710,10 +751,10 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
       for (int t = 0; t < NT; ++t) qo[t] = qs[t] * a.scale;
     };
     auto store = [&](int c) { op.store(c, qo); };
-    qp.load(qf, 0);
+    qp.load(qf, c0);
     load_tri<NO>(pf, pp, pat, true, high);
     f32x4 gam = *reinterpret_cast<const f32x4*>(gp + (unsigned)ib);
-    for (int c = 0; c < nc; ++c) {
+    for (int c = c0; c < c1; ++c) {
       lds_barrier();
 #pragma unroll
       for (int t = 0; t < NT; ++t) qn[t] = zero;
@@ -725,21 +766,118 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
           sb::load_frag<NO>(b, sl + (16 * t + lr) * LDS_S + 32 * kb + 8 * lg, VT * LDS_S);
           sb::mma<NP, NO>(qn[t], qf[kb], b);
         }
-      qp.load(qf, min(c + 1, nc - 1));
-      if (c > 1) store(c - 2);
+      qp.load(qf, min(c + 1, c1 - 1));
+      if (c > c0 + 1) store(c - 2);
       lds_barrier();
-      if (c > 0) second(c - 1);
+      if (c > c0) second(c - 1);
 #pragma unroll
       for (int t = 0; t < NT; ++t) qs[t] = qn[t] * gam;
-      gp += c + 1 < nc ? (long)a.Hv * kVecs * kC : 0;
+      gp += c + 1 < c1 ? (long)a.Hv * kVecs * kC : 0;
       gam = *reinterpret_cast<const f32x4*>(gp + (unsigned)ib);
       lds_barrier();
       pw(c, 0);
-      load_half<NO>(pf[0], pp + min(c + 1, nc - 1) * pstep, pat);
+      load_half<NO>(pf[0], pp + (min(c + 1, c1 - 1) - c0) * pstep, pat);
     }
-    if (nc > 1) store(nc - 2);
-    second(nc - 1);
-    store(nc - 1);
+    if (c1 - c0 > 1) store(c1 - 2);
+    second(c1 - 1);
+    store(c1 - 1);
+  }
+}
+
+// Long sequences with few heads: the chunks of a sequence are cut into segments that all run at once.  A segment moves the
+// state it is given to M S + N; one launch finds M and N of every segment but the last (the chain alone, on the columns of
+// V from a zero state and on K columns without a v from the unit state), one joins the states along the segments, and the
+// scan then runs with every segment's own first state.  The chain is walked twice, and K / V more columns of it the first
+// time, by eight times the workgroups.
+template <typename T, int NP, int KB2>
+__global__ __launch_bounds__(256, 2) void gdr_segment_kernel(GdrArgs a) {
+  constexpr int NT = 2;
+  using L = ScanLds<NP, KB2, NT>;
+  constexpr int Kp = L::Kp, VT = L::VT;
+  extern __shared__ __align__(16) char smem[];
+  __bf16* const sl = reinterpret_cast<__bf16*>(smem);
+  __bf16* const xl = sl + L::S;
+  __bf16* const ul = xl + L::X;
+  int n, hv, v0, seg;
+  if (!scan_tile(a, VT, n, hv, v0, seg)) return;           // tiles: the columns of V, then Kp of the unit state
+  long start, slot0;
+  int len;
+  seq_range(a, n, start, len, slot0);
+  const int nc = (len + kC - 1) / kC, c0 = seg * a.seg_chunks, c1 = c0 + a.seg_chunks;
+  if (c1 >= nc) return;                                    // the last segment's end is nobody's beginning
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
+  const bool unit = v0 >= a.vp;
+  const int j0 = v0 - a.vp;
+  f32x4 S[KB2][NT];
+#pragma unroll
+  for (int t = 0; t < KB2; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[t][u][e] = unit && 16 * (KB2 * w + t) + 4 * lg + e == j0 + 16 * u + lr ? 1.f : 0.f;
+  scan_chain<T, NP, KB2, NT, false, true>(a, S, sl, xl, ul, nullptr, hv, unit ? 0 : a.V, unit ? 0 : v0, start, len, slot0, c0, c1);
+  const long at = ((long)n * a.Hv + hv) * a.segs + seg;
+  if (unit) {
+    store_seg<KB2, NT>(S, a.seg_m + at * Kp * Kp, Kp, w, j0, lr, lg);
+    if (a.train) {                                         // and transposed, for the gradients' way back
+#pragma unroll
+      for (int t = 0; t < KB2; ++t)
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+          *reinterpret_cast<f32x4*>(a.seg_mt + (at * Kp + j0 + 16 * u + lr) * Kp + 16 * (KB2 * w + t) + 4 * lg) = S[t][u];
+    }
+  } else {
+    store_seg<KB2, NT>(S, a.seg_n + at * Kp * a.vp, a.vp, w, v0, lr, lg);
+  }
+}
+
+// The first states of the segments behind the first, one after the other (backward: the gradients behind the segments in
+// front of the last, from the last): S <- M S + N, 16 columns per workgroup.
+template <int KB2>
+__global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
+  constexpr int Kp = 64 * KB2, KB = Kp / 32, LDS_S = Kp + 8;
+  __shared__ __align__(16) __bf16 sl[3 * 16 * LDS_S];
+  int n, hv, v0, seg;
+  if (!scan_tile(a, 16, n, hv, v0, seg)) return;
+  long start, slot0;
+  int len;
+  seq_range(a, n, start, len, slot0);
+  const int nc = (len + kC - 1) / kC, ns = (nc + a.seg_chunks - 1) / a.seg_chunks;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
+  const long nh = (long)n * a.Hv + hv;
+  f32x4 S[KB2][1];
+  load_state<KB2, 1>(S, bwd ? a.d_s1 : a.s0, a, nh, w, v0, lr, lg);
+  for (int i = 0; i + 1 < ns; ++i) {
+    const int g = bwd ? ns - 1 - i : i;
+    const long at = nh * a.segs + g;
+    const float* const m = (bwd ? a.seg_mt : a.seg_m) + (at * Kp + 16 * KB2 * w + lr) * Kp + 8 * lg;
+    f32x4 next[KB2][1];
+    load_seg<KB2, 1>(next, a.seg_n + at * Kp * a.vp, a.vp, w, v0, lr, lg);
+#pragma unroll
+    for (int t = 0; t < KB2; ++t) sb::split_store4<3>(sl + lr * LDS_S + 16 * (KB2 * w + t) + 4 * lg, 16 * LDS_S, S[t][0]);
+    __syncthreads();
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      bf16x8 b[3];
+      sb::load_frag<3>(b, sl + lr * LDS_S + 32 * kb + 8 * lg, 16 * LDS_S);
+#pragma unroll
+      for (int t = 0; t < KB2; ++t) {
+        float x[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4 y = *reinterpret_cast<const f32x4*>(m + 16 * t * Kp + 32 * kb + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[4 * h + e] = y[e];
+        }
+        bf16x8 f[3];
+        sb::split8<3>(x, f);
+        sb::mma<3, 3>(next[t][0], f, b);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < KB2; ++t) S[t][0] = next[t][0];
+    store_seg<KB2, 1>(S, a.seg_s + (nh * a.segs + (bwd ? g - 1 : g + 1)) * Kp * a.vp, a.vp, w, v0, lr, lg);
   }
 }
 
@@ -755,8 +893,8 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
   __bf16* const ol = yl + L::X;                            // [NP][VT][kLdT] dO
   float* const zp = reinterpret_cast<float*>(ol + NP * VT * kLdT);   // [VT][kLdM] scale P^T dO
   float* const yf = zp + L::F;                             // [2][VT][kLdM] Y, of the chunk at hand and the one behind it
-  int n, hv, v0;
-  if (!scan_tile(a, VT, n, hv, v0)) return;
+  int n, hv, v0, seg;
+  if (!scan_tile(a, VT, n, hv, v0, seg)) return;
   const int hk = hv / a.rep;
   const int tid = threadIdx.x, lane = tid & 63, w = (tid >> 6) & 3, lr = lane & 15, lg = lane >> 4;
   long start, slot0;
@@ -1455,6 +1593,22 @@ long slots_of(int n_seq, long rows, bool packed) {
   return packed ? rows / kC + n_seq : (long)n_seq * ((rows / n_seq + kC - 1) / kC);
 }
 
+// Segments per sequence and their chunks.  Cutting a sequence in s pays a second walk of 1/s of the chunks with K / V more
+// columns and a join of s steps, about two chunks each: from three segments on, where the chip's 256 CUs hold them side by side
+// (32-column workgroups) and each is long enough.  Packed sequences may all be one.
+#ifndef GDR_SEGS
+#define GDR_SEGS 1
+#endif
+int segments_of(int n_seq, long rows, bool packed, int Hv, int vp, int* chunks) {
+  const long most = packed ? rows / kC + 1 : (rows / n_seq + kC - 1) / kC, wgs = (long)n_seq * Hv * (vp / 32);
+  long segs = GDR_SEGS ? 256 / wgs : 1;
+  if (segs > most / 16) segs = most / 16;
+  if (segs > 16) segs = 16;
+  if (segs < 3) segs = 1;
+  *chunks = (int)((most + segs - 1) / segs);
+  return (int)segs;
+}
+
 // ws: offsets in floats (every array a multiple of 64 floats); returns the total.  Rows that the scans read in place
 // (bf16, K = 64 or 128, 16-byte aligned) are not packed; the size leaves room for them where alignment may forbid it.
 long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, int Hk, int Hv, int K, int V, bool train) {
@@ -1478,7 +1632,17 @@ long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, 
     t.s = take(ns * Hv * kp * vp);
     t.ds = take(ns * Hv * kp * vp);
   }
+  int chunks;
+  const int segs = segments_of(n_seq, rows, packed, Hv, (int)vp, &chunks);
+  const long pairs = (long)n_seq * Hv;
+  if (segs > 1) {
+    t.seg_m = take(pairs * segs * kp * kp);
+    t.seg_n = take(pairs * segs * kp * vp);
+    t.seg_s = take(pairs * segs * kp * vp);
+    if (train) t.seg_mt = take(pairs * segs * kp * kp);
+  }
   if (a) {
+    a->segs = segs; a->seg_chunks = chunks; a->seg_m = t.seg_m; a->seg_mt = t.seg_mt; a->seg_n = t.seg_n; a->seg_s = t.seg_s;
     a->kpk = t.kpk; a->qpk = t.qpk; a->kt = t.kt; a->qt = t.qt; a->m = t.m; a->p = t.p; a->mt = t.mt; a->pt = t.pt;
     a->vec = t.vec; a->w = t.w; a->y = t.y; a->s = t.s; a->ds = t.ds;
     a->n_slots = ns; a->vp = (int)vp;
@@ -1503,7 +1667,7 @@ int gdr_check(const hhrl_gdr_desc* d, const char* who) {
   HHRL_REQUIRE(d->ldq < most && d->ldk < most && d->ldv < most, "%s: leading dimension of an input beyond %ld", who, most - 1);
   const long ns = slots_of(d->n_seq, d->rows, d->starts != nullptr);
   HHRL_REQUIRE(ns < (1L << 31), "%s: %ld chunks", who, ns);
-  const long blocks = ((long)d->n_seq * d->Hv + 7) / 8 * 8 * ((d->V + 31) / 32 * 2);
+  const long blocks = ((long)d->n_seq * d->Hv + 7) / 8 * 8 * ((d->V + 31) / 32 * 2) * 16;     // up to 16 segments
   HHRL_REQUIRE(blocks < (1L << 31), "%s: n_seq*Hv too large", who);
   return HHRL_OK;
 }
@@ -1531,28 +1695,53 @@ int gdr_fill(const hhrl_gdr_desc* d, GdrArgs& a, bool train, const char* who) {
 #ifndef SCAN_NT
 #define SCAN_NT(wgs32) ((wgs32) >= 256 ? 2 : 1)
 #endif
-int scan_tiles(const GdrArgs& a) { return SCAN_NT((long)a.n_seq * a.Hv * (a.vp / 32)); }
+int scan_tiles(const GdrArgs& a) { return a.segs > 1 ? 2 : SCAN_NT((long)a.n_seq * a.Hv * (a.vp / 32)); }
+unsigned scan_grid(const GdrArgs& a) { return (unsigned)(((long)a.n_seq * a.Hv * a.grid_segs + 7) / 8 * 8 * a.nvt); }
 
 template <typename T, int NP, int KB2, int NT>
 int run_scan(GdrArgs a, bool bwd, hipStream_t st, double flops) {
   a.nvt = a.vp / (16 * NT);
-  const unsigned grid = (unsigned)(((long)a.n_seq * a.Hv + 7) / 8 * 8 * a.nvt);
   if (bwd) {
+    a.grid_segs = 1;
     constexpr int lds = ScanLds<NP, KB2, NT>::bwd_bytes;
     HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(&gdr_scan_bwd_kernel<T, NP, KB2, NT>), lds, "gdr_backward"));
     ProfScope ps("gdr_scan_bwd_kernel", st, flops, 0.0);
-    hipLaunchKernelGGL((gdr_scan_bwd_kernel<T, NP, KB2, NT>), dim3(grid), dim3(512), lds, st, a);
+    hipLaunchKernelGGL((gdr_scan_bwd_kernel<T, NP, KB2, NT>), dim3(scan_grid(a)), dim3(512), lds, st, a);
   } else {
+    a.grid_segs = a.segs;
     constexpr int lds = ScanLds<NP, KB2, NT>::fwd_bytes;
     void (*const fn)(GdrArgs) = a.train ? gdr_scan_fwd_kernel<T, NP, KB2, NT, true> : gdr_scan_fwd_kernel<T, NP, KB2, NT, false>;
     HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(fn), lds, "gdr_forward"));
     ProfScope ps("gdr_scan_fwd_kernel", st, flops, 0.0);
-    hipLaunchKernelGGL(fn, dim3(grid), dim3(512), lds, st, a);
+    hipLaunchKernelGGL(fn, dim3(scan_grid(a)), dim3(512), lds, st, a);
   }
   return launch_status(bwd ? "gdr_scan_bwd_kernel" : "gdr_scan_fwd_kernel");
 }
+// M and N of the segments
+template <typename T, int NP, int KB2>
+int run_segments(GdrArgs a, hipStream_t st) {
+  constexpr int lds = 2 * (ScanLds<NP, KB2, 2>::S + 2 * ScanLds<NP, KB2, 2>::X);
+  HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(&gdr_segment_kernel<T, NP, KB2>), lds, "gdr_forward"));
+  a.grid_segs = a.segs - 1;
+  a.nvt = (a.vp + 64 * KB2) / 32;
+  ProfScope ps("gdr_segment_kernel", st, 0.0, 0.0);
+  hipLaunchKernelGGL((gdr_segment_kernel<T, NP, KB2>), dim3(scan_grid(a)), dim3(256), lds, st, a);
+  return launch_status("gdr_segment_kernel");
+}
+template <int KB2>
+int run_join(GdrArgs a, bool bwd, hipStream_t st) {
+  a.grid_segs = 1;
+  a.nvt = a.vp / 16;
+  ProfScope ps("gdr_join_kernel", st, 0.0, 0.0);
+  hipLaunchKernelGGL((gdr_join_kernel<KB2>), dim3(scan_grid(a)), dim3(256), 0, st, a, bwd);
+  return launch_status("gdr_join_kernel");
+}
 template <typename T, int NP, int KB2>
 int run_scan(const GdrArgs& a, bool bwd, hipStream_t st, double flops) {
+  if (a.segs > 1 && !bwd) {
+    HHRL_TRY((run_segments<T, NP, KB2>(a, st)));
+    HHRL_TRY(run_join<KB2>(a, bwd, st));
+  }
   return scan_tiles(a) == 2 ? run_scan<T, NP, KB2, 2>(a, bwd, st, flops) : run_scan<T, NP, KB2, 1>(a, bwd, st, flops);
 }
 

@@ -128,11 +128,19 @@ def test_gdr_packed(seq, dtype, Hk, Hv, K, V, lens):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
-@pytest.mark.parametrize("T,lens", [(70, None), (130, [130, 0, 64, 1]), (3, [1, 2, 3])])
+@pytest.mark.parametrize("T,lens", [(70, None), (130, [130, 0, 64, 1]), (3, [1, 2, 3]), (3201, [3201, 1601, 0])])
 def test_gdr_padded(seq, dtype, T, lens):
     B = 4 if lens is None else len(lens)
     ranges = [(b * T, b * T + (T if lens is None else lens[b])) for b in range(B)]
     check_gdr(seq, dtype, 2, 2, 64, 48, ranges, (B, T), lens=lens, seed=T)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("K,V,Hv,lens", [(64, 32, 2, [3333]), (65, 40, 1, [70, 0, 3200, 1]), (16, 128, 2, [5000])])
+def test_gdr_long_sequences_with_few_heads(seq, dtype, K, V, Hv, lens):
+    """Long enough for the walk over the chunks to be cut into segments that run side by side."""
+    ranges, lead, starts = packed(lens, tail=1)
+    check_gdr(seq, dtype, 1, Hv, K, V, ranges, lead, starts=starts, seed=K + V, gscale=0.05)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
