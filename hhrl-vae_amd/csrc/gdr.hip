@@ -850,6 +850,11 @@ __global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
   for (int i = 0; i + 1 < ns; ++i) {
     const int g = bwd ? ns - 1 - i : i;
     const long at = nh * a.segs + g;
+    if (bwd && i == 0) {                                   // the last segment has been walked from d_s1
+      load_seg<KB2, 1>(S, a.seg_n + at * Kp * a.vp, a.vp, w, v0, lr, lg);
+      store_seg<KB2, 1>(S, a.seg_s + (nh * a.segs + g - 1) * Kp * a.vp, a.vp, w, v0, lr, lg);
+      continue;
+    }
     const float* const m = (bwd ? a.seg_mt : a.seg_m) + (at * Kp + 16 * KB2 * w + lr) * Kp + 8 * lg;
     f32x4 next[KB2][1];
     load_seg<KB2, 1>(next, a.seg_n + at * Kp * a.vp, a.vp, w, v0, lr, lg);
@@ -881,7 +886,8 @@ __global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
   }
 }
 
-template <typename T, int NP, int KB2, int NT>
+// BARE: a segment from a zero gradient (the last one: from d_s1), which leaves only the gradient in front of it, in seg_n.
+template <typename T, int NP, int KB2, int NT, bool BARE>
 __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
   using L = ScanLds<NP, KB2, NT>;
   constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT, LDS_S = L::LDS_S;
@@ -901,17 +907,21 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
   int len;
   seq_range(a, n, start, len, slot0);
   const int nc = (len + kC - 1) / kC;
+  if (BARE) ++seg;                                         // in front of the first segment there is none
+  const int c0 = seg * a.seg_chunks, c1 = min(nc, c0 + a.seg_chunks);
+  if (seg > 0 && c0 >= nc) return;
   const int ib = 16 * w + 4 * lg, ia = 16 * w + lr;
   const bool low = w < 2;                                  // P^T and M^T are upper triangular: rows >= 32 read the last 32 columns
   const long nh = (long)n * a.Hv + hv;
-  const long slot1 = slot0 + nc - 1;                       // the last chunk, where the walk begins
+  const long slot1 = slot0 + c1 - 1;                       // the last chunk, where the walk begins
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
   // Barriers of a chunk: 1 (dl), 2 (zl), 3 (yl, yf; gl, zp by the others).  Two more in front of the walk.
   if (tid < 256) {                                         // ---- the chain
     f32x4 dS[KB2][NT];
-    load_state<KB2, NT>(dS, a.d_s1, a, nh, w, v0, lr, lg);
-    if (nc > 0) {
+    if (BARE || c1 == nc) load_state<KB2, NT>(dS, c1 == nc ? a.d_s1 : nullptr, a, nh, w, v0, lr, lg);
+    else load_seg<KB2, NT>(dS, a.seg_s + (nh * a.segs + seg) * Kp * a.vp, a.vp, w, v0, lr, lg);
+    if (c0 < c1) {
       bf16x8 kf[KB][NP], mf[2][3], ktf[KB2][2][NP], qtf[KB2][2][NP];
       const RowPtr<NP, KB> kp(a, a.k, a.ldk, a.kpk, slot0, hk, start, len, ia, lg);
       ScanVec vn;
@@ -923,14 +933,14 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
         load_kt<NP, KB2>(qtf, qtp, ktat);
         load_kt<NP, KB2>(ktf, ktp, ktat);
       };
-      kp.load(kf, nc - 1);
+      kp.load(kf, c1 - 1);
       vn.load(vecp, ib);
       load_tri<3>(mf, mp, mat, low, true);
       load_t();
       lds_barrier();
       lds_barrier();
-      for (int c = nc - 1; c >= 0; --c) {
-        const int next = max(c - 1, 0);
+      for (int c = c1 - 1; c >= c0; --c) {
+        const int next = max(c - 1, c0);
         const long adv = c - next;
         vecp -= adv * a.Hv * kVecs * kC;
         mp -= adv * a.Hv * 3 * kC * kC;
@@ -962,14 +972,16 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
           sb::split_store4<3>(zl + (16 * t + lr) * kLdT + ib, VT * kLdT, p + vc.tail * z[t]);
         }
         vn.load(vecp, ib);
-        float* const sp = a.ds + ((vs * (a.vp / 32) + v0 / 32) * Kp) * 32 + (v0 & 16);
-        const unsigned at = (16 * KB2 * w + 4 * lg) * 32 + lr;
+        if constexpr (!BARE) {
+          float* const sp = a.ds + ((vs * (a.vp / 32) + v0 / 32) * Kp) * 32 + (v0 & 16);
+          const unsigned at = (16 * KB2 * w + 4 * lg) * 32 + lr;
 #pragma unroll
-        for (int t = 0; t < KB2; ++t)
+          for (int t = 0; t < KB2; ++t)
 #pragma unroll
-          for (int u = 0; u < NT; ++u)
+            for (int u = 0; u < NT; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sp[at + (16 * t + e) * 32 + 16 * u] = dS[t][u][e];
+              for (int e = 0; e < 4; ++e) sp[at + (16 * t + e) * 32 + 16 * u] = dS[t][u][e];
+        }
         lds_barrier();
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -984,7 +996,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           sb::split_store4<3>(yl + (16 * t + lr) * kLdT + ib, VT * kLdT, -vc.gam * vc.beta * y[t]);
-          *reinterpret_cast<f32x4*>(yf + (c & 1) * L::F + (16 * t + lr) * kLdM + ib) = y[t];
+          if constexpr (!BARE) *reinterpret_cast<f32x4*>(yf + (c & 1) * L::F + (16 * t + lr) * kLdM + ib) = y[t];
         }
         lds_barrier();
 #pragma unroll
@@ -1007,8 +1019,9 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
         load_t();
       }
     }
-    if (a.d_s0) store_state<KB2, NT>(dS, a.d_s0, a, nh, w, v0, lr, lg);
-  } else if (nc > 0) {                                     // ---- dO's share, ahead of the chain; Y and dV, behind it
+    if (BARE) store_seg<KB2, NT>(dS, a.seg_n + (nh * a.segs + seg) * Kp * a.vp, a.vp, w, v0, lr, lg);
+    else if (a.d_s0 && seg == 0) store_state<KB2, NT>(dS, a.d_s0, a, nh, w, v0, lr, lg);
+  } else if (c0 < c1) {                                    // ---- dO's share, ahead of the chain; Y and dV, behind it
     bf16x8 pf[2][3];
     const bool has_do = a.d_o != nullptr;
     ColPtr<T, NT> dp(has_do ? a.d_o : a.v, has_do ? a.lddo : a.ldv, start, len, hv, has_do ? a.V : 0, v0, lr, ib);
@@ -1034,17 +1047,17 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(zp + (16 * t + lr) * kLdM + ib) = a.scale * z[t];
     };
-    dp.load(nc - 1);
-    load_tri<3>(pf, pt + (nc - 1) * pstep, pat, low, true);
+    dp.load(c1 - 1);
+    load_tri<3>(pf, pt + (c1 - 1) * pstep, pat, low, true);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       dn[t] = dp.get(t);
       sb::split_store4<NP>(ol + (16 * t + lr) * kLdT + ib, VT * kLdT, dn[t]);
     }
-    dp.load(max(nc - 2, 0));
+    dp.load(max(c1 - 2, c0));
     lds_barrier();
     share();
-    load_tri<3>(pf, pt + max(nc - 2, 0) * pstep, pat, low, true);
+    load_tri<3>(pf, pt + max(c1 - 2, c0) * pstep, pat, low, true);
     lds_barrier();
     // Y and dV of chunk c, which the chain has left in yf
     auto finish = [&](int c, const f32x4& beta) {
@@ -1059,10 +1072,10 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
       }
       vo.store(c, y);
     };
-    f32x4 gam = *reinterpret_cast<const f32x4*>(vec + (nc - 1) * vstep + kGam * kC + (unsigned)ib), beta = *reinterpret_cast<const f32x4*>(vec + (nc - 1) * vstep + kBeta * kC + (unsigned)ib);
+    f32x4 gam = *reinterpret_cast<const f32x4*>(vec + (c1 - 1) * vstep + kGam * kC + (unsigned)ib), beta = *reinterpret_cast<const f32x4*>(vec + (c1 - 1) * vstep + kBeta * kC + (unsigned)ib);
     f32x4 before = zero;                                   // beta of the chunk behind
-    for (int c = nc - 1; c >= 0; --c) {
-      const int next = max(c - 1, 0), next2 = max(c - 2, 0);
+    for (int c = c1 - 1; c >= c0; --c) {
+      const int next = max(c - 1, c0), next2 = max(c - 2, c0);
 #pragma unroll
       for (int t = 0; t < NT; ++t) { d[t] = dn[t]; dn[t] = dp.get(t); }
       dp.load(next2);
@@ -1076,12 +1089,12 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
       lds_barrier();                                       // 2: the chain has read zp
       share();
       load_tri<3>(pf, pt + next2 * pstep, pat, low, true);
-      if (c < nc - 1) finish(c + 1, before);
+      if (!BARE && c < c1 - 1) finish(c + 1, before);
       before = beta;
       beta = *reinterpret_cast<const f32x4*>(vec + next * vstep + kBeta * kC + (unsigned)ib);
       lds_barrier();                                       // 3
     }
-    finish(0, before);
+    if (!BARE) finish(c0, before);
   }
 }
 
@@ -1699,14 +1712,15 @@ int scan_tiles(const GdrArgs& a) { return a.segs > 1 ? 2 : SCAN_NT((long)a.n_seq
 unsigned scan_grid(const GdrArgs& a) { return (unsigned)(((long)a.n_seq * a.Hv * a.grid_segs + 7) / 8 * 8 * a.nvt); }
 
 template <typename T, int NP, int KB2, int NT>
-int run_scan(GdrArgs a, bool bwd, hipStream_t st, double flops) {
+int run_scan(GdrArgs a, bool bwd, hipStream_t st, double flops, bool bare = false) {
   a.nvt = a.vp / (16 * NT);
   if (bwd) {
-    a.grid_segs = 1;
+    a.grid_segs = bare ? a.segs - 1 : a.segs;
     constexpr int lds = ScanLds<NP, KB2, NT>::bwd_bytes;
-    HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(&gdr_scan_bwd_kernel<T, NP, KB2, NT>), lds, "gdr_backward"));
-    ProfScope ps("gdr_scan_bwd_kernel", st, flops, 0.0);
-    hipLaunchKernelGGL((gdr_scan_bwd_kernel<T, NP, KB2, NT>), dim3(scan_grid(a)), dim3(512), lds, st, a);
+    void (*const fn)(GdrArgs) = bare ? gdr_scan_bwd_kernel<T, NP, KB2, NT, true> : gdr_scan_bwd_kernel<T, NP, KB2, NT, false>;
+    HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(fn), lds, "gdr_backward"));
+    ProfScope ps(bare ? "gdr_segment_bwd_kernel" : "gdr_scan_bwd_kernel", st, flops, 0.0);
+    hipLaunchKernelGGL(fn, dim3(scan_grid(a)), dim3(512), lds, st, a);
   } else {
     a.grid_segs = a.segs;
     constexpr int lds = ScanLds<NP, KB2, NT>::fwd_bytes;
@@ -1738,8 +1752,9 @@ int run_join(GdrArgs a, bool bwd, hipStream_t st) {
 }
 template <typename T, int NP, int KB2>
 int run_scan(const GdrArgs& a, bool bwd, hipStream_t st, double flops) {
-  if (a.segs > 1 && !bwd) {
-    HHRL_TRY((run_segments<T, NP, KB2>(a, st)));
+  if (a.segs > 1) {
+    if (bwd) HHRL_TRY((run_scan<T, NP, KB2, 2>(a, true, st, 0.0, true)));
+    else HHRL_TRY((run_segments<T, NP, KB2>(a, st)));
     HHRL_TRY(run_join<KB2>(a, bwd, st));
   }
   return scan_tiles(a) == 2 ? run_scan<T, NP, KB2, 2>(a, bwd, st, flops) : run_scan<T, NP, KB2, 1>(a, bwd, st, flops);
