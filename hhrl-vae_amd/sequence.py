@@ -76,7 +76,13 @@ def _rows(name: str, t, shape, n: int, width: int, dtype, dev: int):
 def _device() -> int:
     if not torch.cuda.is_initialized():
         _need(torch.cuda.is_available(), "no GPU")
-    return torch.cuda.current_device()
+        torch.cuda.init()
+    return torch._C._cuda_getDevice()
+
+
+def _stream(dev: int) -> int:
+    """The raw stream that is current on a device (the current one, which a call has looked up already)."""
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 class GatedDelta:
@@ -96,6 +102,9 @@ class GatedDelta:
         _need(0 < K <= _lib.GDR_MAX_K and 0 < V <= _lib.GDR_MAX_V, "K=%d V=%d: up to %d, %d supported" % (K, V, _lib.GDR_MAX_K, _lib.GDR_MAX_V))
         self.Hk, self.Hv, self.K, self.V, self.dtype = Hk, Hv, K, V, dtype
         self.scale = float(K) ** -0.5 if scale is None else float(scale)
+        d = _lib.GdrDesc()                        # what every call of this layer has in common
+        d.dtype, d.Hk, d.Hv, d.K, d.V, d.scale = self.code, Hk, Hv, K, V, self.scale
+        self._common = bytes(d)
         self._lib = _lib.load()
 
     def workspace(self, n_seq: int, rows: int, device, packed: bool = True, no_backward: bool = False) -> torch.Tensor:
@@ -106,7 +115,7 @@ class GatedDelta:
         return torch.empty(n, dtype=torch.float32, device=device)
 
     def _desc(self, q, k, v, g, beta, ws, starts, lens, dev):
-        d = _lib.GdrDesc()
+        d = _lib.GdrDesc.from_buffer_copy(self._common)
         _need(isinstance(q, torch.Tensor), "q is not a tensor")
         if starts is not None:
             _need(lens is None, "starts and lens")
@@ -126,8 +135,7 @@ class GatedDelta:
         n = len(lead)
         key, val, head = (lead + (self.Hk, self.K), n, self.Hk * self.K, self.dtype, dev), \
             (lead + (self.Hv, self.V), n, self.Hv * self.V, self.dtype, dev), (lead + (self.Hv,), n, self.Hv, torch.float32, dev)
-        d.dtype, d.n_seq, d.rows = self.code, n_seq, rows
-        d.Hk, d.Hv, d.K, d.V, d.scale = self.Hk, self.Hv, self.K, self.V, self.scale
+        d.n_seq, d.rows = n_seq, rows
         d.q, d.ldq = _rows("q", q, *key)
         d.k, d.ldk = _rows("k", k, *key)
         d.v, d.ldv = _rows("v", v, *val)
@@ -149,7 +157,7 @@ class GatedDelta:
         d.o, d.ldo = _rows("o", o, *val)
         d.s0, d.s1 = self._state("s0", s0, n, dev), self._state("s1", s1, n, dev)
         d.no_backward = int(no_backward)
-        check(self._lib.hhrl_gdr_forward(C.byref(d), _lib.stream_ptr()))
+        check(self._lib.hhrl_gdr_forward(C.byref(d), _stream(dev)))
 
     def bwd(self, q, k, v, g, beta, d_o, dq, dk, dv, dg, dbeta, ws, d_s1=None, d_s0=None, starts=None, lens=None) -> None:
         """Gradients of <d_o, o> + <d_s1, s1> (either None: absent), written to dq, dk, dv, dg, dbeta and d_s0; ws as the
@@ -164,7 +172,7 @@ class GatedDelta:
         d.dv, d.lddv = _rows("dv", dv, *val)
         d.dg, d.lddg = _rows("dg", dg, *head)
         d.dbeta, d.lddbeta = _rows("dbeta", dbeta, *head)
-        check(self._lib.hhrl_gdr_backward(C.byref(d), _lib.stream_ptr()))
+        check(self._lib.hhrl_gdr_backward(C.byref(d), _stream(dev)))
 
     def step(self, q, k, v, g, beta, o, state, state_out=None, slots=None) -> None:
         """One token for each of B rows (q, k [B, Hk, K], v, o [B, Hv, V], g, beta [B, Hv]) against a pool of states
@@ -186,7 +194,7 @@ class GatedDelta:
             _need(B <= n, "%d rows for %d states" % (B, n))
         check(self._lib.hhrl_gdr_step(self.code, B, Hk, Hv, K, V, self.scale, *_rows("q", q, *key), *_rows("k", k, *key),
                                       *_rows("v", v, *val), *_rows("g", g, *head), *_rows("beta", beta, *head), *_rows("o", o, *val),
-                                      sp, so, n, sl, _lib.stream_ptr()))
+                                      sp, so, n, sl, _stream(dev)))
 
 
 class BlockNorm:
@@ -211,7 +219,11 @@ class BlockNorm:
         _need(eps >= 0, "eps=%g" % eps)
         self.D, self.H, self.post, self.pre, self.gate_act, self.gate_rows = D, H, post, pre, gate_act, gate_rows
         self.alpha, self.scale, self.eps, self.dtype = float(alpha), float(scale), float(eps), dtype
-        self._kinds = _NORMS[post], _NORMS[pre], _GATES[gate_act], gate_rows
+        d = _lib.BlockNormDesc()                  # what every call of this plan has in common
+        d.dtype, d.H, d.D = self.code, H, D
+        d.post, d.pre, d.gate_act, d.gate_rows = _NORMS[post], _NORMS[pre], _GATES[gate_act], gate_rows
+        d.alpha, d.scale, d.eps = self.alpha, self.scale, self.eps
+        self._common = bytes(d)
         self._lib = _lib.load()
 
     def workspace(self, M: int, device) -> torch.Tensor:
@@ -232,38 +244,46 @@ class BlockNorm:
         return ((n, self.D) if isinstance(t, torch.Tensor) and t.dim() == 2 else (n, 1, self.D), 1, self.D, torch.float32, dev)
 
     def _desc(self, x, y, gate, params, dev):
-        d = _lib.BlockNormDesc()
+        d = _lib.BlockNormDesc.from_buffer_copy(self._common)
         first = x if x is not None else y
         _need(isinstance(first, torch.Tensor) and first.dim() > 0, "neither x nor y")
         M = first.shape[0]
         _need(M > 0, "no rows")
         _need(y is not None or (gate is None and self.post == "none"), "a gate or a post norm without y")
         act = self._shape(first, M, dev)
-        d.dtype, d.M, d.H, d.D = self.code, M, self.H, self.D
-        d.post, d.pre, d.gate_act, d.gate_rows = self._kinds
-        d.alpha, d.scale, d.eps = self.alpha, self.scale, self.eps
+        d.M = M
         if x is not None:
             d.x, d.ldx = _rows("x", x, *act)
         if y is not None:
             d.y, d.ldy = _rows("y", y, *act)
         if gate is not None:
             d.gate, d.ldgate = _rows("gate", gate, *self._gate_shape(gate, M, act, dev))
-        for name, t in zip(self.PARAMS, params):
-            if t is not None:
-                _need(getattr(self, name[2:]) != "none", "%s without a %s norm" % (name, name[2:]))
-                setattr(d, name, _tensor(name, t, (self.D,), torch.float32, dev))
+        w_post, b_post, w_pre, b_pre = params
+        if w_post is not None or b_post is not None:
+            _need(self.post != "none", "parameters without a post norm")
+            if w_post is not None:
+                d.w_post = _tensor("w_post", w_post, (self.D,), torch.float32, dev)
+            if b_post is not None:
+                d.b_post = _tensor("b_post", b_post, (self.D,), torch.float32, dev)
+        if w_pre is not None or b_pre is not None:
+            _need(self.pre != "none", "parameters without a pre norm")
+            if w_pre is not None:
+                d.w_pre = _tensor("w_pre", w_pre, (self.D,), torch.float32, dev)
+            if b_pre is not None:
+                d.b_pre = _tensor("b_pre", b_pre, (self.D,), torch.float32, dev)
         return d, M, act
 
     def fwd(self, x=None, y=None, gate=None, w_post=None, b_post=None, w_pre=None, b_pre=None, out=None, h=None) -> None:
         """Writes r to out and pre(r) to h (either may be None; both may be x or y)."""
-        d, M, act = self._desc(x, y, gate, (w_post, b_post, w_pre, b_pre), _device())
+        dev = _device()
+        d, M, act = self._desc(x, y, gate, (w_post, b_post, w_pre, b_pre), dev)
         _need(out is not None or h is not None, "neither out nor h")
         _need(self.pre == "none" or h is not None, "a pre norm without h")
         if out is not None:
             d.out, d.ldo = _rows("out", out, *act)
         if h is not None:
             d.h, d.ldh = _rows("h", h, *act)
-        check(self._lib.hhrl_block_norm_forward(C.byref(d), _lib.stream_ptr()))
+        check(self._lib.hhrl_block_norm_forward(C.byref(d), _stream(dev)))
 
     def bwd(self, x=None, y=None, gate=None, w_post=None, b_post=None, w_pre=None, b_pre=None, d_out=None, d_h=None,
             dx=None, dy=None, dgate=None, dw_post=None, db_post=None, dw_pre=None, db_pre=None, ws=None) -> None:
@@ -293,4 +313,4 @@ class BlockNorm:
             _need(isinstance(ws, torch.Tensor), "ws is not a tensor")
             d.ws_floats = ws.numel()
             d.ws = _tensor("ws", ws, (d.ws_floats,), torch.float32, dev)
-        check(self._lib.hhrl_block_norm_backward(C.byref(d), _lib.stream_ptr()))
+        check(self._lib.hhrl_block_norm_backward(C.byref(d), _stream(dev)))

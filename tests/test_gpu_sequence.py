@@ -530,6 +530,52 @@ def test_block_norm_captured_and_replayed(seq):
             assert torch.equal(grads[k], g2[k])
 
 
+# --------------------------------------------------------------------------------------------------------- refusals
+def test_refusals_on_the_gpu(seq):
+    """Wrong types, shapes, strides and places raise ValueError, too small a workspace HipError, before anything is launched."""
+    from hhrl_vae_amd._lib import HipError
+    layer = seq.GatedDelta(1, 1, 64, 64, dtype=BF)
+    q, k, v, g, beta, d_o = (t.to(DEV) for t in make((1, 70), 1, 1, 64, 64, BF, 0))
+    o, ws = torch.full_like(v, 7.0), layer.workspace(1, 70, DEV)
+    good = dict(q=q, k=k, v=v, g=g, beta=beta, o=o, ws=ws)
+    for bad in (dict(q=q.float()), dict(q=q.cpu()), dict(q=q[0]), dict(v=v[:, :69]), dict(g=g.to(BF)), dict(k=k.transpose(2, 3)), dict(o=None),
+                dict(beta=beta[..., None]), dict(starts=torch.tensor([0, 70], device=DEV)), dict(lens=torch.tensor([70], dtype=torch.int32)),
+                dict(lens=torch.tensor([70, 1], dtype=torch.int32, device=DEV)), dict(s0=torch.zeros(2, 1, 64, 64, device=DEV)),
+                dict(s1=torch.zeros(1, 1, 64, 64, device=DEV, dtype=BF)), dict(ws=ws.view(-1, 1)), dict(ws=None)):
+        with pytest.raises(ValueError):
+            layer.fwd(**{**good, **bad})
+    for small in (ws[:1000], ws[1:]):
+        with pytest.raises(HipError):
+            layer.fwd(**{**good, "ws": small})
+    with pytest.raises(HipError):                   # a forward pass alone leaves no room for the backward pass
+        layer.fwd(**{**good, "ws": layer.workspace(1, 70, DEV, no_backward=True)})
+    with pytest.raises(HipError):
+        layer.bwd(q, k, v, g, beta, None, *[torch.empty_like(t) for t in (q, k, v, g, beta)], ws)
+    pool = torch.zeros(3, 1, 64, 64, device=DEV)
+    row = [t[0, :4].contiguous() for t in (q, k, v, g, beta, v)]
+    for bad in (dict(state=pool[:, 0]), dict(state=pool.to(BF)), dict(slots=torch.zeros(4, dtype=torch.int64, device=DEV)), dict(slots=None),
+                dict(state_out=torch.zeros(4, 1, 64, 64, device=DEV)), dict(slots=torch.zeros(3, dtype=torch.int32, device=DEV))):
+        with pytest.raises(ValueError):
+            layer.step(*row, **{**dict(state=pool, slots=torch.zeros(4, dtype=torch.int32, device=DEV)), **bad})
+    x = torch.zeros(5, 64, device=DEV)
+    w = torch.ones(64, device=DEV)
+    plan = seq.BlockNorm(64, post="rms", pre="rms", gate_act="silu", gate_rows=2)
+    ok = dict(x=x, y=x, gate=x[:3], out=torch.full_like(x, 7.0), h=torch.empty_like(x), w_post=w, w_pre=w)
+    for bad in (dict(x=x.to(BF)), dict(y=x[:4]), dict(gate=x[:2]), dict(gate=x[:3].to(BF)), dict(w_post=w[:63]), dict(w_pre=w.to(BF)), dict(h=None), dict(y=None),
+                dict(out=x.t().contiguous().t()), dict(x=None, y=None)):
+        with pytest.raises(ValueError):
+            plan.fwd(**{**ok, **bad})
+    back = {k_: v_ for k_, v_ in ok.items() if k_ not in ("out", "h")}
+    for bad in (dict(), dict(d_out=x, d_h=x, dw_pre=w[:3]), dict(d_out=x, dw_pre=w), dict(d_out=x[:4]), dict(d_out=x, ws=torch.zeros(4, dtype=torch.int32, device=DEV))):
+        with pytest.raises(ValueError):
+            plan.bwd(**back, **bad)
+    for ws_ in (None, torch.zeros(16, device=DEV)):
+        with pytest.raises(HipError):
+            plan.bwd(**back, d_out=x, dw_post=w.clone(), ws=ws_)
+    torch.cuda.synchronize()
+    assert bool((o == 7.0).all()) and bool((ok["out"] == 7.0).all())
+
+
 # ---------------------------------------------------------------------------------------------------------- together
 def test_layer_of_all_of_them(seq):
     """A residual layer as it would be built: norm before the block, q, k, v, gate and output projections (hhrl_linear_*),
