@@ -703,8 +703,8 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
 
   if (tid < 256) {                                         // ---- the chain
     f32x4 S[KB2][NT];
-    if (seg == 0) load_state<KB2, NT>(S, a.s0, a, nh, w, v0, lr, lg);
-    else load_seg<KB2, NT>(S, a.seg_s + (nh * a.segs + seg) * Kp * a.vp, a.vp, w, v0, lr, lg);
+    if (a.segs == 1) load_state<KB2, NT>(S, a.s0, a, nh, w, v0, lr, lg);
+    else load_seg<KB2, NT>(S, a.seg_s + (nh * a.segs + seg) * Kp * a.vp, a.vp, w, v0, lr, lg);   // s0 may be s1 by now
     if (c0 < c1) scan_chain<T, NP, KB2, NT, TRAIN, false>(a, S, sl, xl, ul, wl, hv, a.V, v0, start, len, slot0, c0, c1);
     if (a.s1 && c1 == nc) store_state<KB2, NT>(S, a.s1, a, nh, w, v0, lr, lg);
   } else if (c0 < c1) {                                    // ---- the output, between the chain's barriers
@@ -831,8 +831,9 @@ __global__ __launch_bounds__(256, 2) void gdr_segment_kernel(GdrArgs a) {
   }
 }
 
-// The first states of the segments behind the first, one after the other (backward: the gradients behind the segments in
-// front of the last, from the last): S <- M S + N, 16 columns per workgroup.
+// The first states of the segments, one after the other (backward: the gradients behind the segments, from the last):
+// S <- M S + N, 16 columns per workgroup.  The scan takes all of them from here, s0 (d_s1) too: the workgroup of another
+// segment may have written s1 over it by then.
 template <int KB2>
 __global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
   constexpr int Kp = 64 * KB2, KB = Kp / 32, LDS_S = Kp + 8;
@@ -847,6 +848,7 @@ __global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
   const long nh = (long)n * a.Hv + hv;
   f32x4 S[KB2][1];
   load_state<KB2, 1>(S, bwd ? a.d_s1 : a.s0, a, nh, w, v0, lr, lg);
+  store_seg<KB2, 1>(S, a.seg_s + (nh * a.segs + (bwd ? max(ns - 1, 0) : 0)) * Kp * a.vp, a.vp, w, v0, lr, lg);
   for (int i = 0; i + 1 < ns; ++i) {
     const int g = bwd ? ns - 1 - i : i;
     const long at = nh * a.segs + g;
@@ -919,7 +921,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
   // Barriers of a chunk: 1 (dl), 2 (zl), 3 (yl, yf; gl, zp by the others).  Two more in front of the walk.
   if (tid < 256) {                                         // ---- the chain
     f32x4 dS[KB2][NT];
-    if (BARE || c1 == nc) load_state<KB2, NT>(dS, c1 == nc ? a.d_s1 : nullptr, a, nh, w, v0, lr, lg);
+    if (BARE || a.segs == 1) load_state<KB2, NT>(dS, c1 == nc ? a.d_s1 : nullptr, a, nh, w, v0, lr, lg);
     else load_seg<KB2, NT>(dS, a.seg_s + (nh * a.segs + seg) * Kp * a.vp, a.vp, w, v0, lr, lg);
     if (c0 < c1) {
       bf16x8 kf[KB][NP], mf[2][3], ktf[KB2][2][NP], qtf[KB2][2][NP];

@@ -143,6 +143,27 @@ def test_gdr_long_sequences_with_few_heads(seq, dtype, K, V, Hv, lens):
     check_gdr(seq, dtype, 1, Hv, K, V, ranges, lead, starts=starts, seed=K + V, gscale=0.05)
 
 
+@pytest.mark.parametrize("T", [100, 3333])
+def test_gdr_states_in_place(seq, T):
+    """s1 over s0 and d_s0 over d_s1, of one walk and of segments that run side by side: the same bits as apart."""
+    q, k, v, g, beta, d_o = (t.to(DEV) for t in make((2, T), 1, 1, 64, 32, BF, T, 0.05))
+    layer = seq.GatedDelta(1, 1, 64, 32, dtype=BF)
+    ws = layer.workspace(2, 2 * T, DEV, packed=False)
+    gen = torch.Generator().manual_seed(T)
+    s0, d_s1 = (torch.randn(2, 1, 64, 32, generator=gen).to(DEV) for _ in range(2))
+
+    def go(s, s1, d, d0):
+        o, grads = torch.empty_like(v), [torch.empty_like(t) for t in (q, k, v, g, beta)]
+        layer.fwd(q, k, v, g, beta, o, ws, s0=s, s1=s1)
+        layer.bwd(q, k, v, g, beta, d_o, *grads, ws, d_s1=d, d_s0=d0)
+        return [o, s1, d0] + grads
+    want = go(s0, torch.empty_like(s0), d_s1, torch.empty_like(d_s1))
+    for _ in range(3):
+        s, d = s0.clone(), d_s1.clone()
+        for a, b in zip(go(s, s, d, d), want):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("wide", [8, 3])
 def test_gdr_columns_of_wider_buffers(seq, dtype, wide):
