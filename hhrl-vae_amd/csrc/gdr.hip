@@ -1681,9 +1681,9 @@ int gdr_check(const hhrl_gdr_desc* d, const char* who) {
   const long most = 1L << 22;                    // offsets inside a chunk are 31-bit byte numbers
   HHRL_REQUIRE(d->ldq < most && d->ldk < most && d->ldv < most, "%s: leading dimension of an input beyond %ld", who, most - 1);
   const long ns = slots_of(d->n_seq, d->rows, d->starts != nullptr);
-  HHRL_REQUIRE(ns < (1L << 31), "%s: %ld chunks", who, ns);
-  const long blocks = ((long)d->n_seq * d->Hv + 7) / 8 * 8 * ((d->V + 31) / 32 * 2) * 16;     // up to 16 segments
-  HHRL_REQUIRE(blocks < (1L << 31), "%s: n_seq*Hv too large", who);
+  const long threads = 1L << 32;                 // a launch has fewer than this; workgroups of a scan (segments and 16-column tiles: few heads only)
+  const long scan = (((long)d->n_seq * d->Hv + 7) / 8 * 8) * ((d->V + 31) / 32);
+  HHRL_REQUIRE(ns < threads / 512 && scan < threads / 512, "%s: %ld chunks, n_seq*Hv*V/32 = %ld: too many for a launch", who, ns, scan);
   return HHRL_OK;
 }
 
@@ -1857,7 +1857,7 @@ int hhrl_gdr_step(int dtype, int B, int Hk, int Hv, int K, int V, float scale, c
   a.o = o; a.ldo = ldo; a.sin = state_in; a.sout = state_out; a.slots = slots;
   a.nvt = ceil_div(V, vec ? 64 : 16);
   const long grid = (long)B * Hv * a.nvt;
-  HHRL_REQUIRE(grid < (1L << 31), "gdr_step: B*Hv*V too large");
+  HHRL_REQUIRE(grid < (1L << 24), "gdr_step: B*Hv*V too large: %ld workgroups of 256 threads", grid);
   hipStream_t st = as_stream(stream);
   ProfScope ps("gdr_step_kernel", st, 6.0 * B * Hv * K * V, 8.0 * B * Hv * K * V);
   if (dtype == HHRL_BF16) {

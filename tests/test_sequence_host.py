@@ -48,6 +48,19 @@ def test_gdr_refuses(lib, over, word):
         assert word in lib.hhrl_last_error(), lib.hhrl_last_error()
 
 
+@pytest.mark.parametrize("over", [dict(n_seq=1 << 23, rows=1 << 23), dict(n_seq=4096, rows=4096, Hk=1, Hv=128, V=512, K=1, ldv=1 << 16, ldg=128, ldbeta=128)])
+def test_gdr_refuses_more_than_a_launch_holds(lib, over):
+    """A launch has fewer than 2^32 threads: 512 for each chunk, and for each 32 columns of a sequence's head."""
+    for fn in (lib.hhrl_gdr_forward, lib.hhrl_gdr_backward):
+        assert fn(C.byref(gdr_desc(ldo=1 << 16, lddo=1 << 16, lddv=1 << 16, lddg=128, lddbeta=128, **over)), None) == 1
+        assert b"too many" in lib.hhrl_last_error(), lib.hhrl_last_error()
+
+
+def test_gdr_step_refuses_more_than_a_launch_holds(lib):
+    assert lib.hhrl_gdr_step(1, 8192, 1, 256, 32, 512, 1.0, FAKE, 32, FAKE, 32, FAKE, 1 << 17, FAKE, 256, FAKE, 256, FAKE, 1 << 17, FAKE, FAKE, 8192, None, None) == 1
+    assert b"too large" in lib.hhrl_last_error(), lib.hhrl_last_error()
+
+
 @pytest.mark.parametrize("over", [dict(o=None), dict(ldo=255), dict(ldo=1 << 22)])
 def test_gdr_forward_refuses(lib, over):
     assert lib.hhrl_gdr_forward(C.byref(gdr_desc(**over)), None) == 1
