@@ -37,9 +37,26 @@ using sb::bf16x8;
 using sb::f32x4;
 
 constexpr int kC = 64;             // tokens per chunk
-constexpr int kLdT = kC + 8;       // row stride of an LDS image that runs along the tokens (16 rows: 16 distinct bank groups)
-constexpr int kLdM = kC + 4;       // row stride of an fp32 image
+constexpr int kLdM = kC + 4;       // row stride of prep's fp32 images
 constexpr float kGMin = -1e4f;     // log decays are clamped here: exp() of it is 0, and infinities would leave NaN differences
+
+// Images in LDS that matrix fragments are read from: rows of P pieces of 16 bytes, without padding, the pieces of a row
+// exchanged by its number.  A fragment read (lane: row l & 15, piece p + (l >> 4)) goes in four cycles of 16 lanes, rows
+// 0-3, 12-15 of one piece with rows 4-11 of the next or the other way round, and the exchange gives these 16 different
+// places in the 256 bytes of a cycle; so it does for the 8-byte stores of 16 rows.  Measured per wave: read 4.2 cycles,
+// 8.0 from rows padded by 16 bytes, which the grads kernel was bound by; store 8 either way (16 with 32 bytes of padding,
+// which read in 4.2 as well).
+template <int P>
+__device__ __forceinline__ int place(int row, int piece) {
+  static_assert(P == 4 || P == 8 || P == 16, "pieces of a row");
+  const int x = row >> 2 & 3;
+  return row * P + (piece ^ (P == 16 ? row & 15 : P == 8 ? row >> 1 & 7 : (((x << 1) ^ x) & 2) | x >> 1));
+}
+// element i of a row of N bf16 (fp32: multiples of 4)
+template <int N>
+__device__ __forceinline__ int at16(int row, int i) { return place<N / 8>(row, i >> 3) * 8 + (i & 7); }
+template <int N>
+__device__ __forceinline__ int at32(int row, int i) { return place<N / 4>(row, i >> 2) * 4; }
 
 struct GdrArgs {
   int n_seq, Hk, Hv, K, V, rep;
@@ -62,7 +79,7 @@ struct GdrArgs {
   long lddq, lddk, lddv;
   float *dg, *dbeta;
   long lddg, lddbeta;
-  int pack, wide, train, vp, nvt;
+  int pack, wide, wide_v, train, vp, nvt;
   // ws, per chunk and key head: k, q [64][terms][Kp] (pack), their transposes [Kp][terms][64];
   //     per chunk and value head: M, P (two terms for bf16: what o takes) and their transposes [64][terms][64], five rows of 64 floats, and for the
   //     backward pass W, Y [vp/32][64][32] and S, dS [vp/32][Kp][32], fp32 (tiles of 32 columns).  The terms of a row lie side by side, so that a lane's
@@ -134,8 +151,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, lo
 // blocks beyond the diagonal are neither written nor read.
 template <int NP, int KB2>
 struct PrepLds {
-  static constexpr int Kp = 64 * KB2, LDK = Kp + 8;
-  static constexpr int kq = 2 * NP * kC * LDK * 2;             // bytes: k and q as terms
+  static constexpr int Kp = 64 * KB2;
+  static constexpr int kq = 2 * NP * kC * Kp * 2;             // bytes: k and q as terms
   static constexpr int img = (2 * kC + 32) * kLdM * 4;         // I + A, its inverse, a product of the solve: over them once they are used
   static constexpr int over = kq > img ? kq : img;
   static constexpr int bytes = over + 3 * kC * 4;
@@ -143,10 +160,10 @@ struct PrepLds {
 template <typename T, int NP, int KB2>
 __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs a) {
   using L = PrepLds<NP, KB2>;
-  constexpr int Kp = L::Kp, LDK = L::LDK, KG = Kp / 8, NO = NP == 1 ? 2 : 3;
+  constexpr int Kp = L::Kp, KG = Kp / 8, NO = NP == 1 ? 2 : 3;
   extern __shared__ __align__(16) char smem[];
-  __bf16* const kl = reinterpret_cast<__bf16*>(smem);          // [NP][64][LDK]
-  __bf16* const ql = kl + NP * kC * LDK;
+  __bf16* const kl = reinterpret_cast<__bf16*>(smem);          // [NP][64][Kp]
+  __bf16* const ql = kl + NP * kC * Kp;
   float* const lm = reinterpret_cast<float*>(smem);            // [64][kLdM] I + A
   float* const mm = lm + kC * kLdM;                            // [64][kLdM] its inverse
   float* const tm = mm + kC * kLdM;                            // [32][kLdM]
@@ -181,7 +198,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int g = u * 256 + tid, i = g / KG, c = (g - i * KG) * 8;
-        *reinterpret_cast<bf16x8*>((side ? ql : kl) + i * LDK + c) = x[side][u];
+        *reinterpret_cast<bf16x8*>((side ? ql : kl) + at16<Kp>(i, c)) = x[side][u];
       }
   } else {
     for (int side = 0; side < 2; ++side) {
@@ -211,7 +228,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
         sb::split8<NP>(x, t);
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
-          *reinterpret_cast<bf16x8*>(dst + (p * kC + i) * LDK + c) = t[p];
+          *reinterpret_cast<bf16x8*>(dst + p * kC * Kp + at16<Kp>(i, c)) = t[p];
           if (a.pack) *reinterpret_cast<bf16x8*>(pk + ((long)i * NP + p) * Kp + c) = t[p];
         }
       }
@@ -226,7 +243,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
       const int k = u % (Kp / 2) * 2, r = u / (Kp / 2), i0 = (r & 7) * 8, p = r >> 3;
       unsigned x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const unsigned*>(src + (p * kC + i0 + e) * LDK + k);
+      for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const unsigned*>(src + p * kC * Kp + at16<Kp>(i0 + e, k));
       u32x4 lo, hi;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -245,14 +262,14 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
 #pragma unroll
   for (int kb = 0; kb < Kp / 32; ++kb) {
     bf16x8 ka[NP], qa[NP];
-    const int off = (16 * wave + lr) * LDK + 32 * kb + 8 * lg;
-    sb::load_frag<NP>(ka, kl + off, kC * LDK);
-    sb::load_frag<NP>(qa, ql + off, kC * LDK);
+    const int off = at16<Kp>(lr, 32 * kb + 8 * lg);
+    sb::load_frag<NP>(ka, kl + 16 * wave * Kp + off, kC * Kp);
+    sb::load_frag<NP>(qa, ql + 16 * wave * Kp + off, kC * Kp);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if (t <= wave) {
         bf16x8 b[NP];
-        sb::load_frag<NP>(b, kl + (16 * t + lr) * LDK + 32 * kb + 8 * lg, kC * LDK);
+        sb::load_frag<NP>(b, kl + 16 * t * Kp + off, kC * Kp);
         sb::mma<NP, NP>(kk[t], ka, b);
         if (a.train) sb::mma<NP, NP>(qk[t], qa, b);
         sb::mma<NP, NP>(kq[t], b, qa);                         // row 16*t + ..: k's token j, column 16*wave + lr: q's token i
@@ -397,10 +414,10 @@ __device__ __forceinline__ bool scan_tile(const GdrArgs& a, int vt, int& n, int&
 // a row per state column
 template <int NP, int KB2, int NT>
 struct ScanLds {
-  static constexpr int Kp = 64 * KB2, VT = 16 * NT, LDS_S = Kp + 8;
-  static constexpr int S = 3 * VT * LDS_S, X = 3 * VT * kLdT, F = VT * kLdM;     // elements
+  static constexpr int Kp = 64 * KB2, VT = 16 * NT;
+  static constexpr int S = 3 * VT * Kp, X = 3 * VT * kC, F = VT * kC;     // elements
   static constexpr int fwd_bytes = 2 * (S + 2 * X) + 8 * F;
-  static constexpr int bwd_bytes = 2 * (S + 3 * X + NP * VT * kLdT) + 12 * F;
+  static constexpr int bwd_bytes = 2 * (S + 3 * X + NP * VT * kC) + 12 * F;
 };
 
 // Operand rows of k or q, token 16*w + lr of a chunk, from the packed terms (whose rows behind the sequence are 0) or from
@@ -580,7 +597,7 @@ template <typename T, int NP, int KB2, int NT, bool TRAIN, bool BARE>
 __device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT], __bf16* sl, __bf16* xl, __bf16* ul, float* wl, int hv, int vcols,
                                            int v0, long start, int len, long slot0, int c0, int c1) {
   using L = ScanLds<NP, KB2, NT>;
-  constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT, LDS_S = L::LDS_S;
+  constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT;
   const int hk = hv / a.rep, lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
   const int ib = 16 * w + 4 * lg, ia = 16 * w + lr;        // first of four result rows; operand row
   const bool high = w >= 2;                                // M is lower triangular: rows < 32 read 32 columns
@@ -609,7 +626,7 @@ __device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT]
     for (int t = 0; t < KB2; ++t)
 #pragma unroll
       for (int u = 0; u < NT; ++u)
-        sb::split_store4<3>(sl + (16 * u + lr) * LDS_S + 16 * (KB2 * w + t) + 4 * lg, VT * LDS_S, S[t][u]);
+        sb::split_store4<3>(sl + 16 * u * Kp + at16<Kp>(lr, 16 * (KB2 * w + t) + 4 * lg), VT * Kp, S[t][u]);
     lds_barrier();
     f32x4 ks[NT];
 #pragma unroll
@@ -619,14 +636,14 @@ __device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT]
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         bf16x8 b[3];
-        sb::load_frag<3>(b, sl + (16 * t + lr) * LDS_S + 32 * kb + 8 * lg, VT * LDS_S);
+        sb::load_frag<3>(b, sl + 16 * t * Kp + at16<Kp>(lr, 32 * kb + 8 * lg), VT * Kp);
         sb::mma<NP, 3>(ks[t], kf[kb], b);
       }
     kp.load(kf, next);
     const ScanVec vc = vn;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-      sb::split_store4<3>(xl + (16 * t + lr) * kLdT + ib, VT * kLdT, vc.beta * (vp.get(t) - vc.gam * ks[t]));
+      sb::split_store4<3>(xl + 16 * t * kC + at16<kC>(lr, ib), VT * kC, vc.beta * (vp.get(t) - vc.gam * ks[t]));
     vp.load(next);
     vn.load(vecp, ib);
     if constexpr (TRAIN) {
@@ -649,14 +666,14 @@ __device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT]
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           bf16x8 b[3];
-          sb::load_frag<3>(b, xl + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+          sb::load_frag<3>(b, xl + 16 * t * kC + at16<kC>(lr, 32 * kb + 8 * lg), VT * kC);
           sb::mma<3, 3>(wt[t], mf[kb], b);
         }
     load_tri<3>(mf, mp, mat, true, high);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      sb::split_store4<3>(ul + (16 * t + lr) * kLdT + ib, VT * kLdT, vc.tail * wt[t]);
-      if constexpr (!BARE) *reinterpret_cast<f32x4*>(wl + (c & 1) * L::F + (16 * t + lr) * kLdM + ib) = wt[t];
+      sb::split_store4<3>(ul + 16 * t * kC + at16<kC>(lr, ib), VT * kC, vc.tail * wt[t]);
+      if constexpr (!BARE) *reinterpret_cast<f32x4*>(wl + (c & 1) * L::F + 16 * t * kC + at32<kC>(lr, ib)) = wt[t];
     }
     lds_barrier();
 #pragma unroll
@@ -668,7 +685,7 @@ __device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT]
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
         bf16x8 b[3];
-        sb::load_frag<3>(b, ul + (16 * u + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+        sb::load_frag<3>(b, ul + 16 * u * kC + at16<kC>(lr, 32 * kb + 8 * lg), VT * kC);
 #pragma unroll
         for (int t = 0; t < KB2; ++t) sb::mma<NP, 3>(S[t][u], ktf[t][kb], b);
       }
@@ -679,13 +696,13 @@ __device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT]
 template <typename T, int NP, int KB2, int NT, bool TRAIN>
 __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
   using L = ScanLds<NP, KB2, NT>;
-  constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT, LDS_S = L::LDS_S;
+  constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT;
   constexpr int NO = NP == 1 ? 2 : 3;                      // terms behind o: a bf16 o takes 2^-17, an fp32 one all three
   extern __shared__ __align__(16) char smem[];
-  __bf16* const sl = reinterpret_cast<__bf16*>(smem);      // [3][VT][LDS_S] S
-  __bf16* const xl = sl + L::S;                            // [3][VT][kLdT]  beta (V - gam K S)
-  __bf16* const ul = xl + L::X;                            // [3][VT][kLdT]  exp(G_C - G) W
-  float* const wl = reinterpret_cast<float*>(ul + L::X);   // [2][VT][kLdM]  W, of the chunk at hand and the one in front of it
+  __bf16* const sl = reinterpret_cast<__bf16*>(smem);      // [3][VT][Kp] S
+  __bf16* const xl = sl + L::S;                            // [3][VT][kC]  beta (V - gam K S)
+  __bf16* const ul = xl + L::X;                            // [3][VT][kC]  exp(G_C - G) W
+  float* const wl = reinterpret_cast<float*>(ul + L::X);   // [2][VT][kC]  W, of the chunk at hand and the one in front of it
   int n, hv, v0, seg;
   if (!scan_tile(a, VT, n, hv, v0, seg)) return;
   const int hk = hv / a.rep;
@@ -723,10 +740,9 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float x[8];
-        const float* const src = wc + (16 * t + lr) * kLdM + 32 * kb + 8 * lg;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(src + 4 * h);
+          const f32x4 y = *reinterpret_cast<const f32x4*>(wc + 16 * t * kC + at32<kC>(lr, 32 * kb + 8 * lg + 4 * h));
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[4 * h + e] = y[e];
         }
@@ -742,7 +758,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
         float* const wp = a.w + ((((slot0 + c) * a.Hv + hv) * (a.vp / 32) + v0 / 32) * kC) * 32 + (v0 & 16);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(wl + (c & 1) * L::F + (16 * t + lr) * kLdM + ib);
+          const f32x4 y = *reinterpret_cast<const f32x4*>(wl + (c & 1) * L::F + 16 * t * kC + at32<kC>(lr, ib));
 #pragma unroll
           for (int e = 0; e < 4; ++e) wp[(unsigned)(ib * 32 + lr) + e * 32 + 16 * t] = y[e];
         }
@@ -763,7 +779,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           bf16x8 b[NO];
-          sb::load_frag<NO>(b, sl + (16 * t + lr) * LDS_S + 32 * kb + 8 * lg, VT * LDS_S);
+          sb::load_frag<NO>(b, sl + 16 * t * Kp + at16<Kp>(lr, 32 * kb + 8 * lg), VT * Kp);
           sb::mma<NP, NO>(qn[t], qf[kb], b);
         }
       qp.load(qf, min(c + 1, c1 - 1));
@@ -836,8 +852,8 @@ __global__ __launch_bounds__(256, 2) void gdr_segment_kernel(GdrArgs a) {
 // segment may have written s1 over it by then.
 template <int KB2>
 __global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
-  constexpr int Kp = 64 * KB2, KB = Kp / 32, LDS_S = Kp + 8;
-  __shared__ __align__(16) __bf16 sl[3 * 16 * LDS_S];
+  constexpr int Kp = 64 * KB2, KB = Kp / 32;
+  __shared__ __align__(16) __bf16 sl[3 * 16 * Kp];
   int n, hv, v0, seg;
   if (!scan_tile(a, 16, n, hv, v0, seg)) return;
   long start, slot0;
@@ -861,12 +877,12 @@ __global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
     f32x4 next[KB2][1];
     load_seg<KB2, 1>(next, a.seg_n + at * Kp * a.vp, a.vp, w, v0, lr, lg);
 #pragma unroll
-    for (int t = 0; t < KB2; ++t) sb::split_store4<3>(sl + lr * LDS_S + 16 * (KB2 * w + t) + 4 * lg, 16 * LDS_S, S[t][0]);
+    for (int t = 0; t < KB2; ++t) sb::split_store4<3>(sl + at16<Kp>(lr, 16 * (KB2 * w + t) + 4 * lg), 16 * Kp, S[t][0]);
     __syncthreads();
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       bf16x8 b[3];
-      sb::load_frag<3>(b, sl + lr * LDS_S + 32 * kb + 8 * lg, 16 * LDS_S);
+      sb::load_frag<3>(b, sl + at16<Kp>(lr, 32 * kb + 8 * lg), 16 * Kp);
 #pragma unroll
       for (int t = 0; t < KB2; ++t) {
         float x[8];
@@ -892,15 +908,15 @@ __global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
 template <typename T, int NP, int KB2, int NT, bool BARE>
 __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
   using L = ScanLds<NP, KB2, NT>;
-  constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT, LDS_S = L::LDS_S;
+  constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT;
   extern __shared__ __align__(16) char smem[];
-  __bf16* const dl = reinterpret_cast<__bf16*>(smem);      // [3][VT][LDS_S] dS'
-  __bf16* const gl = dl + L::S;                            // [3][VT][kLdT]  scale gam dO
-  __bf16* const zl = gl + L::X;                            // [3][VT][kLdT]  Z
-  __bf16* const yl = zl + L::X;                            // [3][VT][kLdT]  -gam beta Y
-  __bf16* const ol = yl + L::X;                            // [NP][VT][kLdT] dO
-  float* const zp = reinterpret_cast<float*>(ol + NP * VT * kLdT);   // [VT][kLdM] scale P^T dO
-  float* const yf = zp + L::F;                             // [2][VT][kLdM] Y, of the chunk at hand and the one behind it
+  __bf16* const dl = reinterpret_cast<__bf16*>(smem);      // [3][VT][Kp] dS'
+  __bf16* const gl = dl + L::S;                            // [3][VT][kC]  scale gam dO
+  __bf16* const zl = gl + L::X;                            // [3][VT][kC]  Z
+  __bf16* const yl = zl + L::X;                            // [3][VT][kC]  -gam beta Y
+  __bf16* const ol = yl + L::X;                            // [NP][VT][kC] dO
+  float* const zp = reinterpret_cast<float*>(ol + NP * VT * kC);   // [VT][kC] scale P^T dO
+  float* const yf = zp + L::F;                             // [2][VT][kC] Y, of the chunk at hand and the one behind it
   int n, hv, v0, seg;
   if (!scan_tile(a, VT, n, hv, v0, seg)) return;
   const int hk = hv / a.rep;
@@ -954,7 +970,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
         for (int t = 0; t < KB2; ++t)
 #pragma unroll
           for (int u = 0; u < NT; ++u)
-            sb::split_store4<3>(dl + (16 * u + lr) * LDS_S + 16 * (KB2 * w + t) + 4 * lg, VT * LDS_S, dS[t][u]);
+            sb::split_store4<3>(dl + 16 * u * Kp + at16<Kp>(lr, 16 * (KB2 * w + t) + 4 * lg), VT * Kp, dS[t][u]);
         lds_barrier();
         f32x4 z[NT], y[NT];
 #pragma unroll
@@ -964,14 +980,14 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             bf16x8 b[3];
-            sb::load_frag<3>(b, dl + (16 * t + lr) * LDS_S + 32 * kb + 8 * lg, VT * LDS_S);
+            sb::load_frag<3>(b, dl + 16 * t * Kp + at16<Kp>(lr, 32 * kb + 8 * lg), VT * Kp);
             sb::mma<NP, 3>(z[t], kf[kb], b);
           }
         kp.load(kf, next);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const f32x4 p = *reinterpret_cast<const f32x4*>(zp + (16 * t + lr) * kLdM + ib);
-          sb::split_store4<3>(zl + (16 * t + lr) * kLdT + ib, VT * kLdT, p + vc.tail * z[t]);
+          const f32x4 p = *reinterpret_cast<const f32x4*>(zp + 16 * t * kC + at32<kC>(lr, ib));
+          sb::split_store4<3>(zl + 16 * t * kC + at16<kC>(lr, ib), VT * kC, p + vc.tail * z[t]);
         }
         vn.load(vecp, ib);
         if constexpr (!BARE) {
@@ -991,14 +1007,14 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               bf16x8 b[3];
-              sb::load_frag<3>(b, zl + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+              sb::load_frag<3>(b, zl + 16 * t * kC + at16<kC>(lr, 32 * kb + 8 * lg), VT * kC);
               sb::mma<3, 3>(y[t], mf[kb], b);
             }
         load_tri<3>(mf, mp, mat, low, true);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          sb::split_store4<3>(yl + (16 * t + lr) * kLdT + ib, VT * kLdT, -vc.gam * vc.beta * y[t]);
-          if constexpr (!BARE) *reinterpret_cast<f32x4*>(yf + (c & 1) * L::F + (16 * t + lr) * kLdM + ib) = y[t];
+          sb::split_store4<3>(yl + 16 * t * kC + at16<kC>(lr, ib), VT * kC, -vc.gam * vc.beta * y[t]);
+          if constexpr (!BARE) *reinterpret_cast<f32x4*>(yf + (c & 1) * L::F + 16 * t * kC + at32<kC>(lr, ib)) = y[t];
         }
         lds_barrier();
 #pragma unroll
@@ -1010,8 +1026,8 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
 #pragma unroll
           for (int u = 0; u < NT; ++u) {
             bf16x8 b[3], g[3];
-            sb::load_frag<3>(g, gl + (16 * u + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
-            sb::load_frag<3>(b, yl + (16 * u + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+            sb::load_frag<3>(g, gl + 16 * u * kC + at16<kC>(lr, 32 * kb + 8 * lg), VT * kC);
+            sb::load_frag<3>(b, yl + 16 * u * kC + at16<kC>(lr, 32 * kb + 8 * lg), VT * kC);
 #pragma unroll
             for (int t = 0; t < KB2; ++t) {
               sb::mma<NP, 3>(dS[t][u], qtf[t][kb], g);
@@ -1043,18 +1059,18 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             bf16x8 b[NP];
-            sb::load_frag<NP>(b, ol + (16 * t + lr) * kLdT + 32 * kb + 8 * lg, VT * kLdT);
+            sb::load_frag<NP>(b, ol + 16 * t * kC + at16<kC>(lr, 32 * kb + 8 * lg), VT * kC);
             sb::mma<3, NP>(z[t], pf[kb], b);
           }
 #pragma unroll
-      for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(zp + (16 * t + lr) * kLdM + ib) = a.scale * z[t];
+      for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(zp + 16 * t * kC + at32<kC>(lr, ib)) = a.scale * z[t];
     };
     dp.load(c1 - 1);
     load_tri<3>(pf, pt + (c1 - 1) * pstep, pat, low, true);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       dn[t] = dp.get(t);
-      sb::split_store4<NP>(ol + (16 * t + lr) * kLdT + ib, VT * kLdT, dn[t]);
+      sb::split_store4<NP>(ol + 16 * t * kC + at16<kC>(lr, ib), VT * kC, dn[t]);
     }
     dp.load(max(c1 - 2, c0));
     lds_barrier();
@@ -1067,7 +1083,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
       f32x4 y[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        y[t] = *reinterpret_cast<const f32x4*>(yf + (c & 1) * L::F + (16 * t + lr) * kLdM + ib);
+        y[t] = *reinterpret_cast<const f32x4*>(yf + (c & 1) * L::F + 16 * t * kC + at32<kC>(lr, ib));
 #pragma unroll
         for (int e = 0; e < 4; ++e) yp[(unsigned)(ib * 32 + lr) + e * 32 + 16 * t] = y[t][e];
         y[t] *= beta;
@@ -1084,8 +1100,8 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
       lds_barrier();                                       // 1: the chain has read the previous chunk's gl
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        sb::split_store4<3>(gl + (16 * t + lr) * kLdT + ib, VT * kLdT, a.scale * gam * d[t]);
-        sb::split_store4<NP>(ol + (16 * t + lr) * kLdT + ib, VT * kLdT, dn[t]);
+        sb::split_store4<3>(gl + 16 * t * kC + at16<kC>(lr, ib), VT * kC, a.scale * gam * d[t]);
+        sb::split_store4<NP>(ol + 16 * t * kC + at16<kC>(lr, ib), VT * kC, dn[t]);
       }
       gam = *reinterpret_cast<const f32x4*>(vec + next * vstep + kGam * kC + (unsigned)ib);
       lds_barrier();                                       // 2: the chain has read zp
@@ -1106,14 +1122,14 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
 // columns at a time as bf16 terms; the next 32 columns are on their way from memory meanwhile.
 template <int NP, int KB2>
 struct GradsLds {
-  static constexpr int Kp = 64 * KB2, LDV = 40;              // 32 columns + 8: 16 rows in 16 distinct bank groups
+  static constexpr int Kp = 64 * KB2, LDV = 32;              // columns at a time
   static constexpr int cols = 3 * LDV * (2 * Kp + 2 * kC) + NP * LDV * kC;       // elements: S, dS', W, Y, dO
   // afterwards, over them: R, B and their transposes; where k and q do not stay in LDS (three terms), 32 tokens of those and
   // of k and q at a time
-  static constexpr int LDH = 32 + 8;
-  static constexpr int tri = NP == 1 ? 4 * 3 * kC * kLdT : 4 * 3 * kC * LDH + 2 * NP * Kp * LDH;
+  static constexpr int LDR = NP == 1 ? kC : 32;
+  static constexpr int tri = 4 * 3 * kC * LDR + (NP == 1 ? 0 : 2 * NP * Kp * LDR);
   static constexpr int over = 2 * (cols > tri ? cols : tri);
-  static constexpr int kq = NP == 1 ? 2 * 2 * Kp * kLdT : 0;                     // bytes: k and q of the chunk, transposed (three terms do not fit)
+  static constexpr int kq = NP == 1 ? 2 * 2 * Kp * kC : 0;                     // bytes: k and q of the chunk, transposed (three terms do not fit)
   static constexpr int bytes = over + kq + (8 * kC + 8) * 4;
 };
 template <typename T, int NP, int KB2, bool GROUP>
@@ -1126,18 +1142,18 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
   __bf16* const wl = dl + 3 * Kp * LDV;                      // [3][64][LDV]
   __bf16* const yl = wl + 3 * kC * LDV;                      // [3][64][LDV]
   __bf16* const ol = yl + 3 * kC * LDV;                      // [NP][64][LDV]
-  constexpr int LDR = NP == 1 ? kLdT : L::LDH;
+  constexpr int LDR = L::LDR;
   __bf16* const rl = reinterpret_cast<__bf16*>(smem);        // [3][64][LDR] each
   __bf16* const bl = rl + 3 * kC * LDR;
   __bf16* const rt = bl + 3 * kC * LDR;
   __bf16* const bt = rt + 3 * kC * LDR;
-  // k and q, transposed: for the kernel's length (one term, [Kp][kLdT] each) or 32 tokens at a time ([NP][Kp][LDH] each)
+  // k and q, transposed: for the kernel's length (one term, [Kp][64] each) or 32 tokens at a time ([NP][Kp][32] each)
   __bf16* const kl = NP == 1 ? reinterpret_cast<__bf16*>(smem + L::over) : bt + 3 * kC * LDR;
-  __bf16* const ql = kl + (NP == 1 ? Kp * kLdT : NP * Kp * L::LDH);
+  __bf16* const ql = kl + NP * Kp * LDR;
   float* const rows = reinterpret_cast<float*>(smem + L::over + L::kq);    // [2 halves][3][64]: shares of dG, of dbeta, k.(tail E3)
   float* const yv = rows + 6 * kC;                                 // [64] Y.v
   float* const red = yv + kC;                                      // [8]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, w = wave >> 1, half = wave & 1, lr = lane & 15, lg = lane >> 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave >> 1, half = wave & 1, kt0 = 16 * KT * half;
   const long slot = blockIdx.x;
   const int hk = blockIdx.y;
   long row0;
@@ -1145,13 +1161,8 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
   slot_chunk(a, slot, row0, valid);
   if (valid == 0) return;
   const long hs = slot * a.Hk + hk;
-  const int ib = 16 * w + 4 * lg, ia = 16 * w + lr, kt0 = 16 * KT * half;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   const bool has_do = a.d_o != nullptr;
-  // cooperative loads: 8 columns of a row per thread
-  const int gi = (tid & 255) >> 2, gc = (tid & 3) * 8;       // token and columns of W, dO (threads 0..255), Y, v (the others)
-  const long rowc = row0 + min(gi, valid - 1);
-
   if constexpr (NP == 1) {
     const bf16x8* const gk = reinterpret_cast<const bf16x8*>(a.kt + hs * Kp * kC);
     const bf16x8* const gq = reinterpret_cast<const bf16x8*>(a.qt + hs * Kp * kC);
@@ -1160,7 +1171,7 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
     for (int u = 0; u < Kp / 64; ++u) { x[u] = gk[u * 512 + tid]; y[u] = gq[u * 512 + tid]; }
 #pragma unroll
     for (int u = 0; u < Kp / 64; ++u) {
-      const int at = (u * 64 + (tid >> 3)) * kLdT + (tid & 7) * 8;
+      const int at = at16<kC>(u * 64 + (tid >> 3), (tid & 7) * 8);
       *reinterpret_cast<bf16x8*>(kl + at) = x[u];
       *reinterpret_cast<bf16x8*>(ql + at) = y[u];
     }
@@ -1170,8 +1181,14 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
     for (int t = 0; t < (GROUP ? KT : 1); ++t) dqs[t] = dks[t] = zero;
   }
-  for (int r = 0; r < a.rep; ++r) {
-    const int hv = hk * a.rep + r;
+  for (int r = 0; r < (GROUP ? a.rep : 1); ++r) {
+    int lane = tid & 63;
+    if (GROUP) asm("" : "+v"(lane));                         // or every address below would be kept over the loop, in registers that are not there
+    const int lr = lane & 15, lg = lane >> 4, ib = 16 * w + 4 * lg;
+    // cooperative loads: 8 columns of a row per thread
+    const int gi = (64 * (wave & 3) + lane) >> 2, gc = (lane & 3) * 8;   // token and columns of W, dO (waves 0 .. 3), Y, v (the others)
+    const long rowc = row0 + min(gi, valid - 1);
+    const int hv = hk * (GROUP ? a.rep : 1) + r;
     const long vs = slot * a.Hv + hv;
     f32x4 e1[KT], e2[KT], e3[KT], dp[2], da[2];
 #pragma unroll
@@ -1179,14 +1196,14 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) dp[t] = da[t] = zero;
     float sdot = 0.f, ydot = 0.f;
-    const bool has_s = KB2 == 2 || tid < 256;
-    const float* const ps = a.s + (vs * (a.vp / 32) * Kp + (tid >> 2) % Kp) * 32 + gc;
-    const float* const pd = a.ds + (vs * (a.vp / 32) * Kp + (tid >> 2) % Kp) * 32 + gc;
-    const float* const pw = (tid < 256 ? a.w : a.y) + (vs * (a.vp / 32) * kC + gi) * 32 + gc;
-    const T* const px = tid < 256 ? (has_do ? static_cast<const T*>(a.d_o) + rowc * a.lddo + (long)hv * a.V : static_cast<const T*>(a.v))
+    const bool has_s = KB2 == 2 || wave < 4;
+    const float* const ps = a.s + (vs * (a.vp / 32) * Kp + ((64 * wave + lane) >> 2) % Kp) * 32 + gc;
+    const float* const pd = a.ds + (vs * (a.vp / 32) * Kp + ((64 * wave + lane) >> 2) % Kp) * 32 + gc;
+    const float* const pw = (wave < 4 ? a.w : a.y) + (vs * (a.vp / 32) * kC + gi) * 32 + gc;
+    const T* const px = wave < 4 ? (has_do ? static_cast<const T*>(a.d_o) + rowc * a.lddo + (long)hv * a.V : static_cast<const T*>(a.v))
                                   : static_cast<const T*>(a.v) + rowc * a.ldv + (long)hv * a.V;
     f32x4 xs[2], xd[2], xw[2];
-    unsigned xo[8];
+    u32x4 xo[sizeof(T) / 2];                                 // eight columns of dO or v, as they come
     auto request = [&](int vb) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -1194,65 +1211,71 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
         xd[h] = *reinterpret_cast<const f32x4*>(pd + vb * Kp + 4 * h);
         xw[h] = *reinterpret_cast<const f32x4*>(pw + vb * kC + 4 * h);
       }
+      if (a.wide_v) {                                          // V a multiple of 8, 16-byte aligned rows
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int v = min(vb + gc + e, a.V - 1);
-        if constexpr (sizeof(T) == 2) xo[e] = *reinterpret_cast<const unsigned short*>(px + v);
-        else xo[e] = *reinterpret_cast<const unsigned*>(px + v);
+        for (int h = 0; h < (int)sizeof(T) / 2; ++h) xo[h] = *reinterpret_cast<const u32x4*>(px + min(vb + gc, a.V - 8) + 4 * h);
+      } else {
+        T raw[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) raw[e] = px[min(vb + gc + e, a.V - 1)];
+        __builtin_memcpy(xo, raw, sizeof(raw));
       }
     };
     request(0);
     for (int vb = 0; vb < a.vp; vb += 32) {
-      __syncthreads();
+      lds_barrier();
       {
         float x[8];
         bf16x8 t[3];
         if (has_s) {
-          const int k = tid >> 2;
+          const int k = (64 * wave + lane) >> 2;
 #pragma unroll
           for (int e = 0; e < 8; ++e) { x[e] = xs[e >> 2][e & 3]; sdot = fmaf(x[e], xd[e >> 2][e & 3], sdot); }
           sb::split8<3>(x, t);
 #pragma unroll
-          for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(sl + (p * Kp + k) * LDV + gc) = t[p];
+          for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(sl + p * Kp * LDV + at16<LDV>(k, gc)) = t[p];
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = xd[e >> 2][e & 3];
           sb::split8<3>(x, t);
 #pragma unroll
-          for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dl + (p * Kp + k) * LDV + gc) = t[p];
+          for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dl + p * Kp * LDV + at16<LDV>(k, gc)) = t[p];
         }
         float o[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          o[e] = gi < valid && vb + gc + e < a.V ? __uint_as_float(sizeof(T) == 2 ? xo[e] << 16 : xo[e]) : 0.f;
-        __bf16* const dst = (tid < 256 ? wl : yl) + gi * LDV + gc;
+        for (int e = 0; e < 8; ++e) {
+          const unsigned y = sizeof(T) == 2 ? e & 1 ? xo[0][e >> 1] & 0xffff0000u : xo[0][e >> 1] << 16 : xo[sizeof(T) / 2 - 1 - (e < 4)][e & 3];
+          o[e] = gi < valid && vb + gc + e < a.V ? __uint_as_float(y) : 0.f;
+        }
+        __bf16* const dst = (wave < 4 ? wl : yl) + at16<LDV>(gi, gc);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = xw[e >> 2][e & 3];
         sb::split8<3>(x, t);
 #pragma unroll
         for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dst + p * kC * LDV) = t[p];
-        if (tid < 256) {
+        if (wave < 4) {
           bf16x8 u[NP];
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] = has_do ? o[e] : 0.f;
           sb::split8<NP>(o, u);
 #pragma unroll
-          for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(ol + (p * kC + gi) * LDV + gc) = u[p];
+          for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(ol + p * kC * LDV + at16<LDV>(gi, gc)) = u[p];
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) ydot = fmaf(x[e], o[e], ydot);
         }
       }
-      __syncthreads();
-      request(min(vb + 32, a.vp - 32));
+      request(min(vb + 32, a.vp - 32));                        // in front of the barrier: behind it the compiler moves them below the products
+      lds_barrier();
       bf16x8 of[NP], yf[3], wf[3];
-      sb::load_frag<NP>(of, ol + ia * LDV + 8 * lg, kC * LDV);
-      sb::load_frag<3>(yf, yl + ia * LDV + 8 * lg, kC * LDV);
-      sb::load_frag<3>(wf, wl + ia * LDV + 8 * lg, kC * LDV);
+      const int fr = at16<LDV>(lr, 8 * lg);
+      sb::load_frag<NP>(of, ol + 16 * w * LDV + fr, kC * LDV);
+      sb::load_frag<3>(yf, yl + 16 * w * LDV + fr, kC * LDV);
+      sb::load_frag<3>(wf, wl + 16 * w * LDV + fr, kC * LDV);
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
         bf16x8 b[3], d[3];
-        sb::load_frag<3>(b, sl + (kt0 + 16 * t + lr) * LDV + 8 * lg, Kp * LDV);
-        sb::load_frag<3>(d, dl + (kt0 + 16 * t + lr) * LDV + 8 * lg, Kp * LDV);
+        sb::load_frag<3>(b, sl + (kt0 + 16 * t) * LDV + fr, Kp * LDV);
+        sb::load_frag<3>(d, dl + (kt0 + 16 * t) * LDV + fr, Kp * LDV);
         sb::mma<NP, 3>(e1[t], of, b);
         sb::mma<3, 3>(e2[t], yf, b);
         sb::mma<3, 3>(e3[t], wf, d);
@@ -1262,7 +1285,7 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
         const int jt = 2 * t + half;
         if (jt <= w) {
           bf16x8 b[3];
-          sb::load_frag<3>(b, wl + (16 * jt + lr) * LDV + 8 * lg, kC * LDV);
+          sb::load_frag<3>(b, wl + 16 * jt * LDV + fr, kC * LDV);
           sb::mma<NP, 3>(dp[t], of, b);
           sb::mma<3, 3>(da[t], yf, b);
         }
@@ -1288,8 +1311,8 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
     if constexpr (NP == 1) {
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
-        kr[t] = *reinterpret_cast<const bf16x4*>(kl + (kt0 + 16 * t + lr) * kLdT + ib);
-        qr[t] = *reinterpret_cast<const bf16x4*>(ql + (kt0 + 16 * t + lr) * kLdT + ib);
+        kr[t] = *reinterpret_cast<const bf16x4*>(kl + at16<kC>(kt0 + 16 * t + lr, ib));
+        qr[t] = *reinterpret_cast<const bf16x4*>(ql + at16<kC>(kt0 + 16 * t + lr, ib));
       }
     } else {
       const __amdgpu_buffer_rsrc_t rk = rows_rsrc(a.k, (row0 * a.ldk + (long)hk * a.K) * 4, ((valid - 1) * a.ldk + a.K) * 4);
@@ -1342,50 +1365,50 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
         __bf16 x[3];
         sb::split3(dp[t][e], x[0], x[1], x[2]);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) rl[(p * kC + ib + e) * LDR + j - j0] = x[p];
+        for (int p = 0; p < 3; ++p) rl[p * kC * LDR + at16<LDR>(ib + e, j - j0)] = x[p];
         sb::split3(da[t][e], x[0], x[1], x[2]);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) bl[(p * kC + ib + e) * LDR + j - j0] = x[p];
+        for (int p = 0; p < 3; ++p) bl[p * kC * LDR + at16<LDR>(ib + e, j - j0)] = x[p];
       }
     };
     auto put_t = [&](int t, int i0) {
       const int j = 16 * (2 * t + half) + lr;
-      sb::split_store4<3>(rt + j * LDR + ib - i0, kC * LDR, dp[t]);
-      sb::split_store4<3>(bt + j * LDR + ib - i0, kC * LDR, beta * da[t]);
+      sb::split_store4<3>(rt + at16<LDR>(j, ib - i0), kC * LDR, dp[t]);
+      sb::split_store4<3>(bt + at16<LDR>(j, ib - i0), kC * LDR, beta * da[t]);
     };
     // the products of 32 tokens: at = where they begin in the images
     auto join = [&](int kb, int at) {
-      constexpr int KS = NP == 1 ? kLdT : L::LDH, KP = NP * Kp;  // from column to column, from term to term (in columns)
-      const __bf16* const kf = kl + (kt0 + lr) * KS + at + 8 * lg;
-      const __bf16* const qf = ql + (kt0 + lr) * KS + at + 8 * lg;
+      const int fr = at16<LDR>(lr, at + 8 * lg);
+      const __bf16* const kf = kl + kt0 * LDR + fr;
+      const __bf16* const qf = ql + kt0 * LDR + fr;
       if (kb == 0 || w >= 2) {
         bf16x8 rf[3], bf[3];
-        sb::load_frag<3>(rf, rl + ia * LDR + at + 8 * lg, kC * LDR);
-        sb::load_frag<3>(bf, bl + ia * LDR + at + 8 * lg, kC * LDR);
+        sb::load_frag<3>(rf, rl + 16 * w * LDR + fr, kC * LDR);
+        sb::load_frag<3>(bf, bl + 16 * w * LDR + fr, kC * LDR);
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
           bf16x8 b[NP];
-          sb::load_frag<NP>(b, kf + 16 * t * KS, Kp * KS);
+          sb::load_frag<NP>(b, kf + 16 * t * LDR, Kp * LDR);
           sb::mma<3, NP>(e1[t], rf, b);
           sb::mma<3, NP>(e2[t], bf, b);
         }
       }
       if (kb == 1 || w < 2) {
         bf16x8 rf[3], bf[3];
-        sb::load_frag<3>(rf, rt + ia * LDR + at + 8 * lg, kC * LDR);
-        sb::load_frag<3>(bf, bt + ia * LDR + at + 8 * lg, kC * LDR);
+        sb::load_frag<3>(rf, rt + 16 * w * LDR + fr, kC * LDR);
+        sb::load_frag<3>(bf, bt + 16 * w * LDR + fr, kC * LDR);
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
           bf16x8 b[NP];
-          sb::load_frag<NP>(b, qf + 16 * t * KS, Kp * KS);
+          sb::load_frag<NP>(b, qf + 16 * t * LDR, Kp * LDR);
           sb::mma<3, NP>(e3[t], rf, b);
-          sb::load_frag<NP>(b, kf + 16 * t * KS, Kp * KS);
+          sb::load_frag<NP>(b, kf + 16 * t * LDR, Kp * LDR);
           sb::mma<3, NP>(e3[t], bf, b);
         }
       }
     };
     __syncthreads();
-    if (tid >= 256 && (tid & 3) == 0) yv[gi] = ydot;
+    if (wave >= 4 && (lane & 3) == 0) yv[gi] = ydot;
     if (lane == 0) red[wave] = sdot;
     if constexpr (NP == 1) {
       put(0, 0);
@@ -1398,13 +1421,13 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
     } else {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        // 16 bytes of a term's row (32 tokens are four) per thread: columns tid/4, tid/4 + 128, ..
+        // 16 bytes of a term's row (32 tokens are four) per thread: columns 16 * wave + lane / 4, + 128, ..
         constexpr int U = (NP * Kp + 127) / 128;
         bf16x8 x[2][U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int row = min(u * 128 + (tid >> 2), NP * Kp - 1), p = row / Kp, k = row - p * Kp;
-          const long at = ((hs * Kp + k) * NP + p) * kC + 32 * kb + 8 * (tid & 3);
+          const int row = min(u * 128 + ((64 * wave + lane) >> 2), NP * Kp - 1), p = row / Kp, k = row - p * Kp;
+          const long at = ((hs * Kp + k) * NP + p) * kC + 32 * kb + 8 * (lane & 3);
           x[0][u] = *reinterpret_cast<const bf16x8*>(a.kt + at);
           x[1][u] = *reinterpret_cast<const bf16x8*>(a.qt + at);
         }
@@ -1416,7 +1439,7 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int at = min(u * 128 + (tid >> 2), NP * Kp - 1) * L::LDH + 8 * (tid & 3);    // (the last row's copies are the same)
+          const int at = at16<LDR>(min(u * 128 + ((64 * wave + lane) >> 2), NP * Kp - 1), 8 * (lane & 3));    // (the last row's copies are the same)
           *reinterpret_cast<bf16x8*>(kl + at) = x[0][u];
           *reinterpret_cast<bf16x8*>(ql + at) = x[1][u];
         }
@@ -1467,7 +1490,7 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
         a.dbeta[(row0 + lane) * a.lddbeta + hv] = yv[lane] + (rows[kC + lane] + rows[4 * kC + lane]);
       }
     }
-    if (r == a.rep - 1) {
+    if (!GROUP || r == a.rep - 1) {
       T* const pq = static_cast<T*>(a.dq) + (row0 + ib) * a.lddq + (long)hk * a.K + kt0 + lr;
       T* const pk = static_cast<T*>(a.dk) + (row0 + ib) * a.lddk + (long)hk * a.K + kt0 + lr;
 #pragma unroll
@@ -1834,6 +1857,7 @@ int hhrl_gdr_backward(const hhrl_gdr_desc* d, void* stream) {
   a.d_o = d->d_o; a.lddo = d->lddo; a.d_s1 = d->d_s1; a.d_s0 = d->d_s0;
   a.dq = d->dq; a.dk = d->dk; a.dv = d->dv; a.lddq = d->lddq; a.lddk = d->lddk; a.lddv = d->lddv;
   a.dg = d->dg; a.dbeta = d->dbeta; a.lddg = d->lddg; a.lddbeta = d->lddbeta;
+  a.wide_v = d->V % 8 == 0 && a16(d->v) && d->ldv % 8 == 0 && (!d->d_o || (a16(d->d_o) && d->lddo % 8 == 0));
   const double flops = 6.0 * d->rows * d->Hv * d->K * d->V;
   hipStream_t st = as_stream(stream);
   if (d->dtype == HHRL_BF16) return d->K <= 64 ? run_bwd<__bf16, 1, 1>(a, st, flops) : run_bwd<__bf16, 1, 2>(a, st, flops);
