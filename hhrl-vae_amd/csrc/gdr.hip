@@ -562,6 +562,15 @@ __device__ __forceinline__ void store_seg(const f32x4 (&S)[KB2][NT], float* s, i
       for (int e = 0; e < 4; ++e) s[(16 * (KB2 * w + t) + 4 * lg + e) * ld + v0 + 16 * u + lr] = S[t][u][e];
 }
 
+// the tile for the gradients, as the registers hold it: [K/16][2 halves of 32 columns][64 lanes][4]
+template <int KB2, int NT>
+__device__ __forceinline__ void store_tile(const f32x4 (&S)[KB2][NT], float* s, int w, int lane) {
+#pragma unroll
+  for (int t = 0; t < KB2; ++t)
+#pragma unroll
+    for (int u = 0; u < NT; ++u) *reinterpret_cast<f32x4*>(s + ((unsigned)(KB2 * w * 512 + lane * 4) + t * 512 + u * 256)) = S[t][u];
+}
+
 // Per-token factors of a chunk, rows ib .. ib + 3
 struct ScanVec {
   f32x4 gam, tail, beta;
@@ -647,14 +656,7 @@ __device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT]
     vp.load(next);
     vn.load(vecp, ib);
     if constexpr (TRAIN) {
-      float* const sp = a.s + ((vs * (a.vp / 32) + v0 / 32) * Kp) * 32 + (v0 & 16);
-      const unsigned at = (16 * KB2 * w + 4 * lg) * 32 + lr;
-#pragma unroll
-      for (int t = 0; t < KB2; ++t)
-#pragma unroll
-        for (int u = 0; u < NT; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sp[at + (16 * t + e) * 32 + 16 * u] = S[t][u][e];
+      store_tile<KB2, NT>(S, a.s + ((vs * (a.vp / 32) + v0 / 32) * Kp) * 32 + (v0 & 16) * 16, w, lane);
     }
     lds_barrier();
     f32x4 wt[NT];
@@ -991,14 +993,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
         }
         vn.load(vecp, ib);
         if constexpr (!BARE) {
-          float* const sp = a.ds + ((vs * (a.vp / 32) + v0 / 32) * Kp) * 32 + (v0 & 16);
-          const unsigned at = (16 * KB2 * w + 4 * lg) * 32 + lr;
-#pragma unroll
-          for (int t = 0; t < KB2; ++t)
-#pragma unroll
-            for (int u = 0; u < NT; ++u)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) sp[at + (16 * t + e) * 32 + 16 * u] = dS[t][u][e];
+          store_tile<KB2, NT>(dS, a.ds + ((vs * (a.vp / 32) + v0 / 32) * Kp) * 32 + (v0 & 16) * 16, w, lane);
         }
         lds_barrier();
 #pragma unroll
@@ -1197,8 +1192,10 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
     for (int t = 0; t < 2; ++t) dp[t] = da[t] = zero;
     float sdot = 0.f, ydot = 0.f;
     const bool has_s = KB2 == 2 || wave < 4;
-    const float* const ps = a.s + (vs * (a.vp / 32) * Kp + ((64 * wave + lane) >> 2) % Kp) * 32 + gc;
-    const float* const pd = a.ds + (vs * (a.vp / 32) * Kp + ((64 * wave + lane) >> 2) % Kp) * 32 + gc;
+    // S, dS': two lanes' registers of a 16 x 16 tile, so four rows of two columns
+    const long st0 = vs * (a.vp / 32) * Kp * 32 + (64 * wave + lane) % (4 * Kp) * 8;
+    const float *const ps = a.s + st0, *const pd = a.ds + st0;
+    const int si = at16<LDV>(16 * (wave % (4 * KB2)) + 4 * (lane >> 3 & 3), 16 * (lane >> 5) + 2 * (lane & 7));
     const float* const pw = (wave < 4 ? a.w : a.y) + (vs * (a.vp / 32) * kC + gi) * 32 + gc;
     const T* const px = wave < 4 ? (has_do ? static_cast<const T*>(a.d_o) + rowc * a.lddo + (long)hv * a.V : static_cast<const T*>(a.v))
                                   : static_cast<const T*>(a.v) + rowc * a.ldv + (long)hv * a.V;
@@ -1228,17 +1225,18 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
         float x[8];
         bf16x8 t[3];
         if (has_s) {
-          const int k = (64 * wave + lane) >> 2;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) { x[e] = xs[e >> 2][e & 3]; sdot = fmaf(x[e], xd[e >> 2][e & 3], sdot); }
-          sb::split8<3>(x, t);
+          for (int e = 0; e < 4; ++e) {
+            sdot = fmaf(xs[0][e], xd[0][e], fmaf(xs[1][e], xd[1][e], sdot));
+            unsigned u[3], v[3];
+            sb::split2<3>(xs[0][e], xs[1][e], u);
+            sb::split2<3>(xd[0][e], xd[1][e], v);
 #pragma unroll
-          for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(sl + p * Kp * LDV + at16<LDV>(k, gc)) = t[p];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = xd[e >> 2][e & 3];
-          sb::split8<3>(x, t);
-#pragma unroll
-          for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dl + p * Kp * LDV + at16<LDV>(k, gc)) = t[p];
+            for (int p = 0; p < 3; ++p) {
+              *reinterpret_cast<unsigned*>(sl + p * Kp * LDV + si + e * LDV) = u[p];
+              *reinterpret_cast<unsigned*>(dl + p * Kp * LDV + si + e * LDV) = v[p];
+            }
+          }
         }
         float o[8];
 #pragma unroll
