@@ -58,6 +58,14 @@ __device__ __forceinline__ int at16(int row, int i) { return place<N / 8>(row, i
 template <int N>
 __device__ __forceinline__ int at32(int row, int i) { return place<N / 4>(row, i >> 2) * 4; }
 
+// Images in the workspace that matrix fragments are read from lie as the fragments do: blocks of 16 rows by 32 columns, the
+// 64 lanes' 16 bytes behind each other ([row block][column block][term][lane][8]).  A wave's request for one is 1 KB in a
+// row and takes the address unit 16 cycles; from rows of 128 bytes and more (every four lanes four rows) it takes 64,
+// and a scan's requests, a hundred per chunk and workgroup, were what bound it.
+constexpr int kFrag = 512;         // elements of a block
+// where element i .. of row lr (of 16) of a block begins
+__device__ __forceinline__ int frag_at(int lr, int i) { return ((i >> 3 & 3) * 16 + lr) * 8 + (i & 7); }
+
 struct GdrArgs {
   int n_seq, Hk, Hv, K, V, rep;
   long rows;
@@ -79,7 +87,7 @@ struct GdrArgs {
   long lddq, lddk, lddv;
   float *dg, *dbeta;
   long lddg, lddbeta;
-  int pack, wide, wide_v, train, vp, nvt;
+  int whole, wide, wide_v, v16, train, vp, nvt;
   // ws, per chunk and key head: k, q [64][terms][Kp] (pack), their transposes [Kp][terms][64];
   //     per chunk and value head: M, P (two terms for bf16: what o takes) and their transposes [64][terms][64], five rows of 64 floats, and for the
   //     backward pass W, Y [vp/32][64][32] and S, dS [vp/32][Kp][32], fp32 (tiles of 32 columns).  The terms of a row lie side by side, so that a lane's
@@ -138,6 +146,7 @@ __device__ __forceinline__ void slot_chunk(const GdrArgs& a, long slot, long& ro
 // dropped.  So rows behind the sequence need no test, no request has a condition (a conditional one would be waited for
 // where its branch joins), and a chunk costs no address arithmetic on the vector unit.
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 constexpr unsigned kNoColumn = 0x80000000u;      // an offset behind every size
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, long offset, long bytes) {
   // (descriptor word 3: 32-bit data, no swizzle)
@@ -180,7 +189,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
   const long hs = slot * a.Hk + hk;
 
   // k and q as bf16 terms; what lies beyond the sequence or the head's width becomes 0 and is not read
-  if (NP == 1 && !a.pack) {                                    // rows of Kp elements, 16-byte aligned
+  if (NP == 1 && a.whole) {                                    // rows of Kp elements, 16-byte aligned
     constexpr int U = kC * KG / 256;
     bf16x8 x[2][U];
 #pragma unroll
@@ -205,7 +214,6 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
       const long ld = side ? a.ldq : a.ldk;
       const T* const src = static_cast<const T*>(side ? a.q : a.k) + row0 * ld + (long)hk * a.K;
       __bf16* const dst = side ? ql : kl;
-      __bf16* const pk = (side ? a.qpk : a.kpk) + hs * kC * NP * Kp;
       for (int u = tid; u < kC * KG; u += 256) {
         const int i = u / KG, c = (u - i * KG) * 8;
         // (unconditional requests of elements that are there, then a choice)
@@ -227,10 +235,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
         bf16x8 t[NP];
         sb::split8<NP>(x, t);
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          *reinterpret_cast<bf16x8*>(dst + p * kC * Kp + at16<Kp>(i, c)) = t[p];
-          if (a.pack) *reinterpret_cast<bf16x8*>(pk + ((long)i * NP + p) * Kp + c) = t[p];
-        }
+        for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(dst + p * kC * Kp + at16<Kp>(i, c)) = t[p];
       }
     }
   }
@@ -250,8 +255,9 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
         lo[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x05040100u);       // low halves of two tokens
         hi[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x07060302u);       // high halves
       }
-      *reinterpret_cast<u32x4*>(dst + ((long)k * NP + p) * kC + i0) = lo;
-      *reinterpret_cast<u32x4*>(dst + ((long)(k + 1) * NP + p) * kC + i0) = hi;
+      __bf16* const to = dst + ((k >> 4) * 2 + (i0 >> 5)) * NP * kFrag + p * kFrag + frag_at(k & 15, i0);
+      *reinterpret_cast<u32x4*>(to) = lo;
+      *reinterpret_cast<u32x4*>(to + 8) = hi;
     }
   }
   // rows 16*wave.. against the tiles of columns in front of them: k k^T, q k^T (its transpose's source), and k q^T with the
@@ -265,6 +271,12 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
     const int off = at16<Kp>(lr, 32 * kb + 8 * lg);
     sb::load_frag<NP>(ka, kl + 16 * wave * Kp + off, kC * Kp);
     sb::load_frag<NP>(qa, ql + 16 * wave * Kp + off, kC * Kp);
+    const long at = hs * kC * NP * Kp + ((wave * (Kp / 32) + kb) * NP) * kFrag + lane * 8;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      *reinterpret_cast<bf16x8*>(a.kpk + at + p * kFrag) = ka[p];
+      *reinterpret_cast<bf16x8*>(a.qpk + at + p * kFrag) = qa[p];
+    }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if (t <= wave) {
@@ -322,11 +334,11 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
         mm[i * kLdM + j] = 0.f;
         x[e] = i >= j ? qk[t][e] * d : 0.f;
       }
-      if (a.train && ((t < 2) || (wave >= 2))) sb::split_store4<3>(pt + j * 3 * kC + ib, kC, x);       // PT rows j >= 32 hold columns i >= 32
+      if (a.train && ((t < 2) || (wave >= 2))) sb::split_store4<3>(pt + (t * 2 + (wave >> 1)) * 3 * kFrag + frag_at(lr, ib), kFrag, x);       // PT rows j >= 32 hold columns i >= 32
       const float hi = gh[iq], lo = gl[iq];
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = iq >= jb + e ? kq[t][e] * decay((hi - gh[jb + e]) + (lo - gl[jb + e])) : 0.f;
-      if (t < 2 || wave >= 2) sb::split_store4<NO>(pp + iq * NO * kC + jb, kC, x);
+      if (t < 2 || wave >= 2) sb::split_store4<NO>(pp + (wave * 2 + (t >> 1)) * NO * kFrag + frag_at(lr, jb), kFrag, x);
     }
     __syncthreads();
     {
@@ -376,10 +388,10 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
     }
     __syncthreads();
     // 16 elements of a row (or of a column, for the transpose the backward scan reads) per thread
-    const int row = tid >> 2, c0 = (tid & 3) * 16;
+    const int row = 16 * wave + lr, c0 = lg * 16;
     for (int what = 0; what < (a.train ? 2 : 1); ++what) {
       if (what == 0 ? row < 32 && c0 >= 32 : row >= 32 && c0 < 32) continue;
-      __bf16* const dst = (what == 0 ? a.m : a.mt) + (vs * kC + row) * 3 * kC + c0;
+      __bf16* const dst = (what == 0 ? a.m : a.mt) + vs * kC * 3 * kC + (wave * 2 + (lg >> 1)) * 3 * kFrag;
       const int si = what == 0 ? kLdM : 1, sj = what == 0 ? 1 : kLdM;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -389,7 +401,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
         bf16x8 t[3];
         sb::split8<3>(x, t);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dst + p * kC + 8 * h) = t[p];
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dst + p * kFrag + frag_at(lr, c0 + 8 * h)) = t[p];
       }
     }
   }
@@ -416,97 +428,117 @@ template <int NP, int KB2, int NT>
 struct ScanLds {
   static constexpr int Kp = 64 * KB2, VT = 16 * NT;
   static constexpr int S = 3 * VT * Kp, X = 3 * VT * kC, F = VT * kC;     // elements
-  static constexpr int fwd_bytes = 2 * (S + 2 * X) + 8 * F;
-  static constexpr int bwd_bytes = 2 * (S + 3 * X + NP * VT * kC) + 12 * F;
+  static constexpr int V = VT * kC * (NP == 1 ? 2 : 4);                            // bytes: rows of v or dO, turned
+  static constexpr int chain_bytes = 2 * (S + 2 * X) + V, fwd_bytes = chain_bytes + V + 12 * F;
+  static constexpr int bwd_bytes = 2 * (S + 3 * X + NP * VT * kC) + 12 * F + V;
 };
 
-// Operand rows of k or q, token 16*w + lr of a chunk, from the packed terms (whose rows behind the sequence are 0) or from
-// the caller's rows
+// Operand rows of k or q, token 16*w + lr of a chunk
 template <int NP, int KB>
-struct RowPtr {
-  static constexpr int Kp = 32 * KB;
-  const char* base;
-  long step, row;                              // bytes from chunk to chunk and from row to row
-  unsigned at;
-  int len;
-  __device__ __forceinline__ RowPtr(const GdrArgs& a, const void* raw, long ld, const __bf16* packed, long slot0, int hk, long start, int len_,
-                                    int i, int lg) : len(len_) {
-    if (NP == 1 && !a.pack) {
-      base = static_cast<const char*>(raw) + (start * ld + (long)hk * Kp) * 2;
-      row = ld * 2;
-      step = kC * row;
-    } else {
-      base = reinterpret_cast<const char*>(packed + (slot0 * a.Hk + hk) * kC * NP * Kp);
-      row = NP * Kp * 2;
-      step = (long)a.Hk * kC * row;
-      len = 0x7fffffff;                        // all rows of a packed chunk are there
-    }
-    at = i * (unsigned)row + 16 * lg;
-  }
-  __device__ __forceinline__ void load(bf16x8 (&f)[KB][NP], int c) const {
-    const int have = min(kC, len - c * kC);
-    const __amdgpu_buffer_rsrc_t r = rows_rsrc(base, c * step, (have - 1) * row + NP * Kp * 2);
+__device__ __forceinline__ void load_rows(bf16x8 (&f)[KB][NP], const __bf16* base, unsigned at) {
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
+  for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int p = 0; p < NP; ++p)
-        f[kb][p] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(r, at + (p * Kp + 32 * kb) * 2, 0, 0));
-  }
-};
-// Elements of v or dO in the layout of a result (rows ib + e, columns v0 + 16*t + lr), kept as they come
-template <typename T, int NT>
-struct ColPtr {
+    for (int p = 0; p < NP; ++p) f[kb][p] = *reinterpret_cast<const bf16x8*>(base + (at + (kb * NP + p) * kFrag));
+}
+// Rows of v, dO, o or dv: lane l holds token 16*w + l/4, columns v0 + 4*NT*(l & 3) + e, so that four lanes read or write
+// neighbours (WIDE: in 16-byte pieces, where V is a multiple of those and rows are aligned to them).
+template <typename T, int NT, bool WIDE>
+struct RowTile {
+  static constexpr int N = 4 * NT, R = N * (int)sizeof(T) / 4;
   const char* base;
   long row, width;
-  int len;
-  unsigned at[NT][4], x[NT][4];
-  __device__ __forceinline__ ColPtr(const void* src, long ld, long start, int len_, int hv, int V, int v0, int lr, int ib) : len(len_) {
+  int len, have;                               // have: columns from the lane's first to the end of the head
+  unsigned at, x[WIDE ? R : N];
+  __device__ __forceinline__ RowTile(const void* src, long ld, long start, int len_, int hv, int V, int v0, int w, int lane)
+      : len(len_), have(V - v0 - N * (lane & 3)) {
     base = static_cast<const char*>(src) + (start * ld + (long)hv * V) * sizeof(T);
     row = ld * sizeof(T);
     width = (long)V * sizeof(T);
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int v = v0 + 16 * t + lr;
-        at[t][e] = v < V ? (ib + e) * (unsigned)row + v * (unsigned)sizeof(T) : kNoColumn;
-      }
+    at = (16 * w + (lane >> 2)) * (unsigned)row + (v0 + N * (lane & 3)) * (unsigned)sizeof(T);
   }
   __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk(int c) const {
     return rows_rsrc(base, (long)c * kC * row, (min(kC, len - c * kC) - 1) * row + width);
   }
+  __device__ __forceinline__ unsigned place_of(int e) const { return e < have ? at + e * (unsigned)sizeof(T) : kNoColumn; }
   __device__ __forceinline__ void load(int c) {
     const __amdgpu_buffer_rsrc_t r = chunk(c);
+    if constexpr (WIDE && R == 2) {
+      const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(r, place_of(0), 0, 0);
+      x[0] = y[0]; x[1] = y[1];
+    } else if constexpr (WIDE) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int h = 0; h < R; h += 4) {
+        const u32x4 y = __builtin_amdgcn_raw_buffer_load_b128(r, place_of(h * 4 / (int)sizeof(T)), 0, 0);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (sizeof(T) == 2) x[t][e] = __builtin_amdgcn_raw_buffer_load_b16(r, at[t][e], 0, 0);
-        else x[t][e] = __builtin_amdgcn_raw_buffer_load_b32(r, at[t][e], 0, 0);
+        for (int e = 0; e < 4; ++e) x[h + e] = y[e];
       }
-  }
-  __device__ __forceinline__ f32x4 get(int t) const {
-    f32x4 r;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = __uint_as_float(sizeof(T) == 2 ? x[t][e] << 16 : x[t][e]);
-    return r;
+      for (int e = 0; e < N; ++e) {
+        if constexpr (sizeof(T) == 2) x[e] = __builtin_amdgcn_raw_buffer_load_b16(r, place_of(e), 0, 0);
+        else x[e] = __builtin_amdgcn_raw_buffer_load_b32(r, place_of(e), 0, 0);
+      }
+    }
+  }
+  // what was loaded into an image in LDS, columns by tokens
+  __device__ __forceinline__ void put(T* img, int w, int lane) const {
+    const int i = 16 * w + (lane >> 2);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int col = N * (lane & 3) + e;
+      if constexpr (sizeof(T) == 2) {
+        const unsigned y = WIDE ? e & 1 ? x[e >> 1] >> 16 : x[e >> 1] : x[e];
+        reinterpret_cast<unsigned short*>(img)[at16<kC>(col, i)] = (unsigned short)y;
+      } else {
+        reinterpret_cast<unsigned*>(img)[at32<kC>(col, i) + (i & 3)] = x[e];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(int c, const float (&y)[N]) const {
+    const __amdgpu_buffer_rsrc_t r = chunk(c);
+    if constexpr (WIDE && R == 2) {
+      __builtin_amdgcn_raw_buffer_store_b64(u32x2{sb::pack2(y[0], y[1]), sb::pack2(y[2], y[3])}, r, place_of(0), 0, 0);
+    } else if constexpr (WIDE) {
+#pragma unroll
+      for (int h = 0; h < R; h += 4) {
+        u32x4 z;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (sizeof(T) == 2) z[e] = sb::pack2(y[2 * e], y[2 * e + 1]);
+          else z[e] = __float_as_uint(y[h + e]);
+        }
+        __builtin_amdgcn_raw_buffer_store_b128(z, r, place_of(h * 4 / (int)sizeof(T)), 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)y[e]), r, place_of(e), 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y[e]), r, place_of(e), 0, 0);
+      }
+    }
   }
 };
-// a result tile of o or dv into the caller's rows
-template <typename T, int NT>
-struct ColOut : ColPtr<T, NT> {
-  using ColPtr<T, NT>::ColPtr;
-  __device__ __forceinline__ void store(int c, const f32x4 (&y)[NT]) const {
-    const __amdgpu_buffer_rsrc_t r = this->chunk(c);
+// four tokens (i ..) of a column from such an image
+template <typename T>
+using Four = T __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ Four<T> column4(const T* img, int col, int i) {
+  return *reinterpret_cast<const Four<T>*>(img + (sizeof(T) == 2 ? at16<kC>(col, i) : at32<kC>(col, i)));
+}
+__device__ __forceinline__ f32x4 wide4(const f32x4& x) { return x; }
+__device__ __forceinline__ f32x4 wide4(const bf16x4& x) { return f32x4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]}; }
+// N columns of token i from an fp32 image of columns by tokens, and into rows of 32 floats
+template <int N>
+__device__ __forceinline__ void token_row(float (&y)[N], const float* img, int i, int col) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+  for (int e = 0; e < N; ++e) y[e] = img[at32<kC>(col + e, i) + (i & 3)];
+}
+template <int N>
+__device__ __forceinline__ void store_row(float* to, const float (&y)[N]) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)y[t][e]), r, this->at[t][e], 0, 0);
-        else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(y[t][e]), r, this->at[t][e], 0, 0);
-      }
-  }
-};
+  for (int h = 0; h < N; h += 4) *reinterpret_cast<f32x4*>(to + h) = f32x4{y[h], y[h + 1], y[h + 2], y[h + 3]};
+}
 template <int NP, int KB2>
 __device__ __forceinline__ void load_kt(bf16x8 (&f)[KB2][2][NP], const __bf16* base, unsigned at) {
 #pragma unroll
@@ -514,7 +546,7 @@ __device__ __forceinline__ void load_kt(bf16x8 (&f)[KB2][2][NP], const __bf16* b
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int p = 0; p < NP; ++p) f[t][kb][p] = *reinterpret_cast<const bf16x8*>(base + (at + (16 * t * NP + p) * kC + 32 * kb));
+      for (int p = 0; p < NP; ++p) f[t][kb][p] = *reinterpret_cast<const bf16x8*>(base + (at + ((t * 2 + kb) * NP + p) * kFrag));
 }
 // the state tile of a scan's chain wave w: rows 16*(KB2*w + t) + 4*lg + e, columns v0 + 16*u + lr
 template <int KB2, int NT>
@@ -587,12 +619,12 @@ struct ScanVec {
 template <int N>
 __device__ __forceinline__ void load_half(bf16x8 (&f)[N], const __bf16* base, unsigned at) {
 #pragma unroll
-  for (int q = 0; q < N; ++q) f[q] = *reinterpret_cast<const bf16x8*>(base + (at + q * kC));
+  for (int q = 0; q < N; ++q) f[q] = *reinterpret_cast<const bf16x8*>(base + (at + q * kFrag));
 }
 template <int N>
 __device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* base, unsigned at, bool low, bool high) {
-  load_half<N>(f[0], base, at + (low ? 0 : 32));
-  load_half<N>(f[1], base, at + (high ? 32 : 0));
+  load_half<N>(f[0], base, at + (low ? 0 : N * kFrag));
+  load_half<N>(f[1], base, at + (high ? N * kFrag : 0));
 }
 
 // A scan is bound by its chain: state -> K S -> W -> state, chunk after chunk, and inside it by the instructions its waves
@@ -601,35 +633,40 @@ __device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* base, 
 // on dO, one chunk ahead, and the stores of Y and dV (backward).  Everything a chunk needs from memory is requested while
 // the chunk in front of it is worked on, behind the last use of its registers.
 // The chain: chunks c0 .. c1 - 1 of a sequence, four waves, S in their registers.  BARE: nobody hangs on it (no W is left in
-// wl).  vcols: V, or 0 for columns without a v (and v0 what it may).
-template <typename T, int NP, int KB2, int NT, bool TRAIN, bool BARE>
-__device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT], __bf16* sl, __bf16* xl, __bf16* ul, float* wl, int hv, int vcols,
+// wl, and v comes into vl by these waves).  vcols: V, or 0 for columns without a v (and v0 what it may).
+template <typename T, int NP, int KB2, int NT, bool TRAIN, bool BARE, bool WIDE>
+__device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT], __bf16* sl, __bf16* xl, __bf16* ul, T* vl, float* wl, int hv, int vcols,
                                            int v0, long start, int len, long slot0, int c0, int c1) {
   using L = ScanLds<NP, KB2, NT>;
   constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT;
   const int hk = hv / a.rep, lane = threadIdx.x & 63, w = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
-  const int ib = 16 * w + 4 * lg, ia = 16 * w + lr;        // first of four result rows; operand row
+  const int ib = 16 * w + 4 * lg;                          // first of four result rows
   const bool high = w >= 2;                                // M is lower triangular: rows < 32 read 32 columns
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   bf16x8 kf[KB][NP], mf[2][3], ktf[KB2][2][NP];
-  const RowPtr<NP, KB> kp(a, a.k, a.ldk, a.kpk, slot0, hk, start, len, ia, lg);
-  ColPtr<T, NT> vp(a.v, a.ldv, start, len, hv, vcols, v0, lr, ib);
+  const __bf16* kp = a.kpk + ((slot0 + c0) * a.Hk + hk) * kC * NP * Kp;
+  RowTile<T, NT, WIDE> vp(a.v, a.ldv, start, len, hv, vcols, v0, w, lane);
   ScanVec vn;
   const float* vecp = a.vec + ((slot0 + c0) * a.Hv + hv) * kVecs * kC;
   const __bf16* mp = a.m + ((slot0 + c0) * a.Hv + hv) * 3 * kC * kC;
   const __bf16* ktp = a.kt + ((slot0 + c0) * a.Hk + hk) * Kp * NP * kC;
-  const unsigned mat = ia * 3 * kC + 8 * lg, ktat = (16 * KB2 * w + lr) * NP * kC + 8 * lg;
-  kp.load(kf, c0);
-  vp.load(c0);
+  const unsigned kat = w * KB * NP * kFrag + lane * 8, mat = w * 2 * 3 * kFrag + lane * 8, ktat = KB2 * w * 2 * NP * kFrag + lane * 8;
+  if constexpr (BARE) vp.load(c0);
+  load_rows<NP, KB>(kf, kp, kat);
   vn.load(vecp, ib);
   load_tri<3>(mf, mp, mat, true, high);
   load_kt<NP, KB2>(ktf, ktp, ktat);
+  if constexpr (BARE) {
+    vp.put(vl, w, lane);
+    vp.load(min(c0 + 1, c1 - 1));
+  }
   for (int c = c0; c < c1; ++c) {
     const int next = min(c + 1, c1 - 1);
     const long adv = next - c;                         // 0 behind the last chunk: its operands are read again, to no use
     vecp += adv * a.Hv * kVecs * kC;
     mp += adv * a.Hv * 3 * kC * kC;
     ktp += adv * a.Hk * NP * Kp * kC;
+    kp += adv * a.Hk * NP * Kp * kC;
     const long vs = (slot0 + c) * a.Hv + hv;
 #pragma unroll
     for (int t = 0; t < KB2; ++t)
@@ -637,9 +674,14 @@ __device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT]
       for (int u = 0; u < NT; ++u)
         sb::split_store4<3>(sl + 16 * u * Kp + at16<Kp>(lr, 16 * (KB2 * w + t) + 4 * lg), VT * Kp, S[t][u]);
     lds_barrier();
+    const ScanVec vc = vn;
     f32x4 ks[NT];
+    Four<T> vv[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) ks[t] = zero;
+    for (int t = 0; t < NT; ++t) {
+      ks[t] = zero;
+      vv[t] = column4<T>(vl + ((BARE ? 0 : (c & 1) * L::VT) + 16 * t) * kC, lr, ib);
+    }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -648,13 +690,15 @@ __device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT]
         sb::load_frag<3>(b, sl + 16 * t * Kp + at16<Kp>(lr, 32 * kb + 8 * lg), VT * Kp);
         sb::mma<NP, 3>(ks[t], kf[kb], b);
       }
-    kp.load(kf, next);
-    const ScanVec vc = vn;
+    load_rows<NP, KB>(kf, kp, kat);
+    vn.load(vecp, ib);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-      sb::split_store4<3>(xl + 16 * t * kC + at16<kC>(lr, ib), VT * kC, vc.beta * (vp.get(t) - vc.gam * ks[t]));
-    vp.load(next);
-    vn.load(vecp, ib);
+      sb::split_store4<3>(xl + 16 * t * kC + at16<kC>(lr, ib), VT * kC, vc.beta * (wide4(vv[t]) - vc.gam * ks[t]));
+    if constexpr (BARE) {                                  // (a wave's tokens are read by nobody else)
+      vp.put(vl, w, lane);
+      vp.load(min(c + 2, c1 - 1));
+    }
     if constexpr (TRAIN) {
       store_tile<KB2, NT>(S, a.s + ((vs * (a.vp / 32) + v0 / 32) * Kp) * 32 + (v0 & 16) * 16, w, lane);
     }
@@ -695,7 +739,7 @@ __device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT]
   }
 }
 
-template <typename T, int NP, int KB2, int NT, bool TRAIN>
+template <typename T, int NP, int KB2, int NT, bool TRAIN, bool WIDE>
 __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
   using L = ScanLds<NP, KB2, NT>;
   constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT;
@@ -705,6 +749,8 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
   __bf16* const xl = sl + L::S;                            // [3][VT][kC]  beta (V - gam K S)
   __bf16* const ul = xl + L::X;                            // [3][VT][kC]  exp(G_C - G) W
   float* const wl = reinterpret_cast<float*>(ul + L::X);   // [2][VT][kC]  W, of the chunk at hand and the one in front of it
+  T* const vl = reinterpret_cast<T*>(wl + 2 * L::F);       // [2][VT][kC]  v, of the chunk at hand and the next one
+  float* const ot = reinterpret_cast<float*>(vl + 2 * VT * kC);   // [4 waves][16][VT]  o on its way to rows
   int n, hv, v0, seg;
   if (!scan_tile(a, VT, n, hv, v0, seg)) return;
   const int hk = hv / a.rep;
@@ -715,7 +761,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
   const int nc = (len + kC - 1) / kC;
   const int c0 = seg * a.seg_chunks, c1 = min(nc, c0 + a.seg_chunks);
   if (seg > 0 && c0 >= nc) return;
-  const int ib = 16 * w + 4 * lg, ia = 16 * w + lr;        // first of four result rows; operand row
+  const int ia = 16 * w + lr;                              // operand row
   const bool high = w >= 2;                                // M and P are lower triangular: rows < 32 read 32 columns
   const long nh = (long)n * a.Hv + hv;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -724,18 +770,25 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
     f32x4 S[KB2][NT];
     if (a.segs == 1) load_state<KB2, NT>(S, a.s0, a, nh, w, v0, lr, lg);
     else load_seg<KB2, NT>(S, a.seg_s + (nh * a.segs + seg) * Kp * a.vp, a.vp, w, v0, lr, lg);   // s0 may be s1 by now
-    if (c0 < c1) scan_chain<T, NP, KB2, NT, TRAIN, false>(a, S, sl, xl, ul, wl, hv, a.V, v0, start, len, slot0, c0, c1);
+    if (c0 < c1) scan_chain<T, NP, KB2, NT, TRAIN, false, WIDE>(a, S, sl, xl, ul, vl, wl, hv, a.V, v0, start, len, slot0, c0, c1);
     if (a.s1 && c1 == nc) store_state<KB2, NT>(S, a.s1, a, nh, w, v0, lr, lg);
   } else if (c0 < c1) {                                    // ---- the output, between the chain's barriers
     // Chunk c: Q S behind barrier 1, the first half of P W behind barrier 3, the second behind the next chunk's barrier 2,
     // the store behind its barrier 1 after that: no stretch between two barriers is longer than the chain's.
     bf16x8 qf[KB][NP], pf[2][NO];
     f32x4 qn[NT], qs[NT], qo[NT];
-    const RowPtr<NP, KB> qp(a, a.q, a.ldq, a.qpk, slot0, hk, start, len, ia, lg);
+    const __bf16* const qp = a.qpk + ((slot0 + c0) * a.Hk + hk) * kC * NP * Kp;
+    const long qstep = (long)a.Hk * kC * NP * Kp;
+    const unsigned qat = w * KB * NP * kFrag + lane * 8;
     const __bf16* const pp = a.p + ((slot0 + c0) * a.Hv + hv) * NO * kC * kC;
     const long pstep = (long)a.Hv * NO * kC * kC;
-    const unsigned pat = ia * NO * kC + 8 * lg;
-    ColOut<T, NT> op(a.o, a.ldo, start, len, hv, a.V, v0, lr, ib);
+    const unsigned pat = w * 2 * NO * kFrag + lane * 8;
+    // The products are formed turned (S^T Q^T, W^T P^T): a lane then holds four columns of a token, and four lanes' worth of
+    // neighbours is one exchange inside the wave away (through its part of ot)
+    const RowTile<T, NT, WIDE> op(a.o, a.ldo, start, len, hv, a.V, v0, w, lane);
+    RowTile<T, NT, WIDE> vp(a.v, a.ldv, start, len, hv, a.V, v0, w, lane);
+    const int ta = 16 * w + (lane >> 2), cb = 4 * NT * (lane & 3);
+    float* const ow = ot + 16 * w * VT;
     const float* gp = a.vec + ((slot0 + c0) * a.Hv + hv) * kVecs * kC + kGam * kC;
     auto pw = [&](int c, int kb) {                         // qs += P W, columns 32*kb of P; W as the chain left it in wl
       const float* const wc = wl + (c & 1) * L::F;
@@ -750,28 +803,39 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
         }
         bf16x8 b[NO];
         sb::split8<NO>(x, b);
-        sb::mma<NO, NO>(qs[t], pf[kb], b);
+        sb::mma<NO, NO>(qs[t], b, pf[kb]);
       }
     };
     auto second = [&](int c) {                             // the second half, and W for the backward pass
       if (high) pw(c, 1);
-      load_half<NO>(pf[1], pp + (min(c + 1, c1 - 1) - c0) * pstep, pat + (high ? 32 : 0));
+      load_half<NO>(pf[1], pp + (min(c + 1, c1 - 1) - c0) * pstep, pat + (high ? NO * kFrag : 0));
       if constexpr (TRAIN) {
         float* const wp = a.w + ((((slot0 + c) * a.Hv + hv) * (a.vp / 32) + v0 / 32) * kC) * 32 + (v0 & 16);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(wl + (c & 1) * L::F + 16 * t * kC + at32<kC>(lr, ib));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) wp[(unsigned)(ib * 32 + lr) + e * 32 + 16 * t] = y[e];
-        }
+float y[4 * NT];
+        token_row<4 * NT>(y, wl + (c & 1) * L::F, ta, cb);
+        store_row<4 * NT>(wp + (unsigned)(ta * 32 + cb), y);
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) qo[t] = qs[t] * a.scale;
     };
-    auto store = [&](int c) { op.store(c, qo); };
-    qp.load(qf, c0);
+    auto store = [&](int c) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(ow + at32<VT>(lr, 16 * t + 4 * lg)) = qo[t];
+      float y[4 * NT];
+#pragma unroll
+      for (int h = 0; h < NT; ++h) {
+        const f32x4 z = *reinterpret_cast<const f32x4*>(ow + at32<VT>(lane >> 2, cb + 4 * h));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[4 * h + e] = z[e];
+      }
+      op.store(c, y);
+    };
+    vp.load(c0);
+    load_rows<NP, KB>(qf, qp, qat);
     load_tri<NO>(pf, pp, pat, true, high);
-    f32x4 gam = *reinterpret_cast<const f32x4*>(gp + (unsigned)ib);
+    float gam = gp[(unsigned)ia];
+    vp.put(vl + (c0 & 1) * VT * kC, w, lane);
+    vp.load(min(c0 + 1, c1 - 1));
     for (int c = c0; c < c1; ++c) {
       lds_barrier();
 #pragma unroll
@@ -782,16 +846,18 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
         for (int t = 0; t < NT; ++t) {
           bf16x8 b[NO];
           sb::load_frag<NO>(b, sl + 16 * t * Kp + at16<Kp>(lr, 32 * kb + 8 * lg), VT * Kp);
-          sb::mma<NP, NO>(qn[t], qf[kb], b);
+          sb::mma<NO, NP>(qn[t], b, qf[kb]);
         }
-      qp.load(qf, min(c + 1, c1 - 1));
+      load_rows<NP, KB>(qf, qp + (min(c + 1, c1 - 1) - c0) * qstep, qat);
       if (c > c0 + 1) store(c - 2);
+      vp.put(vl + (~c & 1) * VT * kC, w, lane);
+      vp.load(min(c + 2, c1 - 1));
       lds_barrier();
       if (c > c0) second(c - 1);
 #pragma unroll
       for (int t = 0; t < NT; ++t) qs[t] = qn[t] * gam;
       gp += c + 1 < c1 ? (long)a.Hv * kVecs * kC : 0;
-      gam = *reinterpret_cast<const f32x4*>(gp + (unsigned)ib);
+      gam = gp[(unsigned)ia];
       lds_barrier();
       pw(c, 0);
       load_half<NO>(pf[0], pp + (min(c + 1, c1 - 1) - c0) * pstep, pat);
@@ -807,7 +873,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
 // V from a zero state and on K columns without a v from the unit state), one joins the states along the segments, and the
 // scan then runs with every segment's own first state.  The chain is walked twice, and K / V more columns of it the first
 // time, by eight times the workgroups.
-template <typename T, int NP, int KB2>
+template <typename T, int NP, int KB2, bool WIDE>
 __global__ __launch_bounds__(256, 2) void gdr_segment_kernel(GdrArgs a) {
   constexpr int NT = 2;
   using L = ScanLds<NP, KB2, NT>;
@@ -816,6 +882,7 @@ __global__ __launch_bounds__(256, 2) void gdr_segment_kernel(GdrArgs a) {
   __bf16* const sl = reinterpret_cast<__bf16*>(smem);
   __bf16* const xl = sl + L::S;
   __bf16* const ul = xl + L::X;
+  T* const vl = reinterpret_cast<T*>(ul + L::X);
   int n, hv, v0, seg;
   if (!scan_tile(a, VT, n, hv, v0, seg)) return;           // tiles: the columns of V, then Kp of the unit state
   long start, slot0;
@@ -833,7 +900,7 @@ __global__ __launch_bounds__(256, 2) void gdr_segment_kernel(GdrArgs a) {
     for (int u = 0; u < NT; ++u)
 #pragma unroll
       for (int e = 0; e < 4; ++e) S[t][u][e] = unit && 16 * (KB2 * w + t) + 4 * lg + e == j0 + 16 * u + lr ? 1.f : 0.f;
-  scan_chain<T, NP, KB2, NT, false, true>(a, S, sl, xl, ul, nullptr, hv, unit ? 0 : a.V, unit ? 0 : v0, start, len, slot0, c0, c1);
+  scan_chain<T, NP, KB2, NT, false, true, WIDE>(a, S, sl, xl, ul, vl, nullptr, hv, unit ? 0 : a.V, unit ? 0 : v0, start, len, slot0, c0, c1);
   const long at = ((long)n * a.Hv + hv) * a.segs + seg;
   if (unit) {
     store_seg<KB2, NT>(S, a.seg_m + at * Kp * Kp, Kp, w, j0, lr, lg);
@@ -907,7 +974,7 @@ __global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
 }
 
 // BARE: a segment from a zero gradient (the last one: from d_s1), which leaves only the gradient in front of it, in seg_n.
-template <typename T, int NP, int KB2, int NT, bool BARE>
+template <typename T, int NP, int KB2, int NT, bool BARE, bool WIDE>
 __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
   using L = ScanLds<NP, KB2, NT>;
   constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT;
@@ -919,6 +986,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
   __bf16* const ol = yl + L::X;                            // [NP][VT][kC] dO
   float* const zp = reinterpret_cast<float*>(ol + NP * VT * kC);   // [VT][kC] scale P^T dO
   float* const yf = zp + L::F;                             // [2][VT][kC] Y, of the chunk at hand and the one behind it
+  T* const rl = reinterpret_cast<T*>(yf + 2 * L::F);       // [VT][kC] dO as it comes
   int n, hv, v0, seg;
   if (!scan_tile(a, VT, n, hv, v0, seg)) return;
   const int hk = hv / a.rep;
@@ -930,7 +998,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
   if (BARE) ++seg;                                         // in front of the first segment there is none
   const int c0 = seg * a.seg_chunks, c1 = min(nc, c0 + a.seg_chunks);
   if (seg > 0 && c0 >= nc) return;
-  const int ib = 16 * w + 4 * lg, ia = 16 * w + lr;
+  const int ib = 16 * w + 4 * lg;
   const bool low = w < 2;                                  // P^T and M^T are upper triangular: rows >= 32 read the last 32 columns
   const long nh = (long)n * a.Hv + hv;
   const long slot1 = slot0 + c1 - 1;                       // the last chunk, where the walk begins
@@ -943,17 +1011,17 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
     else load_seg<KB2, NT>(dS, a.seg_s + (nh * a.segs + seg) * Kp * a.vp, a.vp, w, v0, lr, lg);
     if (c0 < c1) {
       bf16x8 kf[KB][NP], mf[2][3], ktf[KB2][2][NP], qtf[KB2][2][NP];
-      const RowPtr<NP, KB> kp(a, a.k, a.ldk, a.kpk, slot0, hk, start, len, ia, lg);
+      const __bf16* kp = a.kpk + (slot1 * a.Hk + hk) * kC * NP * Kp;
       ScanVec vn;
       const float* vecp = a.vec + (slot1 * a.Hv + hv) * kVecs * kC;
       const __bf16* mp = a.mt + (slot1 * a.Hv + hv) * 3 * kC * kC;
       const __bf16 *ktp = a.kt + (slot1 * a.Hk + hk) * Kp * NP * kC, *qtp = a.qt + (slot1 * a.Hk + hk) * Kp * NP * kC;
-      const unsigned mat = ia * 3 * kC + 8 * lg, ktat = (16 * KB2 * w + lr) * NP * kC + 8 * lg;
+      const unsigned kat = w * KB * NP * kFrag + lane * 8, mat = w * 2 * 3 * kFrag + lane * 8, ktat = KB2 * w * 2 * NP * kFrag + lane * 8;
       auto load_t = [&]() {
         load_kt<NP, KB2>(qtf, qtp, ktat);
         load_kt<NP, KB2>(ktf, ktp, ktat);
       };
-      kp.load(kf, c1 - 1);
+      load_rows<NP, KB>(kf, kp, kat);
       vn.load(vecp, ib);
       load_tri<3>(mf, mp, mat, low, true);
       load_t();
@@ -966,6 +1034,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
         mp -= adv * a.Hv * 3 * kC * kC;
         ktp -= adv * a.Hk * NP * Kp * kC;
         qtp -= adv * a.Hk * NP * Kp * kC;
+        kp -= adv * a.Hk * NP * Kp * kC;
         const ScanVec vc = vn;
         const long vs = (slot0 + c) * a.Hv + hv;
 #pragma unroll
@@ -985,7 +1054,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
             sb::load_frag<3>(b, dl + 16 * t * Kp + at16<Kp>(lr, 32 * kb + 8 * lg), VT * Kp);
             sb::mma<NP, 3>(z[t], kf[kb], b);
           }
-        kp.load(kf, next);
+        load_rows<NP, KB>(kf, kp, kat);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const f32x4 p = *reinterpret_cast<const f32x4*>(zp + 16 * t * kC + at32<kC>(lr, ib));
@@ -1037,10 +1106,11 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
   } else if (c0 < c1) {                                    // ---- dO's share, ahead of the chain; Y and dV, behind it
     bf16x8 pf[2][3];
     const bool has_do = a.d_o != nullptr;
-    ColPtr<T, NT> dp(has_do ? a.d_o : a.v, has_do ? a.lddo : a.ldv, start, len, hv, has_do ? a.V : 0, v0, lr, ib);
+    RowTile<T, NT, WIDE> dp(has_do ? a.d_o : a.v, has_do ? a.lddo : a.ldv, start, len, hv, has_do ? a.V : 0, has_do ? v0 : 0, w, lane);
     const __bf16* const pt = a.pt + (slot0 * a.Hv + hv) * 3 * kC * kC;
-    const unsigned pat = ia * 3 * kC + 8 * lg;
-    ColOut<T, NT> vo(a.dv, a.lddv, start, len, hv, a.V, v0, lr, ib);
+    const unsigned pat = w * 2 * 3 * kFrag + lane * 8;
+    const RowTile<T, NT, WIDE> vo(a.dv, a.lddv, start, len, hv, a.V, v0, w, lane);
+    const int ta = 16 * w + (lane >> 2), cb = 4 * NT * (lane & 3);
     const float* const vec = a.vec + (slot0 * a.Hv + hv) * kVecs * kC;
     const long pstep = (long)a.Hv * 3 * kC * kC, vstep = (long)a.Hv * kVecs * kC;
     f32x4 d[NT], dn[NT];                                   // dO of the chunk at hand and of the next one
@@ -1064,7 +1134,8 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
     load_tri<3>(pf, pt + (c1 - 1) * pstep, pat, low, true);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      dn[t] = dp.get(t);
+      if (t == 0) dp.put(rl, w, lane);                      // (a wave's tokens are read by nobody else)
+      dn[t] = wide4(column4<T>(rl + 16 * t * kC, lr, ib));
       sb::split_store4<NP>(ol + 16 * t * kC + at16<kC>(lr, ib), VT * kC, dn[t]);
     }
     dp.load(max(c1 - 2, c0));
@@ -1073,24 +1144,24 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
     load_tri<3>(pf, pt + max(c1 - 2, c0) * pstep, pat, low, true);
     lds_barrier();
     // Y and dV of chunk c, which the chain has left in yf
-    auto finish = [&](int c, const f32x4& beta) {
+    auto finish = [&](int c, float beta) {
       float* const yp = a.y + ((((slot0 + c) * a.Hv + hv) * (a.vp / 32) + v0 / 32) * kC) * 32 + (v0 & 16);
-      f32x4 y[NT];
+      float y[4 * NT];
+      token_row<4 * NT>(y, yf + (c & 1) * L::F, ta, cb);
+      store_row<4 * NT>(yp + (unsigned)(ta * 32 + cb), y);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        y[t] = *reinterpret_cast<const f32x4*>(yf + (c & 1) * L::F + 16 * t * kC + at32<kC>(lr, ib));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) yp[(unsigned)(ib * 32 + lr) + e * 32 + 16 * t] = y[t][e];
-        y[t] *= beta;
-      }
+      for (int e = 0; e < 4 * NT; ++e) y[e] *= beta;
       vo.store(c, y);
     };
-    f32x4 gam = *reinterpret_cast<const f32x4*>(vec + (c1 - 1) * vstep + kGam * kC + (unsigned)ib), beta = *reinterpret_cast<const f32x4*>(vec + (c1 - 1) * vstep + kBeta * kC + (unsigned)ib);
-    f32x4 before = zero;                                   // beta of the chunk behind
+    f32x4 gam = *reinterpret_cast<const f32x4*>(vec + (c1 - 1) * vstep + kGam * kC + (unsigned)ib);
+    float beta = vec[(c1 - 1) * vstep + kBeta * kC + (unsigned)ta], before = 0.f;                                   // beta of the chunk behind
     for (int c = c1 - 1; c >= c0; --c) {
       const int next = max(c - 1, c0), next2 = max(c - 2, c0);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) { d[t] = dn[t]; dn[t] = dp.get(t); }
+      for (int t = 0; t < NT; ++t) d[t] = dn[t];
+      dp.put(rl, w, lane);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) dn[t] = wide4(column4<T>(rl + 16 * t * kC, lr, ib));
       dp.load(next2);
       lds_barrier();                                       // 1: the chain has read the previous chunk's gl
 #pragma unroll
@@ -1104,7 +1175,7 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
       load_tri<3>(pf, pt + next2 * pstep, pat, low, true);
       if (!BARE && c < c1 - 1) finish(c + 1, before);
       before = beta;
-      beta = *reinterpret_cast<const f32x4*>(vec + next * vstep + kBeta * kC + (unsigned)ib);
+      beta = vec[next * vstep + kBeta * kC + (unsigned)ta];
       lds_barrier();                                       // 3
     }
     if (!BARE) finish(c0, before);
@@ -1166,7 +1237,7 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
     for (int u = 0; u < Kp / 64; ++u) { x[u] = gk[u * 512 + tid]; y[u] = gq[u * 512 + tid]; }
 #pragma unroll
     for (int u = 0; u < Kp / 64; ++u) {
-      const int at = at16<kC>(u * 64 + (tid >> 3), (tid & 7) * 8);
+      const int blk = u * 8 + wave, at = at16<kC>(16 * (blk >> 1) + (tid & 15), 32 * (blk & 1) + 8 * (tid >> 4 & 3));
       *reinterpret_cast<bf16x8*>(kl + at) = x[u];
       *reinterpret_cast<bf16x8*>(ql + at) = y[u];
     }
@@ -1419,13 +1490,13 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
     } else {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        // 16 bytes of a term's row (32 tokens are four) per thread: columns 16 * wave + lane / 4, + 128, ..
-        constexpr int U = (NP * Kp + 127) / 128;
+        // a block of 16 columns of k (q) by 32 tokens per wave
+        constexpr int U = (NP * Kp / 16 + 7) / 8;
         bf16x8 x[2][U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int row = min(u * 128 + ((64 * wave + lane) >> 2), NP * Kp - 1), p = row / Kp, k = row - p * Kp;
-          const long at = ((hs * Kp + k) * NP + p) * kC + 32 * kb + 8 * (lane & 3);
+          const int blk = min(u * 8 + wave, NP * Kp / 16 - 1), t = blk / NP, p = blk - t * NP;
+          const long at = hs * Kp * NP * kC + ((t * 2 + kb) * NP + p) * kFrag + lane * 8;
           x[0][u] = *reinterpret_cast<const bf16x8*>(a.kt + at);
           x[1][u] = *reinterpret_cast<const bf16x8*>(a.qt + at);
         }
@@ -1437,7 +1508,8 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int at = at16<LDR>(min(u * 128 + ((64 * wave + lane) >> 2), NP * Kp - 1), 8 * (lane & 3));    // (the last row's copies are the same)
+          const int blk = min(u * 8 + wave, NP * Kp / 16 - 1), t = blk / NP, p = blk - t * NP;      // (the last block's copies are the same)
+          const int at = at16<LDR>(p * Kp + 16 * t + lr, 8 * lg);
           *reinterpret_cast<bf16x8*>(kl + at) = x[0][u];
           *reinterpret_cast<bf16x8*>(ql + at) = x[1][u];
         }
@@ -1624,6 +1696,11 @@ __global__ __launch_bounds__(256) void gdr_step_kernel(GdrStepArgs a) {
 namespace {
 
 bool a16(const void* p) { return (reinterpret_cast<unsigned long long>(p) & 15) == 0; }
+// rows of V elements that may be taken in 16-byte pieces
+int rows16(int dtype, int V, const void* p, long ld) {
+  const int n = dtype == HHRL_BF16 ? 8 : 4;
+  return V % n == 0 && ld % n == 0 && a16(p);
+}
 int padded_k(int K) { return K <= 64 ? 64 : 128; }
 long slots_of(int n_seq, long rows, bool packed) {
   return packed ? rows / kC + n_seq : (long)n_seq * ((rows / n_seq + kC - 1) / kC);
@@ -1721,33 +1798,34 @@ int gdr_fill(const hhrl_gdr_desc* d, GdrArgs& a, bool train, const char* who) {
   a.q = d->q; a.k = d->k; a.v = d->v; a.ldq = d->ldq; a.ldk = d->ldk; a.ldv = d->ldv;
   a.g = d->g; a.beta = d->beta; a.ldg = d->ldg; a.ldbeta = d->ldbeta;
   a.train = train;
+  a.v16 = rows16(d->dtype, d->V, d->v, d->ldv);
   a.wide = d->K % 8 == 0 && a16(d->q) && a16(d->k) && d->ldq % 8 == 0 && d->ldk % 8 == 0;
-  a.pack = !(d->dtype == HHRL_BF16 && d->K == padded_k(d->K) && a.wide);
+  a.whole = d->K == padded_k(d->K) && a.wide;
   return HHRL_OK;
 }
 
 // Columns per workgroup of a scan: 32 (two result tiles per wave) where that fills the chip's 256 CUs, else 16: twice the
 // workgroups, and a shorter chain from chunk to chunk.
 #ifndef SCAN_NT
-#define SCAN_NT(wgs32) ((wgs32) >= 256 ? 2 : 1)
+#define SCAN_NT(wgs32) ((wgs32) > 128 ? 2 : 1)
 #endif
 int scan_tiles(const GdrArgs& a) { return a.segs > 1 ? 2 : SCAN_NT((long)a.n_seq * a.Hv * (a.vp / 32)); }
 unsigned scan_grid(const GdrArgs& a) { return (unsigned)(((long)a.n_seq * a.Hv * a.grid_segs + 7) / 8 * 8 * a.nvt); }
 
-template <typename T, int NP, int KB2, int NT>
+template <typename T, int NP, int KB2, int NT, bool WIDE>
 int run_scan(GdrArgs a, bool bwd, hipStream_t st, double flops, bool bare = false) {
   a.nvt = a.vp / (16 * NT);
   if (bwd) {
     a.grid_segs = bare ? a.segs - 1 : a.segs;
     constexpr int lds = ScanLds<NP, KB2, NT>::bwd_bytes;
-    void (*const fn)(GdrArgs) = bare ? gdr_scan_bwd_kernel<T, NP, KB2, NT, true> : gdr_scan_bwd_kernel<T, NP, KB2, NT, false>;
+    void (*const fn)(GdrArgs) = bare ? gdr_scan_bwd_kernel<T, NP, KB2, NT, true, WIDE> : gdr_scan_bwd_kernel<T, NP, KB2, NT, false, WIDE>;
     HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(fn), lds, "gdr_backward"));
     ProfScope ps(bare ? "gdr_segment_bwd_kernel" : "gdr_scan_bwd_kernel", st, flops, 0.0);
     hipLaunchKernelGGL(fn, dim3(scan_grid(a)), dim3(512), lds, st, a);
   } else {
     a.grid_segs = a.segs;
     constexpr int lds = ScanLds<NP, KB2, NT>::fwd_bytes;
-    void (*const fn)(GdrArgs) = a.train ? gdr_scan_fwd_kernel<T, NP, KB2, NT, true> : gdr_scan_fwd_kernel<T, NP, KB2, NT, false>;
+    void (*const fn)(GdrArgs) = a.train ? gdr_scan_fwd_kernel<T, NP, KB2, NT, true, WIDE> : gdr_scan_fwd_kernel<T, NP, KB2, NT, false, WIDE>;
     HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(fn), lds, "gdr_forward"));
     ProfScope ps("gdr_scan_fwd_kernel", st, flops, 0.0);
     hipLaunchKernelGGL(fn, dim3(scan_grid(a)), dim3(512), lds, st, a);
@@ -1755,14 +1833,14 @@ int run_scan(GdrArgs a, bool bwd, hipStream_t st, double flops, bool bare = fals
   return launch_status(bwd ? "gdr_scan_bwd_kernel" : "gdr_scan_fwd_kernel");
 }
 // M and N of the segments
-template <typename T, int NP, int KB2>
+template <typename T, int NP, int KB2, bool WIDE>
 int run_segments(GdrArgs a, hipStream_t st) {
-  constexpr int lds = 2 * (ScanLds<NP, KB2, 2>::S + 2 * ScanLds<NP, KB2, 2>::X);
-  HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(&gdr_segment_kernel<T, NP, KB2>), lds, "gdr_forward"));
+  constexpr int lds = ScanLds<NP, KB2, 2>::chain_bytes;
+  HHRL_TRY(ensure_dyn_lds(reinterpret_cast<const void*>(&gdr_segment_kernel<T, NP, KB2, WIDE>), lds, "gdr_forward"));
   a.grid_segs = a.segs - 1;
   a.nvt = (a.vp + 64 * KB2) / 32;
   ProfScope ps("gdr_segment_kernel", st, 0.0, 0.0);
-  hipLaunchKernelGGL((gdr_segment_kernel<T, NP, KB2>), dim3(scan_grid(a)), dim3(256), lds, st, a);
+  hipLaunchKernelGGL((gdr_segment_kernel<T, NP, KB2, WIDE>), dim3(scan_grid(a)), dim3(256), lds, st, a);
   return launch_status("gdr_segment_kernel");
 }
 template <int KB2>
@@ -1773,14 +1851,18 @@ int run_join(GdrArgs a, bool bwd, hipStream_t st) {
   hipLaunchKernelGGL((gdr_join_kernel<KB2>), dim3(scan_grid(a)), dim3(256), 0, st, a, bwd);
   return launch_status("gdr_join_kernel");
 }
-template <typename T, int NP, int KB2>
-int run_scan(const GdrArgs& a, bool bwd, hipStream_t st, double flops) {
+template <typename T, int NP, int KB2, bool WIDE>
+int run_scans(const GdrArgs& a, bool bwd, hipStream_t st, double flops) {
   if (a.segs > 1) {
-    if (bwd) HHRL_TRY((run_scan<T, NP, KB2, 2>(a, true, st, 0.0, true)));
-    else HHRL_TRY((run_segments<T, NP, KB2>(a, st)));
+    if (bwd) HHRL_TRY((run_scan<T, NP, KB2, 2, WIDE>(a, true, st, 0.0, true)));
+    else HHRL_TRY((run_segments<T, NP, KB2, WIDE>(a, st)));
     HHRL_TRY(run_join<KB2>(a, bwd, st));
   }
-  return scan_tiles(a) == 2 ? run_scan<T, NP, KB2, 2>(a, bwd, st, flops) : run_scan<T, NP, KB2, 1>(a, bwd, st, flops);
+  return scan_tiles(a) == 2 ? run_scan<T, NP, KB2, 2, WIDE>(a, bwd, st, flops) : run_scan<T, NP, KB2, 1, WIDE>(a, bwd, st, flops);
+}
+template <typename T, int NP, int KB2>
+int run_scans(const GdrArgs& a, bool bwd, hipStream_t st, double flops) {
+  return a.v16 ? run_scans<T, NP, KB2, true>(a, bwd, st, flops) : run_scans<T, NP, KB2, false>(a, bwd, st, flops);
 }
 
 template <typename T, int NP, int KB2>
@@ -1792,7 +1874,7 @@ int run_fwd(const GdrArgs& a, hipStream_t st, double flops) {
     hipLaunchKernelGGL((gdr_prep_kernel<T, NP, KB2>), dim3((unsigned)a.n_slots, a.Hk), dim3(256), lds_prep, st, a);
   }
   HHRL_TRY(launch_status("gdr_prep_kernel"));
-  return run_scan<T, NP, KB2>(a, false, st, flops);
+  return run_scans<T, NP, KB2>(a, false, st, flops);
 }
 
 template <typename T, int NP, int KB2, bool GROUP>
@@ -1806,7 +1888,7 @@ int run_grads(const GdrArgs& a, hipStream_t st, double flops) {
 
 template <typename T, int NP, int KB2>
 int run_bwd(const GdrArgs& a, hipStream_t st, double flops) {
-  HHRL_TRY((run_scan<T, NP, KB2>(a, true, st, flops)));
+  HHRL_TRY((run_scans<T, NP, KB2>(a, true, st, flops)));
   return a.rep > 1 ? run_grads<T, NP, KB2, true>(a, st, flops) : run_grads<T, NP, KB2, false>(a, st, flops);
 }
 
@@ -1836,6 +1918,7 @@ int hhrl_gdr_forward(const hhrl_gdr_desc* d, void* stream) {
   HHRL_REQUIRE(d->ldo < (1L << 22), "gdr_forward: ldo=%ld too large", d->ldo);
   GdrArgs a = {};
   HHRL_TRY(gdr_fill(d, a, !d->no_backward, "gdr_forward"));
+  a.v16 = a.v16 && rows16(d->dtype, d->V, d->o, d->ldo);
   a.o = d->o; a.ldo = d->ldo; a.s0 = d->s0; a.s1 = d->s1;
   const double flops = 6.0 * d->rows * d->Hv * d->K * d->V;
   hipStream_t st = as_stream(stream);
@@ -1852,6 +1935,7 @@ int hhrl_gdr_backward(const hhrl_gdr_desc* d, void* stream) {
   HHRL_REQUIRE((!d->d_o || d->lddo < (1L << 22)) && d->lddv < (1L << 22), "gdr_backward: leading dimension of d_o or dv too large");
   GdrArgs a = {};
   HHRL_TRY(gdr_fill(d, a, true, "gdr_backward"));
+  a.v16 = (d->d_o ? rows16(d->dtype, d->V, d->d_o, d->lddo) : a.v16) && rows16(d->dtype, d->V, d->dv, d->lddv);
   a.d_o = d->d_o; a.lddo = d->lddo; a.d_s1 = d->d_s1; a.d_s0 = d->d_s0;
   a.dq = d->dq; a.dk = d->dk; a.dv = d->dv; a.lddq = d->lddq; a.lddk = d->lddk; a.lddv = d->lddv;
   a.dg = d->dg; a.dbeta = d->dbeta; a.lddg = d->lddg; a.lddbeta = d->lddbeta;
