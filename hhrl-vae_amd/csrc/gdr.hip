@@ -903,14 +903,17 @@ __global__ __launch_bounds__(256, 2) void gdr_segment_kernel(GdrArgs a) {
   scan_chain<T, NP, KB2, NT, false, true, WIDE>(a, S, sl, xl, ul, vl, nullptr, hv, unit ? 0 : a.V, unit ? 0 : v0, start, len, slot0, c0, c1);
   const long at = ((long)n * a.Hv + hv) * a.segs + seg;
   if (unit) {
-    store_seg<KB2, NT>(S, a.seg_m + at * Kp * Kp, Kp, w, j0, lr, lg);
-    if (a.train) {                                         // and transposed, for the gradients' way back
+    // as operand blocks (fp32), and transposed for the gradients' way back
 #pragma unroll
-      for (int t = 0; t < KB2; ++t)
+    for (int t = 0; t < KB2; ++t)
 #pragma unroll
-        for (int u = 0; u < NT; ++u)
-          *reinterpret_cast<f32x4*>(a.seg_mt + (at * Kp + j0 + 16 * u + lr) * Kp + 16 * (KB2 * w + t) + 4 * lg) = S[t][u];
-    }
+      for (int u = 0; u < NT; ++u) {
+        const int k0 = 16 * (KB2 * w + t), c0 = j0 + 16 * u;
+        float* const m = a.seg_m + at * Kp * Kp + ((k0 >> 4) * (Kp / 32) + (c0 >> 5)) * kFrag;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[frag_at(4 * lg + e, (c0 & 16) + lr)] = S[t][u][e];
+        if (a.train) *reinterpret_cast<f32x4*>(a.seg_mt + at * Kp * Kp + ((c0 >> 4) * (Kp / 32) + (k0 >> 5)) * kFrag + frag_at(lr, (k0 & 16) + 4 * lg)) = S[t][u];
+      }
   } else {
     store_seg<KB2, NT>(S, a.seg_n + at * Kp * a.vp, a.vp, w, v0, lr, lg);
   }
@@ -942,7 +945,7 @@ __global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
       store_seg<KB2, 1>(S, a.seg_s + (nh * a.segs + g - 1) * Kp * a.vp, a.vp, w, v0, lr, lg);
       continue;
     }
-    const float* const m = (bwd ? a.seg_mt : a.seg_m) + (at * Kp + 16 * KB2 * w + lr) * Kp + 8 * lg;
+    const float* const m = (bwd ? a.seg_mt : a.seg_m) + at * Kp * Kp + KB2 * w * KB * kFrag + lane * 8;
     f32x4 next[KB2][1];
     load_seg<KB2, 1>(next, a.seg_n + at * Kp * a.vp, a.vp, w, v0, lr, lg);
 #pragma unroll
@@ -957,7 +960,7 @@ __global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
         float x[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(m + 16 * t * Kp + 32 * kb + 4 * h);
+          const f32x4 y = *reinterpret_cast<const f32x4*>(m + (t * KB + kb) * kFrag + 4 * h);
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[4 * h + e] = y[e];
         }
@@ -1194,29 +1197,26 @@ struct GradsLds {
   // of k and q at a time
   static constexpr int LDR = NP == 1 ? kC : 32;
   static constexpr int tri = 4 * 3 * kC * LDR + (NP == 1 ? 0 : 2 * NP * Kp * LDR);
-  static constexpr int over = 2 * (cols > tri ? cols : tri);
-  static constexpr int kq = NP == 1 ? 2 * 2 * Kp * kC : 0;                     // bytes: k and q of the chunk, transposed (three terms do not fit)
-  static constexpr int bytes = over + kq + (8 * kC + 8) * 4;
+  static constexpr int NB = NP == 1 ? 2 : 1;                 // column images: two where they fit
+  static constexpr int over = 2 * (NB * cols > tri ? NB * cols : tri);
+  static constexpr int bytes = over + (8 * kC + 8) * 4;
 };
 template <typename T, int NP, int KB2, bool GROUP>
 __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
   using L = GradsLds<NP, KB2>;
   constexpr int Kp = L::Kp, LDV = L::LDV, KT = Kp / 32;      // k tiles of a wave
   extern __shared__ __align__(16) char smem[];
-  __bf16* const sl = reinterpret_cast<__bf16*>(smem);        // [3][Kp][LDV]
-  __bf16* const dl = sl + 3 * Kp * LDV;                      // [3][Kp][LDV]
-  __bf16* const wl = dl + 3 * Kp * LDV;                      // [3][64][LDV]
-  __bf16* const yl = wl + 3 * kC * LDV;                      // [3][64][LDV]
-  __bf16* const ol = yl + 3 * kC * LDV;                      // [NP][64][LDV]
+  __bf16* const img = reinterpret_cast<__bf16*>(smem);
+  constexpr int DL = 3 * Kp * LDV, WL = 2 * DL, YL = WL + 3 * kC * LDV, OL = YL + 3 * kC * LDV;   // [3][Kp][LDV] S and dS', [3][64][LDV] W and Y, [NP][64][LDV] dO
   constexpr int LDR = L::LDR;
   __bf16* const rl = reinterpret_cast<__bf16*>(smem);        // [3][64][LDR] each
   __bf16* const bl = rl + 3 * kC * LDR;
   __bf16* const rt = bl + 3 * kC * LDR;
   __bf16* const bt = rt + 3 * kC * LDR;
-  // k and q, transposed: for the kernel's length (one term, [Kp][64] each) or 32 tokens at a time ([NP][Kp][32] each)
-  __bf16* const kl = NP == 1 ? reinterpret_cast<__bf16*>(smem + L::over) : bt + 3 * kC * LDR;
+  // k and q, transposed, 32 tokens at a time ([NP][Kp][32] each; one term comes straight from the workspace)
+  __bf16* const kl = bt + 3 * kC * LDR;
   __bf16* const ql = kl + NP * Kp * LDR;
-  float* const rows = reinterpret_cast<float*>(smem + L::over + L::kq);    // [2 halves][3][64]: shares of dG, of dbeta, k.(tail E3)
+  float* const rows = reinterpret_cast<float*>(smem + L::over);    // [2 halves][3][64]: shares of dG, of dbeta, k.(tail E3)
   float* const yv = rows + 6 * kC;                                 // [64] Y.v
   float* const red = yv + kC;                                      // [8]
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave >> 1, half = wave & 1, kt0 = 16 * KT * half;
@@ -1229,19 +1229,6 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
   const long hs = slot * a.Hk + hk;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   const bool has_do = a.d_o != nullptr;
-  if constexpr (NP == 1) {
-    const bf16x8* const gk = reinterpret_cast<const bf16x8*>(a.kt + hs * Kp * kC);
-    const bf16x8* const gq = reinterpret_cast<const bf16x8*>(a.qt + hs * Kp * kC);
-    bf16x8 x[Kp / 64], y[Kp / 64];
-#pragma unroll
-    for (int u = 0; u < Kp / 64; ++u) { x[u] = gk[u * 512 + tid]; y[u] = gq[u * 512 + tid]; }
-#pragma unroll
-    for (int u = 0; u < Kp / 64; ++u) {
-      const int blk = u * 8 + wave, at = at16<kC>(16 * (blk >> 1) + (tid & 15), 32 * (blk & 1) + 8 * (tid >> 4 & 3));
-      *reinterpret_cast<bf16x8*>(kl + at) = x[u];
-      *reinterpret_cast<bf16x8*>(ql + at) = y[u];
-    }
-  }
   f32x4 dqs[GROUP ? KT : 1], dks[GROUP ? KT : 1];
   if (GROUP) {
 #pragma unroll
@@ -1289,62 +1276,59 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
         __builtin_memcpy(xo, raw, sizeof(raw));
       }
     };
-    request(0);
-    for (int vb = 0; vb < a.vp; vb += 32) {
-      lds_barrier();
-      {
-        float x[8];
-        bf16x8 t[3];
-        if (has_s) {
+    // columns vb .., which have been requested, into an image
+    auto stage = [&](int vb, __bf16* im) {
+      float x[8];
+      bf16x8 t[3];
+      if (has_s) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            sdot = fmaf(xs[0][e], xd[0][e], fmaf(xs[1][e], xd[1][e], sdot));
-            unsigned u[3], v[3];
-            sb::split2<3>(xs[0][e], xs[1][e], u);
-            sb::split2<3>(xd[0][e], xd[1][e], v);
+        for (int e = 0; e < 4; ++e) {
+          sdot = fmaf(xs[0][e], xd[0][e], fmaf(xs[1][e], xd[1][e], sdot));
+          unsigned u[3], v[3];
+          sb::split2<3>(xs[0][e], xs[1][e], u);
+          sb::split2<3>(xd[0][e], xd[1][e], v);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) {
-              *reinterpret_cast<unsigned*>(sl + p * Kp * LDV + si + e * LDV) = u[p];
-              *reinterpret_cast<unsigned*>(dl + p * Kp * LDV + si + e * LDV) = v[p];
-            }
+          for (int p = 0; p < 3; ++p) {
+            *reinterpret_cast<unsigned*>(im + p * Kp * LDV + si + e * LDV) = u[p];
+            *reinterpret_cast<unsigned*>(im + DL + p * Kp * LDV + si + e * LDV) = v[p];
           }
         }
-        float o[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const unsigned y = sizeof(T) == 2 ? e & 1 ? xo[0][e >> 1] & 0xffff0000u : xo[0][e >> 1] << 16 : xo[sizeof(T) / 2 - 1 - (e < 4)][e & 3];
-          o[e] = gi < valid && vb + gc + e < a.V ? __uint_as_float(y) : 0.f;
-        }
-        __bf16* const dst = (wave < 4 ? wl : yl) + at16<LDV>(gi, gc);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = xw[e >> 2][e & 3];
-        sb::split8<3>(x, t);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dst + p * kC * LDV) = t[p];
-        if (wave < 4) {
-          bf16x8 u[NP];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = has_do ? o[e] : 0.f;
-          sb::split8<NP>(o, u);
-#pragma unroll
-          for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(ol + p * kC * LDV + at16<LDV>(gi, gc)) = u[p];
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) ydot = fmaf(x[e], o[e], ydot);
-        }
       }
-      request(min(vb + 32, a.vp - 32));                        // in front of the barrier: behind it the compiler moves them below the products
-      lds_barrier();
+      float o[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const unsigned y = sizeof(T) == 2 ? e & 1 ? xo[0][e >> 1] & 0xffff0000u : xo[0][e >> 1] << 16 : xo[sizeof(T) / 2 - 1 - (e < 4)][e & 3];
+        o[e] = gi < valid && vb + gc + e < a.V ? __uint_as_float(y) : 0.f;
+      }
+      __bf16* const dst = im + (wave < 4 ? WL : YL) + at16<LDV>(gi, gc);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = xw[e >> 2][e & 3];
+      sb::split8<3>(x, t);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(dst + p * kC * LDV) = t[p];
+      if (wave < 4) {
+        bf16x8 u[NP];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = has_do ? o[e] : 0.f;
+        sb::split8<NP>(o, u);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(im + OL + p * kC * LDV + at16<LDV>(gi, gc)) = u[p];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ydot = fmaf(x[e], o[e], ydot);
+      }
+    };
+    auto products = [&](const __bf16* im) {
       bf16x8 of[NP], yf[3], wf[3];
       const int fr = at16<LDV>(lr, 8 * lg);
-      sb::load_frag<NP>(of, ol + 16 * w * LDV + fr, kC * LDV);
-      sb::load_frag<3>(yf, yl + 16 * w * LDV + fr, kC * LDV);
-      sb::load_frag<3>(wf, wl + 16 * w * LDV + fr, kC * LDV);
+      sb::load_frag<NP>(of, im + OL + 16 * w * LDV + fr, kC * LDV);
+      sb::load_frag<3>(yf, im + YL + 16 * w * LDV + fr, kC * LDV);
+      sb::load_frag<3>(wf, im + WL + 16 * w * LDV + fr, kC * LDV);
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
         bf16x8 b[3], d[3];
-        sb::load_frag<3>(b, sl + (kt0 + 16 * t) * LDV + fr, Kp * LDV);
-        sb::load_frag<3>(d, dl + (kt0 + 16 * t) * LDV + fr, Kp * LDV);
+        sb::load_frag<3>(b, im + (kt0 + 16 * t) * LDV + fr, Kp * LDV);
+        sb::load_frag<3>(d, im + DL + (kt0 + 16 * t) * LDV + fr, Kp * LDV);
         sb::mma<NP, 3>(e1[t], of, b);
         sb::mma<3, 3>(e2[t], yf, b);
         sb::mma<3, 3>(e3[t], wf, d);
@@ -1354,10 +1338,54 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
         const int jt = 2 * t + half;
         if (jt <= w) {
           bf16x8 b[3];
-          sb::load_frag<3>(b, wl + 16 * jt * LDV + fr, kC * LDV);
+          sb::load_frag<3>(b, im + WL + 16 * jt * LDV + fr, kC * LDV);
           sb::mma<NP, 3>(dp[t], of, b);
           sb::mma<3, 3>(da[t], yf, b);
         }
+      }
+    };
+    // k and q in the layout of a result: four tokens of one column, from the transposes or from the caller's rows
+    bf16x4 kr[NP == 1 ? KT : 1], qr[NP == 1 ? KT : 1];
+    bf16x8 kf1[2][NP == 1 ? KT : 1], qf1[2][NP == 1 ? KT : 1];   // and as operands of the products below
+    unsigned kx[NP == 1 ? 1 : KT][4], qx[NP == 1 ? 1 : KT][4];
+    auto own = [&]() {
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const long at = hs * Kp * kC + (kt0 / 16 + t) * 2 * kFrag;
+        kr[t] = *reinterpret_cast<const bf16x4*>(a.kt + at + (w >> 1) * kFrag + frag_at(lr, ib));
+        qr[t] = *reinterpret_cast<const bf16x4*>(a.qt + at + (w >> 1) * kFrag + frag_at(lr, ib));
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          kf1[kb][t] = *reinterpret_cast<const bf16x8*>(a.kt + at + kb * kFrag + lane * 8);
+          qf1[kb][t] = *reinterpret_cast<const bf16x8*>(a.qt + at + kb * kFrag + lane * 8);
+        }
+      }
+      asm volatile("" ::: "memory");                         // or the requests would move below the products
+    };
+    request(0);
+    if constexpr (L::NB == 2) {
+      // Two waves share a SIMD: one of them multiplies while the other splits the next columns, then the other way round.
+      stage(0, img);
+      request(min(32, a.vp - 32));
+      lds_barrier();
+      int cur = 0;
+      for (int vb = 32; vb < a.vp; vb += 32) {
+        if (wave < 4) products(img + cur);
+        stage(vb, img + L::cols - cur);
+        request(min(vb + 32, a.vp - 32));
+        if (wave >= 4) products(img + cur);
+        cur = L::cols - cur;
+        lds_barrier();
+      }
+      own();
+      products(img + cur);
+    } else {
+      for (int vb = 0; vb < a.vp; vb += 32) {
+        lds_barrier();
+        stage(vb, img);
+        request(min(vb + 32, a.vp - 32));                    // in front of the barrier: behind it the compiler moves them below the products
+        lds_barrier();
+        products(img);
       }
     }
     // ---- the chunk's own part
@@ -1374,16 +1402,7 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
       hj[t] = vec[kGHi * kC + 16 * (2 * t + half) + lr];
       lj[t] = vec[kGLo * kC + 16 * (2 * t + half) + lr];
     }
-    // k and q in the layout of a result: four tokens of one column, from the transposes or from the caller's rows
-    bf16x4 kr[NP == 1 ? KT : 1], qr[NP == 1 ? KT : 1];
-    unsigned kx[NP == 1 ? 1 : KT][4], qx[NP == 1 ? 1 : KT][4];
-    if constexpr (NP == 1) {
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        kr[t] = *reinterpret_cast<const bf16x4*>(kl + at16<kC>(kt0 + 16 * t + lr, ib));
-        qr[t] = *reinterpret_cast<const bf16x4*>(ql + at16<kC>(kt0 + 16 * t + lr, ib));
-      }
-    } else {
+    if constexpr (NP != 1) {
       const __amdgpu_buffer_rsrc_t rk = rows_rsrc(a.k, (row0 * a.ldk + (long)hk * a.K) * 4, ((valid - 1) * a.ldk + a.K) * 4);
       const __amdgpu_buffer_rsrc_t rq = rows_rsrc(a.q, (row0 * a.ldq + (long)hk * a.K) * 4, ((valid - 1) * a.ldq + a.K) * 4);
 #pragma unroll
@@ -1457,7 +1476,8 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
           bf16x8 b[NP];
-          sb::load_frag<NP>(b, kf + 16 * t * LDR, Kp * LDR);
+          if constexpr (NP == 1) b[0] = kf1[kb][t];
+          else sb::load_frag<NP>(b, kf + 16 * t * LDR, Kp * LDR);
           sb::mma<3, NP>(e1[t], rf, b);
           sb::mma<3, NP>(e2[t], bf, b);
         }
@@ -1469,9 +1489,11 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
           bf16x8 b[NP];
-          sb::load_frag<NP>(b, qf + 16 * t * LDR, Kp * LDR);
+          if constexpr (NP == 1) b[0] = qf1[kb][t];
+          else sb::load_frag<NP>(b, qf + 16 * t * LDR, Kp * LDR);
           sb::mma<3, NP>(e3[t], rf, b);
-          sb::load_frag<NP>(b, kf + 16 * t * LDR, Kp * LDR);
+          if constexpr (NP == 1) b[0] = kf1[kb][t];
+          else sb::load_frag<NP>(b, kf + 16 * t * LDR, Kp * LDR);
           sb::mma<3, NP>(e3[t], bf, b);
         }
       }
@@ -1485,8 +1507,8 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
       put_t(0, 0);
       put_t(1, 0);
       __syncthreads();
-#pragma unroll 1
-      for (int kb = 0; kb < 2; ++kb) join(kb, 32 * kb);      // not unrolled: fragments of both halves at once would not fit the registers
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) join(kb, 32 * kb);
     } else {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
