@@ -923,7 +923,7 @@ __global__ __launch_bounds__(256, 2) void gdr_segment_kernel(GdrArgs a) {
 // S <- M S + N, 16 columns per workgroup.  The scan takes all of them from here, s0 (d_s1) too: the workgroup of another
 // segment may have written s1 over it by then.
 template <int KB2>
-__global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
+__global__ __launch_bounds__(256) void gdr_join_kernel(GdrArgs a, bool bwd) {
   constexpr int Kp = 64 * KB2, KB = Kp / 32;
   __shared__ __align__(16) __bf16 sl[3 * 16 * Kp];
   int n, hv, v0, seg;
@@ -937,20 +937,41 @@ __global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
   f32x4 S[KB2][1];
   load_state<KB2, 1>(S, bwd ? a.d_s1 : a.s0, a, nh, w, v0, lr, lg);
   store_seg<KB2, 1>(S, a.seg_s + (nh * a.segs + (bwd ? max(ns - 1, 0) : 0)) * Kp * a.vp, a.vp, w, v0, lr, lg);
-  for (int i = 0; i + 1 < ns; ++i) {
-    const int g = bwd ? ns - 1 - i : i;
-    const long at = nh * a.segs + g;
-    if (bwd && i == 0) {                                   // the last segment has been walked from d_s1
-      load_seg<KB2, 1>(S, a.seg_n + at * Kp * a.vp, a.vp, w, v0, lr, lg);
-      store_seg<KB2, 1>(S, a.seg_s + (nh * a.segs + g - 1) * Kp * a.vp, a.vp, w, v0, lr, lg);
-      continue;
-    }
+  int i = 0;
+  if (bwd && ns > 1) {                                     // the last segment has been walked from d_s1
+    load_seg<KB2, 1>(S, a.seg_n + (nh * a.segs + ns - 1) * Kp * a.vp, a.vp, w, v0, lr, lg);
+    store_seg<KB2, 1>(S, a.seg_s + (nh * a.segs + ns - 2) * Kp * a.vp, a.vp, w, v0, lr, lg);
+    i = 1;
+  }
+  if (i + 1 >= ns) return;
+  // a step is one chain of latencies: its M and N are requested a step ahead
+  f32x4 mn[KB2][KB][2], nn[KB2][1];
+  auto request = [&](int j) {
+    const long at = nh * a.segs + (bwd ? ns - 1 - j : j);
     const float* const m = (bwd ? a.seg_mt : a.seg_m) + at * Kp * Kp + KB2 * w * KB * kFrag + lane * 8;
-    f32x4 next[KB2][1];
-    load_seg<KB2, 1>(next, a.seg_n + at * Kp * a.vp, a.vp, w, v0, lr, lg);
+#pragma unroll
+    for (int t = 0; t < KB2; ++t)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) mn[t][kb][h] = *reinterpret_cast<const f32x4*>(m + (t * KB + kb) * kFrag + 4 * h);
+    load_seg<KB2, 1>(nn, a.seg_n + at * Kp * a.vp, a.vp, w, v0, lr, lg);
+  };
+  request(i);
+  for (; i + 1 < ns; ++i) {
+    f32x4 m[KB2][KB][2], next[KB2][1];
+#pragma unroll
+    for (int t = 0; t < KB2; ++t) {
+      next[t][0] = nn[t][0];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) m[t][kb][h] = mn[t][kb][h];
+    }
+    request(min(i + 1, ns - 2));
 #pragma unroll
     for (int t = 0; t < KB2; ++t) sb::split_store4<3>(sl + at16<Kp>(lr, 16 * (KB2 * w + t) + 4 * lg), 16 * Kp, S[t][0]);
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       bf16x8 b[3];
@@ -959,20 +980,16 @@ __global__ __launch_bounds__(256, 2) void gdr_join_kernel(GdrArgs a, bool bwd) {
       for (int t = 0; t < KB2; ++t) {
         float x[8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const f32x4 y = *reinterpret_cast<const f32x4*>(m + (t * KB + kb) * kFrag + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[4 * h + e] = y[e];
-        }
+        for (int e = 0; e < 8; ++e) x[e] = m[t][kb][e >> 2][e & 3];
         bf16x8 f[3];
         sb::split8<3>(x, f);
         sb::mma<3, 3>(next[t][0], f, b);
       }
     }
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int t = 0; t < KB2; ++t) S[t][0] = next[t][0];
-    store_seg<KB2, 1>(S, a.seg_s + (nh * a.segs + (bwd ? g - 1 : g + 1)) * Kp * a.vp, a.vp, w, v0, lr, lg);
+    store_seg<KB2, 1>(S, a.seg_s + (nh * a.segs + (bwd ? ns - 2 - i : i + 1)) * Kp * a.vp, a.vp, w, v0, lr, lg);
   }
 }
 
