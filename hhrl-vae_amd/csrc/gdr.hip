@@ -187,6 +187,9 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
   slot_chunk(a, slot, row0, valid);
   if (valid == 0) return;
   const long hs = slot * a.Hk + hk;
+  // every wave holds token `lane`; a head's g and beta are requested a head ahead
+  const long grow = row0 + min(lane, valid - 1);
+  float gn = a.g[grow * a.ldg + hk * a.rep], bn = a.beta[grow * a.ldbeta + hk * a.rep];
 
   // k and q as bf16 terms; what lies beyond the sequence or the head's width becomes 0 and is not read
   if (NP == 1 && a.whole) {                                    // rows of Kp elements, 16-byte aligned
@@ -210,42 +213,58 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
         *reinterpret_cast<bf16x8*>((side ? ql : kl) + at16<Kp>(i, c)) = x[side][u];
       }
   } else {
-    for (int side = 0; side < 2; ++side) {
-      const long ld = side ? a.ldq : a.ldk;
-      const T* const src = static_cast<const T*>(side ? a.q : a.k) + row0 * ld + (long)hk * a.K;
-      __bf16* const dst = side ? ql : kl;
-      for (int u = tid; u < kC * KG; u += 256) {
-        const int i = u / KG, c = (u - i * KG) * 8;
-        // (unconditional requests of elements that are there, then a choice)
-        const T* const p = src + min(i, valid - 1) * ld;
-        T raw[8];
-        if (a.wide) {                                          // K % 8 == 0, 16-byte aligned rows
-          const u32x4* const q = reinterpret_cast<const u32x4*>(p + min(c, a.K - 8));
-          u32x4 y[sizeof(T) / 2];
+    constexpr int U = kC * KG / 256;
+    const T* src[2] = {static_cast<const T*>(a.k) + row0 * a.ldk + (long)hk * a.K, static_cast<const T*>(a.q) + row0 * a.ldq + (long)hk * a.K};
+    auto convert = [&](int side, int u, const T (&raw)[8]) {
+      const int i = (u * 256 + tid) / KG, c = (u * 256 + tid - i * KG) * 8;
+      float x[8];
 #pragma unroll
-          for (int h = 0; h < (int)sizeof(T) / 2; ++h) y[h] = q[h];
-          __builtin_memcpy(raw, y, sizeof(raw));
-        } else {
+      for (int e = 0; e < 8; ++e) x[e] = i < valid && c + e < a.K ? (float)raw[e] : 0.f;
+      bf16x8 t[NP];
+      sb::split8<NP>(x, t);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) raw[e] = p[min(c + e, a.K - 1)];
+      for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>((side ? ql : kl) + p * kC * Kp + at16<Kp>(i, c)) = t[p];
+    };
+    // (requests of elements that are there, all at once where they come in pieces of 16 bytes, then a choice)
+    if (a.wide) {                                              // K % 8 == 0, 16-byte aligned rows
+      u32x4 y[2][U][sizeof(T) / 2];
+#pragma unroll
+      for (int side = 0; side < 2; ++side)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = (u * 256 + tid) / KG, c = (u * 256 + tid - i * KG) * 8;
+          const u32x4* const q = reinterpret_cast<const u32x4*>(src[side] + min(i, valid - 1) * (side ? a.ldq : a.ldk) + min(c, a.K - 8));
+#pragma unroll
+          for (int h = 0; h < (int)sizeof(T) / 2; ++h) y[side][u][h] = q[h];
         }
-        float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = i < valid && c + e < a.K ? (float)raw[e] : 0.f;
-        bf16x8 t[NP];
-        sb::split8<NP>(x, t);
+      for (int side = 0; side < 2; ++side)
 #pragma unroll
-        for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(dst + p * kC * Kp + at16<Kp>(i, c)) = t[p];
-      }
+        for (int u = 0; u < U; ++u) {
+          T raw[8];
+          __builtin_memcpy(raw, y[side][u], sizeof(raw));
+          convert(side, u, raw);
+        }
+    } else {
+      for (int side = 0; side < 2; ++side)
+        for (int u = 0; u < U; ++u) {
+          const int i = (u * 256 + tid) / KG, c = (u * 256 + tid - i * KG) * 8;
+          const T* const q = src[side] + min(i, valid - 1) * (side ? a.ldq : a.ldk);
+          T raw[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) raw[e] = q[min(c + e, a.K - 1)];
+          convert(side, u, raw);
+        }
     }
   }
-  __syncthreads();
+  lds_barrier();
   // the transposes: two columns of eight tokens per thread
   for (int side = 0; side < (a.train ? 2 : 1); ++side) {
     const __bf16* const src = side ? ql : kl;
     __bf16* const dst = (side ? a.qt : a.kt) + hs * NP * Kp * kC;
-    for (int u = tid; u < NP * (Kp / 2) * 8; u += 256) {
-      const int k = u % (Kp / 2) * 2, r = u / (Kp / 2), i0 = (r & 7) * 8, p = r >> 3;
+#pragma unroll
+    for (int v = 0; v < NP * Kp / 64; ++v) {
+      const int u = v * 256 + tid, k = u % (Kp / 2) * 2, r = u / (Kp / 2), i0 = (r & 7) * 8, p = r >> 3;
       unsigned x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const unsigned*>(src + p * kC * Kp + at16<Kp>(i0 + e, k));
@@ -291,33 +310,32 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
   for (int r = 0; r < a.rep; ++r) {
     const int hv = hk * a.rep + r;
     const long vs = slot * a.Hv + hv;
-    __syncthreads();                               // kl and ql have been read, the previous head's images too
-    // every wave holds token `lane`: running sum of the log decays in fp64, kept as two floats
-    {
-      const bool in = lane < valid;
-      const long row = row0 + min(lane, valid - 1);
-      float gi = a.g[row * a.ldg + hv], bi = a.beta[row * a.ldbeta + hv];
-      gi = in ? gi < kGMin ? kGMin : gi : 0.f;
-      bi = in ? bi : 0.f;
-      double G = gi;
+    // running sum of the log decays in fp64, kept as two floats
+    float gi = gn, bi = bn;
+    gi = lane < valid ? gi < kGMin ? kGMin : gi : 0.f;
+    bi = lane < valid ? bi : 0.f;
+    double G = gi;
 #pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const double up = __shfl_up(G, off, 64);
-        if (lane >= off) G += up;
-      }
-      const double end = __shfl(G, 63, 64);
-      const float hi = (float)G, lo = (float)(G - (double)hi);
-      if (wave == 0) {
-        gh[lane] = hi; gl[lane] = lo; be[lane] = bi;
-        float* const v = a.vec + vs * kVecs * kC + lane;
-        v[kGam * kC] = expf(hi) * (1.f + lo);
-        v[kTail * kC] = expf((float)(end - G));
-        v[kBeta * kC] = bi;
-        v[kGHi * kC] = hi;
-        v[kGLo * kC] = lo;
-      }
+    for (int off = 1; off < 64; off <<= 1) {
+      const double up = __shfl_up(G, off, 64);
+      if (lane >= off) G += up;
     }
-    __syncthreads();
+    const float hi = (float)G, lo = (float)(G - (double)hi);
+    lds_barrier();                                 // kl and ql have been read, the previous head's images too
+    if (wave == 0) { gh[lane] = hi; gl[lane] = lo; be[lane] = bi; }
+    lds_barrier();
+    const int hn = hk * a.rep + min(r + 1, a.rep - 1);
+    gn = a.g[grow * a.ldg + hn];
+    bn = a.beta[grow * a.ldbeta + hn];
+    if (wave == 0) {
+      const double end = __shfl(G, 63, 64);
+      float* const v = a.vec + vs * kVecs * kC + lane;
+      v[kGam * kC] = expf(hi) * (1.f + lo);
+      v[kTail * kC] = expf((float)(end - G));
+      v[kBeta * kC] = bi;
+      v[kGHi * kC] = hi;
+      v[kGLo * kC] = lo;
+    }
     const int ib = 16 * wave + 4 * lg, iq = 16 * wave + lr;
     __bf16* const pp = a.p + vs * kC * NO * kC;
     __bf16* const pt = a.pt + vs * kC * 3 * kC;
@@ -335,12 +353,12 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
         x[e] = i >= j ? qk[t][e] * d : 0.f;
       }
       if (a.train && ((t < 2) || (wave >= 2))) sb::split_store4<3>(pt + (t * 2 + (wave >> 1)) * 3 * kFrag + frag_at(lr, ib), kFrag, x);       // PT rows j >= 32 hold columns i >= 32
-      const float hi = gh[iq], lo = gl[iq];
+      const float hq = gh[iq], lq = gl[iq];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = iq >= jb + e ? kq[t][e] * decay((hi - gh[jb + e]) + (lo - gl[jb + e])) : 0.f;
+      for (int e = 0; e < 4; ++e) x[e] = iq >= jb + e ? kq[t][e] * decay((hq - gh[jb + e]) + (lq - gl[jb + e])) : 0.f;
       if (t < 2 || wave >= 2) sb::split_store4<NO>(pp + (wave * 2 + (t >> 1)) * NO * kFrag + frag_at(lr, jb), kFrag, x);
     }
-    __syncthreads();
+    lds_barrier();
     {
       // diagonal block `wave`: column lr of the inverse by substitution
       const float* const D = lm + 16 * wave * kLdM + 16 * wave;
@@ -366,7 +384,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
         for (int i = 0; i < 16; ++i) mm[(16 * wave + i) * kLdM + 16 * wave + lr] = x[i];
       }
     }
-    __syncthreads();
+    lds_barrier();
     const mt::f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     if (wave < 2) {
       // 16 x 16 below the diagonal of the two 32 x 32 blocks
@@ -377,16 +395,16 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
       c = mt::wave_mma16<16, kLdM, 1, kLdM, 1>(mm + o2 * kLdM + o2, tm + 16 * wave * kLdM, lane, zero);
       mt::store_block16<kLdM>(mm, o2, o1, -c, lane);
     }
-    __syncthreads();
+    lds_barrier();
     {
       const int ti = 16 * (wave >> 1), tj = 16 * (wave & 1);
       mt::f32x4 c = mt::wave_mma16<32, kLdM, 1, kLdM, 1>(lm + (32 + ti) * kLdM, mm + tj, lane, zero);
       mt::store_block16<kLdM>(tm, ti, tj, c, lane);
-      __syncthreads();
+      lds_barrier();
       c = mt::wave_mma16<32, kLdM, 1, kLdM, 1>(mm + (32 + ti) * kLdM + 32, tm + tj, lane, zero);
       mt::store_block16<kLdM>(mm, 32 + ti, tj, -c, lane);
     }
-    __syncthreads();
+    lds_barrier();
     // 16 elements of a row (or of a column, for the transpose the backward scan reads) per thread
     const int row = 16 * wave + lr, c0 = lg * 16;
     for (int what = 0; what < (a.train ? 2 : 1); ++what) {
