@@ -9,7 +9,7 @@
 //   W = M (beta * (V - gam * (K S)))                      (row i: what token i adds to the state along k_i)
 //   o = scale * (gam * (Q S) + P W),   S' = gam_C S + K^T (exp(G_C - G) * W)
 // M and P do not depend on the state: one launch forms them for all chunks at once (gdr_prep_kernel).  The launch that
-// follows walks the chunks of a sequence (gdr_scan_fwd_kernel); its workgroups hold 32 columns of one head's state in
+// follows walks the chunks of a sequence (gdr_scan_fwd_kernel); its workgroups hold 16 or 32 columns of one head's state in
 // registers: columns do not meet.  K and Q are multiplied as they are; decays are applied to fp32 results.
 // Backward, with dS' the gradient of the state behind the chunk:
 //   Z = scale P^T dO + exp(G_C - G) * (K dS'),   Y = M^T Z,   dV = beta * Y
@@ -26,6 +26,10 @@
 // corrected state is a difference of numbers much larger than itself, its gradients more so, and dg, dbeta and the
 // states are fp32 results.  The decays' sums are kept as two floats from a sum in fp64, so that exp(G_i - G_j) is exact
 // to fp32 however far G has run.
+//
+// What a whole training call moves: per chunk and head of K = V = 128, bf16, 0.8 MB, of which the caller's tensors are 0.13;
+// 4 x 4096 tokens of 16 heads take 0.12 (prep) + 0.26 + 0.25 (scans) + 0.38 ms (gradients), 3.3 GB at 3.3 TB/s (a copy
+// reaches 4.85).  Larger chunks would move fewer states, and pay for it in the triangles and in accuracy.
 #include "common.h"
 #include "mfma_tiles.h"
 #include "split_bf16.h"
@@ -44,8 +48,7 @@ constexpr float kGMin = -1e4f;     // log decays are clamped here: exp() of it i
 // exchanged by its number.  A fragment read (lane: row l & 15, piece p + (l >> 4)) goes in four cycles of 16 lanes, rows
 // 0-3, 12-15 of one piece with rows 4-11 of the next or the other way round, and the exchange gives these 16 different
 // places in the 256 bytes of a cycle; so it does for the 8-byte stores of 16 rows.  Measured per wave: read 4.2 cycles,
-// 8.0 from rows padded by 16 bytes, which the grads kernel was bound by; store 8 either way (16 with 32 bytes of padding,
-// which read in 4.2 as well).
+// 8.0 from rows padded by 16 bytes; store 8 either way (16 with 32 bytes of padding, which read in 4.2 as well).
 template <int P>
 __device__ __forceinline__ int place(int row, int piece) {
   static_assert(P == 4 || P == 8 || P == 16, "pieces of a row");
@@ -88,14 +91,13 @@ struct GdrArgs {
   float *dg, *dbeta;
   long lddg, lddbeta;
   int whole, wide, wide_v, v16, train, vp, nvt;
-  // ws, per chunk and key head: k, q [64][terms][Kp] (pack), their transposes [Kp][terms][64];
-  //     per chunk and value head: M, P (two terms for bf16: what o takes) and their transposes [64][terms][64], five rows of 64 floats, and for the
-  //     backward pass W, Y [vp/32][64][32] and S, dS [vp/32][Kp][32], fp32 (tiles of 32 columns).  The terms of a row lie side by side, so that a lane's
-  //     fragments are at constant offsets from one address.
+  // ws, all but vec, w, y, s, ds as operand blocks, per chunk and key head: k, q (rows: tokens) and their transposes (rows: K);
+  //     per chunk and value head: M, P (two terms for bf16: what o takes) and their transposes, five rows of 64 floats, and
+  //     for the backward pass W, Y [vp/32][64][32] and S, dS [vp/32][Kp/16][2][64 lanes][4], fp32
   __bf16 *kpk, *qpk, *kt, *qt, *m, *p, *mt, *pt;
   float *vec, *w, *y, *s, *ds;
   // segments of long sequences: segs of seg_chunks chunks each (1: the whole sequence), grid_segs of them in a launch; per
-  // value head and segment M and its transpose [Kp][Kp], N [Kp][vp], and the state (gradient) it starts from [Kp][vp]
+  // value head and segment M and its transpose (operand blocks, fp32), N [Kp][vp], and the state (gradient) it starts from [Kp][vp]
   int segs, seg_chunks, grid_segs;
   float *seg_m, *seg_mt, *seg_n, *seg_s;
 };
@@ -158,6 +160,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, lo
 // the blocks below them, 16 and 32 wide, as -M22 (L21 M11) on the fp32 matrix instruction.  P is written straight from the
 // registers of a product: four elements of a row from k q^T, of a column (for the transpose) from q k^T.  The 32 x 32
 // blocks beyond the diagonal are neither written nor read.
+// Bound by what it writes where there are many chunks (4 x 4096 tokens, 16 heads, K 128, bf16, for training: 0.54 GB in
+// 119 us), else by the latency of its steps (64 chunks in fp32: 18 us, of which the products of the last row of tiles, the
+// decays and the substitution are 4 us each).  Three workgroups per CU fill the waits of each other.
 template <int NP, int KB2>
 struct PrepLds {
   static constexpr int Kp = 64 * KB2;
@@ -645,11 +650,14 @@ __device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* base, 
   load_half<N>(f[1], base, at + (high ? N * kFrag : 0));
 }
 
-// A scan is bound by its chain: state -> K S -> W -> state, chunk after chunk, and inside it by the instructions its waves
-// issue (splitting results into terms, addressing; the matrix products are a third).  So four waves of the workgroup do
-// nothing but the chain, and four others what hangs on it: the output o, one chunk behind (forward), or what only depends
-// on dO, one chunk ahead, and the stores of Y and dV (backward).  Everything a chunk needs from memory is requested while
-// the chunk in front of it is worked on, behind the last use of its registers.
+// A scan is a chain: state -> K S -> W -> state, chunk after chunk.  Four waves of the workgroup do nothing but the chain,
+// and four others what hangs on it: v in front of it and the output o one chunk behind (forward), or what only depends on
+// dO, one chunk ahead, and the stores of Y and dV (backward).  Everything a chunk needs from memory is requested while the
+// chunk in front of it is worked on, behind the last use of its registers.
+// Measured with K = V = 128, bf16: 1.6 us per chunk alone with 16 columns, 2.5 with 32 and the chip full; splitting the
+// state and the two right-hand sides into terms, three barriers and the matrix products share it about evenly.  Training
+// adds the stores of S and W: 64 chunks of 64 heads take 256 us forward, 0.46 GB written, 252 backward.  Two workgroups
+// per CU (128 registers) were slower for all sizes (167 -> 179 us, 256 -> 366 for training): the registers do not hold it.
 // The chain: chunks c0 .. c1 - 1 of a sequence, four waves, S in their registers.  BARE: nobody hangs on it (no W is left in
 // wl, and v comes into vl by these waves).  vcols: V, or 0 for columns without a v (and v0 what it may).
 template <typename T, int NP, int KB2, int NT, bool TRAIN, bool BARE, bool WIDE>
@@ -890,7 +898,7 @@ float y[4 * NT];
 // state it is given to M S + N; one launch finds M and N of every segment but the last (the chain alone, on the columns of
 // V from a zero state and on K columns without a v from the unit state), one joins the states along the segments, and the
 // scan then runs with every segment's own first state.  The chain is walked twice, and K / V more columns of it the first
-// time, by eight times the workgroups.
+// time, by as many times the workgroups.  32768 tokens of 8 heads, 8 segments: 837 us -> 198 + 18 (joining) + 165.
 template <typename T, int NP, int KB2, bool WIDE>
 __global__ __launch_bounds__(256, 2) void gdr_segment_kernel(GdrArgs a) {
   constexpr int NT = 2;
@@ -1224,12 +1232,13 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
 // One workgroup per chunk and key head; the value heads of the key head one after the other, so that dq and dk are summed
 // in registers in a fixed order.  Eight waves: 16 tokens against half of K each.  S, dS', W, Y and dO pass through LDS 32
 // columns at a time as bf16 terms; the next 32 columns are on their way from memory meanwhile.
+// Bound by memory where the chip is full: 4 x 4096 tokens of 16 heads, K = V = 128, bf16, read 1.25 GB and write 0.17 in
+// 375 us (3.8 TB/s); one chunk takes a CU 42 thousand cycles, 11 thousand of them matrix products.
 template <int NP, int KB2>
 struct GradsLds {
   static constexpr int Kp = 64 * KB2, LDV = 32;              // columns at a time
   static constexpr int cols = 3 * LDV * (2 * Kp + 2 * kC) + NP * LDV * kC;       // elements: S, dS', W, Y, dO
-  // afterwards, over them: R, B and their transposes; where k and q do not stay in LDS (three terms), 32 tokens of those and
-  // of k and q at a time
+  // afterwards, over them: R, B and their transposes; with three terms 32 tokens of those and of k and q at a time
   static constexpr int LDR = NP == 1 ? kC : 32;
   static constexpr int tri = 4 * 3 * kC * LDR + (NP == 1 ? 0 : 2 * NP * Kp * LDR);
   static constexpr int NB = NP == 1 ? 2 : 1;                 // column images: two where they fit
@@ -1379,7 +1388,7 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
         }
       }
     };
-    // k and q in the layout of a result: four tokens of one column, from the transposes or from the caller's rows
+    // k and q in the layout of a result: four tokens of one column, from the transposes or (fp32) from the caller's rows
     bf16x4 kr[NP == 1 ? KT : 1], qr[NP == 1 ? KT : 1];
     bf16x8 kf1[2][NP == 1 ? KT : 1], qf1[2][NP == 1 ? KT : 1];   // and as operands of the products below
     unsigned kx[NP == 1 ? 1 : KT][4], qx[NP == 1 ? 1 : KT][4];
@@ -1638,6 +1647,8 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
 // A workgroup holds 16 columns (x VEC) of one row's head: 16 threads along the columns, 16 along K.  The two sums over K
 // that a token needs, S^T k and S^T q, are taken of the state as it is stored: o = scale (a S^T q + (q.k) u) with
 // u = beta (v - a S^T k), so the state is read once, moved in registers and written once, behind one exchange in LDS.
+// Bound by the state's way through memory: 192 rows of 32 heads, K = V = 128: 0.81 GB in 161 us, 5.0 TB/s.  One row of 4
+// heads takes 4.2 us, two latencies of memory.
 struct GdrStepArgs {
   int Hk, Hv, K, V, rep, n_slots, nvt;
   float scale;
@@ -1764,14 +1775,13 @@ long slots_of(int n_seq, long rows, bool packed) {
 }
 
 // Segments per sequence and their chunks.  Cutting a sequence in s pays a second walk of 1/s of the chunks with K / V more
-// columns and a join of s steps, about two chunks each: from three segments on, where the chip's 256 CUs hold them side by side
-// (32-column workgroups) and each is long enough.  Packed sequences may all be one.
-#ifndef GDR_SEGS
-#define GDR_SEGS 1
-#endif
+// columns and a join of s steps, about one chunk each, so it takes three, of 16 chunks or more, and a chip whose 256 CUs
+// hold them side by side (32-column workgroups).  Measured for 32768 tokens, K = V = 128, whole calls: 8 heads (8 segments)
+// 930 -> 475 us, 12 (5) 1005 -> 742, 16 (4) 1043 -> 877, 20 (3) 1152 -> 1112; 4096 tokens, 8 heads (4 of 16 chunks) 98 ->
+// 97; two segments would be slower than none.  Packed sequences may all be one.
 int segments_of(int n_seq, long rows, bool packed, int Hv, int vp, int* chunks) {
   const long most = packed ? rows / kC + 1 : (rows / n_seq + kC - 1) / kC, wgs = (long)n_seq * Hv * (vp / 32);
-  long segs = GDR_SEGS ? 256 / wgs : 1;
+  long segs = 256 / wgs;
   if (segs > most / 16) segs = most / 16;
   if (segs > 16) segs = 16;
   if (segs < 3) segs = 1;
@@ -1779,8 +1789,7 @@ int segments_of(int n_seq, long rows, bool packed, int Hv, int vp, int* chunks) 
   return (int)segs;
 }
 
-// ws: offsets in floats (every array a multiple of 64 floats); returns the total.  Rows that the scans read in place
-// (bf16, K = 64 or 128, 16-byte aligned) are not packed; the size leaves room for them where alignment may forbid it.
+// ws: offsets in floats (every array a multiple of 64 floats); returns the total
 long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, int Hk, int Hv, int K, int V, bool train) {
   const long ns = slots_of(n_seq, rows, packed), kp = padded_k(K), np = dtype == HHRL_BF16 ? 1 : 3, vp = (V + 31) / 32 * 32;
   long off = 0;
@@ -1861,12 +1870,10 @@ int gdr_fill(const hhrl_gdr_desc* d, GdrArgs& a, bool train, const char* who) {
   return HHRL_OK;
 }
 
-// Columns per workgroup of a scan: 32 (two result tiles per wave) where that fills the chip's 256 CUs, else 16: twice the
-// workgroups, and a shorter chain from chunk to chunk.
-#ifndef SCAN_NT
-#define SCAN_NT(wgs32) ((wgs32) > 128 ? 2 : 1)
-#endif
-int scan_tiles(const GdrArgs& a) { return a.segs > 1 ? 2 : SCAN_NT((long)a.n_seq * a.Hv * (a.vp / 32)); }
+// Columns per workgroup of a scan: 16 where twice the workgroups still have a CU each (the chain from chunk to chunk is
+// shorter), else 32.  Measured for 16 chunks, K = V = 128, with 16 / 32 columns: 128 workgroups of 32 27 / 38 us, 144 40 / 39,
+// 224 42 / 40, 256 43 / 41.  Segments fill the chip with 32.
+int scan_tiles(const GdrArgs& a) { return a.segs > 1 || (long)a.n_seq * a.Hv * (a.vp / 32) > 128 ? 2 : 1; }
 unsigned scan_grid(const GdrArgs& a) { return (unsigned)(((long)a.n_seq * a.Hv * a.grid_segs + 7) / 8 * 8 * a.nvt); }
 
 template <typename T, int NP, int KB2, int NT, bool WIDE>

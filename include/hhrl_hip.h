@@ -412,15 +412,16 @@ int hhrl_lstm_backward_group(const hhrl_lstm_desc* descs, int n, int B, int T, i
  * Sequences: `starts` null: n_seq sequences of T = rows / n_seq tokens behind each other, of which the first lens[n]
  * hold data (lens null: all).  `starts` (n_seq + 1 device ints): sequence n is rows starts[n] .. starts[n+1] - 1 of
  * `rows` packed rows; it may be empty.  Numbers outside 0 .. rows (or 0 .. T) are clamped; starts has to ascend.
- * Rows of no sequence are neither read nor written, in any operand; what they hold does not matter.
+ * Rows of no sequence are neither read nor written, in any operand; what they hold does not matter.  ld* of q, k, v, o,
+ * d_o and dv are below 2^22; a launch's 2^32 threads bound the chunks (2^23) and n_seq * Hv * V / 32 (2^23).
  * s0 [n_seq, Hv, K, V]: states before the first token (null: zero); s1: receives the states behind the last (null: not
  * wanted; may be s0).  A sequence without tokens hands its state on.
  * Forward writes o.  Unless no_backward is set it leaves in ws what the backward call reads; ws
- * (hhrl_gdr_workspace_floats, 16-byte aligned) must then stay untouched until that call, which takes the same inputs
- * and writes dq, dk, dv (dtype), dg, dbeta and, where given, d_s0 (gradients with respect to q .. s0 of
- * <d_o, o> + <d_s1, s1>; d_o and d_s1 may not both be null).
+ * (hhrl_gdr_workspace_floats, 16-byte aligned) must then stay untouched until that call, which takes the same inputs,
+ * scale and sequences, and writes dq, dk, dv (dtype), dg, dbeta and, where given, d_s0 (gradients with respect to q .. s0 of
+ * <d_o, o> + <d_s1, s1>; d_o and d_s1 may not both be null; d_s0 may be d_s1).  Other outputs overlap no operand.
  * The products run on bf16 matrix instructions with every fp32 operand as three bf16 terms: results carry fp32
- * accuracy for either dtype, o and the input gradients are rounded once.  No atomics: the same bits on every run.
+ * accuracy for either dtype (a bf16 o 2^-17 of the sums behind it), o and the input gradients are rounded once.  No atomics: the same bits on every run.
  * A non-finite number in a token may spread to the 63 tokens before it (they share a chunk) and to all behind it. */
 #define HHRL_GDR_MAX_K 128
 #define HHRL_GDR_MAX_V 512
