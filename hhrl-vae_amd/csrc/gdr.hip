@@ -28,7 +28,7 @@
 // to fp32 however far G has run.
 //
 // What a whole training call moves: per chunk and head of K = V = 128, bf16, 0.8 MB, of which the caller's tensors are 0.13;
-// 4 x 4096 tokens of 16 heads take 0.12 (prep) + 0.26 + 0.25 (scans) + 0.38 ms (gradients), 3.3 GB at 3.3 TB/s (a copy
+// 4 x 4096 tokens of 16 heads take 0.12 (prep) + 0.26 + 0.25 (scans) + 0.38 ms (gradients), 3.6 GB at 3.6 TB/s (a copy
 // reaches 4.85).  Larger chunks would move fewer states, and pay for it in the triangles and in accuracy.
 #include "common.h"
 #include "mfma_tiles.h"
@@ -1232,8 +1232,8 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
 // One workgroup per chunk and key head; the value heads of the key head one after the other, so that dq and dk are summed
 // in registers in a fixed order.  Eight waves: 16 tokens against half of K each.  S, dS', W, Y and dO pass through LDS 32
 // columns at a time as bf16 terms; the next 32 columns are on their way from memory meanwhile.
-// Bound by memory where the chip is full: 4 x 4096 tokens of 16 heads, K = V = 128, bf16, read 1.25 GB and write 0.17 in
-// 375 us (3.8 TB/s); one chunk takes a CU 42 thousand cycles, 11 thousand of them matrix products.
+// Bound by memory where the chip is full: 4 x 4096 tokens of 16 heads, K = V = 128, bf16, read 1.06 GB and write 0.15 in
+// 375 us (3.2 TB/s); one chunk takes a CU 42 thousand cycles, 11 thousand of them matrix products.
 template <int NP, int KB2>
 struct GradsLds {
   static constexpr int Kp = 64 * KB2, LDV = 32;              // columns at a time
