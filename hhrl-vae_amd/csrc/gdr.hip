@@ -650,6 +650,10 @@ __device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* base, 
   load_half<N>(f[1], base, at + (high ? N * kFrag : 0));
 }
 
+// Requests are counted in their order, so those in front of a loop are made in the order of the loop's: in another one the
+// compiler's first wait of every pass would be for what has just been requested.
+#define GDR_IN_ORDER __builtin_amdgcn_sched_barrier(0)
+
 // A scan is a chain: state -> K S -> W -> state, chunk after chunk.  Four waves of the workgroup do nothing but the chain,
 // and four others what hangs on it: v in front of it and the output o one chunk behind (forward), or what only depends on
 // dO, one chunk ahead, and the stores of Y and dV (backward).  Everything a chunk needs from memory is requested while the
@@ -678,10 +682,15 @@ __device__ __forceinline__ void scan_chain(const GdrArgs& a, f32x4 (&S)[KB2][NT]
   const __bf16* ktp = a.kt + ((slot0 + c0) * a.Hk + hk) * Kp * NP * kC;
   const unsigned kat = w * KB * NP * kFrag + lane * 8, mat = w * 2 * 3 * kFrag + lane * 8, ktat = KB2 * w * 2 * NP * kFrag + lane * 8;
   if constexpr (BARE) vp.load(c0);
+  GDR_IN_ORDER;
   load_rows<NP, KB>(kf, kp, kat);
+  GDR_IN_ORDER;
   vn.load(vecp, ib);
+  GDR_IN_ORDER;
   load_tri<3>(mf, mp, mat, true, high);
+  GDR_IN_ORDER;
   load_kt<NP, KB2>(ktf, ktp, ktat);
+  GDR_IN_ORDER;
   if constexpr (BARE) {
     vp.put(vl, w, lane);
     vp.load(min(c0 + 1, c1 - 1));
@@ -815,7 +824,6 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
     RowTile<T, NT, WIDE> vp(a.v, a.ldv, start, len, hv, a.V, v0, w, lane);
     const int ta = 16 * w + (lane >> 2), cb = 4 * NT * (lane & 3);
     float* const ow = ot + 16 * w * VT;
-    const float* gp = a.vec + ((slot0 + c0) * a.Hv + hv) * kVecs * kC + kGam * kC;
     auto pw = [&](int c, int kb) {                         // qs += P W, columns 32*kb of P; W as the chain left it in wl
       const float* const wc = wl + (c & 1) * L::F;
 #pragma unroll
@@ -856,12 +864,20 @@ float y[4 * NT];
       }
       op.store(c, y);
     };
-    vp.load(c0);
+    const float* gp = a.vec + ((slot0 + c0) * a.Hv + hv) * kVecs * kC + kGam * kC;
+    RowTile<T, NT, WIDE> first = vp;
+    first.load(c0);
+    GDR_IN_ORDER;
     load_rows<NP, KB>(qf, qp, qat);
-    load_tri<NO>(pf, pp, pat, true, high);
-    float gam = gp[(unsigned)ia];
-    vp.put(vl + (c0 & 1) * VT * kC, w, lane);
+    GDR_IN_ORDER;
     vp.load(min(c0 + 1, c1 - 1));
+    GDR_IN_ORDER;
+    load_half<NO>(pf[1], pp, pat + (high ? NO * kFrag : 0));
+    float gam = gp[(unsigned)ia];
+    GDR_IN_ORDER;
+    load_half<NO>(pf[0], pp, pat);
+    GDR_IN_ORDER;
+    first.put(vl + (c0 & 1) * VT * kC, w, lane);
     for (int c = c0; c < c1; ++c) {
       lds_barrier();
 #pragma unroll
@@ -1068,9 +1084,13 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
         load_kt<NP, KB2>(ktf, ktp, ktat);
       };
       load_rows<NP, KB>(kf, kp, kat);
+      GDR_IN_ORDER;
       vn.load(vecp, ib);
+      GDR_IN_ORDER;
       load_tri<3>(mf, mp, mat, low, true);
+      GDR_IN_ORDER;
       load_t();
+      GDR_IN_ORDER;
       lds_barrier();
       lds_barrier();
       for (int c = c1 - 1; c >= c0; --c) {
