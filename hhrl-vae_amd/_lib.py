@@ -94,6 +94,13 @@ class GdrDesc(C.Structure):
                 ("dg", _P), ("dbeta", _P), ("lddg", _L), ("lddbeta", _L), ("ws", _P), ("ws_floats", _L)]
 
 
+class GdrStepDesc(C.Structure):
+    """hhrl_gdr_step_desc of include/hhrl_hip.h."""
+    _fields_ = [("dtype", _I), ("B", _I), ("Hk", _I), ("Hv", _I), ("K", _I), ("V", _I), ("scale", _F), ("n_slots", _I),
+                ("q", _P), ("k", _P), ("v", _P), ("ldq", _L), ("ldk", _L), ("ldv", _L), ("g", _P), ("beta", _P), ("ldg", _L), ("ldbeta", _L),
+                ("o", _P), ("ldo", _L), ("state_in", _P), ("state_out", _P), ("slots", _P)]
+
+
 class BlockNormDesc(C.Structure):
     """hhrl_block_norm_desc of include/hhrl_hip.h."""
     _fields_ = [("dtype", _I), ("M", _L), ("H", _I), ("D", _I), ("post", _I), ("pre", _I), ("gate_act", _I), ("gate_rows", _L),
@@ -151,7 +158,7 @@ SIGNATURES = {
     "hhrl_gdr_workspace_floats": (_L, [_I, _I, _L, _I, _I, _I, _I, _I, _I]),
     "hhrl_gdr_forward": (_I, [_P, _P]),
     "hhrl_gdr_backward": (_I, [_P, _P]),
-    "hhrl_gdr_step": (_I, [_I, _I, _I, _I, _I, _I, _F, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _I, _P, _P]),
+    "hhrl_gdr_step": (_I, [_P, _P]),
     "hhrl_block_norm_workspace_floats": (_L, [_L, _I, _I, _L]),
     "hhrl_block_norm_forward": (_I, [_P, _P]),
     "hhrl_block_norm_backward": (_I, [_P, _P]),

@@ -2030,27 +2030,26 @@ int hhrl_gdr_backward(const hhrl_gdr_desc* d, void* stream) {
   return d->K <= 64 ? run_bwd<float, 3, 1>(a, st, flops) : run_bwd<float, 3, 2>(a, st, flops);
 }
 
-int hhrl_gdr_step(int dtype, int B, int Hk, int Hv, int K, int V, float scale, const void* q, long ldq, const void* k, long ldk,
-                  const void* v, long ldv, const float* g, long ldg, const float* beta, long ldbeta, void* o, long ldo,
-                  const float* state_in, float* state_out, int n_slots, const int* slots, void* stream) {
-  HHRL_REQUIRE(dtype == HHRL_F32 || dtype == HHRL_BF16, "gdr_step: dtype %d", dtype);
-  HHRL_REQUIRE(B > 0 && n_slots > 0 && Hk > 0 && Hv > 0 && Hv % Hk == 0, "gdr_step: B=%d n_slots=%d Hk=%d Hv=%d", B, n_slots, Hk, Hv);
-  HHRL_REQUIRE(slots || B <= n_slots, "gdr_step: %d rows for %d states", B, n_slots);
-  HHRL_REQUIRE(K > 0 && K <= HHRL_GDR_MAX_K && V > 0 && V <= HHRL_GDR_MAX_V, "gdr_step: K=%d V=%d (up to %d, %d supported)", K, V, HHRL_GDR_MAX_K, HHRL_GDR_MAX_V);
-  HHRL_REQUIRE(q && k && v && g && beta && o && state_in && state_out, "gdr_step: null pointer");
-  HHRL_REQUIRE(ldq >= (long)Hk * K && ldk >= (long)Hk * K && ldv >= (long)Hv * V && ldo >= (long)Hv * V && ldg >= Hv && ldbeta >= Hv,
+int hhrl_gdr_step(const hhrl_gdr_step_desc* d, void* stream) {
+  HHRL_REQUIRE(d != nullptr, "gdr_step: null descriptor");
+  HHRL_REQUIRE(d->dtype == HHRL_F32 || d->dtype == HHRL_BF16, "gdr_step: dtype %d", d->dtype);
+  HHRL_REQUIRE(d->B > 0 && d->n_slots > 0 && d->Hk > 0 && d->Hv > 0 && d->Hv % d->Hk == 0, "gdr_step: B=%d n_slots=%d Hk=%d Hv=%d", d->B, d->n_slots, d->Hk, d->Hv);
+  HHRL_REQUIRE(d->slots || d->B <= d->n_slots, "gdr_step: %d rows for %d states", d->B, d->n_slots);
+  HHRL_REQUIRE(d->K > 0 && d->K <= HHRL_GDR_MAX_K && d->V > 0 && d->V <= HHRL_GDR_MAX_V, "gdr_step: K=%d V=%d (up to %d, %d supported)", d->K, d->V, HHRL_GDR_MAX_K, HHRL_GDR_MAX_V);
+  HHRL_REQUIRE(d->q && d->k && d->v && d->g && d->beta && d->o && d->state_in && d->state_out, "gdr_step: null pointer");
+  HHRL_REQUIRE(d->ldq >= (long)d->Hk * d->K && d->ldk >= (long)d->Hk * d->K && d->ldv >= (long)d->Hv * d->V && d->ldo >= (long)d->Hv * d->V && d->ldg >= d->Hv && d->ldbeta >= d->Hv,
                "gdr_step: leading dimension too small");
-  const bool vec = V % 4 == 0 && a16(state_in) && a16(state_out);
+  const bool vec = d->V % 4 == 0 && a16(d->state_in) && a16(d->state_out);
   GdrStepArgs a = {};
-  a.Hk = Hk; a.Hv = Hv; a.K = K; a.V = V; a.rep = Hv / Hk; a.n_slots = n_slots; a.scale = scale;
-  a.q = q; a.k = k; a.v = v; a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.g = g; a.beta = beta; a.ldg = ldg; a.ldbeta = ldbeta;
-  a.o = o; a.ldo = ldo; a.sin = state_in; a.sout = state_out; a.slots = slots;
-  a.nvt = ceil_div(V, vec ? 64 : 16);
-  const long grid = (long)B * Hv * a.nvt;
+  a.Hk = d->Hk; a.Hv = d->Hv; a.K = d->K; a.V = d->V; a.rep = d->Hv / d->Hk; a.n_slots = d->n_slots; a.scale = d->scale;
+  a.q = d->q; a.k = d->k; a.v = d->v; a.ldq = d->ldq; a.ldk = d->ldk; a.ldv = d->ldv; a.g = d->g; a.beta = d->beta; a.ldg = d->ldg; a.ldbeta = d->ldbeta;
+  a.o = d->o; a.ldo = d->ldo; a.sin = d->state_in; a.sout = d->state_out; a.slots = d->slots;
+  a.nvt = ceil_div(d->V, vec ? 64 : 16);
+  const long grid = (long)d->B * d->Hv * a.nvt;
   HHRL_REQUIRE(grid < (1L << 24), "gdr_step: B*Hv*V too large: %ld workgroups of 256 threads", grid);
   hipStream_t st = as_stream(stream);
-  ProfScope ps("gdr_step_kernel", st, 6.0 * B * Hv * K * V, 8.0 * B * Hv * K * V);
-  if (dtype == HHRL_BF16) {
+  ProfScope ps("gdr_step_kernel", st, 6.0 * d->B * d->Hv * d->K * d->V, 8.0 * d->B * d->Hv * d->K * d->V);
+  if (d->dtype == HHRL_BF16) {
     if (vec) launch_step<__bf16, 4>(a, (unsigned)grid, st);
     else launch_step<__bf16, 1>(a, (unsigned)grid, st);
   } else {

@@ -11,6 +11,7 @@ any torch operation."""
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
 
 import torch
@@ -20,6 +21,9 @@ from ._lib import ACT_NONE, ACT_SIGMOID, ACT_SILU, check
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}            # HHRL_F32, HHRL_BF16
 _NORMS = {"none": 0, "rms": 1, "layer": 2}                 # HHRL_NORM_*
+# hhrl_gdr_step_desc: acting is bound by the host, and packing a struct takes a third of what setting its fields takes
+_STEP = struct.Struct("@6ifi15q")
+assert _STEP.size == C.sizeof(_lib.GdrStepDesc)
 _GATES = {"none": ACT_NONE, "sigmoid": ACT_SIGMOID, "silu": ACT_SILU}
 
 
@@ -44,7 +48,11 @@ def _fail(name: str, t, shape, dtype, dev: int) -> None:
 
 def _tensor(name: str, t, shape, dtype, dev: int) -> int:
     """Checks a contiguous tensor of a given shape; its address."""
-    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype or t.get_device() != dev:
+    try:
+        bad = t.shape != shape or t.dtype is not dtype or t.get_device() != dev
+    except AttributeError:
+        bad = True
+    if bad:
         _fail(name, t, shape, dtype, dev)
     _need(t.is_contiguous(), "%s is not contiguous" % name)
     return t.data_ptr()
@@ -53,7 +61,11 @@ def _tensor(name: str, t, shape, dtype, dev: int) -> int:
 def _rows(name: str, t, shape, n: int, width: int, dtype, dev: int):
     """Checks a tensor whose first n dimensions are rows of `width` contiguous elements, at one distance from each other
     (a column range of a wider buffer qualifies): its address and that distance in elements."""
-    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype or t.get_device() != dev:
+    try:
+        bad = t.shape != shape or t.dtype is not dtype or t.get_device() != dev
+    except AttributeError:
+        bad = True
+    if bad:
         _fail(name, t, shape, dtype, dev)
     if t.is_contiguous():
         return t.data_ptr(), width
@@ -187,14 +199,19 @@ class GatedDelta:
         key, val, head = ((B, Hk, K), 1, Hk * K, dt, dev), ((B, Hv, V), 1, Hv * V, dt, dev), ((B, Hv), 1, Hv, torch.float32, dev)
         sp = self._state("state", state, n, dev)
         so = sp if state_out is None else self._state("state_out", state_out, n, dev)
-        sl = None
+        sl = 0
         if slots is not None:
             sl = _tensor("slots", slots, (B,), torch.int32, dev)
         else:
             _need(B <= n, "%d rows for %d states" % (B, n))
-        check(self._lib.hhrl_gdr_step(self.code, B, Hk, Hv, K, V, self.scale, *_rows("q", q, *key), *_rows("k", k, *key),
-                                      *_rows("v", v, *val), *_rows("g", g, *head), *_rows("beta", beta, *head), *_rows("o", o, *val),
-                                      sp, so, n, sl, _stream(dev)))
+        qp, ldq = _rows("q", q, *key)
+        kp, ldk = _rows("k", k, *key)
+        vp, ldv = _rows("v", v, *val)
+        gp, ldg = _rows("g", g, *head)
+        bp, ldb = _rows("beta", beta, *head)
+        op, ldo = _rows("o", o, *val)
+        check(self._lib.hhrl_gdr_step(_STEP.pack(self.code, B, Hk, Hv, K, V, self.scale, n, qp, kp, vp, ldq, ldk, ldv, gp, bp, ldg, ldb,
+                                                 op, ldo, sp, so, sl), _stream(dev)))
 
 
 class BlockNorm:

@@ -450,9 +450,17 @@ int hhrl_gdr_backward(const hhrl_gdr_desc* d, void* stream);
  * states (may be state_in; slots that no row names are left alone).  A row whose slot is negative is idle: its output
  * is zero and no state moves.  A slot >= n_slots, or one that an earlier row of the call names already, is an error
  * that only the device sees: that row's output is NaN and no state moves for it.  No workspace. */
-int hhrl_gdr_step(int dtype, int B, int Hk, int Hv, int K, int V, float scale, const void* q, long ldq, const void* k, long ldk,
-                  const void* v, long ldv, const float* g, long ldg, const float* beta, long ldbeta, void* o, long ldo,
-                  const float* state_in, float* state_out, int n_slots, const int* slots, void* stream);
+typedef struct {
+  int dtype;
+  int B, Hk, Hv, K, V;
+  float scale;
+  int n_slots;
+  const void *q, *k, *v; long ldq, ldk, ldv;
+  const float *g, *beta; long ldg, ldbeta;
+  void* o; long ldo;
+  const float* state_in; float* state_out; const int* slots;
+} hhrl_gdr_step_desc;
+int hhrl_gdr_step(const hhrl_gdr_step_desc* d, void* stream);
 
 /* Norms before and after a block with its gate and residual scale, one pass over the rows:
  *   r = alpha*x + scale * a(gate) * post(y);    h = pre(r)

@@ -57,7 +57,7 @@ def test_gdr_refuses_more_than_a_launch_holds(lib, over):
 
 
 def test_gdr_step_refuses_more_than_a_launch_holds(lib):
-    assert lib.hhrl_gdr_step(1, 8192, 1, 256, 32, 512, 1.0, FAKE, 32, FAKE, 32, FAKE, 1 << 17, FAKE, 256, FAKE, 256, FAKE, 1 << 17, FAKE, FAKE, 8192, None, None) == 1
+    assert lib.hhrl_gdr_step(step_desc(B=8192, Hk=1, Hv=256, K=32, V=512, ldv=1 << 17, ldg=256, ldbeta=256, ldo=1 << 17, n_slots=8192, slots=None), None) == 1
     assert b"too large" in lib.hhrl_last_error(), lib.hhrl_last_error()
 
 
@@ -76,15 +76,25 @@ def test_null_descriptors(lib):
         assert fn(None, None) == 1 and b"descriptor" in lib.hhrl_last_error()
 
 
-@pytest.mark.parametrize("i,v", [(0, 5), (1, 0), (2, 0), (3, 5), (4, 129), (5, 513), (7, None), (9, None), (8, 127), (12, 255), (18, 255), (19, None), (20, None), (21, 0)])
-def test_gdr_step_refuses(lib, i, v):
-    args = [1, 3, 2, 4, 64, 64, 0.1, FAKE, 128, FAKE, 128, FAKE, 256, FAKE, 4, FAKE, 4, FAKE, 256, FAKE, FAKE, 8, FAKE, None]
-    args[i] = v
-    assert lib.hhrl_gdr_step(*args) == 1
+def step_desc(**over):
+    from hhrl_vae_amd import _lib
+    d = _lib.GdrStepDesc()
+    f = dict(dtype=1, B=3, Hk=2, Hv=4, K=64, V=64, scale=0.1, n_slots=8, q=FAKE, k=FAKE, v=FAKE, ldq=128, ldk=128, ldv=256, g=FAKE, beta=FAKE, ldg=4,
+             ldbeta=4, o=FAKE, ldo=256, state_in=FAKE, state_out=FAKE, slots=FAKE)
+    f.update(over)
+    for k, v in f.items():
+        setattr(d, k, v)
+    return C.byref(d)
+
+
+@pytest.mark.parametrize("over", [dict(dtype=5), dict(B=0), dict(Hk=0), dict(Hv=5), dict(K=129), dict(V=513), dict(q=None), dict(k=None), dict(ldq=127), dict(ldv=255),
+                                  dict(ldo=255), dict(state_in=None), dict(state_out=None), dict(n_slots=0)])
+def test_gdr_step_refuses(lib, over):
+    assert lib.hhrl_gdr_step(step_desc(**over), None) == 1
 
 
 def test_gdr_step_refuses_more_rows_than_states(lib):
-    assert lib.hhrl_gdr_step(1, 9, 2, 4, 64, 64, 0.1, FAKE, 128, FAKE, 128, FAKE, 256, FAKE, 4, FAKE, 4, FAKE, 256, FAKE, FAKE, 8, None, None) == 1
+    assert lib.hhrl_gdr_step(step_desc(B=9, slots=None), None) == 1 and lib.hhrl_gdr_step(None, None) == 1
 
 
 def norm_desc(**over):
