@@ -28,7 +28,7 @@
 // to fp32 however far G has run.
 //
 // What a whole training call moves: per chunk and head of K = V = 128, bf16, 0.8 MB, of which the caller's tensors are 0.13;
-// 4 x 4096 tokens of 16 heads take 0.12 (prep) + 0.26 + 0.25 (scans) + 0.38 ms (gradients), 3.6 GB at 3.6 TB/s (a copy
+// 4 x 4096 tokens of 16 heads take 0.12 (prep) + 0.25 + 0.24 (scans) + 0.37 ms (gradients), 3.6 GB at 3.7 TB/s (a copy
 // reaches 4.85).  Larger chunks would move fewer states, and pay for it in the triangles and in accuracy.
 #include "common.h"
 #include "mfma_tiles.h"
@@ -658,9 +658,9 @@ __device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* base, 
 // and four others what hangs on it: v in front of it and the output o one chunk behind (forward), or what only depends on
 // dO, one chunk ahead, and the stores of Y and dV (backward).  Everything a chunk needs from memory is requested while the
 // chunk in front of it is worked on, behind the last use of its registers.
-// Measured with K = V = 128, bf16: 1.6 us per chunk alone with 16 columns, 2.5 with 32 and the chip full; splitting the
+// Measured with K = V = 128, bf16: 1.6 us per chunk alone with 16 columns, 2.4 with 32 and the chip full; splitting the
 // state and the two right-hand sides into terms, three barriers and the matrix products share it about evenly.  Training
-// adds the stores of S and W: 64 chunks of 64 heads take 256 us forward, 0.46 GB written, 252 backward.  Two workgroups
+// adds the stores of S and W: 64 chunks of 64 heads take 249 us forward, 0.46 GB written, 240 backward.  Two workgroups
 // per CU (128 registers) were slower for all sizes (167 -> 179 us, 256 -> 366 for training): the registers do not hold it.
 // The chain: chunks c0 .. c1 - 1 of a sequence, four waves, S in their registers.  BARE: nobody hangs on it (no W is left in
 // wl, and v comes into vl by these waves).  vcols: V, or 0 for columns without a v (and v0 what it may).
@@ -914,7 +914,7 @@ float y[4 * NT];
 // state it is given to M S + N; one launch finds M and N of every segment but the last (the chain alone, on the columns of
 // V from a zero state and on K columns without a v from the unit state), one joins the states along the segments, and the
 // scan then runs with every segment's own first state.  The chain is walked twice, and K / V more columns of it the first
-// time, by as many times the workgroups.  32768 tokens of 8 heads, 8 segments: 837 us -> 198 + 18 (joining) + 165.
+// time, by as many times the workgroups.  32768 tokens of 8 heads, 8 segments: 837 us -> 180 + 18 (joining) + 151.
 template <typename T, int NP, int KB2, bool WIDE>
 __global__ __launch_bounds__(256, 2) void gdr_segment_kernel(GdrArgs a) {
   constexpr int NT = 2;
