@@ -552,6 +552,53 @@ def test_block_norm_captured_and_replayed(seq):
 
 
 # --------------------------------------------------------------------------------------------------------- refusals
+def test_offsets_beyond_32_bits(seq):
+    """Rows 8 MB apart (the last ones begin 9 GB behind the first), as columns of one buffer: the bits of contiguous rows."""
+    T, ld = 1100, (1 << 22) - 64
+    big = torch.empty(T * ld, dtype=BF, device=DEV)
+    at = iter(range(0, ld, 64))
+    far = lambda: big.as_strided((1, T, 1, 64), (T * ld, ld, 64, 1), next(at))
+    near = [t.to(DEV) for t in make((1, T), 1, 1, 64, 64, BF, 3, 0.05)]
+    layer = seq.GatedDelta(1, 1, 64, 64, dtype=BF)
+    ws = layer.workspace(1, T, DEV, packed=False)
+    g, beta, got = near[3], near[4], []
+    for new in (lambda t: torch.empty_like(t), lambda t: far()):
+        q, k, v, d_o = (new(t) for t in (near[0], near[1], near[2], near[5]))
+        for a, b in zip((q, k, v, d_o), (near[0], near[1], near[2], near[5])):
+            a.copy_(b)
+        o, dq, dk, dv = (new(t) for t in (v, q, k, v))
+        dg, db = torch.empty_like(g), torch.empty_like(beta)
+        layer.fwd(q, k, v, g, beta, o, ws)
+        layer.bwd(q, k, v, g, beta, d_o, dq, dk, dv, dg, db, ws)
+        n = seq.BlockNorm(64, post="rms", pre="layer", dtype=BF)
+        r, h, dx, dy = (new(v) for _ in range(4))
+        flat = lambda t: t.view(T, 64) if t.is_contiguous() else t.as_strided((T, 64), (ld, 1), t.storage_offset())
+        n.fwd(x=flat(v), y=flat(o), out=flat(r), h=flat(h))
+        n.bwd(x=flat(v), y=flat(o), d_out=flat(d_o), d_h=flat(dv), dx=flat(dx), dy=flat(dy))
+        got.append([t.clone() for t in (o, dq, dk, dv, dg, db, r, h, dx, dy)])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_step_in_a_pool_beyond_32_bits(seq):
+    """2^31 state elements and more: the last states of the pool move as the first."""
+    n = (1 << 31) // (2 * 128 * 128) + 3
+    pool = torch.empty(n, 2, 128, 128, device=DEV)
+    layer = seq.GatedDelta(1, 2, 128, 128, dtype=BF)
+    q, k, v, g, beta, _ = (t[0].to(DEV) for t in make((1, 2), 1, 2, 128, 128, BF, 8))
+    s0 = torch.randn(2, 2, 128, 128, generator=torch.Generator().manual_seed(0)).to(DEV)
+    want, small = torch.empty_like(v), s0.clone()
+    layer.step(q, k, v, g, beta, want, small)
+    slots = [n - 1, n - 2]
+    for i, p in enumerate(slots):
+        pool[p] = s0[i]
+    o = torch.empty_like(v)
+    layer.step(q, k, v, g, beta, o, pool, slots=torch.tensor(slots, dtype=torch.int32, device=DEV))
+    assert torch.equal(o, want)
+    for i, p in enumerate(slots):
+        assert torch.equal(pool[p], small[i])
+
+
 def test_refusals_on_the_gpu(seq):
     """Wrong types, shapes, strides and places raise ValueError, too small a workspace HipError, before anything is launched."""
     from hhrl_vae_amd._lib import HipError
