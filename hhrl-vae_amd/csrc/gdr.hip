@@ -90,7 +90,7 @@ struct GdrArgs {
   long lddq, lddk, lddv;
   float *dg, *dbeta;
   long lddg, lddbeta;
-  int whole, wide, wide_v, v16, train, vp, nvt;
+  int whole, wide, wide_v, v16, train, vp, nvt, by_length;
   // ws, all but vec, w, y, s, ds as operand blocks, per chunk and key head: k, q (rows: tokens) and their transposes (rows: K);
   //     per chunk and value head: M, P (two terms for bf16: what o takes) and their transposes, five rows of 64 floats, and
   //     for the backward pass W, Y [vp/32][64][32] and S, dS [vp/32][Kp/16][2][64 lanes][4], fp32
@@ -431,8 +431,27 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
 }
 
 // --------------------------------------------------------------------------------------------------------- scans
-// Workgroup -> (sequence, value head, segment, column tile).  Workgroups go to the eight XCDs in turn: the column tiles of one
-// head read the same k, q, M and P, so they are dealt to one XCD (one L2), eight workgroups apart.
+// the r-th longest of up to 64 sequences (a lane each; equal ones in their order)
+__device__ __forceinline__ int longest(const GdrArgs& a, int r) {
+  const int lane = threadIdx.x & 63, n = min(lane, a.n_seq - 1);
+  int len;
+  if (a.starts) {
+    const long start = clampl(a.starts[n], 0, a.rows);
+    len = (int)(clampl(a.starts[n + 1], start, a.rows) - start);
+  } else {
+    len = (int)clampl(a.lens[n], 0, a.T);
+  }
+  int rank = 0;
+  for (int j = 0; j < a.n_seq; ++j) {
+    const int other = __builtin_amdgcn_readlane(len, j);
+    rank += other > len || (other == len && j < lane);
+  }
+  return __ffsll((unsigned long long)__ballot(lane < a.n_seq && rank == r)) - 1;
+}
+// Workgroup -> (sequence, value head, segment, column tile).  Sequences of different lengths go from the longest (by_length),
+// so that the last workgroups are short ones: 13 sequences of 12345 tokens, 16 heads 160 -> 132 us.  Workgroups go to the
+// eight XCDs in turn: the column tiles of one head read the same k, q, M and P, so they are dealt to one XCD (one L2),
+// eight workgroups apart.
 __device__ __forceinline__ bool scan_tile(const GdrArgs& a, int vt, int& n, int& hv, int& v0, int& seg) {
   const int xcd = blockIdx.x & 7, u = blockIdx.x >> 3;
   v0 = (u % a.nvt) * vt;
@@ -442,6 +461,7 @@ __device__ __forceinline__ bool scan_tile(const GdrArgs& a, int vt, int& n, int&
   seg = __builtin_amdgcn_readfirstlane((int)(unit - pair * a.grid_segs));
   n = __builtin_amdgcn_readfirstlane((int)(pair / a.Hv));
   hv = __builtin_amdgcn_readfirstlane((int)(pair - (long)n * a.Hv));
+  if (a.by_length) n = longest(a, n);
   return true;
 }
 
@@ -1899,6 +1919,7 @@ unsigned scan_grid(const GdrArgs& a) { return (unsigned)(((long)a.n_seq * a.Hv *
 template <typename T, int NP, int KB2, int NT, bool WIDE>
 int run_scan(GdrArgs a, bool bwd, hipStream_t st, double flops, bool bare = false) {
   a.nvt = a.vp / (16 * NT);
+  a.by_length = (a.starts || a.lens) && a.n_seq > 1 && a.n_seq <= 64 && a.segs == 1 && (long)a.n_seq * a.Hv * a.nvt > 256;    // (else all run at once)
   if (bwd) {
     a.grid_segs = bare ? a.segs - 1 : a.segs;
     constexpr int lds = ScanLds<NP, KB2, NT>::bwd_bytes;

@@ -143,6 +143,17 @@ def test_gdr_long_sequences_with_few_heads(seq, dtype, K, V, Hv, lens):
     check_gdr(seq, dtype, 1, Hv, K, V, ranges, lead, starts=starts, seed=K + V, gscale=0.05)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("lens", [[70, 0, 1, 64, 65, 130, 3, 3, 200], [1] * 64, [3] * 65 + [70]])
+def test_gdr_more_sequences_than_run_at_once(seq, dtype, lens):
+    """Enough workgroups for the order of the sequences to matter (the longest go first, up to 64 of them)."""
+    Hv = 576 // (2 * len(lens)) + 1 if len(lens) > 9 else 32
+    ranges, lead, starts = packed(lens)
+    check_gdr(seq, dtype, 1, Hv, 8, 33, ranges, lead, starts=starts, seed=len(lens))
+    T = max(lens)
+    check_gdr(seq, dtype, 1, Hv, 8, 33, [(i * T, i * T + n) for i, n in enumerate(lens)], (len(lens), T), lens=lens, seed=1 + len(lens))
+
+
 @pytest.mark.parametrize("T", [100, 3333])
 def test_gdr_states_in_place(seq, T):
     """s1 over s0 and d_s0 over d_s1, of one walk and of segments that run side by side: the same bits as apart."""
