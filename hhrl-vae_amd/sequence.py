@@ -27,23 +27,23 @@ assert _STEP.size == C.sizeof(_lib.GdrStepDesc)
 _GATES = {"none": ACT_NONE, "sigmoid": ACT_SIGMOID, "silu": ACT_SILU}
 
 
-def _need(ok: bool, msg: str) -> None:
+def _need(ok: bool, msg: str, *args) -> None:
     if not ok:
-        raise ValueError(msg)
+        raise ValueError(msg % args)
 
 
 def _dtype_code(dtype) -> int:
-    _need(dtype in _DTYPES, "dtype %s: float32 and bfloat16 are supported" % (dtype,))
+    _need(dtype in _DTYPES, "dtype %s: float32 and bfloat16 are supported", dtype)
     return _DTYPES[dtype]
 
 
 def _fail(name: str, t, shape, dtype, dev: int) -> None:
     """Says what is wrong with an operand that failed a check."""
-    _need(isinstance(t, torch.Tensor), "%s is not a tensor" % name)
-    _need(tuple(t.shape) == tuple(shape), "%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
-    _need(t.dtype == dtype, "%s is %s, not %s" % (name, t.dtype, dtype))
-    _need(t.is_cuda, "%s is on %s, not on a GPU" % (name, t.device))
-    _need(t.get_device() == dev, "%s is on %s, the current device is cuda:%d" % (name, t.device, dev))
+    _need(isinstance(t, torch.Tensor), "%s is not a tensor", name)
+    _need(tuple(t.shape) == tuple(shape), "%s has shape %s, not %s", name, tuple(t.shape), tuple(shape))
+    _need(t.dtype == dtype, "%s is %s, not %s", name, t.dtype, dtype)
+    _need(t.is_cuda, "%s is on %s, not on a GPU", name, t.device)
+    _need(t.get_device() == dev, "%s is on %s, the current device is cuda:%d", name, t.device, dev)
 
 
 def _tensor(name: str, t, shape, dtype, dev: int) -> int:
@@ -54,7 +54,7 @@ def _tensor(name: str, t, shape, dtype, dev: int) -> int:
         bad = True
     if bad:
         _fail(name, t, shape, dtype, dev)
-    _need(t.is_contiguous(), "%s is not contiguous" % name)
+    _need(t.is_contiguous(), "%s is not contiguous", name)
     return t.data_ptr()
 
 
@@ -71,17 +71,17 @@ def _rows(name: str, t, shape, n: int, width: int, dtype, dev: int):
         return t.data_ptr(), width
     strides, inner = t.stride(), 1
     for size, stride in zip(reversed(shape[n:]), reversed(strides[n:])):
-        _need(size == 1 or stride == inner, "%s: the elements of a row are not contiguous (strides %s)" % (name, strides))
+        _need(size == 1 or stride == inner, "%s: the elements of a row are not contiguous (strides %s)", name, strides)
         inner *= size
     ld, inner = None, 1                           # inner: rows below the dimension at hand
     for size, stride in zip(reversed(shape[:n]), reversed(strides[:n])):
         if size > 1:
             if ld is None and stride % inner == 0:
                 ld = stride // inner
-            _need(ld is not None and stride == ld * inner, "%s: its rows are not at one distance (strides %s)" % (name, strides))
+            _need(ld is not None and stride == ld * inner, "%s: its rows are not at one distance (strides %s)", name, strides)
         inner *= size
     ld = width if ld is None else ld
-    _need(ld >= width, "%s: rows overlap (strides %s)" % (name, strides))
+    _need(ld >= width, "%s: rows overlap (strides %s)", name, strides)
     return t.data_ptr(), ld
 
 
@@ -110,8 +110,8 @@ class GatedDelta:
 
     def __init__(self, Hk: int, Hv: int, K: int, V: int, dtype=torch.float32, scale: Optional[float] = None):
         self.code = _dtype_code(dtype)
-        _need(Hk > 0 and Hv > 0 and Hv % Hk == 0, "Hv=%d is not a multiple of Hk=%d" % (Hv, Hk))
-        _need(0 < K <= _lib.GDR_MAX_K and 0 < V <= _lib.GDR_MAX_V, "K=%d V=%d: up to %d, %d supported" % (K, V, _lib.GDR_MAX_K, _lib.GDR_MAX_V))
+        _need(Hk > 0 and Hv > 0 and Hv % Hk == 0, "Hv=%d is not a multiple of Hk=%d", Hv, Hk)
+        _need(0 < K <= _lib.GDR_MAX_K and 0 < V <= _lib.GDR_MAX_V, "K=%d V=%d: up to %d, %d supported", K, V, _lib.GDR_MAX_K, _lib.GDR_MAX_V)
         self.Hk, self.Hv, self.K, self.V, self.dtype = Hk, Hv, K, V, dtype
         self.scale = float(K) ** -0.5 if scale is None else float(scale)
         d = _lib.GdrDesc()                        # what every call of this layer has in common
@@ -123,7 +123,7 @@ class GatedDelta:
         """Workspace for n_seq sequences of `rows` tokens in all (of one padded length if not packed); what serves packed
         sequences serves as many padded ones too."""
         n = self._lib.hhrl_gdr_workspace_floats(self.code, n_seq, rows, int(packed), self.Hk, self.Hv, self.K, self.V, int(no_backward))
-        _need(n > 0, "no workspace for n_seq=%d rows=%d" % (n_seq, rows))
+        _need(n > 0, "no workspace for n_seq=%d rows=%d", n_seq, rows)
         return torch.empty(n, dtype=torch.float32, device=device)
 
     def _desc(self, q, k, v, g, beta, ws, starts, lens, dev):
@@ -131,14 +131,16 @@ class GatedDelta:
         _need(isinstance(q, torch.Tensor), "q is not a tensor")
         if starts is not None:
             _need(lens is None, "starts and lens")
-            _need(q.dim() == 3, "packed q has shape %s, not [rows, Hk, K]" % (tuple(q.shape),))
+            if q.dim() != 3:
+                _need(False, "packed q has shape %s, not [rows, Hk, K]", tuple(q.shape))
             lead = (q.shape[0],)
             rows = lead[0]
             _need(isinstance(starts, torch.Tensor) and starts.dim() == 1 and starts.numel() >= 2, "starts: n_seq + 1 numbers")
             n_seq = starts.numel() - 1
             d.starts = _tensor("starts", starts, (n_seq + 1,), torch.int32, dev)
         else:
-            _need(q.dim() == 4, "q has shape %s, not [B, T, Hk, K]" % (tuple(q.shape),))
+            if q.dim() != 4:
+                _need(False, "q has shape %s, not [B, T, Hk, K]", tuple(q.shape))
             lead = tuple(q.shape[:2])
             n_seq, rows = lead[0], lead[0] * lead[1]
             if lens is not None:
@@ -194,7 +196,7 @@ class GatedDelta:
         _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q is not [B, Hk, K]")
         _need(isinstance(state, torch.Tensor) and state.dim() == 4, "state is not [n, Hv, K, V]")
         B, n = q.shape[0], state.shape[0]
-        _need(B > 0 and n > 0, "%d rows for %d states" % (B, n))
+        _need(B > 0 and n > 0, "%d rows for %d states", B, n)
         Hk, Hv, K, V, dt = self.Hk, self.Hv, self.K, self.V, self.dtype
         key, val, head = ((B, Hk, K), 1, Hk * K, dt, dev), ((B, Hv, V), 1, Hv * V, dt, dev), ((B, Hv), 1, Hv, torch.float32, dev)
         sp = self._state("state", state, n, dev)
@@ -203,7 +205,7 @@ class GatedDelta:
         if slots is not None:
             sl = _tensor("slots", slots, (B,), torch.int32, dev)
         else:
-            _need(B <= n, "%d rows for %d states" % (B, n))
+            _need(B <= n, "%d rows for %d states", B, n)
         qp, ldq = _rows("q", q, *key)
         kp, ldk = _rows("k", k, *key)
         vp, ldv = _rows("v", v, *val)
@@ -229,11 +231,11 @@ class BlockNorm:
     def __init__(self, D: int, H: int = 1, post: str = "none", pre: str = "none", gate_act: str = "none", gate_rows: int = 1,
                  alpha: float = 1.0, scale: float = 1.0, eps: float = 1e-6, dtype=torch.float32):
         self.code = _dtype_code(dtype)
-        _need(post in _NORMS and pre in _NORMS, "norms %r, %r: none, rms or layer" % (post, pre))
-        _need(gate_act in _GATES, "gate_act %r: none, sigmoid or silu" % (gate_act,))
-        _need(0 < D <= 8192 and H > 0, "H=%d D=%d: D up to 8192" % (H, D))
-        _need(gate_rows >= 1 and (gate_rows == 1 or H == 1), "gate_rows=%d with H=%d" % (gate_rows, H))
-        _need(eps >= 0, "eps=%g" % eps)
+        _need(post in _NORMS and pre in _NORMS, "norms %r, %r: none, rms or layer", post, pre)
+        _need(gate_act in _GATES, "gate_act %r: none, sigmoid or silu", gate_act)
+        _need(0 < D <= 8192 and H > 0, "H=%d D=%d: D up to 8192", H, D)
+        _need(gate_rows >= 1 and (gate_rows == 1 or H == 1), "gate_rows=%d with H=%d", gate_rows, H)
+        _need(eps >= 0, "eps=%g", eps)
         self.D, self.H, self.post, self.pre, self.gate_act, self.gate_rows = D, H, post, pre, gate_act, gate_rows
         self.alpha, self.scale, self.eps, self.dtype = float(alpha), float(scale), float(eps), dtype
         d = _lib.BlockNormDesc()                  # what every call of this plan has in common
@@ -246,7 +248,7 @@ class BlockNorm:
     def workspace(self, M: int, device) -> torch.Tensor:
         """Workspace of `bwd` for M rows."""
         n = self._lib.hhrl_block_norm_workspace_floats(M, self.H, self.D, self.gate_rows)
-        _need(n > 0, "no workspace for M=%d" % M)
+        _need(n > 0, "no workspace for M=%d", M)
         return torch.empty(n, dtype=torch.float32, device=device)
 
     def _shape(self, first, M, dev):
@@ -311,7 +313,7 @@ class BlockNorm:
         d, M, act = self._desc(x, y, gate, (w_post, b_post, w_pre, b_pre), dev)
         _need(d_out is not None or d_h is not None, "neither d_out nor d_h")
         for name, t, of in (("dx", dx, x), ("dy", dy, y), ("dgate", dgate, gate)):
-            _need(t is None or of is not None, "%s without %s" % (name, name[1:]))
+            _need(t is None or of is not None, "%s without %s", name, name[1:])
         if d_out is not None:
             d.d_out, d.lddo = _rows("d_out", d_out, *act)
         if d_h is not None:
@@ -324,7 +326,7 @@ class BlockNorm:
             d.dgate, d.lddgate = _rows("dgate", dgate, *self._gate_shape(dgate, M, act, dev))
         for name, t in zip(self.PARAMS, (dw_post, db_post, dw_pre, db_pre)):
             if t is not None:
-                _need(getattr(self, name[2:]) != "none" and (name[2:] == "post" or d_h is not None), "d%s without its norm" % name)
+                _need(getattr(self, name[2:]) != "none" and (name[2:] == "post" or d_h is not None), "d%s without its norm", name)
                 setattr(d, "d" + name, _tensor("d" + name, t, (self.D,), torch.float32, dev))
         if ws is not None:
             _need(isinstance(ws, torch.Tensor), "ws is not a tensor")
