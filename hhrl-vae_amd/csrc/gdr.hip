@@ -161,7 +161,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, lo
 // registers of a product: four elements of a row from k q^T, of a column (for the transpose) from q k^T.  The 32 x 32
 // blocks beyond the diagonal are neither written nor read.
 // Bound by what it writes where there are many chunks (4 x 4096 tokens, 16 heads, K 128, bf16, for training: 0.54 GB in
-// 119 us), else by the latency of its steps (64 chunks in fp32: 18 us, of which the products of the last row of tiles, the
+// 125 us), else by the latency of its steps (64 chunks in fp32: 17 us, of which the products of the last row of tiles, the
 // decays and the substitution are 4 us each).  Three workgroups per CU fill the waits of each other.
 template <int NP, int KB2>
 struct PrepLds {
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
   float* const gh = reinterpret_cast<float*>(smem + L::over);
   float* const gl = gh + kC;
   float* const be = gl + kC;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
   const long slot = blockIdx.x;
   const int hk = blockIdx.y;
   long row0;
@@ -344,24 +344,38 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
     const int ib = 16 * wave + 4 * lg, iq = 16 * wave + lr;
     __bf16* const pp = a.p + vs * kC * NO * kC;
     __bf16* const pt = a.pt + vs * kC * 3 * kC;
+    const f32x4 gi4 = *reinterpret_cast<const f32x4*>(gh + ib), li4 = *reinterpret_cast<const f32x4*>(gl + ib), bi4 = *reinterpret_cast<const f32x4*>(be + ib);
+    const float gq = gh[iq], lq = gl[iq];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int j = 16 * t + lr, jb = 16 * t + 4 * lg;
-      f32x4 x;
-      const float hj = gh[j], lj = gl[j];
+      const bool same = t < 2 || wave >= 2;                  // PT rows j >= 32 hold columns i >= 32, P rows i < 32 columns j < 32
+      __bf16* const to_p = pp + (wave * 2 + (t >> 1)) * NO * kFrag + frag_at(lr, jb);
+      __bf16* const to_pt = pt + (t * 2 + (wave >> 1)) * 3 * kFrag + frag_at(lr, ib);
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      if (t <= wave) {
+        const float hj = gh[j], lj = gl[j];
+        const f32x4 gj4 = *reinterpret_cast<const f32x4*>(gh + jb), lj4 = *reinterpret_cast<const f32x4*>(gl + jb);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = ib + e;
-        const float d = i >= j ? decay((gh[i] - hj) + (gl[i] - lj)) : 0.f;
-        lm[i * kLdM + j] = i > j ? be[i] * kk[t][e] * d : i == j ? 1.f : 0.f;
-        mm[i * kLdM + j] = 0.f;
-        x[e] = i >= j ? qk[t][e] * d : 0.f;
+        for (int e = 0; e < 4; ++e) {
+          const int i = ib + e;
+          const float d = i >= j ? decay((gi4[e] - hj) + (li4[e] - lj)) : 0.f;
+          lm[i * kLdM + j] = i > j ? bi4[e] * kk[t][e] * d : i == j ? 1.f : 0.f;
+          mm[i * kLdM + j] = 0.f;
+          x[e] = i >= j ? qk[t][e] * d : 0.f;
+        }
+        if (a.train && same) sb::split_store4<3>(to_pt, kFrag, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = iq >= jb + e ? kq[t][e] * decay((gq - gj4[e]) + (lq - lj4[e])) : 0.f;
+        if (same) sb::split_store4<NO>(to_p, kFrag, x);
+      } else {                                               // above the diagonal: nothing reads it of I + A
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mm[(ib + e) * kLdM + j] = 0.f;
+        if (t >> 1 == wave >> 1) {
+          if (a.train) sb::split_store4<3>(to_pt, kFrag, x);
+          sb::split_store4<NO>(to_p, kFrag, x);
+        }
       }
-      if (a.train && ((t < 2) || (wave >= 2))) sb::split_store4<3>(pt + (t * 2 + (wave >> 1)) * 3 * kFrag + frag_at(lr, ib), kFrag, x);       // PT rows j >= 32 hold columns i >= 32
-      const float hq = gh[iq], lq = gl[iq];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = iq >= jb + e ? kq[t][e] * decay((hq - gh[jb + e]) + (lq - gl[jb + e])) : 0.f;
-      if (t < 2 || wave >= 2) sb::split_store4<NO>(pp + (wave * 2 + (t >> 1)) * NO * kFrag + frag_at(lr, jb), kFrag, x);
     }
     lds_barrier();
     {
