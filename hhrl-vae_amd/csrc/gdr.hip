@@ -23,8 +23,8 @@
 //   dG_i = q_i.dq_i + beta_i k_i.H_i - k_i.(the other terms of dk_i), dG_C += <dS', S'>, dg = sum of dG from i on.
 //
 // All products run on the bf16 matrix instruction with fp32 operands as three bf16 terms (split_bf16.h): a decayed,
-// corrected state is a difference of numbers much larger than itself, its gradients more so, and dg, dbeta and the
-// states are fp32 results.  The decays' sums are kept as two floats from a sum in fp64, so that exp(G_i - G_j) is exact
+// corrected state is a difference of numbers much larger than itself, its gradients more so, and so may o be; dg, dbeta
+// and the states are fp32 results.  The decays' sums are kept as two floats from a sum in fp64, so that exp(G_i - G_j) is exact
 // to fp32 however far G has run.
 //
 // What a whole training call moves: per chunk and head of K = V = 128, bf16, 0.8 MB, of which the caller's tensors are 0.13;
@@ -92,7 +92,7 @@ struct GdrArgs {
   long lddg, lddbeta;
   int whole, wide, wide_v, v16, train, vp, nvt, by_length;
   // ws, all but vec, w, y, s, ds as operand blocks, per chunk and key head: k, q (rows: tokens) and their transposes (rows: K);
-  //     per chunk and value head: M, P (two terms for bf16: what o takes) and their transposes, five rows of 64 floats, and
+  //     per chunk and value head: M, P and their transposes, five rows of 64 floats, and
   //     for the backward pass W, Y [vp/32][64][32] and S, dS [vp/32][Kp/16][2][64 lanes][4], fp32
   __bf16 *kpk, *qpk, *kt, *qt, *m, *p, *mt, *pt;
   float *vec, *w, *y, *s, *ds;
@@ -174,7 +174,7 @@ struct PrepLds {
 template <typename T, int NP, int KB2>
 __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs a) {
   using L = PrepLds<NP, KB2>;
-  constexpr int Kp = L::Kp, KG = Kp / 8, NO = NP == 1 ? 2 : 3;
+  constexpr int Kp = L::Kp, KG = Kp / 8;
   extern __shared__ __align__(16) char smem[];
   __bf16* const kl = reinterpret_cast<__bf16*>(smem);          // [NP][64][Kp]
   __bf16* const ql = kl + NP * kC * Kp;
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
       v[kGLo * kC] = lo;
     }
     const int ib = 16 * wave + 4 * lg, iq = 16 * wave + lr;
-    __bf16* const pp = a.p + vs * kC * NO * kC;
+    __bf16* const pp = a.p + vs * kC * 3 * kC;
     __bf16* const pt = a.pt + vs * kC * 3 * kC;
     const f32x4 gi4 = *reinterpret_cast<const f32x4*>(gh + ib), li4 = *reinterpret_cast<const f32x4*>(gl + ib), bi4 = *reinterpret_cast<const f32x4*>(be + ib);
     const float gq = gh[iq], lq = gl[iq];
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
     for (int t = 0; t < 4; ++t) {
       const int j = 16 * t + lr, jb = 16 * t + 4 * lg;
       const bool same = t < 2 || wave >= 2;                  // PT rows j >= 32 hold columns i >= 32, P rows i < 32 columns j < 32
-      __bf16* const to_p = pp + (wave * 2 + (t >> 1)) * NO * kFrag + frag_at(lr, jb);
+      __bf16* const to_p = pp + (wave * 2 + (t >> 1)) * 3 * kFrag + frag_at(lr, jb);
       __bf16* const to_pt = pt + (t * 2 + (wave >> 1)) * 3 * kFrag + frag_at(lr, ib);
       f32x4 x = {0.f, 0.f, 0.f, 0.f};
       if (t <= wave) {
@@ -367,13 +367,13 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
         if (a.train && same) sb::split_store4<3>(to_pt, kFrag, x);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = iq >= jb + e ? kq[t][e] * decay((gq - gj4[e]) + (lq - lj4[e])) : 0.f;
-        if (same) sb::split_store4<NO>(to_p, kFrag, x);
+        if (same) sb::split_store4<3>(to_p, kFrag, x);
       } else {                                               // above the diagonal: nothing reads it of I + A
 #pragma unroll
         for (int e = 0; e < 4; ++e) mm[(ib + e) * kLdM + j] = 0.f;
         if (t >> 1 == wave >> 1) {
           if (a.train) sb::split_store4<3>(to_pt, kFrag, x);
-          sb::split_store4<NO>(to_p, kFrag, x);
+          sb::split_store4<3>(to_p, kFrag, x);
         }
       }
     }
@@ -812,7 +812,6 @@ template <typename T, int NP, int KB2, int NT, bool TRAIN, bool WIDE>
 __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
   using L = ScanLds<NP, KB2, NT>;
   constexpr int Kp = L::Kp, KB = Kp / 32, VT = L::VT;
-  constexpr int NO = NP == 1 ? 2 : 3;                      // terms behind o: a bf16 o takes 2^-17, an fp32 one all three
   extern __shared__ __align__(16) char smem[];
   __bf16* const sl = reinterpret_cast<__bf16*>(smem);      // [3][VT][Kp] S
   __bf16* const xl = sl + L::S;                            // [3][VT][kC]  beta (V - gam K S)
@@ -844,14 +843,14 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
   } else if (c0 < c1) {                                    // ---- the output, between the chain's barriers
     // Chunk c: Q S behind barrier 1, the first half of P W behind barrier 3, the second behind the next chunk's barrier 2,
     // the store behind its barrier 1 after that: no stretch between two barriers is longer than the chain's.
-    bf16x8 qf[KB][NP], pf[2][NO];
+    bf16x8 qf[KB][NP], pf[2][3];
     f32x4 qn[NT], qs[NT], qo[NT];
     const __bf16* const qp = a.qpk + ((slot0 + c0) * a.Hk + hk) * kC * NP * Kp;
     const long qstep = (long)a.Hk * kC * NP * Kp;
     const unsigned qat = w * KB * NP * kFrag + lane * 8;
-    const __bf16* const pp = a.p + ((slot0 + c0) * a.Hv + hv) * NO * kC * kC;
-    const long pstep = (long)a.Hv * NO * kC * kC;
-    const unsigned pat = w * 2 * NO * kFrag + lane * 8;
+    const __bf16* const pp = a.p + ((slot0 + c0) * a.Hv + hv) * 3 * kC * kC;
+    const long pstep = (long)a.Hv * 3 * kC * kC;
+    const unsigned pat = w * 2 * 3 * kFrag + lane * 8;
     // The products are formed turned (S^T Q^T, W^T P^T): a lane then holds four columns of a token, and four lanes' worth of
     // neighbours is one exchange inside the wave away (through its part of ot)
     const RowTile<T, NT, WIDE> op(a.o, a.ldo, start, len, hv, a.V, v0, w, lane);
@@ -869,14 +868,14 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_fwd_kernel(GdrArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[4 * h + e] = y[e];
         }
-        bf16x8 b[NO];
-        sb::split8<NO>(x, b);
-        sb::mma<NO, NO>(qs[t], b, pf[kb]);
+        bf16x8 b[3];
+        sb::split8<3>(x, b);
+        sb::mma<3, 3>(qs[t], b, pf[kb]);
       }
     };
     auto second = [&](int c) {                             // the second half, and W for the backward pass
       if (high) pw(c, 1);
-      load_half<NO>(pf[1], pp + (min(c + 1, c1 - 1) - c0) * pstep, pat + (high ? NO * kFrag : 0));
+      load_half<3>(pf[1], pp + (min(c + 1, c1 - 1) - c0) * pstep, pat + (high ? 3 * kFrag : 0));
       if constexpr (TRAIN) {
         float* const wp = a.w + ((((slot0 + c) * a.Hv + hv) * (a.vp / 32) + v0 / 32) * kC) * 32 + (v0 & 16);
 float y[4 * NT];
@@ -906,10 +905,10 @@ float y[4 * NT];
     GDR_IN_ORDER;
     vp.load(min(c0 + 1, c1 - 1));
     GDR_IN_ORDER;
-    load_half<NO>(pf[1], pp, pat + (high ? NO * kFrag : 0));
+    load_half<3>(pf[1], pp, pat + (high ? 3 * kFrag : 0));
     float gam = gp[(unsigned)ia];
     GDR_IN_ORDER;
-    load_half<NO>(pf[0], pp, pat);
+    load_half<3>(pf[0], pp, pat);
     GDR_IN_ORDER;
     first.put(vl + (c0 & 1) * VT * kC, w, lane);
     for (int c = c0; c < c1; ++c) {
@@ -920,9 +919,9 @@ float y[4 * NT];
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          bf16x8 b[NO];
-          sb::load_frag<NO>(b, sl + 16 * t * Kp + at16<Kp>(lr, 32 * kb + 8 * lg), VT * Kp);
-          sb::mma<NO, NP>(qn[t], b, qf[kb]);
+          bf16x8 b[3];
+          sb::load_frag<3>(b, sl + 16 * t * Kp + at16<Kp>(lr, 32 * kb + 8 * lg), VT * Kp);
+          sb::mma<3, NP>(qn[t], b, qf[kb]);
         }
       load_rows<NP, KB>(qf, qp + (min(c + 1, c1 - 1) - c0) * qstep, qat);
       if (c > c0 + 1) store(c - 2);
@@ -936,7 +935,7 @@ float y[4 * NT];
       gam = gp[(unsigned)ia];
       lds_barrier();
       pw(c, 0);
-      load_half<NO>(pf[0], pp + (min(c + 1, c1 - 1) - c0) * pstep, pat);
+      load_half<3>(pf[0], pp + (min(c + 1, c1 - 1) - c0) * pstep, pat);
     }
     if (c1 - c0 > 1) store(c1 - 2);
     second(c1 - 1);
@@ -1854,7 +1853,7 @@ long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, 
   t.qpk = take16(ns * Hk * np * kC * kp);
   t.kt = take16(ns * Hk * np * kC * kp);
   t.m = take16(ns * Hv * 3 * kC * kC);
-  t.p = take16(ns * Hv * (np == 1 ? 2 : 3) * kC * kC);
+  t.p = take16(ns * Hv * 3 * kC * kC);
   t.vec = take(ns * Hv * kVecs * kC);
   if (train) {
     t.qt = take16(ns * Hk * np * kC * kp);

@@ -421,7 +421,7 @@ int hhrl_lstm_backward_group(const hhrl_lstm_desc* descs, int n, int B, int T, i
  * scale and sequences, and writes dq, dk, dv (dtype), dg, dbeta and, where given, d_s0 (gradients with respect to q .. s0 of
  * <d_o, o> + <d_s1, s1>; d_o and d_s1 may not both be null; d_s0 may be d_s1).  Other outputs overlap no operand.
  * The products run on bf16 matrix instructions with every fp32 operand as three bf16 terms: results carry fp32
- * accuracy for either dtype (a bf16 o 2^-17 of the sums behind it), o and the input gradients are rounded once.  No atomics: the same bits on every run.
+ * accuracy for either dtype, o and the input gradients are rounded once.  No atomics: the same bits on every run.
  * A non-finite number in a token may spread to the 63 tokens before it (they share a chunk) and to all behind it. */
 #define HHRL_GDR_MAX_K 128
 #define HHRL_GDR_MAX_V 512
