@@ -23,8 +23,8 @@ struct NormArgs {
   int step_j;
   // backward: rows are dealt in segments that end with a gate group; a workgroup takes segs_per_block of them
   long group_rows, seg_rows, n_groups;
-  int parts, segs_per_block;
-  long n_segs;
+  int parts;
+  long segs_per_block, n_segs;
   float* par_ws;                // [workgroups][n_par][D] partial parameter gradients, order dw_post db_post dw_pre db_pre
   float* gate_ws;               // [n_segs][D] partial gate gradients (parts > 1)
   int par_slot[4], n_par;       // row of each parameter gradient in par_ws, -1: not wanted

@@ -69,15 +69,15 @@ int norm_resident(int tpr, int waves) {
   return 256 * (per_cu > 1 ? per_cu : 1);
 }
 
-struct NormParts { long group_rows, n_groups, seg_rows, n_segs; int parts, segs_per_block, blocks; };
+struct NormParts { long group_rows, n_groups, seg_rows, n_segs, segs_per_block; int parts, blocks; };
 NormParts norm_parts(long M, int H, long gate_rows, int tpr, int waves) {
   NormParts p;
   const long R = M * H;
   const int slots = norm_slots(tpr), top = norm_resident(tpr, waves);
   const bool bcast = gate_rows > 1;
-  p.group_rows = bcast ? gate_rows : R;
+  p.group_rows = bcast && gate_rows < R ? gate_rows : R;     // (a gate may be said to be for any number of rows)
   p.n_groups = (R + p.group_rows - 1) / p.group_rows;
-  const long gr = p.group_rows < R ? p.group_rows : R;
+  const long gr = p.group_rows;
   // at least four rows per slot (a partial row costs as much as a row)
   const long most = (gr + 4L * slots - 1) / (4L * slots);
   long parts = (top + p.n_groups - 1) / p.n_groups;
@@ -86,10 +86,12 @@ NormParts norm_parts(long M, int H, long gate_rows, int tpr, int waves) {
   p.seg_rows = (gr + parts - 1) / parts;
   p.parts = (int)((gr + p.seg_rows - 1) / p.seg_rows);
   p.n_segs = p.n_groups * p.parts;
-  p.segs_per_block = (int)((p.n_segs + top - 1) / top);
+  p.segs_per_block = (p.n_segs + top - 1) / top;
   p.blocks = (int)((p.n_segs + p.segs_per_block - 1) / p.segs_per_block);
   return p;
 }
+
+bool norm_rows_ok(long M, int H) { return M < (1L << 40) / H; }
 
 bool aligned16(const void* p) { return (reinterpret_cast<unsigned long long>(p) & 15) == 0; }
 
@@ -103,7 +105,7 @@ int norm_check(const hhrl_block_norm_desc* d, const char* who) {
   HHRL_REQUIRE(d->dtype == HHRL_F32 || d->dtype == HHRL_BF16, "%s: dtype %d", who, d->dtype);
   HHRL_REQUIRE(d->M > 0 && d->H > 0 && d->D > 0, "%s: bad shape M=%ld H=%d D=%d", who, d->M, d->H, d->D);
   HHRL_REQUIRE(d->D <= kNormMaxD, "%s: D=%d (up to %d supported)", who, d->D, kNormMaxD);
-  HHRL_REQUIRE(d->M < (1L << 40) / d->H, "%s: M*H too large", who);
+  HHRL_REQUIRE(norm_rows_ok(d->M, d->H), "%s: M*H too large", who);
   HHRL_REQUIRE(d->post >= HHRL_NORM_NONE && d->post <= HHRL_NORM_LAYER && d->pre >= HHRL_NORM_NONE && d->pre <= HHRL_NORM_LAYER,
                "%s: norm kinds %d, %d", who, d->post, d->pre);
   HHRL_REQUIRE(d->gate_act == HHRL_ACT_NONE || d->gate_act == HHRL_ACT_SIGMOID || d->gate_act == HHRL_ACT_SILU, "%s: gate_act %d", who, d->gate_act);
@@ -156,7 +158,7 @@ using namespace hhrl;
 extern "C" {
 
 long hhrl_block_norm_workspace_floats(long M, int H, int D, long gate_rows) {
-  if (M <= 0 || H <= 0 || D <= 0 || D > kNormMaxD || gate_rows < 1 || (gate_rows > 1 && H != 1)) return 0;
+  if (M <= 0 || H <= 0 || !norm_rows_ok(M, H) || D <= 0 || D > kNormMaxD || gate_rows < 1 || (gate_rows > 1 && H != 1)) return 0;
   long most = 0;
   for (int waves : {2, 4}) {                          // the backward launch chooses by type, alignment and biases
     const NormParts p = norm_parts(M, H, gate_rows, norm_tpr(D), waves);

@@ -234,7 +234,7 @@ class BlockNorm:
         _need(post in _NORMS and pre in _NORMS, "norms %r, %r: none, rms or layer", post, pre)
         _need(gate_act in _GATES, "gate_act %r: none, sigmoid or silu", gate_act)
         _need(0 < D <= 8192 and H > 0, "H=%d D=%d: D up to 8192", H, D)
-        _need(gate_rows >= 1 and (gate_rows == 1 or H == 1), "gate_rows=%d with H=%d", gate_rows, H)
+        _need(1 <= gate_rows < 1 << 63 and (gate_rows == 1 or H == 1), "gate_rows=%d with H=%d", gate_rows, H)
         _need(eps >= 0, "eps=%g", eps)
         self.D, self.H, self.post, self.pre, self.gate_act, self.gate_rows = D, H, post, pre, gate_act, gate_rows
         self.alpha, self.scale, self.eps, self.dtype = float(alpha), float(scale), float(eps), dtype

@@ -1,0 +1,60 @@
+"""Sizes at the ends of their ranges, on the host: what the norms' workspace function and checks answer, without a GPU."""
+import ctypes as C
+import subprocess
+import sys
+
+import pytest
+
+FAKE = 1 << 20                     # an address that no check looks behind
+LONG_MAX = (1 << 63) - 1
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from hhrl_vae_amd import _lib
+    return _lib.load()
+
+
+def norm_desc(M, D, gate_rows, ws_floats, gate=FAKE, **over):
+    from hhrl_vae_amd import _lib
+    d = _lib.BlockNormDesc()
+    f = dict(dtype=0, M=M, H=1, D=D, post=2, pre=2, gate_act=0, gate_rows=gate_rows, alpha=1.0, scale=1.0, eps=1e-6, x=FAKE, y=FAKE, gate=gate, ldx=D, ldy=D,
+             ldgate=D, d_out=FAKE, d_h=FAKE, lddo=D, lddh=D, dx=FAKE, dy=FAKE, lddx=D, lddy=D, dw_post=1 * FAKE, db_post=2 * FAKE, dw_pre=3 * FAKE,
+             db_pre=4 * FAKE, ws=FAKE, ws_floats=ws_floats)
+    f.update(over)
+    for k, v in f.items():
+        setattr(d, k, v)
+    return d
+
+
+def run(code):
+    """In a process of its own, which a mistake here would end."""
+    p = subprocess.run([sys.executable, "-c", "import sys; sys.path[:0] = ['.', 'tests']\nimport test_sequence_sizes as t, ctypes as C\n"
+                        "from hhrl_vae_amd import _lib, sequence\nlib = _lib.load()\n" + code], capture_output=True, text=True, timeout=120)
+    assert p.returncode == 0, (p.returncode, p.stderr[-500:])
+    return p.stdout.split()
+
+
+def test_a_gate_shared_by_more_rows_than_there_are():
+    """One learned gate per channel, however many rows it is said to be for: as for the rows that there are."""
+    rows = (LONG_MAX, LONG_MAX - 9, 1 << 62, 101, 100)
+    sizes = run("for r in %r: print(lib.hhrl_block_norm_workspace_floats(100, 1, 64, r), sequence.BlockNorm(64, gate_rows=r).workspace(100, 'cpu').numel())" % (rows,))
+    assert len(set(sizes)) == 1 and len(sizes) == 2 * len(rows) and int(sizes[0]) > 0
+    # the backward call divides the rows the same way, and asks for its workspace
+    for line in run("for r in %r: print(lib.hhrl_block_norm_backward(C.byref(t.norm_desc(100, 64, r, 16)), None), 'workspace' in lib.hhrl_last_error().decode(), sep=',')" % (rows,)):
+        assert line == "1,True"
+
+
+def test_more_rows_than_a_call_takes(lib):
+    size = lib.hhrl_block_norm_workspace_floats
+    for M, H in ((1 << 40, 1), (1 << 30, 1 << 10), (LONG_MAX, 1), (LONG_MAX, (1 << 31) - 1)):
+        assert size(M, H, 64, 1) == 0
+    for M, gate_rows in (((1 << 40) - 1, 1), ((1 << 40) - 1, 2), ((1 << 40) - 1, LONG_MAX)):
+        assert 0 < size(M, 1, 64, gate_rows) < 1 << 60
+
+
+@pytest.mark.parametrize("rows", [1 << 63, (1 << 64) + 3, -(1 << 64) + 1])
+def test_rows_of_a_gate_that_no_long_holds(rows):
+    from hhrl_vae_amd import sequence
+    with pytest.raises(ValueError):
+        sequence.BlockNorm(64, post="rms", gate_rows=rows)
