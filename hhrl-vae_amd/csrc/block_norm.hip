@@ -160,11 +160,12 @@ extern "C" {
 long hhrl_block_norm_workspace_floats(long M, int H, int D, long gate_rows) {
   if (M <= 0 || H <= 0 || !norm_rows_ok(M, H) || D <= 0 || D > kNormMaxD || gate_rows < 1 || (gate_rows > 1 && H != 1)) return 0;
   long most = 0;
-  for (int waves : {2, 4}) {                          // the backward launch chooses by type, alignment and biases
-    const NormParts p = norm_parts(M, H, gate_rows, norm_tpr(D), waves);
-    const long n = (long)p.blocks * 4 * D + (p.parts > 1 && gate_rows > 1 ? p.n_segs * D : 0);
-    if (n > most) most = n;
-  }
+  for (int waves : {2, 4})                            // the backward launch chooses by type, alignment and biases,
+    for (long rows : {1L, gate_rows}) {               // and by whether the gate is there
+      const NormParts p = norm_parts(M, H, rows, norm_tpr(D), waves);
+      const long n = (long)p.blocks * 4 * D + (p.parts > 1 && rows > 1 ? p.n_segs * D : 0);
+      if (n > most) most = n;
+    }
   return most;
 }
 

@@ -24,3 +24,20 @@ def test_block_norm_gate_for_any_number_of_rows(M):
         want = want or got
         for a, b in zip(got, want):
             assert torch.equal(a, b) and bool(torch.isfinite(a).all())
+
+
+def test_block_norm_shared_gate_plan_without_its_gate():
+    """A plan whose gate is shared by 4465 rows, called without the gate in the workspace it gives: the bits of a plan without one."""
+    from hhrl_vae_amd import sequence
+    M, D, gen = 9201, 8192, torch.Generator(device=DEV).manual_seed(0)
+    y, d_out = (torch.randn(M, D, generator=gen, device=DEV).bfloat16() for _ in range(2))
+    got = []
+    for rows in (4465, 1):
+        plan = sequence.BlockNorm(D, post="layer", gate_rows=rows, dtype=torch.bfloat16)
+        dy, dw, db = torch.empty_like(y), torch.zeros(D, device=DEV), torch.zeros(D, device=DEV)
+        ws = plan.workspace(M, DEV)
+        ws.fill_(float("nan"))
+        plan.bwd(y=y, d_out=d_out, dy=dy, dw_post=dw, db_post=db, ws=ws)
+        got.append((dy, dw, db))
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and bool(torch.isfinite(a).all())

@@ -1,5 +1,7 @@
 """Sizes at the ends of their ranges, on the host: what the norms' workspace function and checks answer, without a GPU."""
 import ctypes as C
+import random
+import re
 import subprocess
 import sys
 
@@ -58,3 +60,20 @@ def test_rows_of_a_gate_that_no_long_holds(rows):
     from hhrl_vae_amd import sequence
     with pytest.raises(ValueError):
         sequence.BlockNorm(64, post="rms", gate_rows=rows)
+
+
+def test_workspace_serves_a_call_without_the_optional_gate(lib):
+    """A plan with a shared gate, called without one: its rows are dealt as one group, and the workspace holds those parts too.
+    (A workspace one float short of what the call needs is refused and says how many that is, before anything is launched.)"""
+    rng = random.Random(7)
+    cases = [(9201, 8192, 4465), (10400, 8192, 40), (1002, 4096, 1001), (70, 64, 3), (1, 1, 1 << 40)]
+    cases += [(rng.randint(1, 20000), rng.choice([1, 17, 100, 512, 1024, 2056, 4096, 8192]), rng.randint(2, 20000)) for _ in range(3000)]
+    for M, D, gate_rows in cases:
+        size = lib.hhrl_block_norm_workspace_floats(M, 1, D, gate_rows)
+        for dtype in (0, 1):
+            for over in (dict(), dict(db_post=None, db_pre=None)):
+                for gate in (None, FAKE):
+                    d = norm_desc(M, D, gate_rows, 0, gate=gate, dtype=dtype, dgate=gate, lddgate=D, **over)
+                    assert lib.hhrl_block_norm_backward(C.byref(d), None) == 1
+                    need = int(re.search(rb"(\d+) needed", lib.hhrl_last_error()).group(1))
+                    assert need <= size, (M, D, gate_rows, dtype, gate, need, size)
