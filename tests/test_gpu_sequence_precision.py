@@ -63,3 +63,71 @@ def test_gdr_output_is_a_difference_of_fp32_numbers(seq, dtype, K, V, what):
         off = (o[0].cpu().double() - want).abs()
         tol = 20 * U + (UBF if dtype is BF else 0.0) * want.abs()
         assert bool((off <= tol).all()), "off by %g u" % float(((off - tol) / U).max())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+def test_block_norm_fp32_results_of_gates(seq, dtype, act):
+    """A shared gate, its gradient and those of the parameters are fp32 for either type.  Gates down to -80, results of one
+    row: sigmoid 6 u (exponential 2, sum 1, quotient 1, argument exact), its slope s (1 - s) 3 more, the products with
+    scale, w, n and d_out 5, silu's slope 2: relative, where the factor next to s is of one sign."""
+    D = 512
+    gen = torch.Generator().manual_seed(1)
+    gate = -80 * torch.rand(1, D, generator=gen) - 3.0
+    y, d_out = (torch.randn(2, D, generator=gen).to(dtype) for _ in range(2))
+    d_out[1] = 0                                                     # two rows share the gate, one of them counts
+    plan = seq.BlockNorm(D, gate_act=act, gate_rows=2, dtype=dtype)
+    dgate, dy = torch.empty(1, D, device=DEV), torch.empty(2, D, dtype=dtype, device=DEV)
+    ws = plan.workspace(2, DEV)
+    plan.bwd(y=y.to(DEV), gate=gate.to(DEV), d_out=d_out.to(DEV), dgate=dgate, dy=dy, ws=ws)
+    z = gate.double().requires_grad_(True)
+    s = torch.sigmoid(z)
+    (s if act == "sigmoid" else z * s).sum().backward()
+    want = (z.grad * y[:1].double() * d_out[:1].double()).detach()
+    assert bool(((dgate.cpu().double() - want).abs() <= 16 * U * want.abs() + 1e-37).all()), float(((dgate.cpu().double() - want).abs() / want.abs()).max() / U)
+    # the gradient of the norm's bias: scale * value of the gate * d_out, of one row
+    plan = seq.BlockNorm(D, post="rms", gate_act=act, gate_rows=2, dtype=dtype)
+    db, b = torch.zeros(D, device=DEV), torch.zeros(D, device=DEV)
+    plan.bwd(y=y.to(DEV), gate=gate.to(DEV), b_post=b, d_out=d_out.to(DEV), db_post=db, ws=plan.workspace(2, DEV))
+    want = ((s if act == "sigmoid" else z * s).detach() * d_out[:1].double())[0]
+    assert bool(((db.cpu().double() - want).abs() <= 16 * U * want.abs() + 1e-37).all()), float(((db.cpu().double() - want).abs() / want.abs()).max() / U)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+def test_block_norm_parameter_gradients_behind_a_gate_per_element(seq, dtype, act):
+    """The same for a gate with an element for every element: db_post of one row."""
+    D = 520
+    gen = torch.Generator().manual_seed(2)
+    gate = (-80 * torch.rand(1, D, generator=gen) - 3.0).to(dtype)
+    y, d_out = (torch.randn(1, D, generator=gen).to(dtype) for _ in range(2))
+    plan = seq.BlockNorm(D, post="rms", gate_act=act, dtype=dtype)
+    db, b = torch.zeros(D, device=DEV), torch.zeros(D, device=DEV)
+    plan.bwd(y=y.to(DEV), gate=gate.to(DEV), b_post=b, d_out=d_out.to(DEV), db_post=db, ws=plan.workspace(1, DEV))
+    z = gate.double()
+    want = ((torch.sigmoid(z) if act == "sigmoid" else z * torch.sigmoid(z)) * d_out.double())[0]
+    assert bool(((db.cpu().double() - want).abs() <= 16 * U * want.abs() + 1e-37).all()), float(((db.cpu().double() - want).abs() / want.abs()).max() / U)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("gate_rows", [1, 2])
+def test_block_norm_gates_at_the_ends(seq, dtype, gate_rows):
+    """Gates that are no number stay none, infinite and very large ones give 0, 1 and themselves, and slopes of 0."""
+    vals = torch.tensor([math.nan, math.inf, -math.inf, 200.0, -200.0, 88.5, -88.5, 0.0] * 8)
+    D = vals.numel()
+    y = torch.ones(1, D, dtype=dtype, device=DEV)
+    gate = vals[None].to(DEV) if gate_rows > 1 else vals[None].to(dtype).to(DEV)
+    for act in ("sigmoid", "silu"):
+        plan = seq.BlockNorm(D, gate_act=act, gate_rows=gate_rows, dtype=dtype)
+        out, dgate = torch.empty_like(y), torch.empty_like(gate)
+        plan.fwd(y=y, gate=gate, out=out)
+        plan.bwd(y=y, gate=gate, d_out=y, dgate=dgate, ws=plan.workspace(1, DEV))
+        o, d = out.float().cpu()[0], dgate.float().cpu()[0]
+        assert bool(torch.isnan(o[0::8]).all()) and bool(torch.isnan(d[0::8]).all())
+        # 88.5 and -200 are multiples of their own last places in bf16 too
+        want = torch.tensor([1.0, 0.0, 1.0, 0.0, 1.0, 0.0, 0.5] if act == "sigmoid" else [math.inf, math.nan, 200.0, 0.0, 88.5, 0.0, 0.0])
+        slope = torch.tensor([0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.25] if act == "sigmoid" else [math.nan, math.nan, 1.0, 0.0, 1.0, 0.0, 0.5])
+        for got, ref in ((o, want), (d, slope)):
+            for i in range(7):
+                if not math.isnan(ref[i]):             # (infinity times 0 at the far end: no value that is asked for)
+                    assert bool(torch.isclose(got[i + 1::8], ref[i], rtol=0, atol=1e-35).all()), (act, i, got[i + 1], ref[i])
