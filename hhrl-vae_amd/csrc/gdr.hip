@@ -103,8 +103,24 @@ struct GdrArgs {
 };
 enum { kGam = 0, kTail = 1, kBeta = 2, kGHi = 3, kGLo = 4, kVecs = 5 };
 
-// exp(x) for x <= 0, to 2^-24 |x| of itself, so to 2^-25 of the largest decay, 1 (the exponential instruction is base two)
-__device__ __forceinline__ float decay(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+// exp(x + low), |low| <= 2^-24 |x|, to 2^-22 of itself however large x is: the exponential instruction (base two) takes the
+// rounded product with log2 e, and what that, the constant and x leave out multiplies the result.
+__device__ __forceinline__ float exp_of(float x, float low) {
+  const float t = x * 1.44269502f;
+  const float r = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269502f, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  return fmaf(e, fmaf(r, 0.693147181f, low), e);
+}
+// exp((a + al) - (b + bl)) for a <= b <= 0, each sum of log decays as two floats.  What a - b leaves out is exact since
+// |a| >= |b|, and the sum of both is split anew, so that only the difference matters.
+__device__ __forceinline__ float decay(float a, float al, float b, float bl) {
+  const float s = a - b, low = (al - bl) + ((a - s) - b), x = s + low;
+  return exp_of(x, (s - x) + low);
+}
+__device__ __forceinline__ float decay(double x) {
+  const float hi = (float)x;
+  return exp_of(hi, (float)(x - (double)hi));
+}
 
 __device__ __forceinline__ long clampl(long v, long lo, long hi) { return v < lo ? lo : v > hi ? hi : v; }
 
@@ -335,8 +351,8 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
     if (wave == 0) {
       const double end = __shfl(G, 63, 64);
       float* const v = a.vec + vs * kVecs * kC + lane;
-      v[kGam * kC] = expf(hi) * (1.f + lo);
-      v[kTail * kC] = expf((float)(end - G));
+      v[kGam * kC] = decay(G);
+      v[kTail * kC] = decay(end - G);
       v[kBeta * kC] = bi;
       v[kGHi * kC] = hi;
       v[kGLo * kC] = lo;
@@ -359,14 +375,14 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int i = ib + e;
-          const float d = i >= j ? decay((gi4[e] - hj) + (li4[e] - lj)) : 0.f;
+          const float d = i >= j ? decay(gi4[e], li4[e], hj, lj) : 0.f;
           lm[i * kLdM + j] = i > j ? bi4[e] * kk[t][e] * d : i == j ? 1.f : 0.f;
           mm[i * kLdM + j] = 0.f;
           x[e] = i >= j ? qk[t][e] * d : 0.f;
         }
         if (a.train && same) sb::split_store4<3>(to_pt, kFrag, x);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = iq >= jb + e ? kq[t][e] * decay((gq - gj4[e]) + (lq - lj4[e])) : 0.f;
+        for (int e = 0; e < 4; ++e) x[e] = iq >= jb + e ? kq[t][e] * decay(gq, lq, gj4[e], lj4[e]) : 0.f;
         if (same) sb::split_store4<3>(to_p, kFrag, x);
       } else {                                               // above the diagonal: nothing reads it of I + A
 #pragma unroll
@@ -1529,7 +1545,7 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = ib + e;
-        const float d = i >= j ? decay((ghi[e] - hj[t]) + (glo[e] - lj[t])) : 0.f;
+        const float d = i >= j ? decay(ghi[e], glo[e], hj[t], lj[t]) : 0.f;
         dp[t][e] = i >= j ? a.scale * dp[t][e] * d : 0.f;
         da[t][e] = i > j ? -da[t][e] * d : 0.f;
       }

@@ -1,7 +1,7 @@
 // fp32-accurate products on the bf16 matrix instructions (gfx950, wave64).
 //
 // An fp32 number is the sum of three bf16 numbers up to 2^-27 of itself (8 + 8 + 8 significand bits and the signs of the
-// remainders), so a product of two such operands is the sum of the six partial products whose weights are above 2^-25,
+// remainders; terms below 2^-126, the least normal number, are lost, so numbers below 2^-109 are kept to 2^-126), so a product of two such operands is the sum of the six partial products whose weights are above 2^-25,
 // accumulated in fp32 by the matrix instruction; an operand that is bf16 to begin with needs three.  At 16384 FLOPs in 16
 // cycles (v_mfma_f32_16x16x32_bf16) against 2048 in 32 (v_mfma_f32_16x16x4_f32) six of them still cost 2.7 times less
 // than the fp32 instruction, three 5.3 times less.

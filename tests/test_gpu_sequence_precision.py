@@ -65,6 +65,35 @@ def test_gdr_output_is_a_difference_of_fp32_numbers(seq, dtype, K, V, what):
         assert bool((off <= tol).all()), "off by %g u" % float(((off - tol) / U).max())
 
 
+@pytest.mark.parametrize("T", [64, 150])
+def test_gdr_decays_far_from_one(seq, T):
+    """One token is written and every later one reads it through the decays in between, down to 2^-120: results are one
+    product of decays each and carry a relative accuracy.  Inside a chunk: the decay 4 u (its exponential 2, the
+    correction 1, the sums behind its argument less than 1), its product with q.k 1, three terms 3, scale 1.  Behind it: the
+    decays of the first chunk's end, of the chunks between and of the token, 4 each and 2 for the product, six sums of at most 2.
+    And 2^-124: a term of a number is lost where it is below the least normal bf16 number, 2^-126 (the third term of a number
+    below 2^-109), which is up to 2^-126 for each number that is split: P or R, or tail W and S, and half of that for W."""
+    gen = torch.Generator().manual_seed(T)
+    g = -2 * 80.0 / T * torch.rand(T, generator=gen)
+    g[1::2] *= 1.0 + 2.0 ** -11
+    q, k = torch.zeros(T, 8), torch.zeros(T, 8)
+    q[:, 3] = k[0, 3] = 1.0
+    beta, v, d_o = torch.zeros(T), torch.ones(T, 1), torch.ones(T, 1)
+    beta[0] = 1.0
+    G = g.double().cumsum(0)
+    want = (G - G[0]).exp()
+    layer = seq.GatedDelta(1, 1, 8, 1, scale=1.0)
+    dev = [t[None, :, None].contiguous().to(DEV) for t in (q, k, v, g, beta)]
+    ws, o = layer.workspace(1, T, DEV), torch.empty(1, T, 1, 1, device=DEV)
+    layer.fwd(*dev, o, ws)
+    grads = [torch.empty_like(t) for t in dev]
+    layer.bwd(*dev, d_o[None, :, None].contiguous().to(DEV), *grads, ws)
+    n = 12 if T <= 64 else 12 + 6 * (T // 64)
+    for name, got in (("o", o), ("dq", grads[0][..., 3])):          # dq_t = S_t d_o: the same numbers
+        off = (got.flatten().cpu().double() - want).abs()
+        assert bool((off <= n * U * want + 2.0 ** -124).all()), "%s: %g u" % (name, float((off / want).max() / U))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("act", ["sigmoid", "silu"])
 def test_block_norm_fp32_results_of_gates(seq, dtype, act):
