@@ -91,7 +91,10 @@ struct GdrArgs {
   float *dg, *dbeta;
   long lddg, lddbeta;
   int whole, wide, wide_v, v16, train, vp, nvt, by_length;
-  // ws, all but vec, w, y, s, ds as operand blocks, per chunk and key head: k, q (rows: tokens) and their transposes (rows: K);
+  // what ws holds: a number of the shapes whose forward pass was the last one in it, 0 if that was for no backward pass.  A
+  // backward pass that finds another number starts its sums from NaN: only the device knows.
+  unsigned long long *mark, key;
+  // ws behind it, all but vec, w, y, s, ds as operand blocks, per chunk and key head: k, q (rows: tokens) and their transposes (rows: K);
   //     per chunk and value head: M, P and their transposes, five rows of 64 floats, and
   //     for the backward pass W, Y [vp/32][64][32] and S, dS [vp/32][Kp/16][2][64 lanes][4], fp32
   __bf16 *kpk, *qpk, *kt, *qt, *m, *p, *mt, *pt;
@@ -123,6 +126,9 @@ __device__ __forceinline__ float decay(double x) {
 }
 
 __device__ __forceinline__ long clampl(long v, long lo, long hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// 0, or NaN for a backward pass without its forward
+__device__ __forceinline__ float poison(const GdrArgs& a) { return *a.mark == a.key ? 0.f : __builtin_nanf(""); }
 
 // rows [start, start + len) of sequence n (the same n in the whole wave) and the place of its first chunk.  Packed sequences of any lengths:
 // floor(start/64) + n leaves every sequence at least ceil(len/64) places.
@@ -203,6 +209,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void gdr_prep_kernel(GdrArgs 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
   const long slot = blockIdx.x;
   const int hk = blockIdx.y;
+  if (slot == 0 && hk == 0 && tid == 0) *a.mark = a.train ? a.key : 0;
   long row0;
   int valid;
   slot_chunk(a, slot, row0, valid);
@@ -1118,8 +1125,13 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
   // Barriers of a chunk: 1 (dl), 2 (zl), 3 (yl, yf; gl, zp by the others).  Two more in front of the walk.
   if (tid < 256) {                                         // ---- the chain
     f32x4 dS[KB2][NT];
+    const float bad = poison(a);
     if (BARE || a.segs == 1) load_state<KB2, NT>(dS, c1 == nc ? a.d_s1 : nullptr, a, nh, w, v0, lr, lg);
     else load_seg<KB2, NT>(dS, a.seg_s + (nh * a.segs + seg) * Kp * a.vp, a.vp, w, v0, lr, lg);
+#pragma unroll
+    for (int t = 0; t < KB2; ++t)
+#pragma unroll
+      for (int u = 0; u < NT; ++u) dS[t][u] += bad;          // from here to dv, d_s0 and, through Y and dS', dk, dg and dbeta
     if (c0 < c1) {
       bf16x8 kf[KB][NP], mf[2][3], ktf[KB2][2][NP], qtf[KB2][2][NP];
       const __bf16* kp = a.kpk + (slot1 * a.Hk + hk) * kC * NP * Kp;
@@ -1342,6 +1354,7 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
   const long hs = slot * a.Hk + hk;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   const bool has_do = a.d_o != nullptr;
+  const float bad = poison(a);
   f32x4 dqs[GROUP ? KT : 1], dks[GROUP ? KT : 1];
   if (GROUP) {
 #pragma unroll
@@ -1358,7 +1371,10 @@ __global__ __launch_bounds__(512, 1) void gdr_grads_kernel(GdrArgs a) {
     const long vs = slot * a.Hv + hv;
     f32x4 e1[KT], e2[KT], e3[KT], dp[2], da[2];
 #pragma unroll
-    for (int t = 0; t < KT; ++t) e1[t] = e2[t] = e3[t] = zero;
+    for (int t = 0; t < KT; ++t) {
+      e1[t] = zero + bad;                                    // (dq)
+      e2[t] = e3[t] = zero;
+    }
 #pragma unroll
     for (int t = 0; t < 2; ++t) dp[t] = da[t] = zero;
     float sdot = 0.f, ydot = 0.f;
@@ -1865,6 +1881,7 @@ long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, 
   auto take = [&](long floats) { float* p = ws ? ws + off : nullptr; off += (floats + 63) & ~63L; return p; };
   auto take16 = [&](long n) { return reinterpret_cast<__bf16*>(take((n + 1) / 2)); };
   GdrArgs t = {};
+  t.mark = reinterpret_cast<unsigned long long*>(take(2));      // (first, so that a forward pass for no backward pass finds it too)
   t.kpk = take16(ns * Hk * np * kC * kp);
   t.qpk = take16(ns * Hk * np * kC * kp);
   t.kt = take16(ns * Hk * np * kC * kp);
@@ -1891,7 +1908,7 @@ long carve(GdrArgs* a, float* ws, int dtype, int n_seq, long rows, bool packed, 
   }
   if (a) {
     a->segs = segs; a->seg_chunks = chunks; a->seg_m = t.seg_m; a->seg_mt = t.seg_mt; a->seg_n = t.seg_n; a->seg_s = t.seg_s;
-    a->kpk = t.kpk; a->qpk = t.qpk; a->kt = t.kt; a->qt = t.qt; a->m = t.m; a->p = t.p; a->mt = t.mt; a->pt = t.pt;
+    a->mark = t.mark; a->kpk = t.kpk; a->qpk = t.qpk; a->kt = t.kt; a->qt = t.qt; a->m = t.m; a->p = t.p; a->mt = t.mt; a->pt = t.pt;
     a->vec = t.vec; a->w = t.w; a->y = t.y; a->s = t.s; a->ds = t.ds;
     a->n_slots = ns; a->vp = (int)vp;
   }
@@ -1933,6 +1950,9 @@ int gdr_fill(const hhrl_gdr_desc* d, GdrArgs& a, bool train, const char* who) {
   a.q = d->q; a.k = d->k; a.v = d->v; a.ldq = d->ldq; a.ldk = d->ldk; a.ldv = d->ldv;
   a.g = d->g; a.beta = d->beta; a.ldg = d->ldg; a.ldbeta = d->ldbeta;
   a.train = train;
+  a.key = 0xcbf29ce484222325ull;                 // FNV-1a over the shapes
+  for (long x : {(long)d->dtype, (long)d->n_seq, d->rows, (long)(d->starts != nullptr), (long)d->Hk, (long)d->Hv, (long)d->K, (long)d->V})
+    for (int i = 0; i < 8; ++i) a.key = (a.key ^ (x >> 8 * i & 255)) * 0x100000001b3ull;
   a.v16 = rows16(d->dtype, d->V, d->v, d->ldv);
   a.wide = d->K % 8 == 0 && a16(d->q) && a16(d->k) && d->ldq % 8 == 0 && d->ldk % 8 == 0;
   a.whole = d->K == padded_k(d->K) && a.wide;

@@ -175,7 +175,8 @@ class GatedDelta:
 
     def bwd(self, q, k, v, g, beta, d_o, dq, dk, dv, dg, dbeta, ws, d_s1=None, d_s0=None, starts=None, lens=None) -> None:
         """Gradients of <d_o, o> + <d_s1, s1> (either None: absent), written to dq, dk, dv, dg, dbeta and d_s0; ws as the
-        forward call of the same inputs left it.  d_s0 may be d_s1."""
+        forward call of the same inputs left it (where the last one in it was of other shapes, or with no_backward, every
+        gradient is NaN).  d_s0 may be d_s1."""
         dev = _device()
         d, n, key, val, head = self._desc(q, k, v, g, beta, ws, starts, lens, dev)
         if d_o is not None:

@@ -418,7 +418,8 @@ int hhrl_lstm_backward_group(const hhrl_lstm_desc* descs, int n, int B, int T, i
  * wanted; may be s0).  A sequence without tokens hands its state on.
  * Forward writes o.  Unless no_backward is set it leaves in ws what the backward call reads; ws
  * (hhrl_gdr_workspace_floats, 16-byte aligned) must then stay untouched until that call, which takes the same inputs,
- * scale and sequences, and writes dq, dk, dv (dtype), dg, dbeta and, where given, d_s0 (gradients with respect to q .. s0 of
+ * scale and sequences (whose last forward pass in ws was for other shapes, or with no_backward, is an error that only the
+ * device sees: every gradient is NaN), and writes dq, dk, dv (dtype), dg, dbeta and, where given, d_s0 (gradients with respect to q .. s0 of
  * <d_o, o> + <d_s1, s1>; d_o and d_s1 may not both be null; d_s0 may be d_s1).  Other outputs overlap no operand.
  * The products run on bf16 matrix instructions with every fp32 operand as three bf16 terms: results carry fp32
  * accuracy for either dtype, o and the input gradients are rounded once.  No atomics: the same bits on every run.
