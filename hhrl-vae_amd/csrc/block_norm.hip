@@ -16,7 +16,7 @@ namespace hhrl {
 void norm_launch_f32(const NormArgs& a, bool vec, int tpr, int blocks, bool bwd, hipStream_t st) { norm_launch<float, 4>(a, vec, tpr, blocks, bwd, st); }
 
 // Sums the partial rows in their order: the parameter gradients (ADDED to dst) over all workgroups, and the gate rows
-// (written) over the parts of their group.  32 columns x 32 row lanes per workgroup: 1024 rows of 128 columns are few
+// (written) over the parts of their group.  Parameters with one gradient (a weight that both norms share) are one job.  32 columns x 32 row lanes per workgroup: 1024 rows of 128 columns are few
 // workgroups and a long walk (8 row lanes: 8.0 us).
 struct NormFoldArgs {
   const float* par_ws;
@@ -32,20 +32,27 @@ __global__ __launch_bounds__(1024) void block_norm_fold_kernel(NormFoldArgs a) {
   for (long job = blockIdx.y; job < a.n_par + a.n_groups; job += gridDim.y) {
     const bool par = job < a.n_par;
     const long grp = job - a.n_par;
-    const float* src = par ? a.par_ws + job * a.D : a.gate_ws + grp * a.parts * a.D;
+    float* const dst = par ? a.dst[job] : a.dgate + grp * a.lddg;
+    bool first = true;
+    for (int q = 0; par && q < job; ++q) first &= a.dst[q] != dst;
+    if (!first) continue;
     const long stride = par ? (long)a.n_par * a.D : a.D;
     const int rows = par ? a.blocks : a.parts;
     float s = 0.f;
-    if (col < a.D) {
+    for (long q = job; q < (par ? a.n_par : job + 1); ++q) {
+      if (par && a.dst[q] != dst) continue;
+      const float* const src = par ? a.par_ws + q * a.D : a.gate_ws + grp * a.parts * a.D;
+      if (col < a.D) {
 #pragma unroll 8
-      for (int r = ry; r < rows; r += 32) s += src[r * stride + col];
+        for (int r = ry; r < rows; r += 32) s += src[r * stride + col];
+      }
     }
     red[ry][cx] = s;
     __syncthreads();
     if (ry == 0 && col < a.D) {
       for (int r = 1; r < 32; ++r) s += red[r][cx];
-      if (par) a.dst[job][col] += s;
-      else a.dgate[grp * a.lddg + col] = s;
+      if (par) dst[col] += s;
+      else dst[col] = s;
     }
     __syncthreads();
   }
@@ -220,6 +227,10 @@ int hhrl_block_norm_backward(const hhrl_block_norm_desc* d, void* stream) {
   const bool fold_gate = a.gate_bcast && a.dgate && p.parts > 1;
   const long need = (long)p.blocks * a.n_par * a.D + (fold_gate ? p.n_segs * a.D : 0);
   HHRL_REQUIRE(need == 0 || (d->ws && d->ws_floats >= need), "block_norm_backward: workspace of %ld floats, %ld needed", d->ws ? d->ws_floats : 0L, need);
+  for (int q = 0; q < 4; ++q)
+    for (int o = 0; o < q; ++o)
+      HHRL_REQUIRE(!dst[q] || !dst[o] || dst[q] == dst[o] || dst[q] + a.D <= dst[o] || dst[o] + a.D <= dst[q],
+                   "block_norm_backward: two parameter gradients overlap (they may be the same array)");
   a.par_ws = d->ws;
   a.gate_ws = fold_gate ? d->ws + (long)p.blocks * a.n_par * a.D : nullptr;
   const double el = d->dtype == HHRL_BF16 ? 2.0 : 4.0;

@@ -473,7 +473,7 @@ int hhrl_gdr_step(const hhrl_gdr_step_desc* d, void* stream);
  * fp32 gate row (modulation of a sequence; gate_rows >= M: one learned gate per channel).
  * out (r) and h are rounded from the same fp32 row; either may be null; both may be x or y.
  * Backward forms everything again from the inputs (no saved statistics).  d_out, d_h: gradients of r and h, either may
- * be null.  dx, dy, dgate are written, dw_*, db_* ADDED to; any may be null.  Parameter gradients and a shared gate's
+ * be null.  dx, dy, dgate are written, dw_*, db_* ADDED to (two of them may be one array: it gets both); any may be null.  Parameter gradients and a shared gate's
  * need ws (hhrl_block_norm_workspace_floats, 16-byte aligned); sums are made in a fixed order.  D <= 8192. */
 typedef struct {
   int dtype;

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+import seq_reference as R
+
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 
@@ -41,3 +43,40 @@ def test_block_norm_shared_gate_plan_without_its_gate():
         got.append((dy, dw, db))
     for a, b in zip(*got):
         assert torch.equal(a, b) and bool(torch.isfinite(a).all())
+
+
+@pytest.mark.parametrize("M,D,gate_rows", [(1, 33, 1), (700, 72, 1), (5000, 4096, 1), (3000, 64, 700)])
+def test_block_norm_parameters_shared_by_both_norms(M, D, gate_rows):
+    """One array for the gradients of both norms' weights and one for those of both biases: each gets both, the same bits on
+    every run."""
+    from hhrl_vae_amd import sequence
+    gen = torch.Generator().manual_seed(D)
+    rn = lambda *s: torch.randn(*s, generator=gen).to(DEV)
+    ins = dict(x=rn(M, D), y=rn(M, D), gate=rn(-(-M // gate_rows), D), w_post=rn(D), b_post=rn(D))
+    ins.update(w_pre=ins["w_post"], b_pre=ins["b_post"])
+    plan = sequence.BlockNorm(D, post="rms", pre="layer", gate_act="sigmoid", gate_rows=gate_rows)
+    ws, d_out, d_h = plan.workspace(M, DEV), rn(M, D), rn(M, D)
+
+    def grads(shared):
+        w, b = torch.zeros(D, device=DEV), torch.zeros(D, device=DEV)
+        w2, b2 = (w, b) if shared else (torch.zeros(D, device=DEV), torch.zeros(D, device=DEV))
+        dgate = torch.empty_like(ins["gate"])
+        plan.bwd(d_out=d_out, d_h=d_h, dgate=dgate, dw_post=w, db_post=b, dw_pre=w2, db_pre=b2, ws=ws, **ins)
+        return w, b, w2, b2, dgate
+    *_, dgate = grads(False)
+    first = grads(True)
+    for r in range(4):
+        sw, sb, _, _, sg = grads(True) if r else first
+        assert torch.equal(sw, first[0]) and torch.equal(sb, first[1]) and torch.equal(sg, dgate)
+    # what the terms of both add up to in size, in 64 bits; either way a thread's rows, its slots, 32 lanes of partial rows and
+    # at last the two parameters: fewer than M / 8 + 256 sums, and the terms' own 128 roundings
+    d64 = {k: v.double() for k, v in ins.items()}
+    act = torch.sigmoid(d64["gate"])[torch.arange(M, device=DEV) // gate_rows]
+    n = R.norm(d64["y"], "rms", None, None, 1e-6)
+    r = (d64["x"] + act * (n * d64["w_post"] + d64["b_post"])).requires_grad_(True)
+    m = R.norm(r, "layer", None, None, 1e-6)
+    ((r * d_out.double()).sum() + ((m * d64["w_pre"] + d64["b_pre"]) * d_h.double()).sum()).backward()
+    db = r.grad * act
+    for got, parts in ((first[0], (db * n, d_h.double() * m.detach())), (first[1], (db, d_h.double()))):
+        want, size = sum(p.sum(0) for p in parts), sum(p.abs().sum(0) for p in parts) + 128 / max(M, 128) * sum(p.abs().max() for p in parts)
+        assert bool(((got.double() - want).abs() <= (M / 8 + 384) * R.U32 * size).all())

@@ -77,3 +77,12 @@ def test_workspace_serves_a_call_without_the_optional_gate(lib):
                     assert lib.hhrl_block_norm_backward(C.byref(d), None) == 1
                     need = int(re.search(rb"(\d+) needed", lib.hhrl_last_error()).group(1))
                     assert need <= size, (M, D, gate_rows, dtype, gate, need, size)
+
+
+@pytest.mark.parametrize("a,b", [("dw_post", "dw_pre"), ("dw_post", "db_post"), ("db_post", "db_pre"), ("dw_pre", "db_pre"), ("dw_post", "db_pre")])
+@pytest.mark.parametrize("apart", [4, -4, 63 * 4, -63 * 4])
+def test_parameter_gradients_that_overlap_are_refused(lib, a, b, apart):
+    """Two parameter gradients are added to by different workgroups at once: arrays that overlap in part would lose sums."""
+    base = 16 * FAKE
+    d = norm_desc(10, 64, 1, 1 << 40, **{a: base, b: base + apart})
+    assert lib.hhrl_block_norm_backward(C.byref(d), None) == 1 and b"overlap" in lib.hhrl_last_error(), lib.hhrl_last_error()
