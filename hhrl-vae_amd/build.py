@@ -25,6 +25,7 @@ def sources():
 def _deps():
     hdrs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")]
     hdrs.append(os.path.join(os.path.dirname(HERE), "include", "hhrl_hip.h"))
+    hdrs.append(os.path.abspath(__file__))            # the flags
     return sources() + hdrs
 
 
@@ -62,7 +63,7 @@ def _build(force: bool, verbose: bool, defines, tag: str) -> str:
         obj = os.path.join(obj_dir, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)
         if not force and os.path.exists(obj) and all(os.path.getmtime(p) <= os.path.getmtime(obj)
-                                                     for p in [src] + [d for d in _deps() if d.endswith(".h")]):
+                                                     for p in [src] + [d for d in _deps() if not d.endswith(".hip")]):
             continue
         cmd = [hipcc] + flags + ["-c", src, "-o", obj]
         if verbose:
