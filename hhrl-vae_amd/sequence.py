@@ -110,7 +110,7 @@ class GatedDelta:
 
     def __init__(self, Hk: int, Hv: int, K: int, V: int, dtype=torch.float32, scale: Optional[float] = None):
         self.code = _dtype_code(dtype)
-        _need(Hk > 0 and Hv > 0 and Hv % Hk == 0, "Hv=%d is not a multiple of Hk=%d", Hv, Hk)
+        _need(Hk > 0 and 0 < Hv < 1 << 31 and Hv % Hk == 0, "Hv=%d is not a multiple of Hk=%d", Hv, Hk)
         _need(0 < K <= _lib.GDR_MAX_K and 0 < V <= _lib.GDR_MAX_V, "K=%d V=%d: up to %d, %d supported", K, V, _lib.GDR_MAX_K, _lib.GDR_MAX_V)
         self.Hk, self.Hv, self.K, self.V, self.dtype = Hk, Hv, K, V, dtype
         self.scale = float(K) ** -0.5 if scale is None else float(scale)
@@ -122,6 +122,7 @@ class GatedDelta:
     def workspace(self, n_seq: int, rows: int, device, packed: bool = True, no_backward: bool = False) -> torch.Tensor:
         """Workspace for n_seq sequences of `rows` tokens in all (of one padded length if not packed); what serves packed
         sequences serves as many padded ones too."""
+        _need(0 < n_seq < 1 << 31 and 0 < rows < 1 << 31, "n_seq=%d rows=%d", n_seq, rows)
         n = self._lib.hhrl_gdr_workspace_floats(self.code, n_seq, rows, int(packed), self.Hk, self.Hv, self.K, self.V, int(no_backward))
         _need(n > 0, "no workspace for n_seq=%d rows=%d", n_seq, rows)
         return torch.empty(n, dtype=torch.float32, device=device)
@@ -234,7 +235,7 @@ class BlockNorm:
         self.code = _dtype_code(dtype)
         _need(post in _NORMS and pre in _NORMS, "norms %r, %r: none, rms or layer", post, pre)
         _need(gate_act in _GATES, "gate_act %r: none, sigmoid or silu", gate_act)
-        _need(0 < D <= 8192 and H > 0, "H=%d D=%d: D up to 8192", H, D)
+        _need(0 < D <= 8192 and 0 < H < 1 << 31, "H=%d D=%d: D up to 8192", H, D)
         _need(1 <= gate_rows < 1 << 63 and (gate_rows == 1 or H == 1), "gate_rows=%d with H=%d", gate_rows, H)
         _need(eps >= 0, "eps=%g", eps)
         self.D, self.H, self.post, self.pre, self.gate_act, self.gate_rows = D, H, post, pre, gate_act, gate_rows
@@ -248,6 +249,7 @@ class BlockNorm:
 
     def workspace(self, M: int, device) -> torch.Tensor:
         """Workspace of `bwd` for M rows."""
+        _need(0 < M < 1 << 40, "M=%d", M)
         n = self._lib.hhrl_block_norm_workspace_floats(M, self.H, self.D, self.gate_rows)
         _need(n > 0, "no workspace for M=%d", M)
         return torch.empty(n, dtype=torch.float32, device=device)

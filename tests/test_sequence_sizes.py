@@ -86,3 +86,17 @@ def test_parameter_gradients_that_overlap_are_refused(lib, a, b, apart):
     base = 16 * FAKE
     d = norm_desc(10, 64, 1, 1 << 40, **{a: base, b: base + apart})
     assert lib.hhrl_block_norm_backward(C.byref(d), None) == 1 and b"overlap" in lib.hhrl_last_error(), lib.hhrl_last_error()
+
+
+BIG = (1 << 32) + 1                # what an int of 32 bits takes for 1
+
+
+@pytest.mark.parametrize("make", [
+    lambda s: s.BlockNorm(64, H=BIG), lambda s: s.GatedDelta(BIG, BIG, 64, 64), lambda s: s.GatedDelta(1, BIG, 64, 64),
+    lambda s: s.GatedDelta(1, 1, 64, 64).workspace(BIG, 10, "cpu"), lambda s: s.GatedDelta(1, 1, 64, 64).workspace(1, (1 << 64) + 10, "cpu"),
+    lambda s: s.BlockNorm(64).workspace((1 << 64) + 10, "cpu"),
+])
+def test_numbers_that_the_library_would_cut_off_are_refused(make):
+    from hhrl_vae_amd import sequence
+    with pytest.raises(ValueError):
+        make(sequence)
