@@ -226,7 +226,8 @@ def run(st):
         p.fwd(out=st["out"], h=st["h"], **args)
         res = {"out": st["out"], "h": st["h"]}
         if case["op"] == "norm_train":
-            torch._foreach_zero_(st["par"])           # parameter gradients are added to
+            if st["par"]:                             # (norms may have no parameters)
+                torch._foreach_zero_(st["par"])       # parameter gradients are added to
             grads = {"d" + k: st["d" + k] for k in args}
             p.bwd(d_out=st["d_out"], d_h=st["d_h"], ws=st["ws"], **args, **grads)
             res.update(grads)
