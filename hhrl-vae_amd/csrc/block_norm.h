@@ -41,6 +41,9 @@ constexpr int kNormE = 8;       // elements of a row per thread
 // Waves per SIMD of the kernels, which the launches fill the chip by: workgroups beyond what is resident at once cost a
 // second round (bf16 rows of 4096, forward: 56 us with 768 workgroups of 512 threads, 71 us with 1024).  A backward pass
 // in bf16 vectors without biases is held to 128 registers for four waves (168 us with one workgroup of 512 threads per CU).
+// Rows of 4097 to 8192 elements take 1024 threads, which have 128 registers at most: their backward kernels spill, most of
+// all those with biases (both norms of 8192 columns trained: bf16 rms 4.3 TB/s, layer 3.3, fp32 4.7 and 3.0; of 5120, where
+// three eighths of the threads idle, 2.9, 2.3, 4.3 and 2.4; of 4096 4.1, 2.9, 4.6 and 4.5).
 constexpr int norm_bwd_waves(int el, int vec, bool bias) { return el == 2 && vec > 1 && !bias ? 4 : 2; }
 constexpr int norm_fwd_waves(int el, int vec) { return el == 2 && vec > 1 ? 6 : 4; }
 
@@ -209,8 +212,8 @@ template <typename T>
 struct Gate {
   // s = sigmoid(z) and c = 1 - s, relative 2^-22 each for either type: parameter gradients and shared gates are fp32 results.
   // exp(-z) as the power of two of the rounded product with log2 e, times 1 + what the product and the constant leave out
-  // (without it 2^-24 |z|); behind +-88 s and c are at fp32's ends.  With expf() and a division norms of 16384 x 16 heads of
-  // 128 with a SiLU gate took 131 us forward and backward.
+  // (without it 2^-24 |z|); behind +-88 s and c are at fp32's ends.  Norms of 16384 x 16 heads of 128 with a SiLU gate take 112 us
+  // forward and backward, 131 with expf() and a division.
   static __device__ __forceinline__ void sigmoid(float z, float& s, float& c) {
     const float x = __builtin_elementwise_maximum(__builtin_elementwise_minimum(z, 88.f), -88.f);   // (NaN stays)
     const float t = x * -1.44269502f;

@@ -27,9 +27,10 @@
 // and the states are fp32 results.  The decays' sums are kept as two floats from a sum in fp64, so that exp(G_i - G_j) is exact
 // to fp32 however far G has run.
 //
-// What a whole training call moves: per chunk and head of K = V = 128, bf16, 0.8 MB, of which the caller's tensors are 0.13;
-// 4 x 4096 tokens of 16 heads take 0.12 (prep) + 0.25 + 0.24 (scans) + 0.37 ms (gradients), 3.6 GB at 3.7 TB/s (a copy
-// reaches 4.85).  Larger chunks would move fewer states, and pay for it in the triangles and in accuracy.
+// What a whole training call moves: per chunk and head of K = V = 128, bf16, 0.9 MB, of which the caller's tensors are 0.13;
+// 4 x 4096 tokens of 16 heads take 0.13 (prep) + 0.26 + 0.24 (scans) + 0.37 ms (gradients), 3.8 GB at 3.7 TB/s (a copy
+// reaches 4.85), with the matrix pipes 6 to 24 % busy: neither is full.  Larger chunks would move fewer states, and pay
+// for it in the triangles and in accuracy.
 #include "common.h"
 #include "mfma_tiles.h"
 #include "split_bf16.h"
@@ -182,8 +183,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, lo
 // the blocks below them, 16 and 32 wide, as -M22 (L21 M11) on the fp32 matrix instruction.  P is written straight from the
 // registers of a product: four elements of a row from k q^T, of a column (for the transpose) from q k^T.  The 32 x 32
 // blocks beyond the diagonal are neither written nor read.
-// Bound by what it writes where there are many chunks (4 x 4096 tokens, 16 heads, K 128, bf16, for training: 0.54 GB in
-// 125 us), else by the latency of its steps (64 chunks in fp32: 17 us, of which the products of the last row of tiles, the
+// Bound by what it writes where there are many chunks (4 x 4096 tokens, 16 heads, K 128, bf16, for training: 0.58 GB in
+// 134 us), else by the latency of its steps (64 chunks in fp32: 17 us, of which the products of the last row of tiles, the
 // decays and the substitution are 4 us each).  Three workgroups per CU fill the waits of each other.
 template <int NP, int KB2>
 struct PrepLds {
@@ -486,7 +487,7 @@ __device__ __forceinline__ int longest(const GdrArgs& a, int r) {
   return __ffsll((unsigned long long)__ballot(lane < a.n_seq && rank == r)) - 1;
 }
 // Workgroup -> (sequence, value head, segment, column tile).  Sequences of different lengths go from the longest (by_length),
-// so that the last workgroups are short ones: 13 sequences of 12345 tokens, 16 heads 160 -> 132 us.  Workgroups go to the
+// so that the last workgroups are short ones: 13 sequences of 12345 tokens, 16 heads 182 -> 151 us.  Workgroups go to the
 // eight XCDs in turn: the column tiles of one head read the same k, q, M and P, so they are dealt to one XCD (one L2),
 // eight workgroups apart.
 __device__ __forceinline__ bool scan_tile(const GdrArgs& a, int vt, int& n, int& hv, int& v0, int& seg) {
@@ -715,9 +716,9 @@ __device__ __forceinline__ void load_tri(bf16x8 (&f)[2][N], const __bf16* base, 
 // and four others what hangs on it: v in front of it and the output o one chunk behind (forward), or what only depends on
 // dO, one chunk ahead, and the stores of Y and dV (backward).  Everything a chunk needs from memory is requested while the
 // chunk in front of it is worked on, behind the last use of its registers.
-// Measured with K = V = 128, bf16: 1.6 us per chunk alone with 16 columns, 2.4 with 32 and the chip full; splitting the
-// state and the two right-hand sides into terms, three barriers and the matrix products share it about evenly.  Training
-// adds the stores of S and W: 64 chunks of 64 heads take 249 us forward, 0.46 GB written, 240 backward.  Two workgroups
+// Measured with K = V = 128, bf16: alone 1.4 us per chunk with 16 columns and 2.2 with 32, 2.6 with 32 and the chip full;
+// splitting the state and the two right-hand sides into terms, three barriers and the matrix products share it about
+// evenly.  Training adds the stores of S and W: 64 chunks of 64 heads take 261 us forward, 0.47 GB written, 240 backward.  Two workgroups
 // per CU (128 registers) were slower for all sizes (167 -> 179 us, 256 -> 366 for training): the registers do not hold it.
 // The chain: chunks c0 .. c1 - 1 of a sequence, four waves, S in their registers.  BARE: nobody hangs on it (no W is left in
 // wl, and v comes into vl by these waves).  vcols: V, or 0 for columns without a v (and v0 what it may).
@@ -970,7 +971,7 @@ float y[4 * NT];
 // state it is given to M S + N; one launch finds M and N of every segment but the last (the chain alone, on the columns of
 // V from a zero state and on K columns without a v from the unit state), one joins the states along the segments, and the
 // scan then runs with every segment's own first state.  The chain is walked twice, and K / V more columns of it the first
-// time, by as many times the workgroups.  32768 tokens of 8 heads, 8 segments: 837 us -> 180 + 18 (joining) + 151.
+// time, by as many times the workgroups.  32768 tokens of 8 heads, 8 segments: 858 us -> 187 + 19 (joining) + 168.
 template <typename T, int NP, int KB2, bool WIDE>
 __global__ __launch_bounds__(256, 2) void gdr_segment_kernel(GdrArgs a) {
   constexpr int NT = 2;
@@ -1313,8 +1314,9 @@ __global__ __launch_bounds__(512, 1) void gdr_scan_bwd_kernel(GdrArgs a) {
 // One workgroup per chunk and key head; the value heads of the key head one after the other, so that dq and dk are summed
 // in registers in a fixed order.  Eight waves: 16 tokens against half of K each.  S, dS', W, Y and dO pass through LDS 32
 // columns at a time as bf16 terms; the next 32 columns are on their way from memory meanwhile.
-// Bound by memory where the chip is full: 4 x 4096 tokens of 16 heads, K = V = 128, bf16, read 1.06 GB and write 0.15 in
-// 375 us (3.2 TB/s); one chunk takes a CU 42 thousand cycles, 11 thousand of them matrix products.
+// Where the chip is full neither memory nor the matrix pipes are: 4 x 4096 tokens of 16 heads, K = V = 128, bf16, read 1.09 GB
+// and write 0.15 in 375 us (3.3 TB/s, two thirds of what a copy reaches); one chunk takes a CU, which it has to itself, 42
+// thousand cycles, 11 thousand of them matrix products.  The rest are splits into terms and waits at barriers and for the next columns.
 template <int NP, int KB2>
 struct GradsLds {
   static constexpr int Kp = 64 * KB2, LDV = 32;              // columns at a time
@@ -1861,9 +1863,9 @@ long slots_of(int n_seq, long rows, bool packed) {
 
 // Segments per sequence and their chunks.  Cutting a sequence in s pays a second walk of 1/s of the chunks with K / V more
 // columns and a join of s steps, about one chunk each, so it takes three, of 16 chunks or more, and a chip whose 256 CUs
-// hold them side by side (32-column workgroups).  Measured for 32768 tokens, K = V = 128, whole calls: 8 heads (8 segments)
-// 930 -> 475 us, 12 (5) 1005 -> 742, 16 (4) 1043 -> 877, 20 (3) 1152 -> 1112; 4096 tokens, 8 heads (4 of 16 chunks) 98 ->
-// 97; two segments would be slower than none.  Packed sequences may all be one.
+// hold them side by side (32-column workgroups).  Measured for 32768 tokens, K = V = 128 (no other widths), whole calls: 8
+// heads (8 segments) 935 -> 457 us, 12 (5) 1013 -> 701, 16 (4) 1034 -> 822, 20 (3) 1139 -> 1036; 4096 tokens, 8 heads (4 of 16
+// chunks) 105 -> 102; two segments would be slower than none.  Packed sequences may all be one.
 int segments_of(int n_seq, long rows, bool packed, int Hv, int vp, int* chunks) {
   const long most = packed ? rows / kC + 1 : (rows / n_seq + kC - 1) / kC, wgs = (long)n_seq * Hv * (vp / 32);
   long segs = 256 / wgs;
@@ -1960,8 +1962,9 @@ int gdr_fill(const hhrl_gdr_desc* d, GdrArgs& a, bool train, const char* who) {
 }
 
 // Columns per workgroup of a scan: 16 where twice the workgroups still have a CU each (the chain from chunk to chunk is
-// shorter), else 32.  Measured for 16 chunks, K = V = 128, with 16 / 32 columns: 128 workgroups of 32 27 / 38 us, 144 40 / 39,
-// 224 42 / 40, 256 43 / 41.  Segments fill the chip with 32.
+// shorter), else 32.  Measured for 16 chunks, K = V = 128, with 16 / 32 columns: 128 workgroups of 32 30 / 41 us, 144 44 / 42,
+// 224 47 / 45, 256 48 / 45; of narrower heads (K <= 64, bf16) two workgroups fit on a CU, and they were not measured apart.
+// Segments fill the chip with 32.
 int scan_tiles(const GdrArgs& a) { return a.segs > 1 || (long)a.n_seq * a.Hv * (a.vp / 32) > 128 ? 2 : 1; }
 unsigned scan_grid(const GdrArgs& a) { return (unsigned)(((long)a.n_seq * a.Hv * a.grid_segs + 7) / 8 * 8 * a.nvt); }
 
