@@ -2118,8 +2118,8 @@ int hhrl_gdr_step(const hhrl_gdr_step_desc* d, void* stream) {
   a.q = d->q; a.k = d->k; a.v = d->v; a.ldq = d->ldq; a.ldk = d->ldk; a.ldv = d->ldv; a.g = d->g; a.beta = d->beta; a.ldg = d->ldg; a.ldbeta = d->ldbeta;
   a.o = d->o; a.ldo = d->ldo; a.sin = d->state_in; a.sout = d->state_out; a.slots = d->slots;
   a.nvt = ceil_div(d->V, vec ? 64 : 16);
-  const long grid = (long)d->B * d->Hv * a.nvt;
-  HHRL_REQUIRE(grid < (1L << 24), "gdr_step: B*Hv*V too large: %ld workgroups of 256 threads", grid);
+  const long grid = (long)d->B * d->Hv < (1L << 24) ? (long)d->B * d->Hv * a.nvt : 1L << 24;
+  HHRL_REQUIRE(grid < (1L << 24), "gdr_step: B*Hv*V too large: %ld or more workgroups of 256 threads", grid);
   hipStream_t st = as_stream(stream);
   ProfScope ps("gdr_step_kernel", st, 6.0 * d->B * d->Hv * d->K * d->V, 8.0 * d->B * d->Hv * d->K * d->V);
   if (d->dtype == HHRL_BF16) {

@@ -100,3 +100,14 @@ def test_numbers_that_the_library_would_cut_off_are_refused(make):
     from hhrl_vae_amd import sequence
     with pytest.raises(ValueError):
         make(sequence)
+
+
+def test_gdr_step_counts_its_workgroups_without_overflow(lib):
+    """2^30 rows of 2^30 heads of 16 column tiles are 2^64 workgroups, which a long takes for none."""
+    from hhrl_vae_amd import _lib
+    d = _lib.GdrStepDesc()
+    n, V = 1 << 30, 256
+    for k, v in dict(dtype=0, B=n, Hk=1, Hv=n, K=1, V=V - 1, scale=1.0, n_slots=n, q=FAKE, k=FAKE, v=FAKE, ldq=1, ldk=1, ldv=n * V, g=FAKE, beta=FAKE, ldg=n,
+                     ldbeta=n, o=FAKE, ldo=n * V, state_in=FAKE, state_out=FAKE).items():
+        setattr(d, k, v)
+    assert lib.hhrl_gdr_step(C.byref(d), None) == 1 and b"too large" in lib.hhrl_last_error(), lib.hhrl_last_error()
