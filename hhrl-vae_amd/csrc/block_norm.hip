@@ -16,8 +16,8 @@ namespace hhrl {
 void norm_launch_f32(const NormArgs& a, bool vec, int tpr, int blocks, bool bwd, hipStream_t st) { norm_launch<float, 4>(a, vec, tpr, blocks, bwd, st); }
 
 // Sums the partial rows in their order: the parameter gradients (ADDED to dst) over all workgroups, and the gate rows
-// (written) over the parts of their group.  Parameters with one gradient (a weight that both norms share) are one job.  32 columns x 32 row lanes per workgroup: 1024 rows of 128 columns are few
-// workgroups and a long walk (8 row lanes: 8.0 us).
+// (written) over the parts of their group.  Parameters with one gradient (a weight that both norms share) are one job.
+// 32 columns x 32 row lanes per workgroup: 1024 rows of 128 columns are few workgroups and a long walk (8 row lanes: 8.0 us).
 struct NormFoldArgs {
   const float* par_ws;
   const float* gate_ws;

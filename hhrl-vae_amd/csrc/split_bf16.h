@@ -1,10 +1,11 @@
 // fp32-accurate products on the bf16 matrix instructions (gfx950, wave64).
 //
 // An fp32 number is the sum of three bf16 numbers up to 2^-27 of itself (8 + 8 + 8 significand bits and the signs of the
-// remainders; terms below 2^-126, the least normal number, are lost, so numbers below 2^-109 are kept to 2^-126), so a product of two such operands is the sum of the six partial products whose weights are above 2^-25,
-// accumulated in fp32 by the matrix instruction; an operand that is bf16 to begin with needs three.  At 16384 FLOPs in 16
-// cycles (v_mfma_f32_16x16x32_bf16) against 2048 in 32 (v_mfma_f32_16x16x4_f32) six of them still cost 2.7 times less
-// than the fp32 instruction, three 5.3 times less.
+// remainders; terms below 2^-126, the least normal number, are lost, so numbers below 2^-109 are kept to 2^-126), so a
+// product of two such operands is the sum of the six partial products whose weights are above 2^-25, accumulated in fp32 by
+// the matrix instruction; an operand that is bf16 to begin with needs three.  At 16384 FLOPs in 16 cycles
+// (v_mfma_f32_16x16x32_bf16) against 2048 in 32 (v_mfma_f32_16x16x4_f32) six of them still cost 2.7 times less than the
+// fp32 instruction, three 5.3 times less.
 //
 // v_mfma_f32_16x16x32_bf16: lane l supplies A[i = l&15][k] and B[k][j = l&15] for the eight k at 8*(l>>4); both operands
 // use the same k, so an operand fragment is 16 contiguous bytes of a row whose memory runs along the reduction.  The four

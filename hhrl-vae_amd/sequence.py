@@ -310,8 +310,8 @@ class BlockNorm:
     def bwd(self, x=None, y=None, gate=None, w_post=None, b_post=None, w_pre=None, b_pre=None, d_out=None, d_h=None,
             dx=None, dy=None, dgate=None, dw_post=None, db_post=None, dw_pre=None, db_pre=None, ws=None) -> None:
         """Gradients of <d_out, r> + <d_h, h> (either None: absent) from the forward call's inputs: dx, dy, dgate are
-        written, parameter gradients added to; those that are None are skipped.  ws: needed for parameter gradients and for
-        the gradient of a gate with gate_rows > 1."""
+        written, parameter gradients added to (two may be one tensor: it gets both); those that are None are skipped.  ws:
+        needed for parameter gradients and for the gradient of a gate with gate_rows > 1."""
         dev = _device()
         d, M, act = self._desc(x, y, gate, (w_post, b_post, w_pre, b_pre), dev)
         _need(d_out is not None or d_h is not None, "neither d_out nor d_h")

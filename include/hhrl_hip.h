@@ -418,9 +418,9 @@ int hhrl_lstm_backward_group(const hhrl_lstm_desc* descs, int n, int B, int T, i
  * wanted; may be s0).  A sequence without tokens hands its state on.
  * Forward writes o.  Unless no_backward is set it leaves in ws what the backward call reads; ws
  * (hhrl_gdr_workspace_floats, 16-byte aligned) must then stay untouched until that call, which takes the same inputs,
- * scale and sequences (whose last forward pass in ws was for other shapes, or with no_backward, is an error that only the
- * device sees: every gradient is NaN), and writes dq, dk, dv (dtype), dg, dbeta and, where given, d_s0 (gradients with respect to q .. s0 of
- * <d_o, o> + <d_s1, s1>; d_o and d_s1 may not both be null; d_s0 may be d_s1).  Other outputs overlap no operand.
+ * scale and sequences, and writes dq, dk, dv (dtype), dg, dbeta and, where given, d_s0 (gradients with respect to q .. s0
+ * of <d_o, o> + <d_s1, s1>; d_o and d_s1 may not both be null; d_s0 may be d_s1).  If the last forward pass in ws was of
+ * other shapes, or with no_backward, every gradient is NaN (only the device sees that error).  Other outputs overlap no operand.
  * The products run on bf16 matrix instructions with every fp32 operand as three bf16 terms: results carry fp32
  * accuracy for either dtype, o and the input gradients are rounded once.  No atomics: the same bits on every run.
  * A non-finite number in a token may spread to the 63 tokens before it (they share a chunk) and to all behind it. */
@@ -473,8 +473,9 @@ int hhrl_gdr_step(const hhrl_gdr_step_desc* d, void* stream);
  * fp32 gate row (modulation of a sequence; gate_rows >= M: one learned gate per channel).
  * out (r) and h are rounded from the same fp32 row; either may be null; both may be x or y.
  * Backward forms everything again from the inputs (no saved statistics).  d_out, d_h: gradients of r and h, either may
- * be null.  dx, dy, dgate are written, dw_*, db_* ADDED to (two of them may be one array: it gets both); any may be null.  Parameter gradients and a shared gate's
- * need ws (hhrl_block_norm_workspace_floats, 16-byte aligned); sums are made in a fixed order.  D <= 8192. */
+ * be null.  dx, dy, dgate are written, dw_*, db_* ADDED to (two of them may be one array: it gets both); any may be null.
+ * Parameter gradients and a shared gate's need ws (hhrl_block_norm_workspace_floats, 16-byte aligned); sums are made in a
+ * fixed order.  D <= 8192. */
 typedef struct {
   int dtype;
   long M; int H, D;
